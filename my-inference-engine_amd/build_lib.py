@@ -1,10 +1,11 @@
-"""Build libmi_fa2.so and libmi_model.so (the HIP kernels + C ABIs) in-tree with hipcc for gfx950.
+"""Build libmi_fa2.so, libmi_model.so and libmi_cache.so (the HIP kernels + C ABIs) in-tree with hipcc for gfx950.
 
     python my-inference-engine_amd/build_lib.py
 
 Compiles every source of csrc/ in parallel into _build/ and links kernels/libmi_fa2.so (attention,
-sampling, step metadata; loaded by kernels/_lib.py) and kernels/libmi_model.so (the projections of
-few rows; loaded by kernels/few_rows.py).  Always rebuilds (a few seconds per file).
+sampling, step metadata; loaded by kernels/_lib.py), kernels/libmi_model.so (the projections of
+few rows; loaded by kernels/few_rows.py) and kernels/libmi_cache.so (block operations and attention
+over shared blocks; loaded by kernels/blocks.py).  Always rebuilds (a few seconds per file).
 """
 import os
 import subprocess
@@ -21,6 +22,7 @@ LIBS = {
     OUT: ["fa2_prefill.hip", "fa2_decode.hip", "fa2_general.hip", "fa2_prefill_dims.hip", "fa2_merge.hip",
           "rope_kv.hip", "sample.hip", "step_meta.hip", "model_ops.hip", "fa2_capi.cpp"],
     PKG / "kernels" / "libmi_model.so": ["linear_rows.hip", "model_capi.cpp"],
+    PKG / "kernels" / "libmi_cache.so": ["block_ops.hip", "shared_attn.hip", "cache_capi.cpp"],
 }
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
