@@ -75,11 +75,11 @@ MI_CACHE_API int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t n
  * first prefix_lens[g] tokens, which are read once for all of them, through the table of the group's
  * first row.  A prefix is used as far as every query of its group sees it and the first row holds it;
  * what is left of it, and a row of no group, is read through the row's own table.  Empty groups may
- * stand anywhere; where groups overlap, the last one holds the row.
+ * stand anywhere; where groups overlap, a row can only be in the one that begins last before it.
  *
  * q, o [cu_seqlens_q[batch]][heads_q][128] with strides (token, head), pools [slots][heads_kv][128]
  * with strides (slot, head), lse strides (head, token).  total_q: the tokens of q, at least
- * cu_seqlens_q[batch].  At most 1,024 rows, n_groups <= batch.  workspace:
+ * cu_seqlens_q[batch].  At most 512 rows and 2^25 (token, head) pairs, n_groups <= batch.  workspace:
  * mi_cache_attend_workspace_size bytes, 16-byte aligned, contents arbitrary; not shared by calls that
  * may overlap in time.
  */

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -34,6 +35,22 @@ int ok() {
 int launched(hipError_t err) {
   if (err != hipSuccess) return fail(kLaunch, "kernel launch failed: %s", hipGetErrorString(err));
   return ok();
+}
+
+// The current device's compute units, read once per device.
+int compute_units(int* out) {
+  static std::atomic<int> known[64];
+  int dev = -1;
+  *out = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err == hipSuccess && dev >= 0 && dev < 64) *out = known[dev].load(std::memory_order_relaxed);
+  if (err == hipSuccess && *out == 0) {
+    err = hipDeviceGetAttribute(out, hipDeviceAttributeMultiprocessorCount, dev);
+    if (err == hipSuccess && dev < 64) known[dev].store(*out, std::memory_order_relaxed);
+  }
+  if (err != hipSuccess || *out <= 0)
+    return fail(kLaunch, "reading the device's CU count failed: %s", hipGetErrorString(err));
+  return kOk;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -68,6 +85,9 @@ int check_table(const int32_t* tables, int64_t stride, int32_t width, int32_t ma
                 (long long)stride);
   return kOk;
 }
+
+// (token, head) pairs of a call: a wave each in the merge, below 2^32 threads.
+constexpr int64_t kMaxPairs = int64_t(1) << 25;
 
 int check_tensor(const char* name, const void* p, const int64_t* strides) {
   if (!p) return fail(kInvalid, "%s is NULL", name);
@@ -172,7 +192,10 @@ int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t num_blocks, in
   return launched(mi_fa2::launch_block_op(p, mi_fa2::kMove, static_cast<hipStream_t>(stream)));
 }
 
-size_t mi_cache_attend_workspace_size(int32_t, int32_t) { return 0; }
+size_t mi_cache_attend_workspace_size(int32_t total_q, int32_t heads_q) {
+  if (total_q <= 0 || heads_q <= 0 || int64_t(total_q) * heads_q > kMaxPairs) return 0;
+  return mi_fa2::shared_space(total_q, heads_q).total;
+}
 
 int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool, const void* v_pool, void* o,
                     float* lse, const int32_t* cu_seqlens_q, const int32_t* block_table,
@@ -193,6 +216,13 @@ int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool, const void
   if (batch > mi_fa2::kShMaxRows || heads_q > 65535)
     return fail(kUnsupported, "batch %d (at most %d), heads_q %d (at most 65535)", batch,
                 mi_fa2::kShMaxRows, heads_q);
+  if (int64_t(total_q) * heads_q > kMaxPairs)
+    return fail(kUnsupported, "%d tokens of %d heads: at most 2^25 pairs", total_q, heads_q);
+  // the units of work are counted in 32 bits: (tiles of 128 pairs, at most one more per range and
+  // head) x (steps of 64 keys)
+  if ((int64_t(total_q) * heads_q / 64 + 4 * int64_t(batch) * heads_kv) *
+          (max_kv_len / 64 + int64_t(1)) >= int64_t(1) << 31)
+    return fail(kUnsupported, "%d tokens over %d keys in one call", total_q, max_kv_len);
   if (n_groups < 0 || n_groups > batch)
     return fail(kInvalid, "n_groups %d: 0 to batch (%d)", n_groups, batch);
   if (max_kv_len < 0) return fail(kInvalid, "max_kv_len %d < 0", max_kv_len);
@@ -249,7 +279,10 @@ int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool, const void
   p.num_blocks = num_blocks;
   p.causal = is_causal ? 1 : 0;
   p.scale_log2 = sm_scale * mi_fa2::kLog2e;
-  return launched(mi_fa2::launch_shared(p, dtype, static_cast<hipStream_t>(stream)));
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  return launched(
+      mi_fa2::launch_shared(p, dtype, cus, workspace, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

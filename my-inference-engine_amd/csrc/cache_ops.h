@@ -29,7 +29,7 @@ enum BlockOp { kCopy = 0, kFork = 1, kMove = 2 };
 hipError_t launch_block_op(const BlockOpParams& p, int op, hipStream_t stream);
 
 // Rows per call of the attention.
-constexpr int kShMaxRows = 1024;
+constexpr int kShMaxRows = 512;
 
 struct SharedParams {
   const uint16_t* q;    // [total_q][Hq][128], token and head strides
@@ -47,7 +47,36 @@ struct SharedParams {
   int32_t G, B, total_q, Hq, Hkv, group;
   int32_t max_kv, bs_shift, num_blocks, causal;
   float scale_log2;
+  // filled by launch_shared
+  FastDiv group_div;
+  float* ws_o;          // parts: [column][128] fp32, unnormalised
+  float* ws_ml;         // [column][2]: maximum (of the unscaled scores) and sum
+  int32_t* ws_where;    // [2][total_q][Hq][2]: where a pair's parts stand, of the prefix and its own keys
+  int32_t columns;      // of the workspace
+  int32_t narrow_base;  // the first column of the waves' parts
 };
-hipError_t launch_shared(const SharedParams& p, int dtype, hipStream_t stream);
+
+// The workspace.  In each of two areas (the work-groups' parts and the waves') an item's parts begin at
+// the number of pairs before the item (prefixes first, total_q * heads_q of them, then rows) and worker
+// w's part of it stands w tiles further: from one (item, worker) to the next either number grows, so no
+// two parts meet.
+constexpr int kSharedWgs = 256, kSharedWaves = 8, kSharedTile = 128, kSharedNarrow = 32;
+struct SharedSpace {
+  int32_t columns, narrow;
+  size_t ml, where, total;   // byte offsets after the O parts
+};
+inline SharedSpace shared_space(int64_t total_q, int64_t heads_q) {
+  const int64_t pairs = 2 * total_q * heads_q;
+  const int64_t narrow = pairs + kSharedTile * kSharedWgs;
+  const int64_t columns = narrow + pairs + kSharedNarrow * kSharedWgs * kSharedWaves;
+  SharedSpace s{};
+  s.columns = (int32_t)columns;
+  s.narrow = (int32_t)narrow;
+  s.ml = (size_t)columns * kHeadDim * sizeof(float);
+  s.where = s.ml + (size_t)columns * 2 * sizeof(float);
+  s.total = s.where + (size_t)pairs * 2 * sizeof(int32_t);
+  return s;
+}
+hipError_t launch_shared(SharedParams p, int dtype, int n_cus, void* workspace, hipStream_t stream);
 
 }  // namespace mi_fa2

@@ -1,84 +1,880 @@
-// Attention of packed new tokens over a paged cache.
+// Attention of packed new tokens over a paged cache, keys that rows share read once.
 //
-// One work-group per (token, query head); its four waves take every fourth key and meet in LDS.  A
-// lane holds two of the head's dims, a score is the sum of the lanes' products, and each wave keeps
-// the running maximum m, sum l and output O of the softmax:
-//   m' = max(m, s), l' = l e^(m - m') + e^(s - m'), O' = O e^(m - m') + e^(s - m') v.
+// The softmax of a query over its keys is the merge of softmaxes over disjoint ranges of them: with
+// m = max s, l = sum e^(s - m), O = sum e^(s - m) v of each range, M = max m:
+//   L = sum l e^(m - M), O = sum O e^(m - M) / L.
+// So the keys are cut by who holds them: the prefix of a group of rows (one range for all the group's
+// queries) and each row's keys behind it.  All query heads of a kv head read the same keys, so a
+// range's queries are its (token, head) pairs: column p of a tile is token p / group, head p % group.
+//
+// Ranges, and the work.  Range s < B is the prefix of the group that row s leads, range B + b row b's
+// own keys.  A range of up to 32 pairs is narrow: its items (kv head) are walked by single waves, 64
+// keys a unit.  A wider one is cut into tiles of up to 128 pairs, whose items (kv head, tile) are walked
+// by whole work-groups, 128 keys a unit.  The units of each kind are dealt out in equal contiguous
+// shares, over the work-groups (one of 8 waves per CU) and over their waves; every work-group finds its
+// shares from the lengths, so a captured launch follows them.  A worker leaves its part of an item in
+// the workspace, and shared_merge_kernel merges the parts of each (token, head).
+//
+// The walks.  K and V travel from memory to LDS (buffer_load ... lds); S^T = K Q^T and O^T += V^T P^T on
+// v_mfma_f32_32x32x16 as in the prefill kernel: one column per lane, P in registers as it comes.  K rows
+// of 256 bytes with chunk ^ row % 16, V with chunk ^ 4 (row % 4), so that the reads of both (V's
+// transposing) are free of bank conflicts.
+//   A wide item's 128-key steps are loaded by all eight waves, one 16-key run each (a run lies in one
+// block), a step ahead; a wave takes 32 columns and 64 keys of a step (up to 128 columns) or 32 keys (up
+// to 64), and the key streams meet in LDS at the end.
+//   A narrow item's 32-key steps are one wave's, in LDS of its own without barriers: once K is in
+// registers the next step's K is sent for, likewise V.
 #include "cache_ops.h"
 
 namespace mi_fa2 {
 
-constexpr int kShWaves = 4;
+constexpr int kShWaves = kSharedWaves, kShThreads = 64 * kShWaves;
+constexpr int kShTile = kSharedTile;            // pairs of a wide tile
+constexpr int kShNarrow = kSharedNarrow;        // pairs a narrow range has at most
+constexpr int kShStep = 32;                     // keys of an MFMA block, and of a narrow step
+constexpr int kShNarrowUnit = 64;
+constexpr int kShWideUnit = 128;                // keys of a wide step
+constexpr int kShRow = kHeadDim * 2;            // bytes of a key
+constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
+constexpr int kShRing = 2 * kShStage / kShWaves;     // a wave's part of the two stages: 16 KB
+static_assert(kShRing == 2 * kShStep * kShRow, "a narrow step's K and V");
+static_assert(kShRing == kShStep * kHeadDim * 4, "a wave's 32 columns of O");
 
-template <typename E>
-__global__ __launch_bounds__(64 * kShWaves) void shared_attn_kernel(const SharedParams p) {
-  const int token = blockIdx.x, h = blockIdx.y, hk = h / p.group;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the row that holds the token: cu_q[b] <= token < cu_q[b + 1]
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (p.cu_q[m] <= token) lo = m; else hi = m;
-  }
-  const int b = lo, q0 = p.cu_q[b], n = p.cu_q[b + 1] - q0;
-  if (token < q0 || token >= q0 + n) return;
-  const int kv = clamp_len(p.kv_lens[b], p.max_kv);
-  const int seen = p.causal ? min(kv, kv - n + 1 + (token - q0)) : kv;
+// What a work-group knows of the call, in LDS.
+struct ShPlan {
+  int wide[2 * kShMaxRows + 1];    // units of the ranges before this one
+  int narrow[2 * kShMaxRows + 1];
+  int cu[kShMaxRows + 1];
+  int kv[kShMaxRows];
+  int prefix[kShMaxRows];          // at a group's first row: keys read for the whole group
+  int16_t lead[kShMaxRows];        // the first row of the row's group, -1: none
+  int16_t end[kShMaxRows];         // at a group's first row: the row after its last
+};
 
-  const uint32_t qw = *reinterpret_cast<const uint32_t*>(p.q + token * p.q_st + h * p.q_sh + 2 * lane);
-  const float qa = E::lo(qw), qb = E::hi(qw);
-  float m = -INFINITY, l = 0.f, oa = 0.f, ob = 0.f;
-  for (int j = wave; j < seen; j += kShWaves) {
-    const int blk = p.table[b * p.bt_stride + (j >> p.bs_shift)];
-    const bool in = (unsigned)blk < (unsigned)p.num_blocks;
-    const int64_t slot = ((int64_t)blk << p.bs_shift) + (j & ((1 << p.bs_shift) - 1));
-    const int64_t at = slot * p.kv_st + hk * p.kv_sh + 2 * lane;
-    const uint32_t kw = in ? *reinterpret_cast<const uint32_t*>(p.k + at) : 0;
-    const uint32_t vw = in ? *reinterpret_cast<const uint32_t*>(p.v + at) : 0;
-    float s = qa * E::lo(kw) + qb * E::hi(kw);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2_fast(m - mu), w = exp2_fast(s - mu);
-    l = l * a + w;
-    oa = oa * a + w * E::lo(vw);
-    ob = ob * a + w * E::hi(vw);
-    m = mn;
-  }
-  __shared__ float sm[kShWaves], sl[kShWaves], so[kShWaves][kHeadDim];
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
-  so[wave][2 * lane] = oa;
-  so[wave][2 * lane + 1] = ob;
-  __syncthreads();
-  if (wave != 0) return;
-  float M = -INFINITY, L = 0.f;
-  oa = ob = 0.f;
-  for (int w = 0; w < kShWaves; ++w) M = fmaxf(M, sm[w]);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  for (int w = 0; w < kShWaves; ++w) {
-    const float f = exp2_fast(sm[w] - Mu);
-    L += sl[w] * f;
-    oa += so[w][2 * lane] * f;
-    ob += so[w][2 * lane + 1] * f;
-  }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  *reinterpret_cast<uint32_t*>(p.o + token * p.o_st + h * p.o_sh + 2 * lane) =
-      E::pack2(oa * inv, ob * inv);
-  if (p.lse && lane == 0)
-    p.lse[h * p.l_sh + token * p.l_st] = L > 0.f ? (M + __builtin_log2f(L)) * kLn2 : -INFINITY;
+// Tokens and keys of range s.
+struct ShRange {
+  int t0, tokens, k0, k1, row;     // keys [k0, k1) through table row `row`
+};
+
+__device__ __forceinline__ int prefix_of(const ShPlan& pl, int b) {
+  return pl.lead[b] >= 0 ? pl.prefix[pl.lead[b]] : 0;
 }
 
-hipError_t launch_shared(const SharedParams& p, int dtype, hipStream_t stream) {
-  const dim3 grid(p.total_q, p.Hq), block(64 * kShWaves);
-  if (dtype == 0)
-    hipLaunchKernelGGL((shared_attn_kernel<BF16>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((shared_attn_kernel<FP16>), grid, block, 0, stream, p);
+__device__ __forceinline__ ShRange range_of(const ShPlan& pl, int B, int s) {
+  ShRange r;
+  if (s < B) {
+    r.row = s;
+    const bool leads = pl.lead[s] == s && pl.prefix[s] > 0;
+    r.t0 = pl.cu[s];
+    r.tokens = leads ? pl.cu[pl.end[s]] - r.t0 : 0;
+    r.k0 = 0;
+    r.k1 = pl.prefix[s];
+  } else {
+    r.row = s - B;
+    r.t0 = pl.cu[r.row];
+    r.tokens = pl.cu[r.row + 1] - r.t0;
+    r.k0 = prefix_of(pl, r.row);
+    r.k1 = pl.kv[r.row];
+  }
+  return r;
+}
+
+__device__ __forceinline__ int wide_tiles(int pairs) { return (pairs + kShTile - 1) / kShTile; }
+// pairs of a tile: the range's, evenly, in whole 32s
+__device__ __forceinline__ int tile_pairs(int pairs, int tiles) {
+  return ((pairs + tiles - 1) / tiles + 31) & ~31;
+}
+__device__ __forceinline__ int key_units(const ShRange& r, int unit) {
+  return max(1, (r.k1 - r.k0 + unit - 1) / unit);
+}
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(x, o);
+    if (lane >= o) x += t;
+  }
+  return x;
+}
+
+__device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = p.B;
+  for (int b = tid; b <= B; b += kShThreads) {
+    // offsets never leave q and never fall
+    int c = p.cu_q[b];
+    c = c < 0 ? 0 : c > p.total_q ? p.total_q : c;
+    pl.cu[b] = c;
+    if (b < B) {
+      pl.kv[b] = clamp_len(p.kv_lens[b], p.max_kv);
+      pl.lead[b] = 0;
+      pl.prefix[b] = 0;
+      pl.end[b] = 0;
+    }
+  }
+  __syncthreads();
+  // groups mark their first rows (of several with one first row, the last group counts)
+  for (int g = tid; g < p.G; g += kShThreads) {
+    const int lo = p.cu_rows[g], hi = p.cu_rows[g + 1];
+    if (lo >= 0 && lo < hi && hi <= B) atomicMax(&pl.prefix[lo], g + 1);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    // the row whose group each row is in: the last first row before it, if that group reaches it
+    int carry = 0, cu_top = 0;
+    for (int base = 0; base < B; base += 64) {
+      const int b = base + lane;
+      int first = b < B && pl.prefix[b] > 0 ? b + 1 : 0;
+      int cu = b <= B ? pl.cu[b] : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(first, o), u = __shfl_up(cu, o);
+        if (lane >= o) first = max(first, t), cu = max(cu, u);
+      }
+      first = max(first, carry);
+      cu = max(cu, cu_top);
+      carry = __shfl(first, 63);
+      cu_top = __shfl(cu, 63);
+      if (b < B) {
+        const int lead = first - 1;
+        const int g = lead >= 0 ? pl.prefix[lead] - 1 : -1;
+        pl.lead[b] = g >= 0 && b < p.cu_rows[g + 1] ? lead : -1;
+        pl.cu[b] = cu;
+      }
+      if (b == B - 1) pl.cu[B] = max(cu, pl.cu[B]);
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < B; b += kShThreads) {
+    const int g = pl.prefix[b] - 1;
+    pl.prefix[b] = g >= 0 ? clamp_len(p.prefix_lens[g], pl.kv[b]) : 0;
+    if (pl.lead[b] >= 0 && (b + 1 == B || pl.lead[b + 1] != pl.lead[b])) pl.end[pl.lead[b]] = b + 1;
+  }
+  __syncthreads();
+  // a prefix goes as far as each query of the group sees it; one row shares with no one
+  for (int b = tid; b < B; b += kShThreads) {
+    const int lead = pl.lead[b], n = pl.cu[b + 1] - pl.cu[b];
+    if (lead >= 0) {
+      if (n > 0) atomicMin(&pl.prefix[lead], max(0, p.causal ? pl.kv[b] - n + 1 : pl.kv[b]));
+      if (pl.end[lead] - lead == 1) atomicMin(&pl.prefix[lead], 0);
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < B; b += kShThreads) pl.prefix[b] &= ~(kShStep - 1);
+  __syncthreads();
+  if (wave < 2) {
+    const bool wide = wave == 0;
+    int* out = wide ? pl.wide : pl.narrow;
+    int carry = 0;
+    if (lane == 0) out[0] = 0;
+    for (int base = 0; base < 2 * B; base += 64) {
+      const int s = base + lane;
+      int n = 0;
+      if (s < 2 * B) {
+        const ShRange r = range_of(pl, B, s);
+        const int pairs = r.tokens * p.group;
+        if (pairs > 0 && (pairs > kShNarrow) == wide)
+          n = p.Hkv * (wide ? wide_tiles(pairs) * key_units(r, kShWideUnit)
+                            : key_units(r, kShNarrowUnit));
+      }
+      n = wave_scan(n, lane);
+      if (s < 2 * B) out[s + 1] = carry + n;
+      carry += __shfl(n, 63);
+    }
+  }
+  __syncthreads();
+}
+
+// The range that holds unit u: R[s] <= u < R[s + 1] (0 <= u < R[n]).
+__device__ __forceinline__ int find_range(const int* R, int n, int u) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (R[m] <= u) lo = m; else hi = m;
+  }
+  return lo;
+}
+
+// First worker (of W over N units) whose share contains unit u.
+__device__ __forceinline__ int first_worker(int64_t u, int64_t N, int W) {
+  return (int)(((u + 1) * W - 1) / N);
+}
+
+// The part of a walk that is the same for all its steps.
+struct ShWalk {
+  const int32_t* table;   // the row's block ids
+  const uint16_t* k;      // pools at the kv head
+  const uint16_t* v;
+  int end;                // keys of the range end here: later rows read as zeros
+  int full;               // keys before this are seen by every column
+};
+
+// One wave's 32 columns.
+struct ShState {
+  u32x4 q[8];             // queries: d = 16 s + 8 g + [0, 8)
+  f32x16 o[4];            // accumulator r of block db: d = 32 db + 8 (r / 4) + 4 g + r % 4
+  float m, l;             // running max (of the unscaled scores) and this lane's part of the sum
+  int lim;                // keys before this are seen by the lane's column
+};
+
+// Lane's offsets in a 16-key run: load instruction j moves rows 4 j + lane / 16 to LDS chunk lane % 16, the
+// chunk of K it takes being that ^ row, of V ^ 4 (row % 4).
+struct ShLanes {
+  int row, k, v;   // bytes: of row lane / 16, of the chunks in instruction 0
+};
+__device__ __forceinline__ ShLanes lane_offsets(int64_t kv_st, int lane) {
+  const int row = lane >> 4;
+  return {row * (int)kv_st * 2, 16 * ((lane & 15) ^ row), 16 * ((lane & 15) ^ (4 * row))};
+}
+
+// The block id of the 16 keys from t on.
+__device__ __forceinline__ int entry_of(const SharedParams& p, const ShWalk& w, int64_t t) {
+  return t < w.end ? w.table[t >> p.bs_shift] : -1;
+}
+
+// 16 keys of K or V from t on, in block blk, to LDS; keys past the range's end become zeros.
+template <bool V>
+__device__ __forceinline__ void load_run(const SharedParams& p, const ShWalk& w, int blk, int t,
+                                         uint32_t lds, const ShLanes& ln) {
+  const bool in = (unsigned)blk < (unsigned)p.num_blocks;
+  const int64_t slot = ((int64_t)(in ? blk : 0) << p.bs_shift) + (t & ((1 << p.bs_shift) - 1));
+  const uint32_t bytes = in ? (uint32_t)(sclamp(w.end - t, 0, 16) * (int)p.kv_st * 2) : 0u;
+  const uint64_t base = uniform_u64(reinterpret_cast<uint64_t>((V ? w.v : w.k) + slot * p.kv_st));
+  const uint32_t n = __builtin_amdgcn_readfirstlane(bytes);
+  const int row = opaque(ln.row);   // the sums are made here, not kept
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    lds_dma16(base, n, lds + 1024 * j, row + j * 8 * (int)p.kv_st + (V ? ln.v : ln.k ^ (64 * j)));
+}
+
+// The operands of 32 keys out of LDS.  MFMA row r of S^T is key pi(r), so that a lane's 8 keys of a
+// 16-key step are consecutive.
+__device__ __forceinline__ int k_offset(int lane) {
+  const int r32 = lane & 31, g = lane >> 5;
+  const int pim = 16 * (r32 >> 4) + 8 * ((r32 >> 2) & 1) + 4 * ((r32 >> 3) & 1) + (r32 & 3);
+  return pim * 256 + 16 * (g ^ (pim & 1)) + 32 * ((pim >> 1) & 7);
+}
+__device__ __forceinline__ void read_k(const uint8_t* k, int lane, u32x4 (&ka)[8]) {
+  const int kx = k_offset(lane);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) ka[s] = *reinterpret_cast<const u32x4*>(k + (kx ^ (32 * s)));
+}
+__device__ __forceinline__ u32x4 read_v(const uint8_t* v, int lane, int kk, int db) {
+  const int g = lane >> 5, vk = (lane >> 2) & 3;
+  const uint8_t* a = v + 2048 * g + 256 * vk + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) +
+                     64 * (db ^ vk) + 4096 * kk;
+  const u32x2 lo = ds_read_tr16(a);
+  const u32x2 hi = ds_read_tr16(a + 1024);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+__device__ __forceinline__ void read_v(const uint8_t* v, int lane, u32x4 (&va)[2][4]) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int db = 0; db < 4; ++db) va[kk][db] = read_v(v, lane, kk, db);
+}
+
+// S^T of 32 keys and the wave's columns.
+template <typename E>
+__device__ __forceinline__ f32x16 scores(const u32x4 (&ka)[8], const u32x4 (&q)[8]) {
+  f32x16 s = f32x16{};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = E::mfma32(ka[k], q[k], s);
+  return s;
+}
+
+// The same for N blocks of 32 keys in LDS, operands read two k-steps ahead of their MFMAs and no further.
+template <typename E, int N>
+__device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x4 (&q)[8],
+                                          f32x16 (&s)[N]) {
+  const int kx = k_offset(lane);
+  u32x4 ka[3][N];
+  const auto rd = [&](int i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      ka[i % 3][n] = *reinterpret_cast<const u32x4*>(k + (kx ^ (32 * i)) + n * kShStep * kShRow);
+  };
+  rd(0);
+  rd(1);
+#pragma unroll
+  for (int n = 0; n < N; ++n) s[n] = f32x16{};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i + 2 < 8) rd(i + 2);
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] = E::mfma32(ka[i % 3][n], q[i], s[n]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// O += P V of N blocks of 32 keys in LDS, likewise a k-step ahead.
+template <typename E, int N>
+__device__ __forceinline__ void add_pv_of(ShState& st, const uint8_t* v, int lane, const u32x4 (&pb)[2 * N]) {
+  u32x4 va[2][4];
+  const auto rd = [&](int i) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      va[i & 1][db] = read_v(v + (i >> 1) * kShStep * kShRow, lane, i & 1, db);
+  };
+  rd(0);
+#pragma unroll
+  for (int i = 0; i < 2 * N; ++i) {
+    if (i + 1 < 2 * N) rd(i + 1);
+#pragma unroll
+    for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i & 1][db], pb[i], st.o[db]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Accumulator r of a block of 32 keys is the lane's key 16 (r / 8) + r % 8 (the lanes with g = 1 start at
+// key 8): those at or past lim are hidden.
+__device__ __forceinline__ void hide(f32x16& s, int lim) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (16 * (r >> 3) + (r & 7) >= lim) s[r] = -INFINITY;
+}
+
+// The online softmax of N blocks of 32 keys: P^T as the B operand (block n's 16-key step kk in pb[2 n +
+// kk]), maximum, sum and O updated.
+//   p = 2^(c (s - m)): the difference first, so that scores of any size keep their weights.  The
+// reference m may lag the true maximum while no p of the lane exceeds 2^8, as in the prefill kernel.
+template <typename E, int N>
+__device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[N], u32x4 (&pb)[2 * N]) {
+  const auto weigh = [&](float ref) {
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x =
+            E::pack2(exp2_fast((s[n][2 * i] - ref) * c), exp2_fast((s[n][2 * i + 1] - ref) * c));
+        pb[2 * n + (i >> 2)][i & 3] = x;
+        sum = E::sum2(x, sum);
+      }
+    return sum;
+  };
+  float sum = weigh(st.m);
+  if (__any(!(sum <= 256.f))) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const bool grow = (mx - st.m) * c > 8.f;
+    if (__any(grow)) {
+      const float alpha = grow ? exp2_fast((st.m - mx) * c) : 1.f;
+      st.l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st.o[i] *= alpha;
+      if (grow) st.m = mx;
+    }
+    sum = weigh(st.m == -INFINITY ? 0.f : st.m);
+  }
+  st.l += sum;
+}
+
+// O += P V of 32 keys.
+template <typename E>
+__device__ __forceinline__ void add_pv(ShState& st, const u32x4 (&va)[2][4], const u32x4* pb) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[kk][db], pb[kk], st.o[db]);
+}
+
+// Whether N blocks of 32 keys in LDS hold a value that is inf or NaN: all its exponent bits set, which a 1
+// added to the exponent carries into the sign's place.
+template <typename E, int N>
+__device__ __forceinline__ bool any_odd(const uint8_t* v, int lane) {
+  constexpr uint32_t kMant = E::kOnes2 == 0x3f803f80u ? 0x007f007fu : 0x03ff03ffu;
+  constexpr uint32_t kUnit = kMant + 0x00010001u, kExp = 0x7fff7fffu & ~kMant;
+  uint32_t odd = 0;
+  lane = opaque(lane);   // rare: its addresses are not kept through the key loop
+#pragma unroll 2
+  for (int i = 0; i < 8 * N; ++i) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(v + 1024 * i + 16 * lane);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= ((x[e] & kExp) + kUnit) & 0x80008000u;
+  }
+  return __any(odd != 0);
+}
+
+// The wave's columns [col0, col0 + 32) of a tile of `cols` that begins with pair `pair0` of the range.
+__device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange& r, bool own, int hk,
+                                           int pair0, int col0, int cols, int lane, ShWalk& w,
+                                           ShState& st) {
+  const int g = lane >> 5, col = col0 + (lane & 31);
+  w.table = p.table + r.row * p.bt_stride;
+  w.k = p.k + hk * p.kv_sh;
+  w.v = p.v + hk * p.kv_sh;
+  w.end = r.k1;
+  // own keys: query i of the row's n sees all but the n - 1 - i last
+  const int first = r.k1 - r.tokens + 1;
+  const int token = fdiv(pair0 + col, p.group_div);
+  w.full = own && p.causal ? min(r.k1, first + fdiv(pair0 + col0, p.group_div)) : r.k1;
+  st.lim = own && p.causal ? min(r.k1, first + token) : r.k1;
+  if (col < cols) {
+    const uint16_t* q = p.q + (int64_t)(r.t0 + token) * p.q_st +
+                        (int64_t)(hk * p.group + (pair0 + col - token * p.group)) * p.q_sh + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) st.q[s] = ld16(q + 16 * s);
+  } else {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) st.q[s] = u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st.o[i] = f32x16{};
+  st.m = -INFINITY;
+  st.l = 0.f;
+}
+
+// Where the parts of the item's pairs stand: written by the worker with the item's first unit.  The
+// record of a pair: its first part's column, and the number of parts with the kind of worker and, for a
+// row's own range, whether the row's group has a prefix.
+__device__ __forceinline__ void record(const SharedParams& p, const ShRange& r, bool own, bool prefix,
+                                       bool wide, int hk, int pair, int column, int parts) {
+  const int token = fdiv(pair, p.group_div);
+  const int64_t at = ((int64_t)(own ? p.total_q : 0) + r.t0 + token) * p.Hq + hk * p.group +
+                     (pair - token * p.group);
+  p.ws_where[2 * at] = column;
+  p.ws_where[2 * at + 1] = parts << 2 | (wide ? 2 : 0) | (prefix ? 1 : 0);
+}
+
+// Columns before the parts of an item's pairs (its kind's workers add theirs).
+__device__ __forceinline__ int item_columns(const SharedParams& p, const ShRange& r, bool own, int hk,
+                                            int pair0) {
+  return ((own ? p.total_q : 0) + r.t0) * p.Hq + hk * r.tokens * p.group + pair0;
+}
+
+// Keys [kb, stop) of a tile's columns, one column a wave at a time, two dims a lane: for items some of
+// whose values are not finite and hidden from some of their queries, where the product of a whole tile
+// would have 0 x inf.  A hidden key is not looked at here.
+template <typename E>
+__device__ __forceinline__ void careful_item(const SharedParams& p, const ShRange& r, bool own, int hk,
+                                             int pair0, int cols, int kb, int stop, int column, int wave,
+                                             int waves, int lane) {
+  lane = opaque(lane);
+  const float c = p.scale_log2;
+  const int32_t* table = p.table + r.row * p.bt_stride;
+  for (int col = wave; col < cols; col += waves) {
+    const int token = fdiv(pair0 + col, p.group_div), h = pair0 + col - token * p.group;
+    const int lim = min(stop, own && p.causal ? r.k1 - r.tokens + 1 + token : r.k1);
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(
+        p.q + (int64_t)(r.t0 + token) * p.q_st + (int64_t)(hk * p.group + h) * p.q_sh + 2 * lane);
+    float m = -INFINITY, l = 0.f, oa = 0.f, ob = 0.f;
+    for (int t = kb; t < lim; ++t) {
+      const int blk = table[t >> p.bs_shift];
+      const bool in = (unsigned)blk < (unsigned)p.num_blocks;
+      const int64_t slot = ((int64_t)(in ? blk : 0) << p.bs_shift) + (t & ((1 << p.bs_shift) - 1));
+      const int64_t at = slot * p.kv_st + hk * p.kv_sh + 2 * lane;
+      const uint32_t k = in ? *reinterpret_cast<const uint32_t*>(p.k + at) : 0;
+      const uint32_t v = in ? *reinterpret_cast<const uint32_t*>(p.v + at) : 0;
+      float s = E::lo(q) * E::lo(k) + E::hi(q) * E::hi(k);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+      const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
+      const float a = exp2_fast((m - mu) * c), w = exp2_fast((s - mu) * c);
+      l = l * a + w;
+      oa = oa * a + w * E::lo(v);
+      ob = ob * a + w * E::hi(v);
+      m = mn;
+    }
+    float* o = p.ws_o + (int64_t)(column + col) * kHeadDim + 2 * lane;
+    o[0] = oa;
+    o[1] = ob;
+    if (lane == 0) {
+      p.ws_ml[2 * (int64_t)(column + col)] = m;
+      p.ws_ml[2 * (int64_t)(column + col) + 1] = l;
+    }
+  }
+}
+
+// Units [c0, c1) of a wide item by the work-group: RG blocks of 32 columns, 8 / RG key streams.
+template <typename E, int RG>
+__device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& r, bool own, int hk,
+                                          int pair0, int cols, int c0, int c1, int column, uint8_t* ring,
+                                          float (*ml)[32][2], int* odd) {
+  constexpr int KS = kShWaves / RG, N = kShWideUnit / KS / kShStep;   // 32-key blocks of a wave and step
+  // (the lane as a value of this item: its many LDS addresses are not kept from one to the next)
+  const int tid = threadIdx.x, lane = opaque(tid & 63);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rg = wave % RG, ks = wave / RG;
+  const int g = lane >> 5;
+  ShWalk w;
+  ShState st;
+  start_tile(p, r, own, hk, pair0, 32 * rg, cols, lane, w, st);
+  const bool active = 32 * rg < cols;
+  const int first = r.k0 + c0 * kShWideUnit, n = c1 - c0;
+  if (tid == 0) *odd = 0;   // (barriers follow)
+  const ShLanes ln = lane_offsets(p.kv_st, lane);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr_of(ring)) + wave * 16 * kShRow;
+  // this wave's run of step i: keys first + 128 i + 16 wave .. ; block ids of 64 steps, a lane each
+  int tbl = entry_of(p, w, first + (int64_t)lane * kShWideUnit + 16 * wave);
+  const auto load = [&](int i) {
+    const int t = first + i * kShWideUnit + 16 * wave;
+    const int blk = __builtin_amdgcn_readlane(tbl, i & 63);
+    const uint32_t at = lds + (i & 1) * kShStage;
+    load_run<false>(p, w, blk, t, at, ln);
+    load_run<true>(p, w, blk, t, at + kShWideUnit * kShRow, ln);
+  };
+  load(0);
+  for (int i = 0; i < n; ++i) {
+    // the step's loads are in LDS, and every wave is done with the other stage
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (i + 1 < n) {
+      if (((i + 1) & 63) == 0)
+        tbl = entry_of(p, w, first + (i + 1 + (int64_t)lane) * kShWideUnit + 16 * wave);
+      load(i + 1);
+    }
+    const int kb = first + i * kShWideUnit + ks * N * kShStep;
+    if (active && kb < w.end) {
+      const uint8_t* k = ring + (i & 1) * kShStage + ks * N * kShStep * kShRow;
+      const uint8_t* v = k + kShWideUnit * kShRow;
+      f32x16 s[N];
+      scores_of<E, N>(k, lane, st.q, s);
+      const bool masked = kb + N * kShStep > w.full;
+      if (masked) {
+#pragma unroll
+        for (int b = 0; b < N; ++b) hide(s[b], st.lim - kb - kShStep * b - 8 * g);
+      }
+      u32x4 pb[2 * N];
+      softmax<E, N>(p.scale_log2, st, s, pb);
+      if (masked && any_odd<E, N>(v, lane)) *odd = 1;
+      add_pv_of<E, N>(st, v, lane, pb);
+    }
+  }
+  // the key streams' parts become one: each scales its own to the common maximum, LDS sums them
+  st.l += __shfl_xor(st.l, 32);
+  const int r32 = opaque(lane & 31);
+  if (g == 0) {
+    ml[wave][r32][0] = st.m;
+    ml[wave][r32][1] = st.l;
+  }
+  __syncthreads();
+  if (*odd) {
+    careful_item<E>(p, r, own, hk, pair0, cols, first, min(r.k1, first + n * kShWideUnit), column, wave,
+                    kShWaves, lane);
+    __syncthreads();
+    return;
+  }
+  {
+    float M = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) M = fmaxf(M, ml[j * RG + rg][r32][0]);
+    const float f = exp2_fast((st.m - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
+    // [wave][column][128], 16-byte pieces at piece ^ column
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr)
+        *reinterpret_cast<f32x4*>(ring + wave * kShRing + r32 * 512 +
+                                  16 * ((8 * db + 2 * rr + g) ^ r32)) =
+            f32x4{st.o[db][4 * rr] * f, st.o[db][4 * rr + 1] * f, st.o[db][4 * rr + 2] * f,
+                  st.o[db][4 * rr + 3] * f};
+  }
+  if (tid < cols) {
+    const int b = tid >> 5, col = tid & 31;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) M = fmaxf(M, ml[j * RG + b][col][0]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+      L += ml[j * RG + b][col][1] * exp2_fast((ml[j * RG + b][col][0] - Mu) * p.scale_log2);
+    p.ws_ml[2 * (int64_t)(column + tid)] = M;
+    p.ws_ml[2 * (int64_t)(column + tid) + 1] = L;
+  }
+  __syncthreads();
+  for (int i = tid; i < cols * 32; i += kShThreads) {
+    const int col = i >> 5, piece = i & 31;
+    const uint8_t* at = ring + (col >> 5) * kShRing + (col & 31) * 512 + 16 * (piece ^ (col & 31));
+    f32x4 sum = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+    for (int j = 1; j < KS; ++j) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(at + j * RG * kShRing);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += x[e];
+    }
+    *reinterpret_cast<f32x4*>(p.ws_o + (int64_t)(column + col) * kHeadDim + 4 * piece) = sum;
+  }
+  __syncthreads();   // the ring and ml are the next item's
+}
+
+// Keys [kb, stop) of a narrow item by one wave, in its own 16 KB of LDS.  Returns whether careful_item
+// has to do it.
+template <typename E>
+__device__ __forceinline__ bool narrow_walk(const SharedParams& p, const ShWalk& w, ShState& st, int kb,
+                                            int stop, const uint8_t* ring, int lane) {
+  if (kb >= stop) return false;
+  bool odd = false;
+  const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_addr_of(ring));
+  const uint32_t lds_v = lds_k + kShStep * kShRow;
+  const ShLanes ln = lane_offsets(p.kv_st, lane);
+  // block ids of the two runs of 32 steps, lane 2 i + run
+  int tbl = entry_of(p, w, kb + (int64_t)lane * 16);
+  const auto load_k = [&](int i, int t) {
+    load_run<false>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i), t, lds_k, ln);
+    load_run<false>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i + 1), t + 16, lds_k + 16 * kShRow, ln);
+  };
+  const auto load_v = [&](int i, int t) {
+    load_run<true>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i), t, lds_v, ln);
+    load_run<true>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i + 1), t + 16, lds_v + 16 * kShRow, ln);
+  };
+  // the last item's reads have left LDS
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  load_k(0, kb);
+  load_v(0, kb);
+  for (int i = 1; kb < stop; ++i, kb += kShStep) {
+    const int next = kb + kShStep;
+    const bool more = next < stop;
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // K is there, V may be on its way
+    u32x4 ka[8];
+    read_k(ring, lane, ka);
+    int ids = tbl;
+    if (more) {
+      if ((i & 31) == 0) ids = entry_of(p, w, next + (int64_t)lane * 16);
+      tbl = ids;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K has left LDS
+      load_k(i & 31, next);
+    }
+    f32x16 s[1] = {scores<E>(ka, st.q)};
+    const int g = lane >> 5;
+    const bool masked = next > w.full;
+    if (masked) hide(s[0], st.lim - kb - 8 * g);
+    u32x4 pb[2];
+    softmax<E, 1>(p.scale_log2, st, s, pb);
+    if (more)
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // V is there, the next K may be on its way
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint8_t* v = ring + kShStep * kShRow;
+    if (masked) odd |= any_odd<E, 1>(v, lane);
+    u32x4 va[2][4];
+    read_v(v, lane, va);
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V has left LDS
+      load_v(i & 31, next);
+    }
+    add_pv<E>(st, va, pb);
+  }
+  return odd;
+}
+
+template <typename E>
+__global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const SharedParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kShWaves * kShRing];
+  __shared__ ShPlan pl;
+  __shared__ float ml[kShWaves][32][2];
+  __shared__ int odd;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  make_plan(p, pl);
+  const int n_ranges = 2 * p.B;
+  const int W = gridDim.x;
+
+  // wide ranges, by work-groups
+  const int N1 = __builtin_amdgcn_readfirstlane(pl.wide[n_ranges]);
+  const int W1 = min(W, N1);
+  if ((int)blockIdx.x < W1) {
+    const int wg = blockIdx.x;
+    int u = (int)((int64_t)wg * N1 / W1);
+    const int stop = (int)((int64_t)(wg + 1) * N1 / W1);
+    int s = find_range(pl.wide, n_ranges, u);
+    while (u < stop) {
+      while (pl.wide[s + 1] <= u) ++s;
+      s = __builtin_amdgcn_readfirstlane(s);
+      ShRange r = range_of(pl, p.B, s);
+      r.t0 = __builtin_amdgcn_readfirstlane(r.t0);
+      r.tokens = __builtin_amdgcn_readfirstlane(r.tokens);
+      r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
+      r.k1 = __builtin_amdgcn_readfirstlane(r.k1);
+      r.row = __builtin_amdgcn_readfirstlane(r.row);
+      const bool own = s >= p.B;
+      const int pairs = r.tokens * p.group, tiles = wide_tiles(pairs), width = tile_pairs(pairs, tiles);
+      const int units = key_units(r, kShWideUnit);
+      const int at = u - __builtin_amdgcn_readfirstlane(pl.wide[s]);
+      const int item = at / units, c0 = at - item * units;
+      const int hk = item / tiles, pair0 = (item - hk * tiles) * width;
+      const int cols = min(width, pairs - pair0);
+      const int c1 = min(units, c0 + stop - u);
+      const int column = item_columns(p, r, own, hk, pair0) + wg * kShTile;
+      if (c0 == 0 && tid < cols)
+        record(p, r, own, own && prefix_of(pl, r.row) > 0, true, hk, pair0 + tid, column + tid,
+               first_worker(u + units - 1, N1, W1) - wg + 1);
+      if (cols <= 64)
+        wide_item<E, 2>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+      else
+        wide_item<E, 4>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+      u += c1 - c0;
+    }
+  }
+
+  // narrow ranges, by waves; the work-groups without a share of the wide ones come first
+  const int N2 = __builtin_amdgcn_readfirstlane(pl.narrow[n_ranges]);
+  const int W2 = min(W * kShWaves, N2);
+  const int wg = (int)blockIdx.x >= W1 ? (int)blockIdx.x - W1 : (int)blockIdx.x + W - W1;
+  // neighbouring shares on different work-groups: a short list of units spreads over the CUs
+  const int worker = wave * W + wg;
+  if (worker < W2) {
+    int u = (int)((int64_t)worker * N2 / W2);
+    const int stop = (int)((int64_t)(worker + 1) * N2 / W2);
+    int s = find_range(pl.narrow, n_ranges, u);
+    while (u < stop) {
+      while (pl.narrow[s + 1] <= u) ++s;
+      s = __builtin_amdgcn_readfirstlane(s);
+      ShRange r = range_of(pl, p.B, s);
+      r.t0 = __builtin_amdgcn_readfirstlane(r.t0);
+      r.tokens = __builtin_amdgcn_readfirstlane(r.tokens);
+      r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
+      r.k1 = __builtin_amdgcn_readfirstlane(r.k1);
+      r.row = __builtin_amdgcn_readfirstlane(r.row);
+      const bool own = s >= p.B;
+      const int pairs = r.tokens * p.group;
+      const int units = key_units(r, kShNarrowUnit);
+      const int at = u - __builtin_amdgcn_readfirstlane(pl.narrow[s]);
+      const int hk = at / units, c0 = at - hk * units, c1 = min(units, c0 + stop - u);
+      const int column = p.narrow_base + item_columns(p, r, own, hk, 0) + worker * kShNarrow;
+      if (c0 == 0 && lane < pairs)
+        record(p, r, own, own && prefix_of(pl, r.row) > 0, false, hk, lane, column + lane,
+               first_worker(u + units - 1, N2, W2) - worker + 1);
+      ShWalk w;
+      ShState st;
+      start_tile(p, r, own, hk, 0, 0, pairs, lane, w, st);
+      const int kb = r.k0 + c0 * kShNarrowUnit, last = min(r.k1, r.k0 + c1 * kShNarrowUnit);
+      if (narrow_walk<E>(p, w, st, kb, last, ring + wave * kShRing, lane)) {
+        careful_item<E>(p, r, own, hk, 0, pairs, kb, last, column, 0, 1, lane);
+        u += c1 - c0;
+        continue;
+      }
+      const int r32 = lane & 31, g = lane >> 5;
+      const float l = st.l + __shfl_xor(st.l, 32);
+      if (r32 < pairs) {
+        float* o = p.ws_o + (int64_t)(column + r32) * kHeadDim + 4 * g;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int rr = 0; rr < 4; ++rr)
+            *reinterpret_cast<f32x4*>(o + 32 * db + 8 * rr) =
+                f32x4{st.o[db][4 * rr], st.o[db][4 * rr + 1], st.o[db][4 * rr + 2],
+                      st.o[db][4 * rr + 3]};
+        if (g == 0) {
+          p.ws_ml[2 * (int64_t)(column + r32)] = st.m;
+          p.ws_ml[2 * (int64_t)(column + r32) + 1] = l;
+        }
+      }
+      u += c1 - c0;
+    }
+  }
+}
+
+// Merges the parts of one (token, head), a wave each: the lanes first take a part's (m, l) each, 64 parts a
+// time, then half the wave each every other part's O, four dims a lane.
+template <typename E>
+__global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p) {
+  const int lane = threadIdx.x & 63;
+  const int pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (pair >= p.total_q * p.Hq) return;
+  const int token = pair / p.Hq, h = pair - token * p.Hq;
+  if (token < p.cu_q[0] || token >= p.cu_q[p.B]) return;
+  const int32_t* where = p.ws_where + 2 * ((int64_t)p.total_q * p.Hq + pair);
+  int col[2], n[2], stride[2];
+  col[1] = where[0];
+  n[1] = where[1] >> 2;
+  stride[1] = where[1] & 2 ? kShTile : kShNarrow;
+  const bool prefix = where[1] & 1;
+  const int32_t* shared = p.ws_where + 2 * (int64_t)pair;
+  col[0] = prefix ? shared[0] : 0;
+  n[0] = prefix ? shared[1] >> 2 : 0;
+  stride[0] = prefix && (shared[1] & 2) ? kShTile : kShNarrow;
+  // a token that no row holds (offsets that fall) has no record: whatever stands there is not followed
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (col[i] < 0 || n[i] < 0 || col[i] + ((int64_t)n[i] - 1) * stride[i] >= p.columns) return;
+
+  const float c = p.scale_log2;
+  const int half = lane >> 5, d = 4 * (lane & 31);
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int total = n[0] + n[1];
+  for (int base = 0; base < total; base += 64) {
+    const int i = base + lane, batch = min(64, total - base);
+    const int64_t at = i < n[0] ? col[0] + (int64_t)i * stride[0]
+                                : col[1] + (int64_t)(i - n[0]) * stride[1];
+    float m = i < total ? p.ws_ml[2 * at] : -INFINITY;
+    const float l = i < total ? p.ws_ml[2 * at + 1] : 0.f;
+    float Mn = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor(Mn, o));
+    Mn = fmaxf(Mn, M);
+    const float Mu = Mn == -INFINITY ? 0.f : Mn;
+    const float old = exp2_fast((M - Mu) * c);
+    const float f = exp2_fast((m - Mu) * c);
+    float ls = l * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+    L = L * old + ls;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= old;
+    M = Mn;
+    constexpr int kFlight = 4;
+    for (int j0 = 0; j0 < batch; j0 += 2 * kFlight) {
+      f32x4 x[kFlight];
+      float wt[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int j = j0 + 2 * k + half;
+        const bool live = j < batch;
+        const int t = base + j;
+        const int64_t a = t < n[0] ? col[0] + (int64_t)t * stride[0]
+                                   : col[1] + (int64_t)(t - n[0]) * stride[1];
+        wt[k] = __shfl(f, j & 63);
+        // a part that saw no key weighs nothing, whatever its O
+        x[k] = live && wt[k] != 0.f
+                   ? *reinterpret_cast<const f32x4*>(p.ws_o + a * kHeadDim + d)
+                   : f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!live) wt[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[k][e], wt[k], acc[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], 32);
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (half == 0)
+    *reinterpret_cast<u32x2*>(p.o + (int64_t)token * p.o_st + (int64_t)h * p.o_sh + d) =
+        u32x2{E::pack2(acc[0] * inv, acc[1] * inv), E::pack2(acc[2] * inv, acc[3] * inv)};
+  if (p.lse && lane == 0)
+    p.lse[h * p.l_sh + token * p.l_st] =
+        L > 0.f ? (M * c + __builtin_log2f(L)) * kLn2 : -INFINITY;
+}
+
+template <typename E>
+static hipError_t launch_shared_t(const SharedParams& p, int n_wg, hipStream_t stream) {
+  hipLaunchKernelGGL((shared_attn_kernel<E>), dim3(n_wg), dim3(kShThreads), 0, stream, p);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL((shared_merge_kernel<E>), dim3((p.total_q * p.Hq + 3) / 4), dim3(256), 0, stream,
+                     p);
   return hipGetLastError();
+}
+
+hipError_t launch_shared(SharedParams p, int dtype, int n_cus, void* workspace, hipStream_t stream) {
+  const SharedSpace s = shared_space(p.total_q, p.Hq);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.ws_o = reinterpret_cast<float*>(ws);
+  p.ws_ml = reinterpret_cast<float*>(ws + s.ml);
+  p.ws_where = reinterpret_cast<int32_t*>(ws + s.where);
+  p.columns = s.columns;
+  p.narrow_base = s.narrow;
+  p.group_div = make_fastdiv(p.group);
+  const int n_wg = n_cus < kSharedWgs ? n_cus : kSharedWgs;
+  return dtype == 0 ? launch_shared_t<BF16>(p, n_wg, stream) : launch_shared_t<FP16>(p, n_wg, stream);
 }
 
 }  // namespace mi_fa2

@@ -12,9 +12,9 @@ import torch
 
 from . import _lib
 from .blocks import check, load
-from .fa2 import HEAD_DIM, _dims_ok, _envelope, _strides
+from .fa2 import HEAD_DIM, _dims_ok, _envelope, _strides, fa2_paged_varlen
 
-MAX_ROWS = 1024   # rows of a call
+MAX_ROWS = 512   # rows of a call of the kernel
 
 
 def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_seqlen_q, cu_rows,
@@ -34,7 +34,8 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
     is_causal    bottom-right aligned per row (query i of row b sees keys <= i + kv_len - T_b)
     out          optional [total_q, Hq, 128] output (any token/head strides); tokens of no row keep
                  what they hold
-    At most 1,024 rows.  Returns O [total_q, Hq, 128] (and the fp32 LSE [Hq, total_q] if return_lse).
+    More than 512 rows go to fa2_paged_varlen, which reads every row's keys for that row alone.
+    Returns O [total_q, Hq, 128] (and the fp32 LSE [Hq, total_q] if return_lse).
     """
     assert q.is_cuda and k_pool.is_cuda and v_pool.is_cuda, "q and the pools must be GPU tensors"
     assert q.dim() == 3, "q is [total_q, Hq, d]"
@@ -56,7 +57,6 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
         f"the pools and the table must be on {dev}"
     assert block_table.stride(-1) == 1 or block_table.shape[1] <= 1, \
         "block_table rows must be contiguous"
-    assert B <= MAX_ROWS, f"at most {MAX_ROWS} rows"
     assert prefix_lens.shape[0] <= B, "at most as many groups as rows"
     assert block_size >= 16 and block_size & (block_size - 1) == 0, "block_size: power of 2, >= 16"
     assert k_pool.shape[0] % block_size == 0, "pool slots must be whole blocks"
@@ -66,6 +66,10 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
     assert 0 <= max_kv_len <= block_table.shape[1] * block_size, \
         "max_kv_len exceeds what the block table can address"
     assert 0 <= max_seqlen_q, "max_seqlen_q must not be negative"
+    if B > MAX_ROWS:
+        return fa2_paged_varlen(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_seqlen_q,
+                                block_size=block_size, max_kv_len=max_kv_len, is_causal=is_causal,
+                                out=out, return_lse=return_lse)
     if not _dims_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)   # 16-byte vector loads
     assert _dims_ok(k_pool) and _dims_ok(v_pool), "pools need 16-byte aligned token rows"

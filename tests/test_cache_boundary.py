@@ -114,7 +114,8 @@ def i64(*v):
 
 @pytest.mark.parametrize("over,status,msg", [
     (dict(dtype=2), 2, "dtype"), (dict(d=64), 2, "head_dim 64"), (dict(heads_kv=5), 1, "bad sizes"),
-    (dict(batch=-1), 1, "bad sizes"), (dict(batch=1025), 2, "1024"), (dict(n_groups=3), 1, "n_groups"),
+    (dict(batch=-1), 1, "bad sizes"), (dict(batch=513), 2, "512"), (dict(total_q=1 << 22), 2, "2^25"),
+    (dict(total_q=1 << 21, max_kv=1 << 23), 2, "in one call"), (dict(n_groups=3), 1, "n_groups"),
     (dict(max_kv=-1), 1, "max_kv_len"), (dict(bs=24), 2, "block_size"), (dict(bs=8), 2, "block_size"),
     (dict(num_blocks=-1), 1, "num_blocks"), (dict(scale=0.0), 1, "sm_scale"),
     (dict(scale=float("nan")), 1, "sm_scale"), (dict(cu_q=None), 1, "cu_seqlens_q"),
@@ -173,6 +174,17 @@ def test_copy_blocks_refuses_pairs(pairs):
         blocks.copy_blocks(pool, pool, pairs, 16)
 
 
+def test_workspace():
+    size = blocks.load().mi_cache_attend_workspace_size
+    # parts of 128 + 2 floats: two columns per (token, head) in either area, 128 for each of 256
+    # work-groups and 32 for each of their 2,048 waves; a record of two words for each column of an area
+    assert size(64, 12) == (4 * 64 * 12 + 98304) * 520 + 2 * 64 * 12 * 8
+    assert size(0, 12) == 0 and size(1 << 22, 12) == 0
+    assert _attend() == 3 and "workspace" in last()
+    assert _attend(ws=24, ws_bytes=1 << 30) == 3
+    assert _attend(ws=16, ws_bytes=size(2, 12) - 1) == 3
+
+
 def test_attention_refuses_bad_arguments():
     i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
     good = dict(q=_gpu_like(3, 12, 128), k_pool=_gpu_like(64, 2, 128), v_pool=_gpu_like(64, 2, 128),
@@ -185,7 +197,6 @@ def test_attention_refuses_bad_arguments():
                 dict(cu_rows=i32(4), prefix_lens=i32(3)), dict(block_table=i32(3, 4)),
                 dict(block_table=i32(2, 8)[:, ::2]), dict(block_size=24), dict(max_kv_len=65),
                 dict(max_kv_len=-1), dict(max_seqlen_q=-1), dict(out=_gpu_like(3, 12, 64)),
-                dict(out=_gpu_like(3, 12, 128, dtype=torch.float16)),
-                dict(cu_seqlens_q=i32(1026), block_table=i32(1025, 4), kv_lens=i32(1025))):
+                dict(out=_gpu_like(3, 12, 128, dtype=torch.float16))):
         with pytest.raises(AssertionError):
             shared.fa2_paged_shared(**{**good, **bad})

@@ -347,13 +347,13 @@ def test_long_cache_offsets_past_32_bits():
     assert torch.equal(b.call(k_pool=far[0], v_pool=far[1], block_table=b.table.contiguous()), want)
 
 
-def test_the_most_rows():
-    b = Batch([(1000, 64), (24, 32)], [1 + i % 5 for i in range(1024)], [1] * 1024, heads=(4, 2), seed=15)
-    b.check(b.call())
-    with pytest.raises(AssertionError, match="1024"):
-        fa2_paged_shared(torch.zeros(1025, 4, 128, dtype=b.dtype, device="cuda"), b.pool[0], b.pool[1],
-                         i32(list(range(1026))), b.table[:1].expand(1025, -1), i32([1] * 1025), 1,
-                         i32([0]), i32([]))
+@pytest.mark.parametrize("rows", [512, 513, 1024])
+def test_many_rows(rows):
+    # 512 on the kernel, more on fa2_paged_varlen
+    b = Batch([(rows - 24, 64), (24, 32)], [1 + i % 5 for i in range(rows)], [1] * rows, heads=(4, 2),
+              seed=15)
+    out, lse = b.call(return_lse=True)
+    b.check(out, lse)
 
 
 def test_nothing_to_do():
