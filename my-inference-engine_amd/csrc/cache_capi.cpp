@@ -218,10 +218,10 @@ int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool, const void
                 mi_fa2::kShMaxRows, heads_q);
   if (int64_t(total_q) * heads_q > kMaxPairs)
     return fail(kUnsupported, "%d tokens of %d heads: at most 2^25 pairs", total_q, heads_q);
-  // the units of work are counted in 32 bits: (tiles of 128 pairs, at most one more per range and
-  // head) x (steps of 64 keys)
+  // the shares of work are counted in 32 bits: (tiles of 128 pairs, at most one more per range and
+  // head) x (64-key units, and what an item costs beside them)
   if ((int64_t(total_q) * heads_q / 64 + 4 * int64_t(batch) * heads_kv) *
-          (max_kv_len / 64 + int64_t(1)) >= int64_t(1) << 31)
+          (max_kv_len / 64 + int64_t(4)) >= int64_t(1) << 31)
     return fail(kUnsupported, "%d tokens over %d keys in one call", total_q, max_kv_len);
   if (n_groups < 0 || n_groups > batch)
     return fail(kInvalid, "n_groups %d: 0 to batch (%d)", n_groups, batch);

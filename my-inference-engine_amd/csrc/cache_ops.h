@@ -48,7 +48,7 @@ struct SharedParams {
   int32_t max_kv, bs_shift, num_blocks, causal;
   float scale_log2;
   // filled by launch_shared
-  FastDiv group_div;
+  FastDiv group_div, heads_div;
   float* ws_o;          // parts: [column][128] fp32, unnormalised
   float* ws_ml;         // [column][2]: maximum (of the unscaled scores) and sum
   int32_t* ws_where;    // [2][total_q][Hq][2]: where a pair's parts stand, of the prefix and its own keys

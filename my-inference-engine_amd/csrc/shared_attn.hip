@@ -34,6 +34,9 @@ constexpr int kShNarrow = kSharedNarrow;        // pairs a narrow range has at m
 constexpr int kShStep = 32;                     // keys of an MFMA block, and of a narrow step
 constexpr int kShNarrowUnit = 64;
 constexpr int kShWideUnit = 128;                // keys of a wide step
+// What an item costs beside its units (queries, the first loads' latency, its part's way out), in units:
+// it takes as many shares more, before its units.
+constexpr int kShItemCost = 2;
 constexpr int kShRow = kHeadDim * 2;            // bytes of a key
 constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
 constexpr int kShRing = 2 * kShStage / kShWaves;     // a wave's part of the two stages: 16 KB
@@ -42,11 +45,13 @@ static_assert(kShRing == kShStep * kHeadDim * 4, "a wave's 32 columns of O");
 
 // What a work-group knows of the call, in LDS.
 struct ShPlan {
-  int wide[2 * kShMaxRows + 1];    // units of the ranges before this one
+  int wide[2 * kShMaxRows + 1];    // shares of the ranges before this one (see item_length)
   int narrow[2 * kShMaxRows + 1];
   int cu[kShMaxRows + 1];
   int kv[kShMaxRows];
-  int prefix[kShMaxRows];          // at a group's first row: keys read for the whole group
+  int prefix[kShMaxRows];          // at a group's first row: keys that could be read for all the group
+  int group_prefix[kShMaxRows];    // by group, as given
+  int16_t group_end[kShMaxRows];
   int16_t lead[kShMaxRows];        // the first row of the row's group, -1: none
   int16_t end[kShMaxRows];         // at a group's first row: the row after its last
 };
@@ -56,24 +61,23 @@ struct ShRange {
   int t0, tokens, k0, k1, row;     // keys [k0, k1) through table row `row`
 };
 
+// Keys read for the whole group of row b, in whole steps.
 __device__ __forceinline__ int prefix_of(const ShPlan& pl, int b) {
-  return pl.lead[b] >= 0 ? pl.prefix[pl.lead[b]] : 0;
+  return pl.lead[b] >= 0 ? pl.prefix[pl.lead[b]] & ~(kShStep - 1) : 0;
 }
 
 __device__ __forceinline__ ShRange range_of(const ShPlan& pl, int B, int s) {
   ShRange r;
+  r.row = s < B ? s : s - B;
+  r.t0 = pl.cu[r.row];
+  const int shared = prefix_of(pl, r.row);
   if (s < B) {
-    r.row = s;
-    const bool leads = pl.lead[s] == s && pl.prefix[s] > 0;
-    r.t0 = pl.cu[s];
-    r.tokens = leads ? pl.cu[pl.end[s]] - r.t0 : 0;
+    r.tokens = pl.lead[s] == s && shared > 0 ? pl.cu[pl.end[s]] - r.t0 : 0;
     r.k0 = 0;
-    r.k1 = pl.prefix[s];
+    r.k1 = shared;
   } else {
-    r.row = s - B;
-    r.t0 = pl.cu[r.row];
     r.tokens = pl.cu[r.row + 1] - r.t0;
-    r.k0 = prefix_of(pl, r.row);
+    r.k0 = shared;
     r.k1 = pl.kv[r.row];
   }
   return r;
@@ -88,116 +92,134 @@ __device__ __forceinline__ int key_units(const ShRange& r, int unit) {
   return max(1, (r.k1 - r.k0 + unit - 1) / unit);
 }
 
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(x, o);
-    if (lane >= o) x += t;
-  }
-  return x;
+__device__ __forceinline__ ShRange uniform(const ShRange& r) {
+  return {__builtin_amdgcn_readfirstlane(r.t0), __builtin_amdgcn_readfirstlane(r.tokens),
+          __builtin_amdgcn_readfirstlane(r.k0), __builtin_amdgcn_readfirstlane(r.k1),
+          __builtin_amdgcn_readfirstlane(r.row)};
 }
 
+// Inclusive sum or maximum (of numbers >= 0) over the wave's lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+template <bool MAX>
+__device__ __forceinline__ int wave_scan(int x) {
+  const auto op = [](int a, int b) { return MAX ? max(a, b) : a + b; };
+  x = op(x, dpp<0x111, 0xf>(x));   // row_shr 1, 2, 4, 8: within 16 lanes
+  x = op(x, dpp<0x112, 0xf>(x));
+  x = op(x, dpp<0x114, 0xf>(x));
+  x = op(x, dpp<0x118, 0xf>(x));
+  x = op(x, dpp<0x142, 0xa>(x));   // lane 15 of a row to the next, lane 31 to the upper half
+  return op(x, dpp<0x143, 0xc>(x));
+}
+
+// One wave's LDS accesses before this come before those after it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Everything by one wave, 64 rows at a time, so that a batch of up to 64 rows needs no barrier but one.
 __device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = p.B;
-  for (int b = tid; b <= B; b += kShThreads) {
-    // offsets never leave q and never fall
-    int c = p.cu_q[b];
-    c = c < 0 ? 0 : c > p.total_q ? p.total_q : c;
-    pl.cu[b] = c;
-    if (b < B) {
-      pl.kv[b] = clamp_len(p.kv_lens[b], p.max_kv);
-      pl.lead[b] = 0;
-      pl.prefix[b] = 0;
-      pl.end[b] = 0;
-    }
-  }
-  __syncthreads();
-  // groups mark their first rows (of several with one first row, the last group counts)
-  for (int g = tid; g < p.G; g += kShThreads) {
-    const int lo = p.cu_rows[g], hi = p.cu_rows[g + 1];
-    if (lo >= 0 && lo < hi && hi <= B) atomicMax(&pl.prefix[lo], g + 1);
-  }
-  __syncthreads();
-  if (wave == 0) {
-    // the row whose group each row is in: the last first row before it, if that group reaches it
-    int carry = 0, cu_top = 0;
-    for (int base = 0; base < B; base += 64) {
-      const int b = base + lane;
-      int first = b < B && pl.prefix[b] > 0 ? b + 1 : 0;
-      int cu = b <= B ? pl.cu[b] : 0;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(first, o), u = __shfl_up(cu, o);
-        if (lane >= o) first = max(first, t), cu = max(cu, u);
-      }
-      first = max(first, carry);
-      cu = max(cu, cu_top);
-      carry = __shfl(first, 63);
-      cu_top = __shfl(cu, 63);
+  const int lane = threadIdx.x & 63, B = p.B;
+  if (threadIdx.x < 64) {
+    for (int b = lane; b <= B; b += 64) {
+      const int c = p.cu_q[b], kv = b < B ? p.kv_lens[b] : 0;
+      const int lo = b < p.G ? p.cu_rows[b] : 0, hi = b < p.G ? p.cu_rows[b + 1] : 0;
+      const int shared = b < p.G ? p.prefix_lens[b] : 0;
+      pl.cu[b] = clamp_len(c, p.total_q);
       if (b < B) {
-        const int lead = first - 1;
-        const int g = lead >= 0 ? pl.prefix[lead] - 1 : -1;
-        pl.lead[b] = g >= 0 && b < p.cu_rows[g + 1] ? lead : -1;
-        pl.cu[b] = cu;
+        pl.kv[b] = clamp_len(kv, p.max_kv);
+        pl.group_prefix[b] = shared;
+        pl.group_end[b] = lo >= 0 && lo < hi && hi <= B ? hi : 0;
+        pl.lead[b] = lo >= 0 && lo < B ? lo : 0;   // for now: the group's first row
+        pl.prefix[b] = 0;
+        pl.end[b] = 0;
       }
-      if (b == B - 1) pl.cu[B] = max(cu, pl.cu[B]);
     }
-  }
-  __syncthreads();
-  for (int b = tid; b < B; b += kShThreads) {
-    const int g = pl.prefix[b] - 1;
-    pl.prefix[b] = g >= 0 ? clamp_len(p.prefix_lens[g], pl.kv[b]) : 0;
-    if (pl.lead[b] >= 0 && (b + 1 == B || pl.lead[b + 1] != pl.lead[b])) pl.end[pl.lead[b]] = b + 1;
-  }
-  __syncthreads();
-  // a prefix goes as far as each query of the group sees it; one row shares with no one
-  for (int b = tid; b < B; b += kShThreads) {
-    const int lead = pl.lead[b], n = pl.cu[b + 1] - pl.cu[b];
-    if (lead >= 0) {
-      if (n > 0) atomicMin(&pl.prefix[lead], max(0, p.causal ? pl.kv[b] - n + 1 : pl.kv[b]));
-      if (pl.end[lead] - lead == 1) atomicMin(&pl.prefix[lead], 0);
+    wave_fence();
+    // groups mark their first rows (of several with one first row, the last group counts)
+    for (int g = lane; g < p.G; g += 64)
+      if (pl.group_end[g] > 0) atomicMax(&pl.prefix[pl.lead[g]], g + 1);
+    wave_fence();
+    // the row whose group each row is in: the last first row up to it, if that group reaches it; and
+    // offsets that never fall
+    int first_top = 0, cu_top = 0;
+    for (int base = 0; base <= B; base += 64) {
+      const int b = base + lane;
+      const int first = max(first_top, wave_scan<true>(b < B && pl.prefix[b] > 0 ? b + 1 : 0));
+      const int cu = max(cu_top, wave_scan<true>(b <= B ? pl.cu[b] : 0));
+      first_top = __builtin_amdgcn_readlane(first, 63);
+      cu_top = __builtin_amdgcn_readlane(cu, 63);
+      const int g = first > 0 ? pl.prefix[first - 1] - 1 : -1;
+      if (b < B) pl.lead[b] = g >= 0 && b < pl.group_end[g] ? first - 1 : -1;
+      if (b <= B) pl.cu[b] = cu;
     }
-  }
-  __syncthreads();
-  for (int b = tid; b < B; b += kShThreads) pl.prefix[b] &= ~(kShStep - 1);
-  __syncthreads();
-  if (wave < 2) {
-    const bool wide = wave == 0;
-    int* out = wide ? pl.wide : pl.narrow;
-    int carry = 0;
-    if (lane == 0) out[0] = 0;
+    wave_fence();
+    for (int b = lane; b < B; b += 64) {
+      const int g = pl.prefix[b] - 1, lead = pl.lead[b];
+      // the first row has to hold it
+      if (g >= 0) pl.prefix[b] = clamp_len(pl.group_prefix[g], pl.kv[b]);
+      if (lead >= 0 && (b + 1 == B || pl.lead[b + 1] != lead)) pl.end[lead] = b + 1;
+    }
+    wave_fence();
+    // a prefix goes as far as each query of the group sees it; one row shares with no one
+    for (int b = lane; b < B; b += 64) {
+      const int lead = pl.lead[b], n = pl.cu[b + 1] - pl.cu[b];
+      if (lead >= 0) {
+        const int seen = n == 0 ? p.max_kv : max(0, p.causal ? pl.kv[b] - n + 1 : pl.kv[b]);
+        atomicMin(&pl.prefix[lead], pl.end[lead] - lead == 1 ? 0 : seen);
+      }
+    }
+    wave_fence();
+    int wide_top = 0, narrow_top = 0;
+    if (lane == 0) pl.wide[0] = pl.narrow[0] = 0;
     for (int base = 0; base < 2 * B; base += 64) {
       const int s = base + lane;
-      int n = 0;
+      int wide = 0, narrow = 0;
       if (s < 2 * B) {
         const ShRange r = range_of(pl, B, s);
         const int pairs = r.tokens * p.group;
-        if (pairs > 0 && (pairs > kShNarrow) == wide)
-          n = p.Hkv * (wide ? wide_tiles(pairs) * key_units(r, kShWideUnit)
-                            : key_units(r, kShNarrowUnit));
+        if (pairs > kShNarrow)
+          wide = p.Hkv * wide_tiles(pairs) * (key_units(r, kShWideUnit) + kShItemCost);
+        else if (pairs > 0)
+          narrow = p.Hkv * (key_units(r, kShNarrowUnit) + kShItemCost);
       }
-      n = wave_scan(n, lane);
-      if (s < 2 * B) out[s + 1] = carry + n;
-      carry += __shfl(n, 63);
+      wide = wide_top + wave_scan<false>(wide);
+      narrow = narrow_top + wave_scan<false>(narrow);
+      wide_top = __builtin_amdgcn_readlane(wide, 63);
+      narrow_top = __builtin_amdgcn_readlane(narrow, 63);
+      if (s < 2 * B) {
+        pl.wide[s + 1] = wide;
+        pl.narrow[s + 1] = narrow;
+      }
     }
   }
   __syncthreads();
 }
 
-// The range that holds unit u: R[s] <= u < R[s + 1] (0 <= u < R[n]).
-__device__ __forceinline__ int find_range(const int* R, int n, int u) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (R[m] <= u) lo = m; else hi = m;
-  }
-  return lo;
+// The range that holds share u: R[s] <= u < R[s + 1] (0 <= u < R[n]), by a whole wave.
+__device__ __forceinline__ int find_range(const int* R, int n, int u, int lane) {
+  int at = -1;
+  for (int base = 0; base < n; base += 64)
+    at += __popcll(__ballot(base + lane < n && R[min(base + lane, n)] <= u));
+  return __builtin_amdgcn_readfirstlane(at);
 }
 
-// First worker (of W over N units) whose share contains unit u.
-__device__ __forceinline__ int first_worker(int64_t u, int64_t N, int W) {
-  return (int)(((u + 1) * W - 1) / N);
+// N shares over W <= N workers: the first `rem` have q + 1, the others q.
+struct ShDeal {
+  int q, rem;
+};
+__device__ __forceinline__ ShDeal make_deal(int N, int W) {
+  const int q = W > 0 ? (unsigned)N / (unsigned)W : 0;
+  return {q, N - q * W};
+}
+__device__ __forceinline__ int first_of(const ShDeal& d, int w) { return w * d.q + min(w, d.rem); }
+__device__ __forceinline__ int worker_of(const ShDeal& d, int u) {
+  const int big = d.rem * (d.q + 1);
+  return u < big ? (unsigned)u / (unsigned)(d.q + 1)
+                 : d.rem + (unsigned)(u - big) / (unsigned)d.q;
 }
 
 // The part of a walk that is the same for all its steps.
@@ -680,35 +702,34 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   const int W1 = min(W, N1);
   if ((int)blockIdx.x < W1) {
     const int wg = blockIdx.x;
-    int u = (int)((int64_t)wg * N1 / W1);
-    const int stop = (int)((int64_t)(wg + 1) * N1 / W1);
-    int s = find_range(pl.wide, n_ranges, u);
+    const ShDeal deal = make_deal(N1, W1);
+    int u = first_of(deal, wg);
+    const int stop = first_of(deal, wg + 1);
+    int s = find_range(pl.wide, n_ranges, u, lane);
     while (u < stop) {
       while (pl.wide[s + 1] <= u) ++s;
       s = __builtin_amdgcn_readfirstlane(s);
-      ShRange r = range_of(pl, p.B, s);
-      r.t0 = __builtin_amdgcn_readfirstlane(r.t0);
-      r.tokens = __builtin_amdgcn_readfirstlane(r.tokens);
-      r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
-      r.k1 = __builtin_amdgcn_readfirstlane(r.k1);
-      r.row = __builtin_amdgcn_readfirstlane(r.row);
+      const ShRange r = uniform(range_of(pl, p.B, s));
       const bool own = s >= p.B;
       const int pairs = r.tokens * p.group, tiles = wide_tiles(pairs), width = tile_pairs(pairs, tiles);
-      const int units = key_units(r, kShWideUnit);
+      const int units = key_units(r, kShWideUnit), length = units + kShItemCost;
       const int at = u - __builtin_amdgcn_readfirstlane(pl.wide[s]);
-      const int item = at / units, c0 = at - item * units;
-      const int hk = item / tiles, pair0 = (item - hk * tiles) * width;
-      const int cols = min(width, pairs - pair0);
-      const int c1 = min(units, c0 + stop - u);
-      const int column = item_columns(p, r, own, hk, pair0) + wg * kShTile;
-      if (c0 == 0 && tid < cols)
-        record(p, r, own, own && prefix_of(pl, r.row) > 0, true, hk, pair0 + tid, column + tid,
-               first_worker(u + units - 1, N1, W1) - wg + 1);
-      if (cols <= 64)
-        wide_item<E, 2>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
-      else
-        wide_item<E, 4>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
-      u += c1 - c0;
+      const int item = (unsigned)at / (unsigned)length, pos = at - item * length;
+      const int hk = (unsigned)item / (unsigned)tiles, pair0 = (item - hk * tiles) * width;
+      const int take = min(length - pos, stop - u);
+      const int c0 = max(0, pos - kShItemCost), c1 = pos + take - kShItemCost;
+      if (c0 < c1) {
+        const int cols = min(width, pairs - pair0);
+        const int column = item_columns(p, r, own, hk, pair0) + wg * kShTile;
+        if (c0 == 0 && tid < cols)
+          record(p, r, own, own && prefix_of(pl, r.row) > 0, true, hk, pair0 + tid, column + tid,
+                 worker_of(deal, u + length - pos - 1) - wg + 1);
+        if (cols <= 64)
+          wide_item<E, 2>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+        else
+          wide_item<E, 4>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+      }
+      u += take;
     }
   }
 
@@ -719,34 +740,33 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   // neighbouring shares on different work-groups: a short list of units spreads over the CUs
   const int worker = wave * W + wg;
   if (worker < W2) {
-    int u = (int)((int64_t)worker * N2 / W2);
-    const int stop = (int)((int64_t)(worker + 1) * N2 / W2);
-    int s = find_range(pl.narrow, n_ranges, u);
+    const ShDeal deal = make_deal(N2, W2);
+    int u = first_of(deal, worker);
+    const int stop = first_of(deal, worker + 1);
+    int s = find_range(pl.narrow, n_ranges, u, lane);
     while (u < stop) {
       while (pl.narrow[s + 1] <= u) ++s;
       s = __builtin_amdgcn_readfirstlane(s);
-      ShRange r = range_of(pl, p.B, s);
-      r.t0 = __builtin_amdgcn_readfirstlane(r.t0);
-      r.tokens = __builtin_amdgcn_readfirstlane(r.tokens);
-      r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
-      r.k1 = __builtin_amdgcn_readfirstlane(r.k1);
-      r.row = __builtin_amdgcn_readfirstlane(r.row);
+      const ShRange r = uniform(range_of(pl, p.B, s));
       const bool own = s >= p.B;
       const int pairs = r.tokens * p.group;
-      const int units = key_units(r, kShNarrowUnit);
+      const int length = key_units(r, kShNarrowUnit) + kShItemCost;
       const int at = u - __builtin_amdgcn_readfirstlane(pl.narrow[s]);
-      const int hk = at / units, c0 = at - hk * units, c1 = min(units, c0 + stop - u);
+      const int hk = (unsigned)at / (unsigned)length, pos = at - hk * length;
+      const int take = min(length - pos, stop - u);
+      const int c0 = max(0, pos - kShItemCost), c1 = pos + take - kShItemCost;
+      u += take;
+      if (c0 >= c1) continue;
       const int column = p.narrow_base + item_columns(p, r, own, hk, 0) + worker * kShNarrow;
       if (c0 == 0 && lane < pairs)
         record(p, r, own, own && prefix_of(pl, r.row) > 0, false, hk, lane, column + lane,
-               first_worker(u + units - 1, N2, W2) - worker + 1);
+               worker_of(deal, u - take + length - pos - 1) - worker + 1);
       ShWalk w;
       ShState st;
       start_tile(p, r, own, hk, 0, 0, pairs, lane, w, st);
       const int kb = r.k0 + c0 * kShNarrowUnit, last = min(r.k1, r.k0 + c1 * kShNarrowUnit);
       if (narrow_walk<E>(p, w, st, kb, last, ring + wave * kShRing, lane)) {
         careful_item<E>(p, r, own, hk, 0, pairs, kb, last, column, 0, 1, lane);
-        u += c1 - c0;
         continue;
       }
       const int r32 = lane & 31, g = lane >> 5;
@@ -765,45 +785,48 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
           p.ws_ml[2 * (int64_t)(column + r32) + 1] = l;
         }
       }
-      u += c1 - c0;
     }
   }
 }
 
-// Merges the parts of one (token, head), a wave each: the lanes first take a part's (m, l) each, 64 parts a
-// time, then half the wave each every other part's O, four dims a lane.
-template <typename E>
+// Merges the parts of one (token, head), by WAVES waves: every lane first takes a part's (m, l), 64 parts a
+// time, then each half wave its share of the parts' O, four dims a lane.
+template <typename E, int WAVES>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p) {
-  const int lane = threadIdx.x & 63;
-  const int pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = blockIdx.x * (4 / WAVES) + wave / WAVES, part = wave % WAVES;
   if (pair >= p.total_q * p.Hq) return;
-  const int token = pair / p.Hq, h = pair - token * p.Hq;
-  if (token < p.cu_q[0] || token >= p.cu_q[p.B]) return;
-  const int32_t* where = p.ws_where + 2 * ((int64_t)p.total_q * p.Hq + pair);
-  int col[2], n[2], stride[2];
-  col[1] = where[0];
-  n[1] = where[1] >> 2;
-  stride[1] = where[1] & 2 ? kShTile : kShNarrow;
-  const bool prefix = where[1] & 1;
-  const int32_t* shared = p.ws_where + 2 * (int64_t)pair;
-  col[0] = prefix ? shared[0] : 0;
-  n[0] = prefix ? shared[1] >> 2 : 0;
-  stride[0] = prefix && (shared[1] & 2) ? kShTile : kShNarrow;
-  // a token that no row holds (offsets that fall) has no record: whatever stands there is not followed
+  const int token = fdiv(pair, p.heads_div), h = pair - token * p.Hq;
+  const int32_t* where = p.ws_where + 2 * (int64_t)pair;
+  const int64_t pairs = 2 * (int64_t)p.total_q * p.Hq;
+  const int first = p.cu_q[0], last = p.cu_q[p.B];
+  int col[2] = {where[0], where[pairs]}, n[2] = {where[1], where[pairs + 1]}, stride[2];
+  const bool prefix = n[1] & 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    stride[i] = n[i] & 2 ? kShTile : kShNarrow;
+    n[i] >>= 2;
+  }
+  if (!prefix) col[0] = n[0] = 0;
+  // Tokens of no row have no record, and offsets that fall leave such tokens between the rows: whatever
+  // stands there is not followed out of the workspace.
+  if (token < first || token >= last) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (col[i] < 0 || n[i] < 0 || col[i] + ((int64_t)n[i] - 1) * stride[i] >= p.columns) return;
 
   const float c = p.scale_log2;
   const int half = lane >> 5, d = 4 * (lane & 31);
+  const auto column = [&](int t) {
+    return t < n[0] ? col[0] + (int64_t)t * stride[0] : col[1] + (int64_t)(t - n[0]) * stride[1];
+  };
   float M = -INFINITY, L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   const int total = n[0] + n[1];
   for (int base = 0; base < total; base += 64) {
     const int i = base + lane, batch = min(64, total - base);
-    const int64_t at = i < n[0] ? col[0] + (int64_t)i * stride[0]
-                                : col[1] + (int64_t)(i - n[0]) * stride[1];
-    float m = i < total ? p.ws_ml[2 * at] : -INFINITY;
+    const int64_t at = column(i);
+    const float m = i < total ? p.ws_ml[2 * at] : -INFINITY;
     const float l = i < total ? p.ws_ml[2 * at + 1] : 0.f;
     float Mn = m;
 #pragma unroll
@@ -819,21 +842,18 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= old;
     M = Mn;
-    constexpr int kFlight = 4;
-    for (int j0 = 0; j0 < batch; j0 += 2 * kFlight) {
+    constexpr int kFlight = 8;
+    for (int j0 = 2 * part; j0 < batch; j0 += 2 * WAVES * kFlight) {
       f32x4 x[kFlight];
       float wt[kFlight];
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const int j = j0 + 2 * k + half;
+        const int j = j0 + 2 * WAVES * k + half;
         const bool live = j < batch;
-        const int t = base + j;
-        const int64_t a = t < n[0] ? col[0] + (int64_t)t * stride[0]
-                                   : col[1] + (int64_t)(t - n[0]) * stride[1];
         wt[k] = __shfl(f, j & 63);
-        // a part that saw no key weighs nothing, whatever its O
+        // a part that weighs nothing (that saw no key) is not looked at: its O may be anything
         x[k] = live && wt[k] != 0.f
-                   ? *reinterpret_cast<const f32x4*>(p.ws_o + a * kHeadDim + d)
+                   ? *reinterpret_cast<const f32x4*>(p.ws_o + column(base + j) * kHeadDim + d)
                    : f32x4{0.f, 0.f, 0.f, 0.f};
         if (!live) wt[k] = 0.f;
       }
@@ -845,6 +865,16 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], 32);
+  if constexpr (WAVES > 1) {
+    __shared__ f32x4 sums[WAVES][32];
+    if (half == 0) sums[part][lane] = acc;
+    __syncthreads();   // (the whole block has one pair)
+    if (part != 0) return;
+#pragma unroll
+    for (int j = 1; j < WAVES; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += sums[j][lane & 31][e];
+  }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   if (half == 0)
     *reinterpret_cast<u32x2*>(p.o + (int64_t)token * p.o_st + (int64_t)h * p.o_sh + d) =
@@ -854,13 +884,19 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
         L > 0.f ? (M * c + __builtin_log2f(L)) * kLn2 : -INFINITY;
 }
 
+constexpr int kShMergePairs = 4096;
+
 template <typename E>
 static hipError_t launch_shared_t(const SharedParams& p, int n_wg, hipStream_t stream) {
   hipLaunchKernelGGL((shared_attn_kernel<E>), dim3(n_wg), dim3(kShThreads), 0, stream, p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL((shared_merge_kernel<E>), dim3((p.total_q * p.Hq + 3) / 4), dim3(256), 0, stream,
-                     p);
+  // four waves for each (token, head) where one would leave most of the device idle
+  const int pairs = p.total_q * p.Hq;
+  if (pairs <= kShMergePairs)
+    hipLaunchKernelGGL((shared_merge_kernel<E, 4>), dim3(pairs), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((shared_merge_kernel<E, 1>), dim3((pairs + 3) / 4), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -873,6 +909,7 @@ hipError_t launch_shared(SharedParams p, int dtype, int n_cus, void* workspace, 
   p.columns = s.columns;
   p.narrow_base = s.narrow;
   p.group_div = make_fastdiv(p.group);
+  p.heads_div = make_fastdiv(p.Hq);
   const int n_wg = n_cus < kSharedWgs ? n_cus : kSharedWgs;
   return dtype == 0 ? launch_shared_t<BF16>(p, n_wg, stream) : launch_shared_t<FP16>(p, n_wg, stream);
 }
