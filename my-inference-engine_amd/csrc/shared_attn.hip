@@ -36,51 +36,44 @@ constexpr int kShNarrowUnit = 64;
 constexpr int kShWideUnit = 128;                // keys of a wide step
 // What an item costs beside its units (queries, the first loads' latency, its part's way out), in units:
 // it takes as many shares more, before its units.
-constexpr int kShItemCost = 2;
+constexpr int kShWideCost = 4, kShNarrowCost = 1;
+constexpr int kShNarrowWeight = 7;
 constexpr int kShRow = kHeadDim * 2;            // bytes of a key
 constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
 constexpr int kShRing = 2 * kShStage / kShWaves;     // a wave's part of the two stages: 16 KB
 static_assert(kShRing == 2 * kShStep * kShRow, "a narrow step's K and V");
 static_assert(kShRing == kShStep * kHeadDim * 4, "a wave's 32 columns of O");
 
+// Tokens and keys of a range: keys [k0, k1) of the row's table (range s: row s, or s - B).
+struct ShRange {
+  int t0, tokens, k0, k1;
+};
+
 // What a work-group knows of the call, in LDS.
 struct ShPlan {
-  int wide[2 * kShMaxRows + 1];    // shares of the ranges before this one (see item_length)
+  int wide[2 * kShMaxRows + 1];    // shares of the ranges before this one (see kShWideCost)
   int narrow[2 * kShMaxRows + 1];
+  ShRange range[2 * kShMaxRows];
+};
+
+// What it is made from, where K and V will be.
+struct ShRows {
   int cu[kShMaxRows + 1];
   int kv[kShMaxRows];
-  int prefix[kShMaxRows];          // at a group's first row: keys that could be read for all the group
+  int prefix[kShMaxRows];          // at a group's first row: keys that can be read for all the group
   int group_prefix[kShMaxRows];    // by group, as given
-  int16_t group_end[kShMaxRows];
-  int16_t lead[kShMaxRows];        // the first row of the row's group, -1: none
-  int16_t end[kShMaxRows];         // at a group's first row: the row after its last
+  int group_end[kShMaxRows];
+  int lead[kShMaxRows];            // the first row of the row's group, -1: none
+  int end[kShMaxRows];             // at a group's first row: the row after its last
 };
 
-// Tokens and keys of range s.
-struct ShRange {
-  int t0, tokens, k0, k1, row;     // keys [k0, k1) through table row `row`
-};
-
-// Keys read for the whole group of row b, in whole steps.
-__device__ __forceinline__ int prefix_of(const ShPlan& pl, int b) {
-  return pl.lead[b] >= 0 ? pl.prefix[pl.lead[b]] & ~(kShStep - 1) : 0;
-}
-
-__device__ __forceinline__ ShRange range_of(const ShPlan& pl, int B, int s) {
-  ShRange r;
-  r.row = s < B ? s : s - B;
-  r.t0 = pl.cu[r.row];
-  const int shared = prefix_of(pl, r.row);
-  if (s < B) {
-    r.tokens = pl.lead[s] == s && shared > 0 ? pl.cu[pl.end[s]] - r.t0 : 0;
-    r.k0 = 0;
-    r.k1 = shared;
-  } else {
-    r.tokens = pl.cu[r.row + 1] - r.t0;
-    r.k0 = shared;
-    r.k1 = pl.kv[r.row];
-  }
-  return r;
+__device__ __forceinline__ ShRange range_of(const ShRows& rows, int B, int s) {
+  const int b = s < B ? s : s - B, lead = rows.lead[b];
+  // in whole steps
+  const int shared = lead >= 0 ? rows.prefix[lead] & ~(kShStep - 1) : 0;
+  const int t0 = rows.cu[b];
+  if (s < B) return {t0, lead == b && shared > 0 ? rows.cu[rows.end[b]] - t0 : 0, 0, shared};
+  return {t0, rows.cu[b + 1] - t0, shared, rows.kv[b]};
 }
 
 __device__ __forceinline__ int wide_tiles(int pairs) { return (pairs + kShTile - 1) / kShTile; }
@@ -94,8 +87,7 @@ __device__ __forceinline__ int key_units(const ShRange& r, int unit) {
 
 __device__ __forceinline__ ShRange uniform(const ShRange& r) {
   return {__builtin_amdgcn_readfirstlane(r.t0), __builtin_amdgcn_readfirstlane(r.tokens),
-          __builtin_amdgcn_readfirstlane(r.k0), __builtin_amdgcn_readfirstlane(r.k1),
-          __builtin_amdgcn_readfirstlane(r.row)};
+          __builtin_amdgcn_readfirstlane(r.k0), __builtin_amdgcn_readfirstlane(r.k1)};
 }
 
 // Inclusive sum or maximum (of numbers >= 0) over the wave's lanes.
@@ -121,55 +113,55 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // Everything by one wave, 64 rows at a time, so that a batch of up to 64 rows needs no barrier but one.
-__device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl) {
+__device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl, ShRows& rows) {
   const int lane = threadIdx.x & 63, B = p.B;
   if (threadIdx.x < 64) {
     for (int b = lane; b <= B; b += 64) {
       const int c = p.cu_q[b], kv = b < B ? p.kv_lens[b] : 0;
       const int lo = b < p.G ? p.cu_rows[b] : 0, hi = b < p.G ? p.cu_rows[b + 1] : 0;
       const int shared = b < p.G ? p.prefix_lens[b] : 0;
-      pl.cu[b] = clamp_len(c, p.total_q);
+      rows.cu[b] = clamp_len(c, p.total_q);
       if (b < B) {
-        pl.kv[b] = clamp_len(kv, p.max_kv);
-        pl.group_prefix[b] = shared;
-        pl.group_end[b] = lo >= 0 && lo < hi && hi <= B ? hi : 0;
-        pl.lead[b] = lo >= 0 && lo < B ? lo : 0;   // for now: the group's first row
-        pl.prefix[b] = 0;
-        pl.end[b] = 0;
+        rows.kv[b] = clamp_len(kv, p.max_kv);
+        rows.group_prefix[b] = shared;
+        rows.group_end[b] = lo >= 0 && lo < hi && hi <= B ? hi : 0;
+        rows.lead[b] = lo >= 0 && lo < B ? lo : 0;   // for now: the group's first row
+        rows.prefix[b] = 0;
+        rows.end[b] = 0;
       }
     }
     wave_fence();
     // groups mark their first rows (of several with one first row, the last group counts)
     for (int g = lane; g < p.G; g += 64)
-      if (pl.group_end[g] > 0) atomicMax(&pl.prefix[pl.lead[g]], g + 1);
+      if (rows.group_end[g] > 0) atomicMax(&rows.prefix[rows.lead[g]], g + 1);
     wave_fence();
     // the row whose group each row is in: the last first row up to it, if that group reaches it; and
     // offsets that never fall
     int first_top = 0, cu_top = 0;
     for (int base = 0; base <= B; base += 64) {
       const int b = base + lane;
-      const int first = max(first_top, wave_scan<true>(b < B && pl.prefix[b] > 0 ? b + 1 : 0));
-      const int cu = max(cu_top, wave_scan<true>(b <= B ? pl.cu[b] : 0));
+      const int first = max(first_top, wave_scan<true>(b < B && rows.prefix[b] > 0 ? b + 1 : 0));
+      const int cu = max(cu_top, wave_scan<true>(b <= B ? rows.cu[b] : 0));
       first_top = __builtin_amdgcn_readlane(first, 63);
       cu_top = __builtin_amdgcn_readlane(cu, 63);
-      const int g = first > 0 ? pl.prefix[first - 1] - 1 : -1;
-      if (b < B) pl.lead[b] = g >= 0 && b < pl.group_end[g] ? first - 1 : -1;
-      if (b <= B) pl.cu[b] = cu;
+      const int g = first > 0 ? rows.prefix[first - 1] - 1 : -1;
+      if (b < B) rows.lead[b] = g >= 0 && b < rows.group_end[g] ? first - 1 : -1;
+      if (b <= B) rows.cu[b] = cu;
     }
     wave_fence();
     for (int b = lane; b < B; b += 64) {
-      const int g = pl.prefix[b] - 1, lead = pl.lead[b];
+      const int g = rows.prefix[b] - 1, lead = rows.lead[b];
       // the first row has to hold it
-      if (g >= 0) pl.prefix[b] = clamp_len(pl.group_prefix[g], pl.kv[b]);
-      if (lead >= 0 && (b + 1 == B || pl.lead[b + 1] != lead)) pl.end[lead] = b + 1;
+      if (g >= 0) rows.prefix[b] = clamp_len(rows.group_prefix[g], rows.kv[b]);
+      if (lead >= 0 && (b + 1 == B || rows.lead[b + 1] != lead)) rows.end[lead] = b + 1;
     }
     wave_fence();
     // a prefix goes as far as each query of the group sees it; one row shares with no one
     for (int b = lane; b < B; b += 64) {
-      const int lead = pl.lead[b], n = pl.cu[b + 1] - pl.cu[b];
+      const int lead = rows.lead[b], n = rows.cu[b + 1] - rows.cu[b];
       if (lead >= 0) {
-        const int seen = n == 0 ? p.max_kv : max(0, p.causal ? pl.kv[b] - n + 1 : pl.kv[b]);
-        atomicMin(&pl.prefix[lead], pl.end[lead] - lead == 1 ? 0 : seen);
+        const int seen = n == 0 ? p.max_kv : max(0, p.causal ? rows.kv[b] - n + 1 : rows.kv[b]);
+        atomicMin(&rows.prefix[lead], rows.end[lead] - lead == 1 ? 0 : seen);
       }
     }
     wave_fence();
@@ -179,12 +171,13 @@ __device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl) {
       const int s = base + lane;
       int wide = 0, narrow = 0;
       if (s < 2 * B) {
-        const ShRange r = range_of(pl, B, s);
+        const ShRange r = range_of(rows, B, s);
+        pl.range[s] = r;
         const int pairs = r.tokens * p.group;
         if (pairs > kShNarrow)
-          wide = p.Hkv * wide_tiles(pairs) * (key_units(r, kShWideUnit) + kShItemCost);
+          wide = p.Hkv * wide_tiles(pairs) * (key_units(r, kShWideUnit) + kShWideCost);
         else if (pairs > 0)
-          narrow = p.Hkv * (key_units(r, kShNarrowUnit) + kShItemCost);
+          narrow = p.Hkv * (key_units(r, kShNarrowUnit) + kShNarrowCost);
       }
       wide = wide_top + wave_scan<false>(wide);
       narrow = narrow_top + wave_scan<false>(narrow);
@@ -254,19 +247,33 @@ __device__ __forceinline__ int entry_of(const SharedParams& p, const ShWalk& w, 
   return t < w.end ? w.table[t >> p.bs_shift] : -1;
 }
 
-// 16 keys of K or V from t on, in block blk, to LDS; keys past the range's end become zeros.
+// 16 keys of K or V from t on, in block blk: where they are; keys past the range's end are outside.
+struct ShRun {
+  uint64_t base;
+  uint32_t bytes;
+};
 template <bool V>
-__device__ __forceinline__ void load_run(const SharedParams& p, const ShWalk& w, int blk, int t,
-                                         uint32_t lds, const ShLanes& ln) {
+__device__ __forceinline__ ShRun run_at(const SharedParams& p, const ShWalk& w, int blk, int t) {
   const bool in = (unsigned)blk < (unsigned)p.num_blocks;
   const int64_t slot = ((int64_t)(in ? blk : 0) << p.bs_shift) + (t & ((1 << p.bs_shift) - 1));
   const uint32_t bytes = in ? (uint32_t)(sclamp(w.end - t, 0, 16) * (int)p.kv_st * 2) : 0u;
-  const uint64_t base = uniform_u64(reinterpret_cast<uint64_t>((V ? w.v : w.k) + slot * p.kv_st));
-  const uint32_t n = __builtin_amdgcn_readfirstlane(bytes);
-  const int row = opaque(ln.row);   // the sums are made here, not kept
+  return {uniform_u64(reinterpret_cast<uint64_t>((V ? w.v : w.k) + slot * p.kv_st)),
+          (uint32_t)__builtin_amdgcn_readfirstlane(bytes)};
+}
+// Load instruction j (0 .. 3) of a run to LDS; what is outside becomes zeros.
+template <bool V>
+__device__ __forceinline__ void load_rows(const SharedParams& p, const ShRun& run, int j, uint32_t lds,
+                                          const ShLanes& ln) {
+  const int row = opaque(ln.row);   // the sum is made here, not kept
+  lds_dma16(run.base, run.bytes, lds + 1024 * j,
+            row + j * 8 * (int)p.kv_st + (V ? ln.v : ln.k ^ (64 * j)));
+}
+template <bool V>
+__device__ __forceinline__ void load_run(const SharedParams& p, const ShWalk& w, int blk, int t,
+                                         uint32_t lds, const ShLanes& ln) {
+  const ShRun run = run_at<V>(p, w, blk, t);
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    lds_dma16(base, n, lds + 1024 * j, row + j * 8 * (int)p.kv_st + (V ? ln.v : ln.k ^ (64 * j)));
+  for (int j = 0; j < 4; ++j) load_rows<V>(p, run, j, lds, ln);
 }
 
 // The operands of 32 keys out of LDS.  MFMA row r of S^T is key pi(r), so that a lane's 8 keys of a
@@ -307,9 +314,10 @@ __device__ __forceinline__ f32x16 scores(const u32x4 (&ka)[8], const u32x4 (&q)[
 }
 
 // The same for N blocks of 32 keys in LDS, operands read two k-steps ahead of their MFMAs and no further.
-template <typename E, int N>
+// between(0 .. 3) is called between the MFMAs (the next step's loads), as in add_pv_of.
+template <typename E, int N, typename F>
 __device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x4 (&q)[8],
-                                          f32x16 (&s)[N]) {
+                                          f32x16 (&s)[N], F&& between) {
   const int kx = k_offset(lane);
   u32x4 ka[3][N];
   const auto rd = [&](int i) {
@@ -326,13 +334,15 @@ __device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x
     if (i + 2 < 8) rd(i + 2);
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] = E::mfma32(ka[i % 3][n], q[i], s[n]);
+    if (i & 1) between(i >> 1);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 // O += P V of N blocks of 32 keys in LDS, likewise a k-step ahead.
-template <typename E, int N>
-__device__ __forceinline__ void add_pv_of(ShState& st, const uint8_t* v, int lane, const u32x4 (&pb)[2 * N]) {
+template <typename E, int N, typename F>
+__device__ __forceinline__ void add_pv_of(ShState& st, const uint8_t* v, int lane, const u32x4 (&pb)[2 * N],
+                                          F&& between) {
   u32x4 va[2][4];
   const auto rd = [&](int i) {
 #pragma unroll
@@ -345,6 +355,8 @@ __device__ __forceinline__ void add_pv_of(ShState& st, const uint8_t* v, int lan
     if (i + 1 < 2 * N) rd(i + 1);
 #pragma unroll
     for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i & 1][db], pb[i], st.o[db]);
+#pragma unroll
+    for (int j = 0; j < 2 / N; ++j) between(i * (2 / N) + j);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -424,11 +436,11 @@ __device__ __forceinline__ bool any_odd(const uint8_t* v, int lane) {
 }
 
 // The wave's columns [col0, col0 + 32) of a tile of `cols` that begins with pair `pair0` of the range.
-__device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange& r, bool own, int hk,
+__device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange& r, int row, bool own, int hk,
                                            int pair0, int col0, int cols, int lane, ShWalk& w,
                                            ShState& st) {
   const int g = lane >> 5, col = col0 + (lane & 31);
-  w.table = p.table + r.row * p.bt_stride;
+  w.table = p.table + row * p.bt_stride;
   w.k = p.k + hk * p.kv_sh;
   w.v = p.v + hk * p.kv_sh;
   w.end = r.k1;
@@ -455,13 +467,13 @@ __device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange&
 // Where the parts of the item's pairs stand: written by the worker with the item's first unit.  The
 // record of a pair: its first part's column, and the number of parts with the kind of worker and, for a
 // row's own range, whether the row's group has a prefix.
-__device__ __forceinline__ void record(const SharedParams& p, const ShRange& r, bool own, bool prefix,
-                                       bool wide, int hk, int pair, int column, int parts) {
+__device__ __forceinline__ void record(const SharedParams& p, const ShRange& r, bool own, bool wide,
+                                       int hk, int pair, int column, int parts) {
   const int token = fdiv(pair, p.group_div);
-  const int64_t at = ((int64_t)(own ? p.total_q : 0) + r.t0 + token) * p.Hq + hk * p.group +
-                     (pair - token * p.group);
-  p.ws_where[2 * at] = column;
-  p.ws_where[2 * at + 1] = parts << 2 | (wide ? 2 : 0) | (prefix ? 1 : 0);
+  const int at = ((own ? p.total_q : 0) + r.t0 + token) * p.Hq + hk * p.group + (pair - token * p.group);
+  const bool prefix = own && r.k0 > 0;
+  *reinterpret_cast<int2*>(p.ws_where + 2 * (int64_t)at) =
+      int2{column, parts << 2 | (wide ? 2 : 0) | (prefix ? 1 : 0)};
 }
 
 // Columns before the parts of an item's pairs (its kind's workers add theirs).
@@ -474,12 +486,12 @@ __device__ __forceinline__ int item_columns(const SharedParams& p, const ShRange
 // whose values are not finite and hidden from some of their queries, where the product of a whole tile
 // would have 0 x inf.  A hidden key is not looked at here.
 template <typename E>
-__device__ __forceinline__ void careful_item(const SharedParams& p, const ShRange& r, bool own, int hk,
-                                             int pair0, int cols, int kb, int stop, int column, int wave,
+__device__ __forceinline__ void careful_item(const SharedParams& p, const ShRange& r, int row, bool own,
+                                             int hk, int pair0, int cols, int kb, int stop, int column, int wave,
                                              int waves, int lane) {
   lane = opaque(lane);
   const float c = p.scale_log2;
-  const int32_t* table = p.table + r.row * p.bt_stride;
+  const int32_t* table = p.table + row * p.bt_stride;
   for (int col = wave; col < cols; col += waves) {
     const int token = fdiv(pair0 + col, p.group_div), h = pair0 + col - token * p.group;
     const int lim = min(stop, own && p.causal ? r.k1 - r.tokens + 1 + token : r.k1);
@@ -515,8 +527,8 @@ __device__ __forceinline__ void careful_item(const SharedParams& p, const ShRang
 
 // Units [c0, c1) of a wide item by the work-group: RG blocks of 32 columns, 8 / RG key streams.
 template <typename E, int RG>
-__device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& r, bool own, int hk,
-                                          int pair0, int cols, int c0, int c1, int column, uint8_t* ring,
+__device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& r, int row, bool own,
+                                          int hk, int pair0, int cols, int c0, int c1, int column, uint8_t* ring,
                                           float (*ml)[32][2], int* odd) {
   constexpr int KS = kShWaves / RG, N = kShWideUnit / KS / kShStep;   // 32-key blocks of a wave and step
   // (the lane as a value of this item: its many LDS addresses are not kept from one to the next)
@@ -526,7 +538,7 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   const int g = lane >> 5;
   ShWalk w;
   ShState st;
-  start_tile(p, r, own, hk, pair0, 32 * rg, cols, lane, w, st);
+  start_tile(p, r, row, own, hk, pair0, 32 * rg, cols, lane, w, st);
   const bool active = 32 * rg < cols;
   const int first = r.k0 + c0 * kShWideUnit, n = c1 - c0;
   if (tid == 0) *odd = 0;   // (barriers follow)
@@ -534,29 +546,36 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr_of(ring)) + wave * 16 * kShRow;
   // this wave's run of step i: keys first + 128 i + 16 wave .. ; block ids of 64 steps, a lane each
   int tbl = entry_of(p, w, first + (int64_t)lane * kShWideUnit + 16 * wave);
-  const auto load = [&](int i) {
-    const int t = first + i * kShWideUnit + 16 * wave;
-    const int blk = __builtin_amdgcn_readlane(tbl, i & 63);
-    const uint32_t at = lds + (i & 1) * kShStage;
-    load_run<false>(p, w, blk, t, at, ln);
-    load_run<true>(p, w, blk, t, at + kShWideUnit * kShRow, ln);
-  };
-  load(0);
+  const auto entry = [&](int i) { return __builtin_amdgcn_readlane(tbl, i & 63); };
+  const auto key_of = [&](int i) { return first + i * kShWideUnit + 16 * wave; };
+  load_run<false>(p, w, entry(0), key_of(0), lds, ln);
+  load_run<true>(p, w, entry(0), key_of(0), lds + kShWideUnit * kShRow, ln);
   for (int i = 0; i < n; ++i) {
     // the step's loads are in LDS, and every wave is done with the other stage
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+    // the next step's loads go out between this one's MFMAs (past the last step: of nothing)
+    ShRun next_k{}, next_v{};
+    const uint32_t next_lds = lds + ((i + 1) & 1) * kShStage;
     if (i + 1 < n) {
       if (((i + 1) & 63) == 0)
         tbl = entry_of(p, w, first + (i + 1 + (int64_t)lane) * kShWideUnit + 16 * wave);
-      load(i + 1);
+      next_k = run_at<false>(p, w, entry(i + 1), key_of(i + 1));
+      next_v = run_at<true>(p, w, entry(i + 1), key_of(i + 1));
     }
+    const bool more = i + 1 < n;
+    const auto load_k = [&](int j) {
+      if (more) load_rows<false>(p, next_k, j, next_lds, ln);
+    };
+    const auto load_v = [&](int j) {
+      if (more) load_rows<true>(p, next_v, j, next_lds + kShWideUnit * kShRow, ln);
+    };
     const int kb = first + i * kShWideUnit + ks * N * kShStep;
     if (active && kb < w.end) {
       const uint8_t* k = ring + (i & 1) * kShStage + ks * N * kShStep * kShRow;
       const uint8_t* v = k + kShWideUnit * kShRow;
       f32x16 s[N];
-      scores_of<E, N>(k, lane, st.q, s);
+      scores_of<E, N>(k, lane, st.q, s, load_k);
       const bool masked = kb + N * kShStep > w.full;
       if (masked) {
 #pragma unroll
@@ -565,7 +584,13 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
       u32x4 pb[2 * N];
       softmax<E, N>(p.scale_log2, st, s, pb);
       if (masked && any_odd<E, N>(v, lane)) *odd = 1;
-      add_pv_of<E, N>(st, v, lane, pb);
+      add_pv_of<E, N>(st, v, lane, pb, load_v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        load_k(j);
+        load_v(j);
+      }
     }
   }
   // the key streams' parts become one: each scales its own to the common maximum, LDS sums them
@@ -577,7 +602,7 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   }
   __syncthreads();
   if (*odd) {
-    careful_item<E>(p, r, own, hk, pair0, cols, first, min(r.k1, first + n * kShWideUnit), column, wave,
+    careful_item<E>(p, r, row, own, hk, pair0, cols, first, min(r.k1, first + n * kShWideUnit), column, wave,
                     kShWaves, lane);
     __syncthreads();
     return;
@@ -693,13 +718,22 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   __shared__ int odd;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  make_plan(p, pl);
-  const int n_ranges = 2 * p.B;
-  const int W = gridDim.x;
-
-  // wide ranges, by work-groups
+  make_plan(p, pl, *reinterpret_cast<ShRows*>(ring));
+  const int n_ranges = 2 * p.B, W = gridDim.x;
   const int N1 = __builtin_amdgcn_readfirstlane(pl.wide[n_ranges]);
-  const int W1 = min(W, N1);
+  const int N2 = __builtin_amdgcn_readfirstlane(pl.narrow[n_ranges]);
+  // The wide ranges take the first W1 work-groups, the waves of the others the narrow ones: a share each
+  // if that fits, else as many as their work weighs (a work-group's wide share takes 2.7 us, eight
+  // narrow shares side by side 1.2 us: kShNarrowWeight of them are one).
+  const int alone = (N2 + kShWaves - 1) / kShWaves;
+  int W3 = alone;
+  if (N1 + alone > W) {
+    const float all = (float)kShNarrowWeight * (float)N1 + (float)N2;
+    W3 = min(alone, (int)((float)W * (float)N2 / all + 0.5f));
+    W3 = __builtin_amdgcn_readfirstlane(min(max(W3, N2 > 0 ? 1 : 0), N1 > 0 ? W - 1 : W));
+  }
+  const int W1 = min(W - W3, N1);
+
   if ((int)blockIdx.x < W1) {
     const int wg = blockIdx.x;
     const ShDeal deal = make_deal(N1, W1);
@@ -709,81 +743,80 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     while (u < stop) {
       while (pl.wide[s + 1] <= u) ++s;
       s = __builtin_amdgcn_readfirstlane(s);
-      const ShRange r = uniform(range_of(pl, p.B, s));
+      const ShRange r = uniform(pl.range[s]);
       const bool own = s >= p.B;
+      const int row = own ? s - p.B : s;
       const int pairs = r.tokens * p.group, tiles = wide_tiles(pairs), width = tile_pairs(pairs, tiles);
-      const int units = key_units(r, kShWideUnit), length = units + kShItemCost;
+      const int units = key_units(r, kShWideUnit), length = units + kShWideCost;
       const int at = u - __builtin_amdgcn_readfirstlane(pl.wide[s]);
       const int item = (unsigned)at / (unsigned)length, pos = at - item * length;
       const int hk = (unsigned)item / (unsigned)tiles, pair0 = (item - hk * tiles) * width;
       const int take = min(length - pos, stop - u);
-      const int c0 = max(0, pos - kShItemCost), c1 = pos + take - kShItemCost;
+      const int c0 = max(0, pos - kShWideCost), c1 = pos + take - kShWideCost;
       if (c0 < c1) {
         const int cols = min(width, pairs - pair0);
         const int column = item_columns(p, r, own, hk, pair0) + wg * kShTile;
         if (c0 == 0 && tid < cols)
-          record(p, r, own, own && prefix_of(pl, r.row) > 0, true, hk, pair0 + tid, column + tid,
+          record(p, r, own, true, hk, pair0 + tid, column + tid,
                  worker_of(deal, u + length - pos - 1) - wg + 1);
         if (cols <= 64)
-          wide_item<E, 2>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+          wide_item<E, 2>(p, r, row, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
         else
-          wide_item<E, 4>(p, r, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
+          wide_item<E, 4>(p, r, row, own, hk, pair0, cols, c0, c1, column, ring, ml, &odd);
       }
       u += take;
     }
+    return;
   }
 
-  // narrow ranges, by waves; the work-groups without a share of the wide ones come first
-  const int N2 = __builtin_amdgcn_readfirstlane(pl.narrow[n_ranges]);
-  const int W2 = min(W * kShWaves, N2);
-  const int wg = (int)blockIdx.x >= W1 ? (int)blockIdx.x - W1 : (int)blockIdx.x + W - W1;
+  const int W2 = min(W3 * kShWaves, N2);
   // neighbouring shares on different work-groups: a short list of units spreads over the CUs
-  const int worker = wave * W + wg;
-  if (worker < W2) {
-    const ShDeal deal = make_deal(N2, W2);
-    int u = first_of(deal, worker);
-    const int stop = first_of(deal, worker + 1);
-    int s = find_range(pl.narrow, n_ranges, u, lane);
-    while (u < stop) {
-      while (pl.narrow[s + 1] <= u) ++s;
-      s = __builtin_amdgcn_readfirstlane(s);
-      const ShRange r = uniform(range_of(pl, p.B, s));
-      const bool own = s >= p.B;
-      const int pairs = r.tokens * p.group;
-      const int length = key_units(r, kShNarrowUnit) + kShItemCost;
-      const int at = u - __builtin_amdgcn_readfirstlane(pl.narrow[s]);
-      const int hk = (unsigned)at / (unsigned)length, pos = at - hk * length;
-      const int take = min(length - pos, stop - u);
-      const int c0 = max(0, pos - kShItemCost), c1 = pos + take - kShItemCost;
-      u += take;
-      if (c0 >= c1) continue;
-      const int column = p.narrow_base + item_columns(p, r, own, hk, 0) + worker * kShNarrow;
-      if (c0 == 0 && lane < pairs)
-        record(p, r, own, own && prefix_of(pl, r.row) > 0, false, hk, lane, column + lane,
-               worker_of(deal, u - take + length - pos - 1) - worker + 1);
-      ShWalk w;
-      ShState st;
-      start_tile(p, r, own, hk, 0, 0, pairs, lane, w, st);
-      const int kb = r.k0 + c0 * kShNarrowUnit, last = min(r.k1, r.k0 + c1 * kShNarrowUnit);
-      if (narrow_walk<E>(p, w, st, kb, last, ring + wave * kShRing, lane)) {
-        careful_item<E>(p, r, own, hk, 0, pairs, kb, last, column, 0, 1, lane);
-        continue;
-      }
-      const int r32 = lane & 31, g = lane >> 5;
-      const float l = st.l + __shfl_xor(st.l, 32);
-      if (r32 < pairs) {
-        float* o = p.ws_o + (int64_t)(column + r32) * kHeadDim + 4 * g;
+  const int worker = wave * W3 + (int)blockIdx.x - (W - W3);
+  if ((int)blockIdx.x < W - W3 || worker >= W2) return;
+  const ShDeal deal = make_deal(N2, W2);
+  int u = first_of(deal, worker);
+  const int stop = first_of(deal, worker + 1);
+  int s = find_range(pl.narrow, n_ranges, u, lane);
+  while (u < stop) {
+    while (pl.narrow[s + 1] <= u) ++s;
+    s = __builtin_amdgcn_readfirstlane(s);
+    const ShRange r = uniform(pl.range[s]);
+    const bool own = s >= p.B;
+    const int row = own ? s - p.B : s;
+    const int pairs = r.tokens * p.group;
+    const int length = key_units(r, kShNarrowUnit) + kShNarrowCost;
+    const int at = u - __builtin_amdgcn_readfirstlane(pl.narrow[s]);
+    const int hk = (unsigned)at / (unsigned)length, pos = at - hk * length;
+    const int take = min(length - pos, stop - u);
+    const int c0 = max(0, pos - kShNarrowCost), c1 = pos + take - kShNarrowCost;
+    u += take;
+    if (c0 >= c1) continue;
+    const int column = p.narrow_base + item_columns(p, r, own, hk, 0) + worker * kShNarrow;
+    if (c0 == 0 && lane < pairs)
+      record(p, r, own, false, hk, lane, column + lane,
+             worker_of(deal, u - take + length - pos - 1) - worker + 1);
+    ShWalk w;
+    ShState st;
+    start_tile(p, r, row, own, hk, 0, 0, pairs, lane, w, st);
+    const int kb = r.k0 + c0 * kShNarrowUnit, last = min(r.k1, r.k0 + c1 * kShNarrowUnit);
+    if (narrow_walk<E>(p, w, st, kb, last, ring + wave * kShRing, lane)) {
+      careful_item<E>(p, r, row, own, hk, 0, pairs, kb, last, column, 0, 1, lane);
+      continue;
+    }
+    const int r32 = lane & 31, g = lane >> 5;
+    const float l = st.l + __shfl_xor(st.l, 32);
+    if (r32 < pairs) {
+      float* o = p.ws_o + (int64_t)(column + r32) * kHeadDim + 4 * g;
 #pragma unroll
-        for (int db = 0; db < 4; ++db)
+      for (int db = 0; db < 4; ++db)
 #pragma unroll
-          for (int rr = 0; rr < 4; ++rr)
-            *reinterpret_cast<f32x4*>(o + 32 * db + 8 * rr) =
-                f32x4{st.o[db][4 * rr], st.o[db][4 * rr + 1], st.o[db][4 * rr + 2],
-                      st.o[db][4 * rr + 3]};
-        if (g == 0) {
-          p.ws_ml[2 * (int64_t)(column + r32)] = st.m;
-          p.ws_ml[2 * (int64_t)(column + r32) + 1] = l;
-        }
+        for (int rr = 0; rr < 4; ++rr)
+          *reinterpret_cast<f32x4*>(o + 32 * db + 8 * rr) =
+              f32x4{st.o[db][4 * rr], st.o[db][4 * rr + 1], st.o[db][4 * rr + 2],
+                    st.o[db][4 * rr + 3]};
+      if (g == 0) {
+        p.ws_ml[2 * (int64_t)(column + r32)] = st.m;
+        p.ws_ml[2 * (int64_t)(column + r32) + 1] = l;
       }
     }
   }
@@ -910,7 +943,8 @@ hipError_t launch_shared(SharedParams p, int dtype, int n_cus, void* workspace, 
   p.narrow_base = s.narrow;
   p.group_div = make_fastdiv(p.group);
   p.heads_div = make_fastdiv(p.Hq);
-  const int n_wg = n_cus < kSharedWgs ? n_cus : kSharedWgs;
+  // (two at least: one for either kind of range)
+  const int n_wg = n_cus < 2 ? 2 : n_cus < kSharedWgs ? n_cus : kSharedWgs;
   return dtype == 0 ? launch_shared_t<BF16>(p, n_wg, stream) : launch_shared_t<FP16>(p, n_wg, stream);
 }
 

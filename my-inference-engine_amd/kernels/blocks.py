@@ -17,6 +17,7 @@ from pathlib import Path
 import torch
 
 from . import _lib
+from .fa2 import _MEMO_MAX
 
 LIB_PATH = Path(os.environ.get("MI_CACHE_LIB", Path(__file__).resolve().parent / "libmi_cache.so"))
 
@@ -61,8 +62,22 @@ def check(status):
             f"libmi_cache status {status}: {load().mi_cache_last_error().decode()}")
 
 
+_POOLS = {}
+
+
 def _planes(pool, name, block_size):
-    """(planes, bytes between them, blocks, bytes of a block) of a pool [..., slots, kv_heads, d]."""
+    """(planes, bytes between them, blocks, bytes of a block) of a pool [..., slots, kv_heads, d].  The
+    checks that its shape, strides and type decide run once per combination."""
+    key = (pool.shape, pool.stride(), pool.dtype, pool.device, block_size)
+    got = _POOLS.get(key)
+    if got is None or type(block_size) is not int:   # (16.0 would find 16's)
+        if len(_POOLS) >= _MEMO_MAX:
+            _POOLS.clear()
+        got = _POOLS[key] = _check_planes(pool, name, block_size)
+    return got
+
+
+def _check_planes(pool, name, block_size):
     assert pool.is_cuda, f"{name}: a GPU tensor"
     assert pool.dim() >= 3, f"{name}: [..., slots, kv_heads, d]"
     slots, heads, d = pool.shape[-3:]
@@ -86,10 +101,11 @@ def _planes(pool, name, block_size):
 
 
 def _ids(t, name, shape, device):
-    assert t.device == device and t.dtype == torch.int32, f"{name}: int32 on {device}"
-    assert t.dim() == len(shape) and t.is_contiguous(), f"{name}: {len(shape)} dims, contiguous"
-    assert all(want is None or n == want for n, want in zip(t.shape, shape)), \
-        f"{name}: shape {tuple(t.shape)}"
+    """The pointer of a contiguous int32 tensor of that shape (its first entry None: any)."""
+    got = t.shape
+    if not (t.dtype == torch.int32 and len(got) == len(shape) and got[1:] == shape[1:]
+            and shape[0] in (None, got[0]) and t.is_contiguous() and t.device == device):
+        raise AssertionError(f"{name}: contiguous int32 of shape {shape} on {device}")
     return t.data_ptr()
 
 
