@@ -26,6 +26,8 @@
 // registers the next step's K is sent for, likewise V.
 #include "cache_ops.h"
 
+#include <type_traits>
+
 namespace mi_fa2 {
 
 constexpr int kShWaves = kSharedWaves, kShThreads = 64 * kShWaves;
@@ -260,6 +262,24 @@ __device__ __forceinline__ ShRun run_at(const SharedParams& p, const ShWalk& w, 
   return {uniform_u64(reinterpret_cast<uint64_t>((V ? w.v : w.k) + slot * p.kv_st)),
           (uint32_t)__builtin_amdgcn_readfirstlane(bytes)};
 }
+// K runs of 64 steps, a lane each, found in a few vector instructions: the lane's first key is t.
+struct ShRuns {
+  uint32_t lo, hi, bytes;
+};
+__device__ __forceinline__ ShRuns find_runs(const SharedParams& p, const ShWalk& w, int64_t t) {
+  const int blk = entry_of(p, w, t);
+  const bool in = (unsigned)blk < (unsigned)p.num_blocks;
+  const int64_t slot = ((int64_t)(in ? blk : 0) << p.bs_shift) + ((int)t & ((1 << p.bs_shift) - 1));
+  const uint64_t at = reinterpret_cast<uint64_t>(w.k + slot * p.kv_st);
+  const int rows = (int)min<int64_t>(max<int64_t>(w.end - t, 0), 16);
+  return {(uint32_t)at, (uint32_t)(at >> 32), in ? (uint32_t)(rows * (int)p.kv_st * 2) : 0u};
+}
+__device__ __forceinline__ ShRun run_of(const ShRuns& runs, int lane) {
+  return {(uint64_t)(uint32_t)__builtin_amdgcn_readlane(runs.hi, lane) << 32 |
+              (uint32_t)__builtin_amdgcn_readlane(runs.lo, lane),
+          (uint32_t)__builtin_amdgcn_readlane(runs.bytes, lane)};
+}
+
 // Load instruction j (0 .. 3) of a run to LDS; what is outside becomes zeros.
 template <bool V>
 __device__ __forceinline__ void load_rows(const SharedParams& p, const ShRun& run, int j, uint32_t lds,
@@ -525,7 +545,13 @@ __device__ __forceinline__ void careful_item(const SharedParams& p, const ShRang
   }
 }
 
-// Units [c0, c1) of a wide item by the work-group: RG blocks of 32 columns, 8 / RG key streams.
+// Units [c0, c1) of a wide item by the work-group: RG blocks of 32 columns, 8 / RG key streams, a unit a
+// step.  Waves w and w + 4 share a SIMD and take keys of a step's two halves half a step apart, so that one's
+// softmax runs beside the other's MFMAs:
+//   first half, step j:  softmax(j), O += PV(j), S(j + 1)      second half:  S(j), O += PV(j - 1), softmax(j)
+// Slot j % 2 of the ring therefore holds, in step j, of the first half V(j) and K(j + 1), of the second
+// K(j) and V(j - 1); it is loaded during step j - 1, each wave its run of either: K of step `ahead`, V of the
+// step before that.
 template <typename E, int RG>
 __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& r, int row, bool own,
                                           int hk, int pair0, int cols, int c0, int c1, int column, uint8_t* ring,
@@ -535,6 +561,7 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   const int tid = threadIdx.x, lane = opaque(tid & 63);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wave % RG, ks = wave / RG;
+  const bool second = wave >= kShWaves / 2;
   const int g = lane >> 5;
   ShWalk w;
   ShState st;
@@ -544,54 +571,115 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   if (tid == 0) *odd = 0;   // (barriers follow)
   const ShLanes ln = lane_offsets(p.kv_st, lane);
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr_of(ring)) + wave * 16 * kShRow;
-  // this wave's run of step i: keys first + 128 i + 16 wave .. ; block ids of 64 steps, a lane each
-  int tbl = entry_of(p, w, first + (int64_t)lane * kShWideUnit + 16 * wave);
-  const auto entry = [&](int i) { return __builtin_amdgcn_readlane(tbl, i & 63); };
-  const auto key_of = [&](int i) { return first + i * kShWideUnit + 16 * wave; };
-  load_run<false>(p, w, entry(0), key_of(0), lds, ln);
-  load_run<true>(p, w, entry(0), key_of(0), lds + kShWideUnit * kShRow, ln);
-  for (int i = 0; i < n; ++i) {
-    // the step's loads are in LDS, and every wave is done with the other stage
+  constexpr uint32_t kV = kShWideUnit * kShRow;   // V of a slot, behind K
+  // this wave's run of step i: keys first + 128 i + 16 wave ..
+  const auto runs_from = [&](int i) {
+    return find_runs(p, w, first + (i + (int64_t)lane) * kShWideUnit + 16 * wave);
+  };
+  ShRuns runs = runs_from(0);
+  const uint64_t v_apart = uniform_u64(reinterpret_cast<uint64_t>(w.v) - reinterpret_cast<uint64_t>(w.k));
+  int ahead = 0;                    // the step whose K run is next_k, and V run v_of(next_k)
+  ShRun next_k = run_of(runs, 0), next_v{};
+  const auto v_of = [&](const ShRun& k) { return ShRun{k.base + v_apart, k.bytes}; };
+  const auto step_ahead = [&]() {
+    ++ahead;
+    if ((ahead & 63) == 0) runs = runs_from(ahead);
+    next_k = run_of(runs, ahead & 63);
+  };
+  const auto load_all = [&](auto v, const ShRun& run, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_rows<decltype(v)::value>(p, run, i, at, ln);
+  };
+  constexpr std::false_type isK{};
+  constexpr std::true_type isV{};
+  if (!second) {
+    load_all(isK, next_k, lds + kShStage);
+    load_all(isV, v_of(next_k), lds + kV);
+    if (n > 1) {
+      step_ahead();
+      load_all(isK, next_k, lds);
+    }
+  } else {
+    load_all(isK, next_k, lds);
+    load_all(isV, v_of(next_k), lds + kShStage + kV);
+  }
+  const auto step_ready = [&]() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    // the next step's loads go out between this one's MFMAs (past the last step: of nothing)
-    ShRun next_k{}, next_v{};
-    const uint32_t next_lds = lds + ((i + 1) & 1) * kShStage;
-    if (i + 1 < n) {
-      if (((i + 1) & 63) == 0)
-        tbl = entry_of(p, w, first + (i + 1 + (int64_t)lane) * kShWideUnit + 16 * wave);
-      next_k = run_at<false>(p, w, entry(i + 1), key_of(i + 1));
-      next_v = run_at<true>(p, w, entry(i + 1), key_of(i + 1));
-    }
-    const bool more = i + 1 < n;
-    const auto load_k = [&](int j) {
-      if (more) load_rows<false>(p, next_k, j, next_lds, ln);
-    };
-    const auto load_v = [&](int j) {
-      if (more) load_rows<true>(p, next_v, j, next_lds + kShWideUnit * kShRow, ln);
-    };
-    const int kb = first + i * kShWideUnit + ks * N * kShStep;
-    if (active && kb < w.end) {
-      const uint8_t* k = ring + (i & 1) * kShStage + ks * N * kShStep * kShRow;
-      const uint8_t* v = k + kShWideUnit * kShRow;
-      f32x16 s[N];
-      scores_of<E, N>(k, lane, st.q, s, load_k);
-      const bool masked = kb + N * kShStep > w.full;
-      if (masked) {
+  };
+
+  // The loads of step j, for slot (j + 1) % 2, between the MFMAs: V of the last step whose K went out, K of
+  // the next (the second half's first V came with the first loads).
+  bool more_k = false, more_v = false;
+  uint32_t next_lds = 0;
+  const auto plan_loads = [&](int j) {
+    next_lds = lds + ((j + 1) & 1) * kShStage;
+    more_v = second ? j > 0 : j + 1 < n;
+    next_v = v_of(next_k);
+    more_k = ahead + 1 < n;
+    if (more_k) step_ahead();
+  };
+  const auto load_k = [&](int i) {
+    if (more_k) load_rows<false>(p, next_k, i, next_lds, ln);
+  };
+  const auto load_v = [&](int i) {
+    if (more_v) load_rows<true>(p, next_v, i, next_lds + kV, ln);
+  };
+
+  const int offset = ks * N * kShStep;   // the stream's keys in a step
+  const auto has = [&](int j) { return active && j < n && first + j * kShWideUnit + offset < w.end; };
+  f32x16 s[N];
+  u32x4 pb[2 * N];
+  const auto do_scores = [&](int j, int slot) {
+    if (has(j)) {
+      scores_of<E, N>(ring + slot * kShStage + offset * kShRow, lane, st.q, s, load_k);
+    } else {
 #pragma unroll
-        for (int b = 0; b < N; ++b) hide(s[b], st.lim - kb - kShStep * b - 8 * g);
-      }
-      u32x4 pb[2 * N];
-      softmax<E, N>(p.scale_log2, st, s, pb);
-      if (masked && any_odd<E, N>(v, lane)) *odd = 1;
+      for (int i = 0; i < 4; ++i) load_k(i);
+    }
+  };
+  const auto do_softmax = [&](int j) {
+    if (!has(j)) return;
+    const int kb = first + j * kShWideUnit + offset;
+    if (kb + N * kShStep > w.full) {
+#pragma unroll
+      for (int b = 0; b < N; ++b) hide(s[b], st.lim - kb - kShStep * b - 8 * g);
+    }
+    softmax<E, N>(p.scale_log2, st, s, pb);
+  };
+  const auto do_pv = [&](int j, int slot) {
+    if (j >= 0 && has(j)) {
+      const uint8_t* v = ring + slot * kShStage + kV + offset * kShRow;
+      if (first + j * kShWideUnit + offset + N * kShStep > w.full && any_odd<E, N>(v, lane)) *odd = 1;
       add_pv_of<E, N>(st, v, lane, pb, load_v);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        load_k(j);
-        load_v(j);
-      }
+      for (int i = 0; i < 4; ++i) load_v(i);
     }
+  };
+  step_ready();
+  // (separate programs of the same barriers)
+  if (!second) {
+    do_scores(0, 1);
+    __syncthreads();
+    for (int j = 0; j < n; ++j) {
+      plan_loads(j);
+      do_softmax(j);
+      do_pv(j, j & 1);
+      do_scores(j + 1, j & 1);
+      step_ready();
+    }
+  } else {
+    __syncthreads();
+    for (int j = 0; j < n; ++j) {
+      plan_loads(j);
+      do_scores(j, j & 1);
+      do_pv(j - 1, j & 1);
+      do_softmax(j);
+      step_ready();
+    }
+    more_v = false;
+    do_pv(n - 1, n & 1);
   }
   // the key streams' parts become one: each scales its own to the common maximum, LDS sums them
   st.l += __shfl_xor(st.l, 32);
