@@ -44,7 +44,6 @@ constexpr int kShRow = kHeadDim * 2;            // bytes of a key
 constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
 constexpr int kShRing = 2 * kShStage / kShWaves;     // a wave's part of the two stages: 16 KB
 static_assert(kShRing == 2 * kShStep * kShRow, "a narrow step's K and V");
-static_assert(kShRing == kShStep * kHeadDim * 4, "a wave's 32 columns of O");
 
 // Tokens and keys of a range: keys [k0, k1) of the row's table (range s: row s, or s - B).
 struct ShRange {
@@ -60,23 +59,18 @@ struct ShPlan {
 
 // What it is made from, where K and V will be.
 struct ShRows {
-  int cu[kShMaxRows + 1];
+  int cu[kShMaxRows + 1];          // as given, inside q
   int kv[kShMaxRows];
-  int prefix[kShMaxRows];          // at a group's first row: keys that can be read for all the group
-  int group_prefix[kShMaxRows];    // by group, as given
-  int group_end[kShMaxRows];
+  int group[kShMaxRows];           // by group: first row and the row after its last, packed; -1: none
+  int group_prefix[kShMaxRows];
+  int mark[kShMaxRows];            // at a group's first row: which group, and the row after its last
+  int t0[kShMaxRows], tokens[kShMaxRows];
   int lead[kShMaxRows];            // the first row of the row's group, -1: none
-  int end[kShMaxRows];             // at a group's first row: the row after its last
+  // at a group's first row:
+  int prefix[kShMaxRows];          // keys that each of its queries sees
+  int last[kShMaxRows];            // the token after its last
+  int alone[kShMaxRows];           // what 128 keys cost without sharing, in shares
 };
-
-__device__ __forceinline__ ShRange range_of(const ShRows& rows, int B, int s) {
-  const int b = s < B ? s : s - B, lead = rows.lead[b];
-  // in whole steps
-  const int shared = lead >= 0 ? rows.prefix[lead] & ~(kShStep - 1) : 0;
-  const int t0 = rows.cu[b];
-  if (s < B) return {t0, lead == b && shared > 0 ? rows.cu[rows.end[b]] - t0 : 0, 0, shared};
-  return {t0, rows.cu[b + 1] - t0, shared, rows.kv[b]};
-}
 
 __device__ __forceinline__ int wide_tiles(int pairs) { return (pairs + kShTile - 1) / kShTile; }
 // pairs of a tile: the range's, evenly, in whole 32s
@@ -114,7 +108,20 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Everything by one wave, 64 rows at a time, so that a batch of up to 64 rows needs no barrier but one.
+// The keys read once for the group that row `lead` leads: whole steps of its prefix, or none where that
+// would cost more shares than every row by itself (one row; rows that fill tiles of their own, and then
+// pay for another item each).
+__device__ __forceinline__ int shared_keys(const SharedParams& p, const ShRows& rows, int lead) {
+  const int keys = rows.prefix[lead] & ~(kShStep - 1);
+  const int pairs = (rows.last[lead] - rows.t0[lead]) * p.group;
+  const float blocks = (float)keys * (1.f / 128.f);
+  const float shared =
+      pairs > kShNarrow ? (float)(kShNarrowWeight * wide_tiles(pairs)) * (blocks + kShWideCost)
+                        : 2.f * blocks + kShNarrowCost;
+  return shared < (float)rows.alone[lead] * blocks ? keys : 0;
+}
+
+// Everything by one wave, 64 rows at a time, so that it needs no barrier but one.
 __device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl, ShRows& rows) {
   const int lane = threadIdx.x & 63, B = p.B;
   if (threadIdx.x < 64) {
@@ -125,45 +132,47 @@ __device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl, ShR
       rows.cu[b] = clamp_len(c, p.total_q);
       if (b < B) {
         rows.kv[b] = clamp_len(kv, p.max_kv);
-        rows.group_prefix[b] = shared;
-        rows.group_end[b] = lo >= 0 && lo < hi && hi <= B ? hi : 0;
-        rows.lead[b] = lo >= 0 && lo < B ? lo : 0;   // for now: the group's first row
-        rows.prefix[b] = 0;
-        rows.end[b] = 0;
+        rows.group[b] = lo >= 0 && lo < hi && hi <= B ? lo << 16 | hi : -1;
+        rows.group_prefix[b] = clamp_len(shared, p.max_kv);
+        rows.mark[b] = 0;
+        rows.prefix[b] = p.max_kv;
+        rows.last[b] = 0;
+        rows.alone[b] = 0;
       }
     }
     wave_fence();
     // groups mark their first rows (of several with one first row, the last group counts)
-    for (int g = lane; g < p.G; g += 64)
-      if (rows.group_end[g] > 0) atomicMax(&rows.prefix[rows.lead[g]], g + 1);
+    for (int g = lane; g < p.G; g += 64) {
+      const int ends = rows.group[g];
+      if (ends >= 0) atomicMax(&rows.mark[ends >> 16], (g + 1) << 10 | (ends & 0xffff));
+    }
     wave_fence();
-    // the row whose group each row is in: the last first row up to it, if that group reaches it; and
-    // offsets that never fall
+    // A row's group is that of the last first row up to it, if it reaches the row; offsets never fall.
+    // Each row tells its group's first row what it sees, holds and costs.
     int first_top = 0, cu_top = 0;
-    for (int base = 0; base <= B; base += 64) {
-      const int b = base + lane;
-      const int first = max(first_top, wave_scan<true>(b < B && rows.prefix[b] > 0 ? b + 1 : 0));
-      const int cu = max(cu_top, wave_scan<true>(b <= B ? rows.cu[b] : 0));
+    for (int base = 0; base < B; base += 64) {
+      const int b = base + lane, at = min(b, B - 1);
+      const int mark = b < B ? rows.mark[at] : 0, next = rows.cu[at + 1], kv = rows.kv[at];
+      const int cu = max(cu_top, wave_scan<true>(b < B ? rows.cu[at] : 0));
+      // first row + 1, group + 1, row after its last: ten bits each
+      const int first = max(first_top, wave_scan<true>(mark ? (b + 1) << 20 | mark : 0));
       first_top = __builtin_amdgcn_readlane(first, 63);
       cu_top = __builtin_amdgcn_readlane(cu, 63);
-      const int g = first > 0 ? rows.prefix[first - 1] - 1 : -1;
-      if (b < B) rows.lead[b] = g >= 0 && b < rows.group_end[g] ? first - 1 : -1;
-      if (b <= B) rows.cu[b] = cu;
-    }
-    wave_fence();
-    for (int b = lane; b < B; b += 64) {
-      const int g = rows.prefix[b] - 1, lead = rows.lead[b];
-      // the first row has to hold it
-      if (g >= 0) rows.prefix[b] = clamp_len(rows.group_prefix[g], rows.kv[b]);
-      if (lead >= 0 && (b + 1 == B || rows.lead[b + 1] != lead)) rows.end[lead] = b + 1;
-    }
-    wave_fence();
-    // a prefix goes as far as each query of the group sees it; one row shares with no one
-    for (int b = lane; b < B; b += 64) {
-      const int lead = rows.lead[b], n = rows.cu[b + 1] - rows.cu[b];
-      if (lead >= 0) {
-        const int seen = n == 0 ? p.max_kv : max(0, p.causal ? rows.kv[b] - n + 1 : rows.kv[b]);
-        atomicMin(&rows.prefix[lead], rows.end[lead] - lead == 1 ? 0 : seen);
+      if (b < B) {
+        const int lead = b < (first & 0x3ff) ? (first >> 20) - 1 : -1;
+        const int tokens = max(next - cu, 0), pairs = tokens * p.group;
+        rows.t0[b] = cu;
+        rows.tokens[b] = tokens;
+        rows.lead[b] = lead;
+        if (lead >= 0) {
+          int seen = tokens == 0 ? p.max_kv : max(0, p.causal ? kv - tokens + 1 : kv);
+          // the first row has to hold the prefix
+          if (lead == b) seen = min(seen, min(kv, rows.group_prefix[((first >> 10) & 0x3ff) - 1]));
+          atomicMin(&rows.prefix[lead], seen);
+          atomicMax(&rows.last[lead], cu + tokens);
+          if (pairs > 0)
+            atomicAdd(&rows.alone[lead], pairs > kShNarrow ? kShNarrowWeight * wide_tiles(pairs) : 2);
+        }
       }
     }
     wave_fence();
@@ -173,7 +182,14 @@ __device__ __forceinline__ void make_plan(const SharedParams& p, ShPlan& pl, ShR
       const int s = base + lane;
       int wide = 0, narrow = 0;
       if (s < 2 * B) {
-        const ShRange r = range_of(rows, B, s);
+        const int b = s < B ? s : s - B, lead = rows.lead[b];
+        const int shared = lead >= 0 ? shared_keys(p, rows, lead) : 0;
+        ShRange r = {rows.t0[b], rows.tokens[b], shared, rows.kv[b]};
+        if (s < B) {
+          r.tokens = lead == b && shared > 0 ? rows.last[b] - r.t0 : 0;
+          r.k0 = 0;
+          r.k1 = shared;
+        }
         pl.range[s] = r;
         const int pairs = r.tokens * p.group;
         if (pairs > kShNarrow)
@@ -202,19 +218,27 @@ __device__ __forceinline__ int find_range(const int* R, int n, int u, int lane) 
   return __builtin_amdgcn_readfirstlane(at);
 }
 
+// a / b of whole numbers >= 0, b > 0.  Below 2^22 by the reciprocal: the product is off by less than one.
+__device__ __forceinline__ int quotient(int a, int b) {
+  if (a >= 1 << 22 || b >= 1 << 22) return (unsigned)a / (unsigned)b;
+  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+  const int r = a - q * b;
+  q += r >= b ? 1 : r < 0 ? -1 : 0;
+  return __builtin_amdgcn_readfirstlane(q);
+}
+
 // N shares over W <= N workers: the first `rem` have q + 1, the others q.
 struct ShDeal {
   int q, rem;
 };
 __device__ __forceinline__ ShDeal make_deal(int N, int W) {
-  const int q = W > 0 ? (unsigned)N / (unsigned)W : 0;
+  const int q = W > 0 ? quotient(N, W) : 0;
   return {q, N - q * W};
 }
 __device__ __forceinline__ int first_of(const ShDeal& d, int w) { return w * d.q + min(w, d.rem); }
 __device__ __forceinline__ int worker_of(const ShDeal& d, int u) {
   const int big = d.rem * (d.q + 1);
-  return u < big ? (unsigned)u / (unsigned)(d.q + 1)
-                 : d.rem + (unsigned)(u - big) / (unsigned)d.q;
+  return u < big ? quotient(u, d.q + 1) : d.rem + quotient(u - big, d.q);
 }
 
 // The part of a walk that is the same for all its steps.
@@ -266,8 +290,7 @@ __device__ __forceinline__ ShRun run_at(const SharedParams& p, const ShWalk& w, 
 struct ShRuns {
   uint32_t lo, hi, bytes;
 };
-__device__ __forceinline__ ShRuns find_runs(const SharedParams& p, const ShWalk& w, int64_t t) {
-  const int blk = entry_of(p, w, t);
+__device__ __forceinline__ ShRuns find_runs(const SharedParams& p, const ShWalk& w, int64_t t, int blk) {
   const bool in = (unsigned)blk < (unsigned)p.num_blocks;
   const int64_t slot = ((int64_t)(in ? blk : 0) << p.bs_shift) + ((int)t & ((1 << p.bs_shift) - 1));
   const uint64_t at = reinterpret_cast<uint64_t>(w.k + slot * p.kv_st);
@@ -393,8 +416,10 @@ __device__ __forceinline__ void hide(f32x16& s, int lim) {
 // kk]), maximum, sum and O updated.
 //   p = 2^(c (s - m)): the difference first, so that scores of any size keep their weights.  The
 // reference m may lag the true maximum while no p of the lane exceeds 2^8, as in the prefill kernel.
+// The first keys of a walk (fresh) have no reference yet.
 template <typename E, int N>
-__device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[N], u32x4 (&pb)[2 * N]) {
+__device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[N], u32x4 (&pb)[2 * N],
+                                        bool fresh) {
   const auto weigh = [&](float ref) {
     float sum = 0.f;
 #pragma unroll
@@ -408,7 +433,8 @@ __device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[
       }
     return sum;
   };
-  float sum = weigh(st.m);
+  float sum = INFINITY;
+  if (!fresh) sum = weigh(st.m);
   if (__any(!(sum <= 256.f))) {
     float mx = -INFINITY;
 #pragma unroll
@@ -456,14 +482,10 @@ __device__ __forceinline__ bool any_odd(const uint8_t* v, int lane) {
 }
 
 // The wave's columns [col0, col0 + 32) of a tile of `cols` that begins with pair `pair0` of the range.
-__device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange& r, int row, bool own, int hk,
+__device__ __forceinline__ void start_tile(const SharedParams& p, const ShRange& r, bool own, int hk,
                                            int pair0, int col0, int cols, int lane, ShWalk& w,
                                            ShState& st) {
   const int g = lane >> 5, col = col0 + (lane & 31);
-  w.table = p.table + row * p.bt_stride;
-  w.k = p.k + hk * p.kv_sh;
-  w.v = p.v + hk * p.kv_sh;
-  w.end = r.k1;
   // own keys: query i of the row's n sees all but the n - 1 - i last
   const int first = r.k1 - r.tokens + 1;
   const int token = fdiv(pair0 + col, p.group_div);
@@ -549,9 +571,9 @@ __device__ __forceinline__ void careful_item(const SharedParams& p, const ShRang
 // step.  Waves w and w + 4 share a SIMD and take keys of a step's two halves half a step apart, so that one's
 // softmax runs beside the other's MFMAs:
 //   first half, step j:  softmax(j), O += PV(j), S(j + 1)      second half:  S(j), O += PV(j - 1), softmax(j)
-// Slot j % 2 of the ring therefore holds, in step j, of the first half V(j) and K(j + 1), of the second
-// K(j) and V(j - 1); it is loaded during step j - 1, each wave its run of either: K of step `ahead`, V of the
-// step before that.
+// (S(0) comes before both).
+// Slot j % 2 of the ring therefore holds, in step j, of the first half V(j) and K(j + 1), of the second K(j)
+// and V(j - 1); it is loaded during step j - 1, each wave its run of either.
 template <typename E, int RG>
 __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& r, int row, bool own,
                                           int hk, int pair0, int cols, int c0, int c1, int column, uint8_t* ring,
@@ -563,27 +585,31 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
   const int rg = wave % RG, ks = wave / RG;
   const bool second = wave >= kShWaves / 2;
   const int g = lane >> 5;
+  const int first = r.k0 + c0 * kShWideUnit, n = c1 - c0;
   ShWalk w;
   ShState st;
-  start_tile(p, r, row, own, hk, pair0, 32 * rg, cols, lane, w, st);
+  w.table = p.table + row * p.bt_stride;
+  w.k = p.k + hk * p.kv_sh;
+  w.v = p.v + hk * p.kv_sh;
+  w.end = r.k1;
+  // this wave's run of step i: keys first + 128 i + 16 wave ..  (The first block ids travel while the
+  // queries are found.)
+  const auto run_key = [&](int i) { return first + (i + (int64_t)lane) * kShWideUnit + 16 * wave; };
+  const int entry = entry_of(p, w, run_key(0));
+  start_tile(p, r, own, hk, pair0, 32 * rg, cols, lane, w, st);
   const bool active = 32 * rg < cols;
-  const int first = r.k0 + c0 * kShWideUnit, n = c1 - c0;
   if (tid == 0) *odd = 0;   // (barriers follow)
   const ShLanes ln = lane_offsets(p.kv_st, lane);
   const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_addr_of(ring)) + wave * 16 * kShRow;
   constexpr uint32_t kV = kShWideUnit * kShRow;   // V of a slot, behind K
-  // this wave's run of step i: keys first + 128 i + 16 wave ..
-  const auto runs_from = [&](int i) {
-    return find_runs(p, w, first + (i + (int64_t)lane) * kShWideUnit + 16 * wave);
-  };
-  ShRuns runs = runs_from(0);
+  ShRuns runs = find_runs(p, w, run_key(0), entry);
   const uint64_t v_apart = uniform_u64(reinterpret_cast<uint64_t>(w.v) - reinterpret_cast<uint64_t>(w.k));
   int ahead = 0;                    // the step whose K run is next_k, and V run v_of(next_k)
   ShRun next_k = run_of(runs, 0), next_v{};
   const auto v_of = [&](const ShRun& k) { return ShRun{k.base + v_apart, k.bytes}; };
   const auto step_ahead = [&]() {
     ++ahead;
-    if ((ahead & 63) == 0) runs = runs_from(ahead);
+    if ((ahead & 63) == 0) runs = find_runs(p, w, run_key(ahead), entry_of(p, w, run_key(ahead)));
     next_k = run_of(runs, ahead & 63);
   };
   const auto load_all = [&](auto v, const ShRun& run, uint32_t at) {
@@ -645,7 +671,7 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
 #pragma unroll
       for (int b = 0; b < N; ++b) hide(s[b], st.lim - kb - kShStep * b - 8 * g);
     }
-    softmax<E, N>(p.scale_log2, st, s, pb);
+    softmax<E, N>(p.scale_log2, st, s, pb, j == 0);
   };
   const auto do_pv = [&](int j, int slot) {
     if (j >= 0 && has(j)) {
@@ -670,8 +696,14 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
       step_ready();
     }
   } else {
+    do_scores(0, 0);
     __syncthreads();
-    for (int j = 0; j < n; ++j) {
+    plan_loads(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_k(i);
+    do_softmax(0);
+    step_ready();
+    for (int j = 1; j < n; ++j) {
       plan_loads(j);
       do_scores(j, j & 1);
       do_pv(j - 1, j & 1);
@@ -681,12 +713,29 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
     more_v = false;
     do_pv(n - 1, n & 1);
   }
-  // the key streams' parts become one: each scales its own to the common maximum, LDS sums them
+  // The key streams' parts become one.  A wave keeps 4 / KS of its four blocks of dims, gives the others away
+  // through LDS, in the accumulators' order, and adds what it gets.
   st.l += __shfl_xor(st.l, 32);
-  const int r32 = opaque(lane & 31);
+  const int out_lane = opaque(lane), r32 = out_lane & 31;
   if (g == 0) {
     ml[wave][r32][0] = st.m;
     ml[wave][r32][1] = st.l;
+  }
+  constexpr int kKeep = 4 / KS;
+  // The second half's waves may still read V of the last step (the last quarter of slot n % 2): the first
+  // half writes to the other slot, the second to the first three quarters of that one.
+  const auto area = [&](int wv, int db) {
+    const int i = KS == 2 ? db & 1 : db - (db > wv / RG ? 1 : 0);   // of the blocks that the wave gives
+    return ring + ((n + (wv < kShWaves / 2 ? 1 : 0)) & 1) * kShStage + (wv & 3) * 12288 + i * 4096 +
+           out_lane * 16;
+  };
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+    if (db / kKeep == ks) continue;   // (uniform)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr)
+      *reinterpret_cast<f32x4*>(area(wave, db) + rr * 1024) =
+          f32x4{st.o[db][4 * rr], st.o[db][4 * rr + 1], st.o[db][4 * rr + 2], st.o[db][4 * rr + 3]};
   }
   __syncthreads();
   if (*odd) {
@@ -695,45 +744,36 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
     __syncthreads();
     return;
   }
-  {
-    float M = -INFINITY;
+  float M = -INFINITY, L = 0.f, f[KS];
 #pragma unroll
-    for (int j = 0; j < KS; ++j) M = fmaxf(M, ml[j * RG + rg][r32][0]);
-    const float f = exp2_fast((st.m - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
-    // [wave][column][128], 16-byte pieces at piece ^ column
+  for (int j = 0; j < KS; ++j) M = fmaxf(M, ml[j * RG + rg][r32][0]);
 #pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int rr = 0; rr < 4; ++rr)
-        *reinterpret_cast<f32x4*>(ring + wave * kShRing + r32 * 512 +
-                                  16 * ((8 * db + 2 * rr + g) ^ r32)) =
-            f32x4{st.o[db][4 * rr] * f, st.o[db][4 * rr + 1] * f, st.o[db][4 * rr + 2] * f,
-                  st.o[db][4 * rr + 3] * f};
+  for (int j = 0; j < KS; ++j) {
+    f[j] = exp2_fast((ml[j * RG + rg][r32][0] - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
+    L = __builtin_fmaf(ml[j * RG + rg][r32][1], f[j], L);
   }
-  if (tid < cols) {
-    const int b = tid >> 5, col = tid & 31;
-    float M = -INFINITY, L = 0.f;
+  const int col = 32 * rg + r32;
+  float* o = p.ws_o + (int64_t)(column + col) * kHeadDim + 4 * g;
 #pragma unroll
-    for (int j = 0; j < KS; ++j) M = fmaxf(M, ml[j * RG + b][col][0]);
-    const float Mu = M == -INFINITY ? 0.f : M;
+  for (int db = 0; db < 4; ++db) {
+    if (db / kKeep != ks) continue;
 #pragma unroll
-    for (int j = 0; j < KS; ++j)
-      L += ml[j * RG + b][col][1] * exp2_fast((ml[j * RG + b][col][0] - Mu) * p.scale_log2);
-    p.ws_ml[2 * (int64_t)(column + tid)] = M;
-    p.ws_ml[2 * (int64_t)(column + tid) + 1] = L;
-  }
-  __syncthreads();
-  for (int i = tid; i < cols * 32; i += kShThreads) {
-    const int col = i >> 5, piece = i & 31;
-    const uint8_t* at = ring + (col >> 5) * kShRing + (col & 31) * 512 + 16 * (piece ^ (col & 31));
-    f32x4 sum = *reinterpret_cast<const f32x4*>(at);
+    for (int rr = 0; rr < 4; ++rr) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 1; j < KS; ++j) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(at + j * RG * kShRing);
+      for (int j = 0; j < KS; ++j) {   // in the streams' order, whoever adds
+        const f32x4 x = j == ks ? f32x4{st.o[db][4 * rr], st.o[db][4 * rr + 1], st.o[db][4 * rr + 2],
+                                        st.o[db][4 * rr + 3]}
+                                : *reinterpret_cast<const f32x4*>(area(j * RG + rg, db) + rr * 1024);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += x[e];
+        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(x[e], f[j], sum[e]);
+      }
+      if (col < cols) *reinterpret_cast<f32x4*>(o + 32 * db + 8 * rr) = sum;
     }
-    *reinterpret_cast<f32x4*>(p.ws_o + (int64_t)(column + col) * kHeadDim + 4 * piece) = sum;
+  }
+  if (ks == 0 && g == 0 && col < cols) {
+    p.ws_ml[2 * (int64_t)(column + col)] = M;
+    p.ws_ml[2 * (int64_t)(column + col) + 1] = L;
   }
   __syncthreads();   // the ring and ml are the next item's
 }
@@ -742,14 +782,13 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
 // has to do it.
 template <typename E>
 __device__ __forceinline__ bool narrow_walk(const SharedParams& p, const ShWalk& w, ShState& st, int kb,
-                                            int stop, const uint8_t* ring, int lane) {
+                                            int stop, int entry, const uint8_t* ring, int lane) {
   if (kb >= stop) return false;
   bool odd = false;
   const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_addr_of(ring));
   const uint32_t lds_v = lds_k + kShStep * kShRow;
   const ShLanes ln = lane_offsets(p.kv_st, lane);
-  // block ids of the two runs of 32 steps, lane 2 i + run
-  int tbl = entry_of(p, w, kb + (int64_t)lane * 16);
+  int tbl = entry;   // block ids of the two runs of 32 steps, lane 2 i + run
   const auto load_k = [&](int i, int t) {
     load_run<false>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i), t, lds_k, ln);
     load_run<false>(p, w, __builtin_amdgcn_readlane(tbl, 2 * i + 1), t + 16, lds_k + 16 * kShRow, ln);
@@ -780,7 +819,7 @@ __device__ __forceinline__ bool narrow_walk(const SharedParams& p, const ShWalk&
     const bool masked = next > w.full;
     if (masked) hide(s[0], st.lim - kb - 8 * g);
     u32x4 pb[2];
-    softmax<E, 1>(p.scale_log2, st, s, pb);
+    softmax<E, 1>(p.scale_log2, st, s, pb, i == 1);
     if (more)
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // V is there, the next K may be on its way
     else
@@ -837,8 +876,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
       const int pairs = r.tokens * p.group, tiles = wide_tiles(pairs), width = tile_pairs(pairs, tiles);
       const int units = key_units(r, kShWideUnit), length = units + kShWideCost;
       const int at = u - __builtin_amdgcn_readfirstlane(pl.wide[s]);
-      const int item = (unsigned)at / (unsigned)length, pos = at - item * length;
-      const int hk = (unsigned)item / (unsigned)tiles, pair0 = (item - hk * tiles) * width;
+      const int item = quotient(at, length), pos = at - item * length;
+      const int hk = quotient(item, tiles), pair0 = (item - hk * tiles) * width;
       const int take = min(length - pos, stop - u);
       const int c0 = max(0, pos - kShWideCost), c1 = pos + take - kShWideCost;
       if (c0 < c1) {
@@ -874,7 +913,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     const int pairs = r.tokens * p.group;
     const int length = key_units(r, kShNarrowUnit) + kShNarrowCost;
     const int at = u - __builtin_amdgcn_readfirstlane(pl.narrow[s]);
-    const int hk = (unsigned)at / (unsigned)length, pos = at - hk * length;
+    const int hk = quotient(at, length), pos = at - hk * length;
     const int take = min(length - pos, stop - u);
     const int c0 = max(0, pos - kShNarrowCost), c1 = pos + take - kShNarrowCost;
     u += take;
@@ -885,9 +924,14 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
              worker_of(deal, u - take + length - pos - 1) - worker + 1);
     ShWalk w;
     ShState st;
-    start_tile(p, r, row, own, hk, 0, 0, pairs, lane, w, st);
+    w.table = p.table + row * p.bt_stride;
+    w.k = p.k + hk * p.kv_sh;
+    w.v = p.v + hk * p.kv_sh;
+    w.end = r.k1;
     const int kb = r.k0 + c0 * kShNarrowUnit, last = min(r.k1, r.k0 + c1 * kShNarrowUnit);
-    if (narrow_walk<E>(p, w, st, kb, last, ring + wave * kShRing, lane)) {
+    const int entry = entry_of(p, w, kb + (int64_t)lane * 16);   // (travels while the queries are found)
+    start_tile(p, r, own, hk, 0, 0, pairs, lane, w, st);
+    if (narrow_walk<E>(p, w, st, kb, last, entry, ring + wave * kShRing, lane)) {
       careful_item<E>(p, r, row, own, hk, 0, pairs, kb, last, column, 0, 1, lane);
       continue;
     }
