@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -69,12 +70,15 @@ int check_pool(const char* name, const void* p, int64_t plane_bytes, int32_t num
   return kOk;
 }
 
-// Work-groups of a launch stay below 2^31 threads' worth of one grid dimension.
-int check_count(int64_t n, int64_t rows, int64_t block_bytes) {
+// A launch stays below 2^31 threads: one work-group of 256 for each 16 KB of a block and plane, and for
+// each table row.
+int check_count(int64_t n, int64_t rows, int64_t block_bytes, int64_t planes) {
   if (n < 0 || rows < 0) return fail(kInvalid, "bad counts: %lld, %lld", (long long)n, (long long)rows);
-  if (n * ((block_bytes >> 14) + 1) + rows >= int64_t(1) << 23)
-    return fail(kUnsupported, "%lld blocks of %lld bytes in one call", (long long)n,
-                (long long)block_bytes);
+  const int64_t pieces = (block_bytes + 16383) / 16384;
+  if (n >= int64_t(1) << 23 || pieces >= int64_t(1) << 23 ||
+      n * pieces >= (int64_t(1) << 23) / std::max<int64_t>(planes, 1) - rows / std::max<int64_t>(planes, 1) - 1)
+    return fail(kUnsupported, "%lld blocks of %lld bytes in %lld planes, %lld rows in one call",
+                (long long)n, (long long)block_bytes, (long long)planes, (long long)rows);
   return kOk;
 }
 
@@ -112,7 +116,7 @@ int mi_cache_copy_blocks(const void* src, int64_t src_plane_bytes, int32_t src_n
                          void* stream) {
   if (int rc = check_pool("src", src, src_plane_bytes, src_num_blocks, planes, block_bytes)) return rc;
   if (int rc = check_pool("dst", dst, dst_plane_bytes, dst_num_blocks, planes, block_bytes)) return rc;
-  if (int rc = check_count(n, 0, block_bytes)) return rc;
+  if (int rc = check_count(n, 0, block_bytes, planes)) return rc;
   if (n == 0 || planes == 0) return ok();
   if (!pairs) return fail(kInvalid, "pairs is NULL");
   BlockOpParams p{};
@@ -136,11 +140,12 @@ int mi_cache_fork_rows(void* pool, int64_t plane_bytes, int32_t num_blocks, int3
   const int64_t block_bytes = block_size * token_bytes;
   if (int rc = check_pool("pool", pool, plane_bytes, num_blocks, planes, block_bytes)) return rc;
   if (int rc = check_table(tables, table_stride, table_width, max_seqs)) return rc;
-  if (int rc = check_count(n, n, block_bytes)) return rc;
+  if (int rc = check_count(n, n, block_bytes, planes)) return rc;
   if (!seq_lens) return fail(kInvalid, "seq_lens is NULL");
   if (planes == 0) return fail(kInvalid, "pool: no planes");
   if (n == 0) return ok();
   if (!children) return fail(kInvalid, "children is NULL");
+  if (!aligned16(children)) return fail(kInvalid, "children is not 16-byte aligned");
   BlockOpParams p{};
   p.src = p.dst = static_cast<uint8_t*>(pool);
   p.src_plane = p.dst_plane = plane_bytes;
@@ -165,7 +170,7 @@ int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t num_blocks, in
                          const int32_t* rows, int32_t n_rows, const int32_t* new_ids,
                          void* stream) {
   if (int rc = check_pool("pool", pool, plane_bytes, num_blocks, planes, block_bytes)) return rc;
-  if (int rc = check_count(n, n_rows, block_bytes)) return rc;
+  if (int rc = check_count(n, n_rows, block_bytes, planes)) return rc;
   if (planes == 0) return fail(kInvalid, "pool: no planes");
   if (n > 0 && !pairs) return fail(kInvalid, "pairs is NULL");
   if (n_rows > 0) {

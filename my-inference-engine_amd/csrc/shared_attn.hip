@@ -39,6 +39,7 @@ constexpr int kShWideUnit = 128;                // keys of a wide step
 // What an item costs beside its units (queries, the first loads' latency, its part's way out), in units:
 // it takes as many shares more, before its units.
 constexpr int kShWideCost = 4, kShNarrowCost = 1;
+constexpr int kShMergeCost = 4;   // of one more wide part for each pair, in the merge
 constexpr int kShNarrowWeight = 7;
 constexpr int kShRow = kHeadDim * 2;            // bytes of a key
 constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
@@ -72,10 +73,19 @@ struct ShRows {
   int alone[kShMaxRows];           // what 128 keys cost without sharing, in shares
 };
 
+// a / b of whole numbers >= 0, b > 0.  Below 2^22 by the reciprocal: the product is off by less than one.
+__device__ __forceinline__ int quotient(int a, int b) {
+  if (a >= 1 << 22 || b >= 1 << 22) return (unsigned)a / (unsigned)b;
+  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+  const int r = a - q * b;
+  q += r >= b ? 1 : r < 0 ? -1 : 0;
+  return __builtin_amdgcn_readfirstlane(q);
+}
+
 __device__ __forceinline__ int wide_tiles(int pairs) { return (pairs + kShTile - 1) / kShTile; }
 // pairs of a tile: the range's, evenly, in whole 32s
 __device__ __forceinline__ int tile_pairs(int pairs, int tiles) {
-  return ((pairs + tiles - 1) / tiles + 31) & ~31;
+  return (quotient(pairs + tiles - 1, tiles) + 31) & ~31;
 }
 __device__ __forceinline__ int key_units(const ShRange& r, int unit) {
   return max(1, (r.k1 - r.k0 + unit - 1) / unit);
@@ -116,8 +126,9 @@ __device__ __forceinline__ int shared_keys(const SharedParams& p, const ShRows& 
   const int pairs = (rows.last[lead] - rows.t0[lead]) * p.group;
   const float blocks = (float)keys * (1.f / 128.f);
   const float shared =
-      pairs > kShNarrow ? (float)(kShNarrowWeight * wide_tiles(pairs)) * (blocks + kShWideCost)
-                        : 2.f * blocks + kShNarrowCost;
+      pairs > kShNarrow
+          ? (float)(kShNarrowWeight * wide_tiles(pairs)) * (blocks + kShWideCost + kShMergeCost)
+          : 2.f * blocks + kShNarrowCost;
   return shared < (float)rows.alone[lead] * blocks ? keys : 0;
 }
 
@@ -216,15 +227,6 @@ __device__ __forceinline__ int find_range(const int* R, int n, int u, int lane) 
   for (int base = 0; base < n; base += 64)
     at += __popcll(__ballot(base + lane < n && R[min(base + lane, n)] <= u));
   return __builtin_amdgcn_readfirstlane(at);
-}
-
-// a / b of whole numbers >= 0, b > 0.  Below 2^22 by the reciprocal: the product is off by less than one.
-__device__ __forceinline__ int quotient(int a, int b) {
-  if (a >= 1 << 22 || b >= 1 << 22) return (unsigned)a / (unsigned)b;
-  int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
-  const int r = a - q * b;
-  q += r >= b ? 1 : r < 0 ? -1 : 0;
-  return __builtin_amdgcn_readfirstlane(q);
 }
 
 // N shares over W <= N workers: the first `rem` have q + 1, the others q.
@@ -357,7 +359,7 @@ __device__ __forceinline__ f32x16 scores(const u32x4 (&ka)[8], const u32x4 (&q)[
 }
 
 // The same for N blocks of 32 keys in LDS, operands read two k-steps ahead of their MFMAs and no further.
-// between(0 .. 3) is called between the MFMAs (the next step's loads), as in add_pv_of.
+// between(0 .. 3) is called between the MFMAs (the next step's loads), as in ShPv.
 template <typename E, int N, typename F>
 __device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x4 (&q)[8],
                                           f32x16 (&s)[N], F&& between) {
@@ -382,27 +384,36 @@ __device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x
   }
 }
 
-// O += P V of N blocks of 32 keys in LDS, likewise a k-step ahead.
-template <typename E, int N, typename F>
-__device__ __forceinline__ void add_pv_of(ShState& st, const uint8_t* v, int lane, const u32x4 (&pb)[2 * N],
-                                          F&& between) {
-  u32x4 va[2][4];
-  const auto rd = [&](int i) {
+// O += P V of N blocks of 32 keys in LDS.  V's operands are read two k-steps ahead, those of the first two
+// (begin) before the softmax or scores that come in between, so that their way is hidden.
+template <typename E, int N>
+struct ShPv {
+  u32x4 va[3][4];
+
+  __device__ __forceinline__ void read(const uint8_t* v, int lane, int i) {
 #pragma unroll
     for (int db = 0; db < 4; ++db)
-      va[i & 1][db] = read_v(v + (i >> 1) * kShStep * kShRow, lane, i & 1, db);
-  };
-  rd(0);
-#pragma unroll
-  for (int i = 0; i < 2 * N; ++i) {
-    if (i + 1 < 2 * N) rd(i + 1);
-#pragma unroll
-    for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i & 1][db], pb[i], st.o[db]);
-#pragma unroll
-    for (int j = 0; j < 2 / N; ++j) between(i * (2 / N) + j);
+      va[i % 3][db] = read_v(v + (i >> 1) * kShStep * kShRow, lane, i & 1, db);
+  }
+  __device__ __forceinline__ void begin(const uint8_t* v, int lane) {
+    read(v, lane, 0);
+    read(v, lane, 1);
     __builtin_amdgcn_sched_barrier(0);
   }
-}
+  template <typename F>
+  __device__ __forceinline__ void add(ShState& st, const uint8_t* v, int lane, const u32x4 (&pb)[2 * N],
+                                      F&& between) {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      if (i + 2 < 2 * N) read(v, lane, i + 2);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i % 3][db], pb[i], st.o[db]);
+#pragma unroll
+      for (int j = 0; j < 2 / N; ++j) between(i * (2 / N) + j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
 
 // Accumulator r of a block of 32 keys is the lane's key 16 (r / 8) + r % 8 (the lanes with g = 1 start at
 // key 8): those at or past lim are hidden.
@@ -443,7 +454,9 @@ __device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     const bool grow = (mx - st.m) * c > 8.f;
-    if (__any(grow)) {
+    if (fresh) {   // nothing to rescale
+      st.m = mx;
+    } else if (__any(grow)) {
       const float alpha = grow ? exp2_fast((st.m - mx) * c) : 1.f;
       st.l *= alpha;
 #pragma unroll
@@ -673,11 +686,16 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
     }
     softmax<E, N>(p.scale_log2, st, s, pb, j == 0);
   };
+  ShPv<E, N> pv;
+  const auto v_in = [&](int slot) { return ring + slot * kShStage + kV + offset * kShRow; };
+  const auto begin_pv = [&](int j, int slot) {
+    if (has(j)) pv.begin(v_in(slot), lane);
+  };
   const auto do_pv = [&](int j, int slot) {
-    if (j >= 0 && has(j)) {
-      const uint8_t* v = ring + slot * kShStage + kV + offset * kShRow;
+    if (has(j)) {
+      const uint8_t* v = v_in(slot);
       if (first + j * kShWideUnit + offset + N * kShStep > w.full && any_odd<E, N>(v, lane)) *odd = 1;
-      add_pv_of<E, N>(st, v, lane, pb, load_v);
+      pv.add(st, v, lane, pb, load_v);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_v(i);
@@ -690,6 +708,7 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
     __syncthreads();
     for (int j = 0; j < n; ++j) {
       plan_loads(j);
+      begin_pv(j, j & 1);
       do_softmax(j);
       do_pv(j, j & 1);
       do_scores(j + 1, j & 1);
@@ -705,12 +724,14 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const ShRange& 
     step_ready();
     for (int j = 1; j < n; ++j) {
       plan_loads(j);
+      begin_pv(j - 1, j & 1);
       do_scores(j, j & 1);
       do_pv(j - 1, j & 1);
       do_softmax(j);
       step_ready();
     }
     more_v = false;
+    begin_pv(n - 1, n & 1);
     do_pv(n - 1, n & 1);
   }
   // The key streams' parts become one.  A wave keeps 4 / KS of its four blocks of dims, gives the others away

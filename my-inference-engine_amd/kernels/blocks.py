@@ -117,6 +117,12 @@ def _table(tables, device):
     return tables.data_ptr(), stride, tables.shape[1]
 
 
+def _parts(n, planes, size, rows=0):
+    """Slices of n blocks, a launch each: 2^23 work-groups of 16 KB at most."""
+    most = max(1, ((1 << 23) - rows) // (planes * -(-size // 16384)) - 2)
+    return [slice(i, min(n, i + most)) for i in range(0, max(n, 1), most)]
+
+
 def copy_blocks(src_pool, dst_pool, pairs, block_size):
     """dst_pool's block pairs[i, 1] = src_pool's block pairs[i, 0], in every plane; returns dst_pool.
 
@@ -133,9 +139,10 @@ def copy_blocks(src_pool, dst_pool, pairs, block_size):
     if size == 0 or planes == 0 or pairs.shape[0] == 0:
         return dst_pool
     with _lib.on_device(src_pool.device) as stream:
-        check(load().mi_cache_copy_blocks(
-            src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), dst_step, dst_blocks,
-            planes, size, ids, pairs.shape[0], stream))
+        for part in _parts(pairs.shape[0], planes, size):
+            check(load().mi_cache_copy_blocks(
+                src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), dst_step, dst_blocks,
+                planes, size, ids + 8 * part.start, part.stop - part.start, stream))
     return dst_pool
 
 
@@ -176,7 +183,10 @@ def move_blocks(pool, tables, rows, pairs, new_ids, block_size):
     ip = _ids(new_ids, "new_ids", (blocks,), pool.device)
     if pairs.shape[0] == 0 and rows.shape[0] == 0:
         return
+    n_rows = rows.shape[0]
     with _lib.on_device(pool.device) as stream:
-        check(load().mi_cache_move_blocks(
-            pool.data_ptr(), step, blocks, planes, size, pp, pairs.shape[0], t, stride, width,
-            tables.shape[0], rp, rows.shape[0], ip, stream))
+        for part in _parts(pairs.shape[0], planes, size, n_rows):
+            check(load().mi_cache_move_blocks(
+                pool.data_ptr(), step, blocks, planes, size, pp + 8 * part.start,
+                part.stop - part.start, t, stride, width, tables.shape[0], rp,
+                n_rows if part.start == 0 else 0, ip, stream))
