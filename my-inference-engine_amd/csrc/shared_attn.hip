@@ -384,20 +384,19 @@ __device__ __forceinline__ void scores_of(const uint8_t* k, int lane, const u32x
   }
 }
 
-// O += P V of N blocks of 32 keys in LDS.  V's operands are read two k-steps ahead, those of the first two
-// (begin) before the softmax or scores that come in between, so that their way is hidden.
+// O += P V of N blocks of 32 keys in LDS.  V's operands are read a k-step ahead, those of the first (begin)
+// before the softmax or scores that come in between.
 template <typename E, int N>
 struct ShPv {
-  u32x4 va[3][4];
+  u32x4 va[2][4];
 
   __device__ __forceinline__ void read(const uint8_t* v, int lane, int i) {
 #pragma unroll
     for (int db = 0; db < 4; ++db)
-      va[i % 3][db] = read_v(v + (i >> 1) * kShStep * kShRow, lane, i & 1, db);
+      va[i & 1][db] = read_v(v + (i >> 1) * kShStep * kShRow, lane, i & 1, db);
   }
   __device__ __forceinline__ void begin(const uint8_t* v, int lane) {
     read(v, lane, 0);
-    read(v, lane, 1);
     __builtin_amdgcn_sched_barrier(0);
   }
   template <typename F>
@@ -405,9 +404,9 @@ struct ShPv {
                                       F&& between) {
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) {
-      if (i + 2 < 2 * N) read(v, lane, i + 2);
+      if (i + 1 < 2 * N) read(v, lane, i + 1);
 #pragma unroll
-      for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i % 3][db], pb[i], st.o[db]);
+      for (int db = 0; db < 4; ++db) st.o[db] = E::mfma32(va[i & 1][db], pb[i], st.o[db]);
 #pragma unroll
       for (int j = 0; j < 2 / N; ++j) between(i * (2 / N) + j);
       __builtin_amdgcn_sched_barrier(0);
@@ -883,7 +882,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   const int W1 = min(W - W3, N1);
 
   if ((int)blockIdx.x < W1) {
-    const int wg = blockIdx.x;
+    // work-group w runs on XCD w % 8: XCD x takes the x-th contiguous share of the work, so that tiles of one
+    // range meet in its L2
+    const int x = blockIdx.x & 7, wg = x * (W1 >> 3) + min(x, W1 & 7) + ((int)blockIdx.x >> 3);
     const ShDeal deal = make_deal(N1, W1);
     int u = first_of(deal, wg);
     const int stop = first_of(deal, wg + 1);
