@@ -25,6 +25,8 @@ of its own: its tokens join the tick's decode step as one more row of a packed m
 several prompts may be admitted per tick, up to max_step_tokens prompt tokens (one prompt is always
 admitted, however long, as the reference's un-chunked prefill is).
 
+fork() makes conversations that go on from another's history, which they share in the cache.
+
 Tokenizer, stop sequences, streaming listeners and the web UI are outside the attention path and
 not rebuilt; conversations carry token ids.
 """
@@ -86,6 +88,33 @@ class Engine:
                   t_submit=time.perf_counter())
         self.queue.append(job)
         return job
+
+    def fork(self, conv, n=1):
+        """n new conversations that go on from where conv is: a message to each, or none (submit(fork,
+        []) samples another continuation of the same history).
+
+        What conv holds in the cache they share (KVCache.fork), all but the history's last token, whose
+        logits their first sample needs, provided that blocks and sequence slots for them can be had by
+        evicting idle conversations; otherwise they start without cache, and their first prompt
+        is their whole history."""
+        forks = [Conversation(ids=list(conv.ids), eos_id=conv.eos_id) for _ in range(n)]
+        if conv.seq is not None and n > 0:
+            held = min(self.cache.length(conv.seq), len(conv.ids) - 1)
+            blocks = n if held % self.cache.block_size else 0
+            busy = {id(j.conv) for j in self.active} | {id(conv)}
+
+            def short():
+                return (self.cache.free_block_count() < blocks
+                        or self.cache.free_slot_count() < n)
+            while short():
+                idle = [c for c in self.resident if id(c) not in busy]
+                if not idle:
+                    return forks
+                self._evict(idle[0])
+            for child, seq in zip(forks, self.cache.fork(conv.seq, n, held)):
+                child.seq = seq
+                self._touch(child)
+        return forks
 
     def release(self, conv):
         """Free a conversation's blocks now (chat.py:325-330)."""
@@ -157,8 +186,8 @@ class Engine:
         raise RuntimeError("scheduler did not drain")
 
     def _fits_after_eviction(self, job):
-        idle_blocks = sum(len(self.cache._block_tables[c.seq]) for c in self.resident
-                          if c.seq is not None and c is not job.conv)
+        idle_blocks = self.cache.reclaimable([c.seq for c in self.resident
+                                              if c.seq is not None and c is not job.conv])
         need = self.cache.blocks_needed(job.conv.seq, self._reserve_len(job))
         return need <= self.cache.free_block_count() + idle_blocks
 
@@ -256,6 +285,9 @@ class Engine:
         if not continuing:
             return
         seqs = [j.conv.seq for j in continuing]
+        # forks beside what they were forked from: a step reads the blocks they share once
+        continuing = [continuing[i] for i in self.cache.order(seqs)]
+        seqs = [j.conv.seq for j in continuing]
         graphs = self.decode_graphs
         if graphs is not None and len(seqs) <= graphs.max_rows:
             last = graphs.run(seqs, [j.next_token for j in continuing])
@@ -268,6 +300,8 @@ class Engine:
 
     def _step_mixed(self, continuing, prompts):
         """One packed step: the decode rows first (one token each), then the admitted prompts."""
+        continuing, prompts = ([jobs[i] for i in self.cache.order([j.conv.seq for j in jobs])]
+                               for jobs in (continuing, prompts))
         jobs = continuing + prompts
         rows = [[j.next_token] for j in continuing] + [j.prefill for j in prompts]
         with torch.no_grad():

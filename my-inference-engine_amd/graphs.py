@@ -17,12 +17,16 @@ Either way W = the most blocks one sequence may hold, so any sequence fits and t
 kernel's grid and workspace (sized for W*block_size keys) never change: its work split follows the
 actual kv_lens on the device.  A batch smaller than its bucket is padded with empty rows (slot -1: no keys,
 nothing written to the cache, zeros from attention), whose logits are ignored.
+
+Steps whose rows share enough of their blocks (KVCache.shared_groups, device tables only) replay
+another graph of the bucket, whose attention reads them once; which rows share what comes up with the
+slots and ids.  It is captured when the first such step comes.
 """
 import numpy as np
 import torch
 
 from kernels.meta import step_metadata
-from kv_cache import StepMeta
+from kv_cache import SharedRows, StepMeta
 
 
 class DecodeGraphs:
@@ -33,6 +37,7 @@ class DecodeGraphs:
         self.W = cache.max_blocks_per_seq
         self.buckets = sorted(buckets)
         self.graphs = {}
+        self.shared_graphs = {}     # by bucket, as they are needed
         # One capture stream for all buckets, alive as long as the graphs: the kernels' workspace
         # is kept per stream, and a stream handle recycled by torch's pool while these graphs
         # exist would hand their workspace to unrelated calls.
@@ -50,28 +55,36 @@ class DecodeGraphs:
                 return b
         raise ValueError(f"batch of {n} rows is larger than the largest captured bucket")
 
-    def _capture(self, rows):
+    def _capture(self, rows, shared=False):
         dev, W, bs = self.cache.device, self.W, self.cache.block_size
         cache = self.cache
         if cache.device_tables:
-            inp = torch.zeros(2 * rows, dtype=torch.int32, device=dev)   # [row slots | ids]
+            # [row slots | ids], and where rows share [cu_rows | prefix lengths]
+            n_in = 4 * rows + 1 if shared else 2 * rows
+            inp = torch.zeros(n_in, dtype=torch.int32, device=dev)
             inp[:rows] = -1                  # padding rows: nothing advances while warming up
-            row_slots, ids_dev = inp[:rows], inp[rows:].view(rows, 1)
+            row_slots, ids_dev = inp[:rows], inp[rows:2 * rows].view(rows, 1)
+            groups = None
+            if shared:
+                groups = SharedRows(rows=rows, cu_q=torch.arange(rows + 1, dtype=torch.int32,
+                                                            device=dev),
+                                    cu_rows=inp[2 * rows:3 * rows + 1],
+                                    prefix_lens=inp[3 * rows + 1:], max_q=1)
             out = torch.zeros(2 * rows + rows * W + rows, dtype=torch.int32, device=dev)
             meta = StepMeta(starts=None, T=1, block_size=bs, starts_dev=out[:rows],
                             kv_lens=out[rows:2 * rows],
                             block_table=out[2 * rows:2 * rows + rows * W].view(rows, W),
                             slot_mapping=None, slot_mapping32=out[2 * rows + rows * W:],
-                            kv_cap=W * bs)
+                            kv_cap=W * bs, shared=groups)
 
             def step():
                 step_metadata(cache, row_slots, None, 1, meta.starts_dev, meta.kv_lens,
                               meta.block_table, meta.slot_mapping32)
                 return self.model.forward_meta(ids_dev, cache, meta)
-            host = torch.zeros(2 * rows, dtype=torch.int32).pin_memory()
+            host = torch.zeros(n_in, dtype=torch.int32).pin_memory()
             # `out` is written by every replay: it lives as long as the graph (it was allocated
             # before the capture, so the graph's own memory pool does not hold it)
-            bufs = (inp, host, out)
+            bufs = (inp, host, out, groups)
         else:
             n_meta = 2 * rows + rows * W + rows
             meta_dev = torch.zeros(n_meta, dtype=torch.int32, device=dev)
@@ -97,7 +110,8 @@ class DecodeGraphs:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph), torch.no_grad():
             logits = step()
-        self.graphs[rows] = (graph, logits, bufs, torch.cuda.Event())
+        kept = self.shared_graphs if shared else self.graphs
+        kept[rows] = (graph, logits, bufs, torch.cuda.Event())
 
     def run(self, seqs, tokens):
         """One decode step for cache sequences `seqs` fed `tokens` (one id per row); returns the
@@ -105,12 +119,15 @@ class DecodeGraphs:
         replay of the same bucket)."""
         n = len(seqs)
         rows = self._bucket(n)
-        graph, logits, bufs, copied = self.graphs[rows]
-        copied.synchronize()             # the previous upload from these host buffers is done
         cache = self.cache
+        groups = cache.shared_groups(seqs) if cache.device_tables else None
+        if groups is not None and rows not in self.shared_graphs:
+            self._capture(rows, shared=True)
+        graph, logits, bufs, copied = (self.graphs if groups is None else self.shared_graphs)[rows]
+        copied.synchronize()             # the previous upload from these host buffers is done
         if cache.device_tables:
             assert len(set(seqs)) == n, "a sequence may appear once per step"
-            inp, host, _ = bufs
+            inp, host = bufs[:2]
             for s in seqs:
                 cache.ensure_capacity(s, cache.length(s) + 1)
             h = host.numpy()
@@ -118,6 +135,11 @@ class DecodeGraphs:
             h[n:rows] = -1
             h[rows:rows + n] = tokens
             h[rows + n:] = 0
+            if groups is not None:
+                cu, prefix = groups
+                h[2 * rows:3 * rows + 1] = n                  # groups that are not there: empty
+                h[2 * rows:2 * rows + len(cu)] = cu
+                h[3 * rows + 1:3 * rows + 1 + len(prefix)] = prefix
             inp.copy_(host, non_blocking=True)
         else:
             meta_dev, ids_dev, host_meta, host_ids = bufs

@@ -32,12 +32,30 @@ prepare_packed() builds the metadata of a mixed step, where each row appends its
 tokens (one for a decoding chat, a whole prompt for a newly admitted one) and the rows' tokens are
 packed back to back: prefix offsets cu_q, every token's position and slot, and each row's last
 token (whose logits are sampled).
+
+Beyond the reference, blocks can have several holders: fork() makes sequences over another's history
+that share its whole blocks (a count per block says when it is free again), copy_from() brings a
+sequence over from another cache and compact() moves the blocks in use together.  A step whose rows
+share enough carries which rows share what (SharedRows), and its attention reads the shared blocks
+once (kernels.shared).
 """
 import math
+import operator
+from collections import Counter
 from dataclasses import dataclass, field
 
 import numpy as np
 import torch
+
+
+@dataclass
+class SharedRows:
+    """Which of a step's first `rows` rows hold the same first blocks: kernels.shared's arguments."""
+    rows: int
+    cu_q: torch.Tensor           # [rows+1] int32: prefix offsets of their new tokens
+    cu_rows: torch.Tensor        # [G+1] int32: rows [cu_rows[g], cu_rows[g+1]) share
+    prefix_lens: torch.Tensor    # [G] int32: this many tokens
+    max_q: int                   # new tokens of a row, at most
 
 
 @dataclass
@@ -53,6 +71,7 @@ class StepMeta:
     slot_mapping32: torch.Tensor = None  # the same slots as int32 (for the fused RoPE + write)
     tables: list = field(default_factory=list)  # host copies of the rows' block lists
     kv_cap: int = None           # fixed upper bound of kv_lens (captured decode graphs)
+    shared: SharedRows = None    # None: no rows that share enough
     packed = False
 
     @property
@@ -82,12 +101,13 @@ class PackedMeta:
     last_idx: torch.Tensor       # [B] int32: packed index of each row's last token
     block_table: torch.Tensor    # [B, W] int32
     tables: list = field(default_factory=list)
+    shared: SharedRows = None    # None: no rows that share enough
     packed = True
 
-    def split(self):
-        """(max kv_len of the leading one-token rows, of the other rows, max new tokens of the
-        other rows): the host bounds each attention launch is sized by."""
-        D = self.n_single
+    def split(self, D=None):
+        """(max kv_len of the leading D rows (default: the one-token rows), of the other rows, max
+        new tokens of the other rows): the host bounds each attention launch is sized by."""
+        D = self.n_single if D is None else D
         kv = [s + c for s, c in zip(self.starts, self.counts)]
         return (max(kv[:D], default=0), max(kv[D:], default=0), max(self.counts[D:], default=0))
 
@@ -104,10 +124,37 @@ class PackedMeta:
         return self.slot_mapping32.long()
 
 
+def _common(a, b):
+    """Leading blocks that two tables have in common: they share those of a fork and none after, so the
+    last one is found by halving."""
+    lo, hi = 0, min(len(a), len(b))
+    if not hi or a[0] != b[0]:
+        return 0
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if a[mid - 1] == b[mid - 1]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
+
+
 class KVCache:
     # Default cap of one sequence's length: Qwen2.5's context window.
     DEFAULT_MAX_TOKENS_PER_SEQ = 32768
     DEFAULT_MAX_SEQS = 4096
+    # K and V bytes that a step would read again in a layer, from which its attention reads the
+    # shared blocks once; with less to save the plain kernels' smaller fixed cost wins.  One new
+    # token, us shared / plain: 16 rows over 1,024 shared keys of 2 heads (15 MB) 14.6 / 12.2, over 2,048
+    # (30 MB) 14.9 / 15.3; 4 rows over 8,192 keys of 4 heads (48 MB) 22.6 / 19.9, over 4,096 of 8
+    # heads (48 MB) 18.0 / 20.5; 8 rows over 4,096 of 4 (56 MB) 15.7 / 20.1; 64 rows over 1,024 of 8
+    # (252 MB) 23.3 / 35.3; 64 rows over 31,000 of 2 (1.9 GB) 39 / 279.
+    SHARED_BYTES = 48 << 20
+    # New tokens of a row up to which that holds: with more, its own tiles are full and the work is
+    # bound by the matrix products (8 rows over 4,096 keys of 8 heads: 8 new tokens 30 / 54, 32 47 / 55,
+    # 64 68 / 57).
+    SHARED_MAX_NEW = 32
+    SHARED_MAX_ROWS = 512     # rows of a call of the kernel
 
     def __init__(self, num_blocks, block_size, device, dtype, num_layers, num_kv_heads, head_dim,
                  *, device_tables=None, max_seqs=None, max_blocks_per_seq=None):
@@ -120,6 +167,9 @@ class KVCache:
         self._block_tables = {}   # seq id -> list of block ids, in logical order
         self._lengths = {}        # seq id -> tokens written so far
         self._next_seq = 0
+        self._holders = [0] * num_blocks   # sequences that hold each block
+        self._extra = 0                    # holders beyond a block's first, over all blocks
+        self._path = {}                    # seq id -> its place among its forks (see order)
         self.device_tables = self.device.type == "cuda" if device_tables is None else device_tables
         # Blocks one sequence may hold.  With device tables this is the width of a table row: the
         # pool, capped at the default context length, so the tables do not grow with the square
@@ -156,22 +206,43 @@ class KVCache:
         return max(0, math.ceil(total_len / self.block_size) - held)
 
     def alloc(self):
+        seq = self._new_seq()
+        if self.device_tables:
+            slot = self.slot[seq]
+            self.dev_lens[slot:slot + 1].zero_()
+        return seq
+
+    def _new_seq(self):
         if not self._free_slots:
             raise RuntimeError(f"all {self.max_seqs} sequence slots are in use")
-        slot = self._free_slots.pop()
         seq = self._next_seq
         self._next_seq += 1
         self._block_tables[seq] = []
         self._lengths[seq] = 0
-        self.slot[seq] = slot
-        if self.device_tables:
-            self.dev_lens[slot:slot + 1].zero_()
+        self.slot[seq] = self._free_slots.pop()
+        self._path[seq] = (seq,)
         return seq
 
     def free(self, seq):
-        self._free_blocks.extend(self._block_tables.pop(seq))
-        del self._lengths[seq]
+        self._release(self._block_tables.pop(seq))
+        del self._lengths[seq], self._path[seq]
         self._free_slots.append(self.slot.pop(seq))
+
+    def _take(self, n):
+        """n free blocks, now held once each."""
+        blocks = [self._free_blocks.pop() for _ in range(n)]
+        for b in blocks:
+            self._holders[b] = 1
+        return blocks
+
+    def _release(self, blocks):
+        """One holder fewer for each; free again are those without."""
+        for b in blocks:
+            self._holders[b] -= 1
+            if self._holders[b] == 0:
+                self._free_blocks.append(b)
+            else:
+                self._extra -= 1
 
     def length(self, seq):
         return self._lengths[seq]
@@ -186,8 +257,7 @@ class KVCache:
                                f"a sequence holds at most {self.max_blocks_per_seq}")
         table = self._block_tables[seq]
         old = len(table)
-        for _ in range(need):
-            table.append(self._free_blocks.pop())
+        table.extend(self._take(need))
         if self.device_tables and need:
             new = torch.tensor(table[old:], dtype=torch.int32)
             self.dev_tables[self.slot[seq], old:old + need].copy_(new)
@@ -195,8 +265,174 @@ class KVCache:
     def trim(self, seq):
         table = self._block_tables[seq]
         keep = math.ceil(self._lengths[seq] / self.block_size)
-        self._free_blocks.extend(table[keep:])
+        self._release(table[keep:])
         del table[keep:]
+
+    # -- blocks with several holders (no counterpart in the reference) ----------------------------
+    def fork(self, seq, n=1, length=None):
+        """n new sequences that begin with the first `length` tokens of seq (default: all it holds).
+
+        They share its whole blocks and get a copy of the one that is only started, so that each
+        writes its next tokens into a block of its own: one launch over all layers.  Returns their
+        ids.  Raises before anything changes if blocks or sequence slots are short."""
+        length = self._lengths[seq] if length is None else operator.index(length)
+        if not 0 <= length <= self._lengths[seq]:
+            raise ValueError(f"seq {seq} holds {self._lengths[seq]} tokens, not {length}")
+        n, bs, table = operator.index(n), self.block_size, self._block_tables[seq]
+        whole, rest = divmod(length, bs)
+        need = n if rest else 0
+        if n < 1:
+            raise ValueError(f"{n} forks")
+        if need > len(self._free_blocks):
+            raise RuntimeError(f"KV cache exhausted: {n} forks of seq {seq} need {need} blocks, "
+                               f"only {len(self._free_blocks)} free")
+        if n > len(self._free_slots):
+            raise RuntimeError(f"{n} forks of seq {seq}: only {len(self._free_slots)} of "
+                               f"{self.max_seqs} sequence slots are free")
+        fresh = self._take(need)
+        forks = []
+        for i in range(n):
+            child = self._new_seq()
+            self._path[child] = self._path[seq] + (child,)
+            self._block_tables[child] = table[:whole] + fresh[i:i + 1]
+            self._lengths[child] = length
+            forks.append(child)
+        for b in table[:whole]:
+            self._holders[b] += n
+        self._extra += n * whole
+        if self.device_tables:
+            from kernels.blocks import fork_rows
+            slot = self.slot[seq]
+            rows = [[slot, self.slot[c], length, fresh[i] if rest else -1]
+                    for i, c in enumerate(forks)]
+            fork_rows(self.buf, self.dev_tables, self.dev_lens, self._upload(rows).view(n, 4), bs)
+        elif rest:
+            self._copy([(table[whole], b) for b in fresh])
+        return forks
+
+    def copy_from(self, other, seq):
+        """A new sequence holding what `seq` of another cache (of the same layers, heads, dtype,
+        block size and device) holds; returns its id."""
+        if self.buf.shape[:2] != other.buf.shape[:2] or self.buf.shape[3:] != other.buf.shape[3:] or (
+                self.buf.dtype, self.buf.device, self.block_size) != (
+                other.buf.dtype, other.buf.device, other.block_size):
+            raise ValueError("copy_from needs caches of one layout, dtype, block size and device")
+        length = other._lengths[seq]
+        mine = self.alloc()
+        try:
+            self.ensure_capacity(mine, length)
+        except RuntimeError:
+            self.free(mine)
+            raise
+        self._lengths[mine] = length
+        self._copy(list(zip(other._block_tables[seq], self._block_tables[mine])), other)
+        if self.device_tables:
+            slot = self.slot[mine]
+            self.dev_lens[slot:slot + 1].fill_(length)
+        return mine
+
+    def compact(self):
+        """Move the blocks in use to the lowest ids, 0 .. n - 1, and return n: buf[:, :, :n *
+        block_size] then holds every sequence.  One launch; the next blocks handed out follow them."""
+        used = sum(h > 0 for h in self._holders)
+        src = [b for b in range(used, self.num_blocks) if self._holders[b]]
+        dst = [b for b in range(used) if not self._holders[b]]
+        new_ids = list(range(self.num_blocks))
+        for a, b in zip(src, dst):
+            new_ids[a] = b
+            self._holders[b], self._holders[a] = self._holders[a], 0
+        self._free_blocks = list(range(self.num_blocks - 1, used - 1, -1))
+        if not src:
+            return used
+        for table in self._block_tables.values():
+            table[:] = [new_ids[b] for b in table]
+        pairs = list(zip(src, dst))
+        if self.device_tables:
+            from kernels.blocks import move_blocks
+            rows = [(self.slot[s], len(t)) for s, t in self._block_tables.items() if t]
+            ids = self._upload(pairs + rows, new_ids)
+            n, m = 2 * len(pairs), 2 * (len(pairs) + len(rows))
+            move_blocks(self.buf, self.dev_tables, ids[n:m].view(-1, 2), ids[:n].view(-1, 2), ids[m:],
+                        self.block_size)
+        else:
+            self._copy(pairs)
+        return used
+
+    def reclaimable(self, seqs):
+        """Blocks that freeing all of `seqs` would give back: those that no other sequence holds."""
+        held = Counter(b for s in seqs for b in self._block_tables[s])
+        return sum(self._holders[b] == n for b, n in held.items())
+
+    def order(self, seqs):
+        """Indices that put sequences which share blocks next to each other: forks after what they
+        were forked from.  Sequences that share nothing keep their order."""
+        if not self._extra:
+            return list(range(len(seqs)))
+        first = {}
+        for i, s in enumerate(seqs):
+            first.setdefault(self._path[s][0], i)
+        return sorted(range(len(seqs)), key=lambda i: (first[self._path[seqs[i]][0]],
+                                                       self._path[seqs[i]]))
+
+    def shared_groups(self, seqs):
+        """(cu_rows, prefix tokens) of neighbouring rows that hold the same first blocks, or None if a
+        step over these rows would gain too little by reading them once."""
+        if not self._extra or not 2 <= len(seqs) <= self.SHARED_MAX_ROWS:
+            return None
+        cu, prefix, saved = [0], [], 0
+        rows, blocks = 1, 0       # of the group being formed
+        tables = [self._block_tables[s] for s in seqs]
+        for a, b in zip(tables, tables[1:]):
+            same = _common(a, b)
+            joined = min(same, blocks) if rows > 1 else same
+            # one more row, at the price of a shorter prefix for all
+            if joined and rows * joined >= (rows - 1) * blocks:
+                rows, blocks = rows + 1, joined
+                continue
+            saved += (rows - 1) * blocks
+            cu.append(cu[-1] + rows)
+            prefix.append(blocks * self.block_size)
+            rows, blocks = 1, 0
+        saved += (rows - 1) * blocks
+        cu.append(cu[-1] + rows)
+        prefix.append(blocks * self.block_size)
+        block = 2 * self.block_size * self.buf.shape[3] * self.buf.shape[4] * self.buf.element_size()
+        return (cu, prefix) if saved * block >= self.SHARED_BYTES else None
+
+    def _shared_rows(self, seqs, counts, cu_q=None):
+        """The SharedRows of a step over `seqs`, or None; cu_q if they are on the device already."""
+        if not self._extra or self.device.type != "cuda":
+            return None
+        rows = 0      # the leading ones with few new tokens
+        while rows < len(seqs) and counts[rows] <= self.SHARED_MAX_NEW:
+            rows += 1
+        groups = self.shared_groups(seqs[:rows])
+        if groups is None:
+            return None
+        cu, prefix = groups
+        g = len(prefix)
+        offsets = [] if cu_q is not None else np.concatenate([[0], np.cumsum(counts[:rows])])
+        up = self._upload(cu, prefix, offsets)
+        return SharedRows(rows=rows, cu_q=up[2 * g + 1:] if cu_q is None else cu_q[:rows + 1],
+                          cu_rows=up[:g + 1], prefix_lens=up[g + 1:2 * g + 1], max_q=max(counts[:rows]))
+
+    def _upload(self, *parts):
+        """Lists of numbers (or of rows of them) as one flat int32 tensor on the device."""
+        host = np.concatenate([np.asarray(p, dtype=np.int32).reshape(-1) for p in parts])
+        return torch.from_numpy(host).pin_memory().to(self.device, non_blocking=True)
+
+    def _copy(self, pairs, source=None):
+        """Whole blocks, (from, to), in every layer; from another cache's buffer if given."""
+        src = (source or self).buf
+        if not pairs:
+            return
+        if self.device.type == "cuda":
+            from kernels.blocks import copy_blocks
+            copy_blocks(src, self.buf, self._upload(pairs).view(-1, 2), self.block_size)
+            return
+        at = torch.arange(self.block_size)
+        a, b = ((torch.tensor(ids)[:, None] * self.block_size + at).reshape(-1) for ids in zip(*pairs))
+        self.buf[:, :, b] = src[:, :, a]
 
     def advance(self, seqs, T):
         """Count T new tokens (an int, or one count per row) as written."""
@@ -253,7 +489,7 @@ class KVCache:
             block_table=dev[2 * B:2 * B + B * W].view(B, W),
             slot_mapping=dev[2 * B + B * W:].long(),
             slot_mapping32=dev[2 * B + B * W:],
-            tables=[list(t) for t in tables])
+            tables=[list(t) for t in tables], shared=self._shared_rows(seqs, [T] * B))
 
     def prepare_packed(self, seqs, counts):
         """Grow the rows' tables for counts[b] new tokens each and build a PackedMeta with one
@@ -297,7 +533,8 @@ class KVCache:
             starts=starts, counts=list(counts), block_size=bs, n_single=n_single,
             cu_q=dev[:B + 1], kv_lens=dev[B + 1:2 * B + 1], positions=dev[o:o + N],
             slot_mapping32=dev[o + N:o + 2 * N], last_idx=dev[o + 2 * N:o + 2 * N + B],
-            block_table=dev[o + 2 * N + B:].view(B, W), tables=[list(t) for t in tables])
+            block_table=dev[o + 2 * N + B:].view(B, W), tables=[list(t) for t in tables],
+            shared=self._shared_rows(seqs, counts, dev[:B + 1]))
 
     def _prepare_device(self, seqs, counts, packed):
         """The device-table path of prepare / prepare_packed: one pinned copy of the rows' slots
@@ -327,13 +564,15 @@ class KVCache:
         if not packed:
             return StepMeta(starts=starts, T=counts[0], block_size=bs, starts_dev=o_starts,
                             kv_lens=o_kv, slot_mapping=None, block_table=o_bt,
-                            slot_mapping32=o_slots, tables=tables)
+                            slot_mapping32=o_slots, tables=tables,
+                            shared=self._shared_rows(seqs, counts))
         n_single = 0
         while n_single < B and counts[n_single] == 1:
             n_single += 1
         return PackedMeta(starts=starts, counts=list(counts), block_size=bs, n_single=n_single,
                           cu_q=cu, kv_lens=o_kv, positions=o_pos, slot_mapping32=o_slots,
-                          last_idx=o_last, block_table=o_bt, tables=tables)
+                          last_idx=o_last, block_table=o_bt, tables=tables,
+                          shared=self._shared_rows(seqs, counts, cu))
 
     # -- data movement --------------------------------------------------------------------------
     def k_pool(self, layer):

@@ -29,6 +29,9 @@ one-token rows and to the paged varlen prefill kernel for the prompt rows, and o
 token reaches the logits.  The reference runs each admitted prompt as a forward of its own
 (chat.py:157-185, one per tick, chat.py:247-253) beside the batched decode step.
 
+Rows that share the blocks of one history (KVCache.fork), a step's metadata says which, go to
+kernels.shared.fa2_paged_shared, which reads the shared blocks once.
+
 On CPU tensors the model takes the reference's own fallback (dense read + fp32 SDPA with the
 bottom-right mask, model.py:104-107,181-195), which only the CPU tests of the scheduler use; the
 attention kernels themselves have no CPU path.
@@ -44,6 +47,7 @@ from kernels import few_rows
 from kernels.fa2 import fa2_paged, fa2_paged_varlen
 from kernels.model_ops import add_rmsnorm, silu_mul
 from kernels.rope import rope_kv_write
+from kernels.shared import fa2_paged_shared
 
 
 @dataclass(frozen=True)
@@ -189,6 +193,14 @@ class Attention(nn.Module):
         if meta.packed:
             out = self._attend_packed(q.view(B * T, cfg.num_heads, cfg.head_dim), cache, layer, meta)
             return out.view(B, T, self.q_size)
+        if meta.shared is not None:
+            # rows over one history (KVCache.fork): its blocks are read once for all of them
+            sh = meta.shared
+            out = fa2_paged_shared(
+                q.view(B * T, cfg.num_heads, cfg.head_dim), cache.k_pool(layer), cache.v_pool(layer),
+                sh.cu_q, meta.block_table, meta.kv_lens, sh.max_q, sh.cu_rows, sh.prefix_lens,
+                block_size=cache.block_size, max_kv_len=meta.max_kv)
+            return out.view(B, T, self.q_size)
         q = q.view(B, T, cfg.num_heads, cfg.head_dim).transpose(1, 2)
         out = fa2_paged(q, cache.k_pool(layer), cache.v_pool(layer), meta.block_table,
                         meta.kv_lens, block_size=cache.block_size, max_kv_len=meta.max_kv,
@@ -218,13 +230,20 @@ class Attention(nn.Module):
 
     def _attend_packed(self, q, cache, layer, meta):
         """q [N, Hq, d] packed queries of a mixed step -> [N, Hq, d]: the leading one-token rows
-        through the paged decode kernel, the rest through the paged varlen prefill kernel, both
-        writing into one packed output."""
+        through the paged decode kernel (or, where rows share blocks, the leading rows through the
+        shared kernel), the rest through the paged varlen prefill kernel, both writing into one
+        packed output."""
         out = torch.empty_like(q)
-        D, B, bs = meta.n_single, len(meta.counts), cache.block_size
-        kv_single, kv_multi, q_multi = meta.split()
+        sh = meta.shared
+        D, B, bs = meta.n_single if sh is None else sh.rows, len(meta.counts), cache.block_size
+        kv_single, kv_multi, q_multi = meta.split(D)
         kp, vp = cache.k_pool(layer), cache.v_pool(layer)
-        if D:
+        if sh is not None:
+            n = sum(meta.counts[:D])
+            fa2_paged_shared(q[:n], kp, vp, sh.cu_q, meta.block_table[:D], meta.kv_lens[:D], sh.max_q,
+                             sh.cu_rows, sh.prefix_lens, block_size=bs, max_kv_len=kv_single,
+                             out=out[:n])
+        elif D:
             fa2_paged(q[:D].unsqueeze(2), kp, vp, meta.block_table[:D], meta.kv_lens[:D],
                       block_size=bs, max_kv_len=kv_single, is_causal=False,
                       out=out[:D].unsqueeze(2))
