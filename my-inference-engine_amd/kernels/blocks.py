@@ -62,22 +62,31 @@ def check(status):
             f"libmi_cache status {status}: {load().mi_cache_last_error().decode()}")
 
 
-_POOLS = {}
+_PLANS = {}   # per entry point and its arguments' shapes, strides, types and devices: what to launch
 
 
-def _planes(pool, name, block_size):
-    """(planes, bytes between them, blocks, bytes of a block) of a pool [..., slots, kv_heads, d].  The
-    checks that its shape, strides and type decide run once per combination."""
-    key = (pool.shape, pool.stride(), pool.dtype, pool.device, block_size)
-    got = _POOLS.get(key)
-    if got is None or type(block_size) is not int:   # (16.0 would find 16's)
-        if len(_POOLS) >= _MEMO_MAX:
-            _POOLS.clear()
-        got = _POOLS[key] = _check_planes(pool, name, block_size)
+def _plan(key, make, *args):
+    """make(*args), which runs every check that those decide, once per combination."""
+    if len(_PLANS) >= _MEMO_MAX:
+        _PLANS.clear()
+    got = _PLANS[key] = make(*args)
     return got
 
 
-def _check_planes(pool, name, block_size):
+def _call(device, fn, *args):
+    """fn(*args, stream) on the device's current stream."""
+    if device == _current():
+        check(fn(*args, _stream(device)))
+        return
+    with _lib.on_device(torch.device("cuda", device)) as stream:
+        check(fn(*args, stream))
+
+
+_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _planes(pool, name, block_size):
+    """(planes, bytes between them, blocks, bytes of a block) of a pool [..., slots, kv_heads, d]."""
     assert pool.is_cuda, f"{name}: a GPU tensor"
     assert pool.dim() >= 3, f"{name}: [..., slots, kv_heads, d]"
     slots, heads, d = pool.shape[-3:]
@@ -101,26 +110,26 @@ def _check_planes(pool, name, block_size):
 
 
 def _ids(t, name, shape, device):
-    """The pointer of a contiguous int32 tensor of that shape (its first entry None: any)."""
+    """A contiguous int32 tensor of that shape (its first entry None: any)."""
     got = t.shape
-    if not (t.dtype == torch.int32 and len(got) == len(shape) and got[1:] == shape[1:]
-            and shape[0] in (None, got[0]) and t.is_contiguous() and t.device == device):
-        raise AssertionError(f"{name}: contiguous int32 of shape {shape} on {device}")
-    return t.data_ptr()
+    assert (t.dtype == torch.int32 and len(got) == len(shape) and got[1:] == shape[1:]
+            and shape[0] in (None, got[0]) and t.is_contiguous() and t.device == device), \
+        f"{name}: contiguous int32 of shape {shape} on {device}"
 
 
 def _table(tables, device):
+    """(entries between rows, entries of a row, rows)."""
     assert tables.device == device and tables.dtype == torch.int32 and tables.dim() == 2, \
         f"tables: [max_seqs, width] int32 on {device}"
     assert tables.stride(1) == 1 or tables.shape[1] <= 1, "tables: rows must be contiguous"
     stride = tables.stride(0) if tables.shape[0] > 1 else tables.shape[1]
-    return tables.data_ptr(), stride, tables.shape[1]
+    return stride, tables.shape[1], tables.shape[0]
 
 
 def _parts(n, planes, size, rows=0):
-    """Slices of n blocks, a launch each: 2^23 work-groups of 16 KB at most."""
+    """(first, count) of n blocks, a launch each: 2^23 work-groups of 16 KB at most."""
     most = max(1, ((1 << 23) - rows) // (planes * -(-size // 16384)) - 2)
-    return [slice(i, min(n, i + most)) for i in range(0, max(n, 1), most)]
+    return [(i, min(n, i + most) - i) for i in range(0, max(n, 1), most)]
 
 
 def copy_blocks(src_pool, dst_pool, pairs, block_size):
@@ -129,21 +138,31 @@ def copy_blocks(src_pool, dst_pool, pairs, block_size):
     pairs [n, 2] int32 on the pools' device.  The pools have the same planes, kv_heads, d and dtype,
     their own numbers of blocks, and may be one pool.  No block may be written twice, nor (in one
     pool) be both read and written.  Pairs outside the pools are skipped."""
+    assert type(block_size) is int, "block_size: a positive int"   # (16.0 would find 16's plan)
+    key = ("copy", block_size, src_pool.shape, src_pool.stride(), src_pool.dtype, src_pool.device,
+           dst_pool.shape, dst_pool.stride(), dst_pool.dtype, dst_pool.device, pairs.shape,
+           pairs.stride(), pairs.dtype, pairs.device)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _copy_plan, src_pool, dst_pool, pairs, block_size)
+    device, fn, src_step, src_blocks, dst, parts = plan
+    for first, n in parts:
+        _call(device, fn, src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), *dst,
+              pairs.data_ptr() + 8 * first, n)
+    return dst_pool
+
+
+def _copy_plan(src_pool, dst_pool, pairs, block_size):
     assert src_pool.dtype == dst_pool.dtype and src_pool.device == dst_pool.device, \
         "pools of one dtype on one device"
     assert src_pool.shape[:-3] == dst_pool.shape[:-3] and src_pool.shape[-2:] == dst_pool.shape[-2:], \
         "pools of the same planes, kv heads and head dim"
     planes, src_step, src_blocks, size = _planes(src_pool, "src_pool", block_size)
     _, dst_step, dst_blocks, _ = _planes(dst_pool, "dst_pool", block_size)
-    ids = _ids(pairs, "pairs", (None, 2), src_pool.device)
-    if size == 0 or planes == 0 or pairs.shape[0] == 0:
-        return dst_pool
-    with _lib.on_device(src_pool.device) as stream:
-        for part in _parts(pairs.shape[0], planes, size):
-            check(load().mi_cache_copy_blocks(
-                src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), dst_step, dst_blocks,
-                planes, size, ids + 8 * part.start, part.stop - part.start, stream))
-    return dst_pool
+    _ids(pairs, "pairs", (None, 2), src_pool.device)
+    nothing = size == 0 or planes == 0 or pairs.shape[0] == 0
+    return (_lib.device_index(src_pool.device), load().mi_cache_copy_blocks, src_step, src_blocks,
+            (dst_step, dst_blocks, planes, size), [] if nothing else _parts(pairs.shape[0], planes, size))
 
 
 def fork_rows(pool, tables, lens, children, block_size):
@@ -155,18 +174,28 @@ def fork_rows(pool, tables, lens, children, block_size):
     into the new block (not looked at where there are none), which is its next entry; its length
     becomes L.  Child slots and new blocks must be distinct, and no child slot may be a parent slot.  A
     child that names anything out of range is skipped whole."""
+    assert type(block_size) is int, "block_size: a positive int"
+    key = ("fork", block_size, pool.shape, pool.stride(), pool.dtype, pool.device, tables.shape,
+           tables.stride(), tables.dtype, tables.device, lens.shape, lens.stride(), lens.dtype,
+           lens.device, children.shape, children.stride(), children.dtype, children.device)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _fork_plan, pool, tables, lens, children, block_size)
+    device, fn, shape, table, n_seqs, n = plan
+    if n:
+        _call(device, fn, pool.data_ptr(), *shape, tables.data_ptr(), *table, lens.data_ptr(), n_seqs,
+              children.data_ptr(), n)
+
+
+def _fork_plan(pool, tables, lens, children, block_size):
     planes, step, blocks, size = _planes(pool, "pool", block_size)
     assert size and planes, "pool: no values"
-    t, stride, width = _table(tables, pool.device)
-    n_seqs = tables.shape[0]
-    lp = _ids(lens, "lens", (n_seqs,), pool.device)
-    cp = _ids(children, "children", (None, 4), pool.device)
-    if children.shape[0] == 0 or n_seqs == 0:
-        return
-    with _lib.on_device(pool.device) as stream:
-        check(load().mi_cache_fork_rows(
-            pool.data_ptr(), step, blocks, planes, block_size, size // block_size, t, stride, width,
-            lp, n_seqs, cp, children.shape[0], stream))
+    stride, width, n_seqs = _table(tables, pool.device)
+    _ids(lens, "lens", (n_seqs,), pool.device)
+    _ids(children, "children", (None, 4), pool.device)
+    return (_lib.device_index(pool.device), load().mi_cache_fork_rows,
+            (step, blocks, planes, block_size, size // block_size), (stride, width), n_seqs,
+            children.shape[0] if n_seqs else 0)
 
 
 def move_blocks(pool, tables, rows, pairs, new_ids, block_size):
@@ -175,18 +204,27 @@ def move_blocks(pool, tables, rows, pairs, new_ids, block_size):
 
     pairs [n, 2], rows [n_rows, 2], new_ids [blocks of the pool] int32 (a block that stays has its own
     id).  No block may be both read and written or written twice, and no slot may occur twice."""
+    assert type(block_size) is int, "block_size: a positive int"
+    key = ("move", block_size, pool.shape, pool.stride(), pool.dtype, pool.device, tables.shape,
+           tables.stride(), tables.dtype, tables.device, rows.shape, rows.stride(), rows.dtype,
+           rows.device, pairs.shape, pairs.stride(), pairs.dtype, pairs.device, new_ids.shape,
+           new_ids.stride(), new_ids.dtype, new_ids.device)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _move_plan, pool, tables, rows, pairs, new_ids, block_size)
+    device, fn, shape, table, n_rows, parts = plan
+    for first, n in parts:
+        _call(device, fn, pool.data_ptr(), *shape, pairs.data_ptr() + 8 * first, n, tables.data_ptr(),
+              *table, rows.data_ptr(), 0 if first else n_rows, new_ids.data_ptr())
+
+
+def _move_plan(pool, tables, rows, pairs, new_ids, block_size):
     planes, step, blocks, size = _planes(pool, "pool", block_size)
     assert size and planes, "pool: no values"
-    t, stride, width = _table(tables, pool.device)
-    pp = _ids(pairs, "pairs", (None, 2), pool.device)
-    rp = _ids(rows, "rows", (None, 2), pool.device)
-    ip = _ids(new_ids, "new_ids", (blocks,), pool.device)
-    if pairs.shape[0] == 0 and rows.shape[0] == 0:
-        return
-    n_rows = rows.shape[0]
-    with _lib.on_device(pool.device) as stream:
-        for part in _parts(pairs.shape[0], planes, size, n_rows):
-            check(load().mi_cache_move_blocks(
-                pool.data_ptr(), step, blocks, planes, size, pp + 8 * part.start,
-                part.stop - part.start, t, stride, width, tables.shape[0], rp,
-                n_rows if part.start == 0 else 0, ip, stream))
+    table = _table(tables, pool.device)
+    _ids(pairs, "pairs", (None, 2), pool.device)
+    _ids(rows, "rows", (None, 2), pool.device)
+    _ids(new_ids, "new_ids", (blocks,), pool.device)
+    n, n_rows = pairs.shape[0], rows.shape[0]
+    return (_lib.device_index(pool.device), load().mi_cache_move_blocks, (step, blocks, planes, size),
+            table, n_rows, _parts(n, planes, size, n_rows) if n or n_rows else [])
