@@ -977,7 +977,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
 }
 
 // Merges the parts of one (token, head), by WAVES waves: every lane first takes a part's (m, l), 64 parts a
-// time, then each half wave its share of the parts' O, four dims a lane.
+// time, then each half wave its share of the parts' O, four dims a lane.  Bound by latency: the launch and
+// three dependent reads, record, (m, l) and O, 4 us for 24 pairs of 2 parts, 6 us for 768 pairs of 44
+// parts (16 MB), 8 us for 10,000 pairs of 5 (20 MB).
 template <typename E, int WAVES>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1013,8 +1015,23 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
   for (int base = 0; base < total; base += 64) {
     const int i = base + lane, batch = min(64, total - base);
     const int64_t at = column(i);
-    const float m = i < total ? p.ws_ml[2 * at] : -INFINITY;
-    const float l = i < total ? p.ws_ml[2 * at + 1] : 0.f;
+    const float2 part_ml = i < total ? *reinterpret_cast<const float2*>(p.ws_ml + 2 * at)
+                                     : float2{-INFINITY, 0.f};
+    // The first parts' O travels while what they weigh is found: 12 tokens over 3,001 keys 25.1 -> 24.0 us, 8
+    // x 150 over 5,000 61.5 -> 60.6 (with four in flight there 61.5, with eight 63.4: the registers
+    // that hold them leave room for fewer waves).
+    constexpr int kFlight = WAVES > 1 ? 4 : 2;
+    f32x4 x[kFlight];
+    const auto send = [&](int j0) {
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int j = j0 + 2 * WAVES * k + half;
+        x[k] = j < batch ? *reinterpret_cast<const f32x4*>(p.ws_o + column(base + j) * kHeadDim + d)
+                         : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    send(2 * part);
+    const float m = part_ml.x, l = part_ml.y;
     float Mn = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor(Mn, o));
@@ -1029,25 +1046,18 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= old;
     M = Mn;
-    constexpr int kFlight = 8;
-    for (int j0 = 2 * part; j0 < batch; j0 += 2 * WAVES * kFlight) {
-      f32x4 x[kFlight];
-      float wt[kFlight];
+    for (int j0 = 2 * part; j0 < batch;) {
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
         const int j = j0 + 2 * WAVES * k + half;
-        const bool live = j < batch;
-        wt[k] = __shfl(f, j & 63);
-        // a part that weighs nothing (that saw no key) is not looked at: its O may be anything
-        x[k] = live && wt[k] != 0.f
-                   ? *reinterpret_cast<const f32x4*>(p.ws_o + column(base + j) * kHeadDim + d)
-                   : f32x4{0.f, 0.f, 0.f, 0.f};
-        if (!live) wt[k] = 0.f;
+        const float wt = __shfl(f, j & 63);
+        // a part that weighs nothing (that saw no key) doesn't count: its O may be anything
+        const bool live = j < batch && wt != 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = live ? __builtin_fmaf(x[k][e], wt, acc[e]) : acc[e];
       }
-#pragma unroll
-      for (int k = 0; k < kFlight; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[k][e], wt[k], acc[e]);
+      j0 += 2 * WAVES * kFlight;
+      if (j0 < batch) send(j0);
     }
   }
 #pragma unroll
