@@ -870,8 +870,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   const int N1 = __builtin_amdgcn_readfirstlane(pl.wide[n_ranges]);
   const int N2 = __builtin_amdgcn_readfirstlane(pl.narrow[n_ranges]);
   // The wide ranges take the first W1 work-groups, the waves of the others the narrow ones: a share each
-  // if that fits, else as many as their work weighs (a work-group's wide share takes 2.7 us, eight
-  // narrow shares side by side 1.2 us: kShNarrowWeight of them are one).
+  // if that fits, else as many as their work weighs (a work-group's wide share takes 2.3 to 2.7 us, one of
+  // eight narrow ones side by side 0.4: kShNarrowWeight of them are one; 5 to 9 differ by 1 %).
   const int alone = (N2 + kShWaves - 1) / kShWaves;
   int W3 = alone;
   if (N1 + alone > W) {
