@@ -120,7 +120,8 @@ class DecodeGraphs:
         n = len(seqs)
         rows = self._bucket(n)
         cache = self.cache
-        groups = cache.shared_groups(seqs) if cache.device_tables else None
+        sharing = cache.device_tables and rows <= cache.SHARED_MAX_ROWS   # (padding rows count)
+        groups = cache.shared_groups(seqs) if sharing else None
         if groups is not None and rows not in self.shared_graphs:
             self._capture(rows, shared=True)
         graph, logits, bufs, copied = (self.graphs if groups is None else self.shared_graphs)[rows]
