@@ -976,14 +976,21 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   }
 }
 
-// Merges the parts of one (token, head), by WAVES waves: every lane first takes a part's (m, l), 64 parts a
-// time, then each half wave its share of the parts' O, four dims a lane.  Bound by latency: the launch and
-// three dependent reads, record, (m, l) and O, 4 us for 24 pairs of 2 parts, 6 us for 768 pairs of 44
-// parts (16 MB), 8 us for 10,000 pairs of 5 (20 MB).
+// Merges the parts of one (token, head), by WAVES waves, or each half wave its own (WAVES = 0): every lane
+// first takes a part's (m, l), as many parts a time as there are lanes, then a half wave its share of the
+// parts' O, four dims a lane.  Bound by latency: the launch and two dependent reads, the record, then (m, l)
+// and O: 4 us for 24 pairs of 2 parts, 6 us for 768 pairs of 44 (16 MB).  (The record, the weights and O one
+// after the other: 25.1 us in all for 12 tokens over 3,001 keys instead of 23.6.)
 template <typename E, int WAVES>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pair = blockIdx.x * (4 / WAVES) + wave / WAVES, part = wave % WAVES;
+  constexpr int kLanes = WAVES > 0 ? 64 : 32;            // that weigh a pair's parts
+  constexpr int kHalves = WAVES > 0 ? 2 * WAVES : 1;     // half waves that share them
+  constexpr int kFlight = 4;                             // 2 to 8 differ by 2 %
+  const int lane = threadIdx.x & 63, half = lane >> 5, d = 4 * (lane & 31);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = WAVES > 0 ? wave : 0, apart = WAVES > 0 ? half : 0;
+  const int pair = WAVES > 0 ? (int)blockIdx.x : (int)blockIdx.x * 8 + 2 * wave + half;
+  static_assert(WAVES == 0 || WAVES == 4, "a work-group's waves");
   if (pair >= p.total_q * p.Hq) return;
   const int token = fdiv(pair, p.heads_div), h = pair - token * p.Hq;
   const int32_t* where = p.ws_where + 2 * (int64_t)pair;
@@ -1005,27 +1012,22 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
     if (col[i] < 0 || n[i] < 0 || col[i] + ((int64_t)n[i] - 1) * stride[i] >= p.columns) return;
 
   const float c = p.scale_log2;
-  const int half = lane >> 5, d = 4 * (lane & 31);
   const auto column = [&](int t) {
     return t < n[0] ? col[0] + (int64_t)t * stride[0] : col[1] + (int64_t)(t - n[0]) * stride[1];
   };
   float M = -INFINITY, L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   const int total = n[0] + n[1];
-  for (int base = 0; base < total; base += 64) {
-    const int i = base + lane, batch = min(64, total - base);
-    const int64_t at = column(i);
-    const float2 part_ml = i < total ? *reinterpret_cast<const float2*>(p.ws_ml + 2 * at)
+  for (int base = 0; base < total; base += kLanes) {
+    const int i = base + (lane & (kLanes - 1)), batch = min(kLanes, total - base);
+    const float2 part_ml = i < total ? *reinterpret_cast<const float2*>(p.ws_ml + 2 * (int64_t)column(i))
                                      : float2{-INFINITY, 0.f};
-    // The first parts' O travels while what they weigh is found: 12 tokens over 3,001 keys 25.1 -> 24.0 us, 8
-    // x 150 over 5,000 61.5 -> 60.6 (with four in flight there 61.5, with eight 63.4: the registers
-    // that hold them leave room for fewer waves).
-    constexpr int kFlight = WAVES > 1 ? 4 : 2;
+    // The first parts' O travels while what they weigh is found.
     f32x4 x[kFlight];
     const auto send = [&](int j0) {
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const int j = j0 + 2 * WAVES * k + half;
+        const int j = j0 + kHalves * k + apart;
         x[k] = j < batch ? *reinterpret_cast<const f32x4*>(p.ws_o + column(base + j) * kHeadDim + d)
                          : f32x4{0.f, 0.f, 0.f, 0.f};
       }
@@ -1034,66 +1036,67 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
     const float m = part_ml.x, l = part_ml.y;
     float Mn = m;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor(Mn, o));
+    for (int o = kLanes / 2; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor(Mn, o));
     Mn = fmaxf(Mn, M);
     const float Mu = Mn == -INFINITY ? 0.f : Mn;
     const float old = exp2_fast((M - Mu) * c);
     const float f = exp2_fast((m - Mu) * c);
     float ls = l * f;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+    for (int o = kLanes / 2; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
     L = L * old + ls;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= old;
     M = Mn;
-    for (int j0 = 2 * part; j0 < batch;) {
+    for (int j0 = 2 * part; j0 < batch;) {   // (a wave's lanes stay together: they read each other's f)
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const int j = j0 + 2 * WAVES * k + half;
-        const float wt = __shfl(f, j & 63);
+        const int j = j0 + kHalves * k + apart;
+        const float wt = __shfl(f, (lane & ~(kLanes - 1)) | (j & (kLanes - 1)));
         // a part that weighs nothing (that saw no key) doesn't count: its O may be anything
         const bool live = j < batch && wt != 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = live ? __builtin_fmaf(x[k][e], wt, acc[e]) : acc[e];
       }
-      j0 += 2 * WAVES * kFlight;
+      j0 += kHalves * kFlight;
       if (j0 < batch) send(j0);
     }
   }
+  if constexpr (WAVES > 0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], 32);
-  if constexpr (WAVES > 1) {
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], 32);
     __shared__ f32x4 sums[WAVES][32];
     if (half == 0) sums[part][lane] = acc;
     __syncthreads();   // (the whole block has one pair)
-    if (part != 0) return;
+    if (part != 0 || half != 0) return;
 #pragma unroll
     for (int j = 1; j < WAVES; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += sums[j][lane & 31][e];
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  if (half == 0)
-    *reinterpret_cast<u32x2*>(p.o + (int64_t)token * p.o_st + (int64_t)h * p.o_sh + d) =
-        u32x2{E::pack2(acc[0] * inv, acc[1] * inv), E::pack2(acc[2] * inv, acc[3] * inv)};
-  if (p.lse && lane == 0)
+  *reinterpret_cast<u32x2*>(p.o + (int64_t)token * p.o_st + (int64_t)h * p.o_sh + d) =
+      u32x2{E::pack2(acc[0] * inv, acc[1] * inv), E::pack2(acc[2] * inv, acc[3] * inv)};
+  if (p.lse && (lane & 31) == 0)
     p.lse[h * p.l_sh + token * p.l_st] =
         L > 0.f ? (M * c + __builtin_log2f(L)) * kLn2 : -INFINITY;
 }
 
-constexpr int kShMergePairs = 4096;
+// From this many pairs on, half a wave merges each (fewer leave most of the device idle, and have more parts
+// each): 1,032 pairs of 60 narrow parts 29.0 us in all by halves and 26.7 by four waves, 1,152 and 1,440 100.3 /
+// 99.4 and 29.4 / 28.8, 2,048 34.2 / 35.6, 2,064 30.7 / 31.6, 4,080 35.7 / 39.5.
+constexpr int kShMergePairs = 2048;
 
 template <typename E>
 static hipError_t launch_shared_t(const SharedParams& p, int n_wg, hipStream_t stream) {
   hipLaunchKernelGGL((shared_attn_kernel<E>), dim3(n_wg), dim3(kShThreads), 0, stream, p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  // four waves for each (token, head) where one would leave most of the device idle
   const int pairs = p.total_q * p.Hq;
-  if (pairs <= kShMergePairs)
+  if (pairs < kShMergePairs)
     hipLaunchKernelGGL((shared_merge_kernel<E, 4>), dim3(pairs), dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((shared_merge_kernel<E, 1>), dim3((pairs + 3) / 4), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((shared_merge_kernel<E, 0>), dim3((pairs + 7) / 8), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
