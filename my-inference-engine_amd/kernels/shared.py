@@ -37,6 +37,8 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
     out          optional [total_q, Hq, 128] output (any token/head strides); tokens of no row keep
                  what they hold
     More than 512 rows go to fa2_paged_varlen, which reads every row's keys for that row alone.
+    Worth it from tens of MB of K and V that the rows would read again (KVCache.SHARED_BYTES has both sides'
+    times); with more than a few tens of new tokens a row fa2_paged_varlen is faster.
     Returns O [total_q, Hq, 128] (and the fp32 LSE [Hq, total_q] if return_lse).
     """
     # plain values only: the plan is looked up by them
