@@ -41,6 +41,12 @@ constexpr int kShWideUnit = 128;                // keys of a wide step
 constexpr int kShWideCost = 4, kShNarrowCost = 1;
 constexpr int kShMergeCost = 4;   // of one more wide part for each pair, in the merge
 constexpr int kShNarrowWeight = 7;
+// Narrow shares go to as many work-groups as there is room for, a wave each, then a second wave of each: 64 keys
+// that a wave has to itself arrive sooner than with seven more of its CU's (2 rows of 100 keys 11.1 -> 10.4 us,
+// drawn rows 14.6 -> 12.3 and 12.9 -> 10.8).  From kShSpread shares for each work-group on a wave takes kShEach, so that
+// an item leaves fewer parts (40 rows in 9 groups, 52 MB, 24.6 -> 21.5 us; two each 22.7), or more where
+// eight waves of each do not do, and no more waves than that takes (172 rows of 34 groups 30.9 -> 29.6).
+constexpr int kShSpread = 4, kShEach = 3;
 constexpr int kShRow = kHeadDim * 2;            // bytes of a key
 constexpr int kShStage = 2 * kShWideUnit * kShRow;   // K, then V, of a wide step: 64 KB
 constexpr int kShRing = 2 * kShStage / kShWaves;     // a wave's part of the two stages: 16 KB
@@ -878,13 +884,15 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   // The wide ranges take the first W1 work-groups, the waves of the others the narrow ones: a share each
   // if that fits, else as many as their work weighs (a work-group's wide share takes 2.3 to 2.7 us, one of
   // eight narrow ones side by side 0.4: kShNarrowWeight of them are one; 5 to 9 differ by 1 %).
-  const int alone = (N2 + kShWaves - 1) / kShWaves;
-  int W3 = alone;
-  if (N1 + alone > W) {
+  int room = W - N1;
+  if (N1 + (N2 + kShWaves - 1) / kShWaves > W) {
     const float all = (float)kShNarrowWeight * (float)N1 + (float)N2;
-    W3 = min(alone, (int)((float)W * (float)N2 / all + 0.5f));
-    W3 = __builtin_amdgcn_readfirstlane(min(max(W3, N2 > 0 ? 1 : 0), N1 > 0 ? W - 1 : W));
+    room = min((N2 + kShWaves - 1) / kShWaves, (int)((float)W * (float)N2 / all + 0.5f));
+    room = __builtin_amdgcn_readfirstlane(min(max(room, N2 > 0 ? 1 : 0), N1 > 0 ? W - 1 : W));
   }
+  int W2 = N2;
+  if (N2 > kShSpread * room) W2 = quotient(N2 - 1, max(kShEach, quotient(N2 - 1, kShWaves * room) + 1)) + 1;
+  const int W3 = min(room, W2);
   const int W1 = min(W - W3, N1);
 
   if ((int)blockIdx.x < W1) {
@@ -924,7 +932,6 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     return;
   }
 
-  const int W2 = min(W3 * kShWaves, N2);
   // neighbouring shares on different work-groups: a short list of units spreads over the CUs
   const int worker = wave * W3 + (int)blockIdx.x - (W - W3);
   if ((int)blockIdx.x < W - W3 || worker >= W2) return;

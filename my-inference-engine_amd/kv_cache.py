@@ -146,13 +146,13 @@ class KVCache:
     # K and V bytes that a step would read again in a layer, from which its attention reads the
     # shared blocks once; with less to save the plain kernels' smaller fixed cost wins.  One new
     # token, us shared / plain: 16 rows over 1,024 shared keys of 2 heads (15 MB) 14.6 / 12.2, over 2,048
-    # (30 MB) 14.9 / 15.3; 4 rows over 8,192 keys of 4 heads (48 MB) 22.6 / 19.9, over 4,096 of 8
-    # heads (48 MB) 18.0 / 20.5; 8 rows over 4,096 of 4 (56 MB) 15.7 / 20.1; 64 rows over 1,024 of 8
-    # (252 MB) 23.3 / 35.3; 64 rows over 31,000 of 2 (1.9 GB) 39 / 279.
-    SHARED_BYTES = 48 << 20
+    # (30 MB) 15.0 / 15.1; 4 rows over 4,096 keys of 4 heads (24 MB) 14.3 / 17.0, of 8 (48 MB) 14.7 /
+    # 20.5; 8 rows over 4,096 of 2 (28 MB) 15.0 / 16.6; 64 rows over 512 of 2 (31 MB) 16.9 / 14.6, over 1,024
+    # of 8 (252 MB) 21.8 / 35.0, over 31,000 of 2 (1.9 GB) 39 / 283.
+    SHARED_BYTES = 24 << 20
     # New tokens of a row up to which that holds: with more, its own tiles are full and the work is
-    # bound by the matrix products (8 rows over 4,096 keys of 8 heads: 8 new tokens 30 / 54, 32 47 / 55,
-    # 64 68 / 57).
+    # bound by the matrix products (8 rows over 4,096 keys of 8 heads: 8 new tokens 29 / 52, 32 43 / 52,
+    # 64 63 / 55).
     SHARED_MAX_NEW = 32
     SHARED_MAX_ROWS = 512     # rows of a call of the kernel
 
