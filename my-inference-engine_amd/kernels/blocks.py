@@ -73,16 +73,13 @@ def _plan(key, make, *args):
     return got
 
 
-def _call(device, fn, *args):
-    """fn(*args, stream) on the device's current stream."""
-    if device == _current():
-        check(fn(*args, _stream(device)))
+def call(device, fn, *args):
+    """fn(*args, stream) on the device's current stream; raises what it reports."""
+    if device == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
         return
     with _lib.on_device(torch.device("cuda", device)) as stream:
         check(fn(*args, stream))
-
-
-_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _planes(pool, name, block_size):
@@ -147,7 +144,7 @@ def copy_blocks(src_pool, dst_pool, pairs, block_size):
         plan = _plan(key, _copy_plan, src_pool, dst_pool, pairs, block_size)
     device, fn, src_step, src_blocks, dst, parts = plan
     for first, n in parts:
-        _call(device, fn, src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), *dst,
+        call(device, fn, src_pool.data_ptr(), src_step, src_blocks, dst_pool.data_ptr(), *dst,
               pairs.data_ptr() + 8 * first, n)
     return dst_pool
 
@@ -161,7 +158,7 @@ def _copy_plan(src_pool, dst_pool, pairs, block_size):
     _, dst_step, dst_blocks, _ = _planes(dst_pool, "dst_pool", block_size)
     _ids(pairs, "pairs", (None, 2), src_pool.device)
     nothing = size == 0 or planes == 0 or pairs.shape[0] == 0
-    return (_lib.device_index(src_pool.device), load().mi_cache_copy_blocks, src_step, src_blocks,
+    return (src_pool.device.index, load().mi_cache_copy_blocks, src_step, src_blocks,
             (dst_step, dst_blocks, planes, size), [] if nothing else _parts(pairs.shape[0], planes, size))
 
 
@@ -183,7 +180,7 @@ def fork_rows(pool, tables, lens, children, block_size):
         plan = _plan(key, _fork_plan, pool, tables, lens, children, block_size)
     device, fn, shape, table, n_seqs, n = plan
     if n:
-        _call(device, fn, pool.data_ptr(), *shape, tables.data_ptr(), *table, lens.data_ptr(), n_seqs,
+        call(device, fn, pool.data_ptr(), *shape, tables.data_ptr(), *table, lens.data_ptr(), n_seqs,
               children.data_ptr(), n)
 
 
@@ -193,7 +190,7 @@ def _fork_plan(pool, tables, lens, children, block_size):
     stride, width, n_seqs = _table(tables, pool.device)
     _ids(lens, "lens", (n_seqs,), pool.device)
     _ids(children, "children", (None, 4), pool.device)
-    return (_lib.device_index(pool.device), load().mi_cache_fork_rows,
+    return (pool.device.index, load().mi_cache_fork_rows,
             (step, blocks, planes, block_size, size // block_size), (stride, width), n_seqs,
             children.shape[0] if n_seqs else 0)
 
@@ -214,7 +211,7 @@ def move_blocks(pool, tables, rows, pairs, new_ids, block_size):
         plan = _plan(key, _move_plan, pool, tables, rows, pairs, new_ids, block_size)
     device, fn, shape, table, n_rows, parts = plan
     for first, n in parts:
-        _call(device, fn, pool.data_ptr(), *shape, pairs.data_ptr() + 8 * first, n, tables.data_ptr(),
+        call(device, fn, pool.data_ptr(), *shape, pairs.data_ptr() + 8 * first, n, tables.data_ptr(),
               *table, rows.data_ptr(), 0 if first else n_rows, new_ids.data_ptr())
 
 
@@ -226,5 +223,5 @@ def _move_plan(pool, tables, rows, pairs, new_ids, block_size):
     _ids(rows, "rows", (None, 2), pool.device)
     _ids(new_ids, "new_ids", (blocks,), pool.device)
     n, n_rows = pairs.shape[0], rows.shape[0]
-    return (_lib.device_index(pool.device), load().mi_cache_move_blocks, (step, blocks, planes, size),
+    return (pool.device.index, load().mi_cache_move_blocks, (step, blocks, planes, size),
             table, n_rows, _parts(n, planes, size, n_rows) if n or n_rows else [])

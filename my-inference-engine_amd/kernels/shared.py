@@ -12,7 +12,7 @@ import operator
 import torch
 
 from . import _lib
-from .blocks import check, load
+from .blocks import call, load
 from .fa2 import (_MEMO_MAX, HEAD_DIM, _contig, _dims_ok, _envelope, _strides, _strides_of,
                   _strides_ok, fa2_paged_varlen)
 
@@ -66,7 +66,8 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
         if len(_PLANS) >= _MEMO_MAX:
             _PLANS.clear()
         _PLANS[key] = pl
-    dtype_code, many, copy_q, table_stride, sizes, q_st, pool_st, o_st, l_st, tail, ws_bytes = pl
+    (device, fn, dtype_code, many, copy_q, table_stride, sizes, q_st, pool_st, o_st, l_st, tail,
+     ws_bytes) = pl
     kp, vp = k_pool.data_ptr(), v_pool.data_ptr()
     assert not (kp | vp) & 15, "pools need 16-byte aligned token rows"
     if many:
@@ -85,12 +86,10 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
     L = torch.empty((q.shape[1], q.shape[0]), device=dev, dtype=torch.float32) if return_lse else None
     # every call has its own (from torch's caching allocator, in stream order): nothing is shared
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev) as stream:
-        check(load().mi_cache_attend(
-            dtype_code, q.data_ptr(), kp, vp, O.data_ptr(), L.data_ptr() if return_lse else None,
-            cu_seqlens_q.data_ptr(), block_table.data_ptr(), table_stride, kv_lens.data_ptr(),
-            cu_rows.data_ptr(), prefix_lens.data_ptr(), *sizes, q_st, pool_st, o_st, l_st, *tail,
-            ws.data_ptr(), ws_bytes, stream))
+    call(device, fn, dtype_code, q.data_ptr(), kp, vp, O.data_ptr(), L.data_ptr() if return_lse else None,
+         cu_seqlens_q.data_ptr(), block_table.data_ptr(), table_stride, kv_lens.data_ptr(),
+         cu_rows.data_ptr(), prefix_lens.data_ptr(), *sizes, q_st, pool_st, o_st, l_st, *tail,
+         ws.data_ptr(), ws_bytes)
     return (O, L) if return_lse else O
 
 
@@ -130,7 +129,7 @@ def _plan(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, cu_rows, prefix
     assert 0 <= max_kv_len <= width * block_size, \
         "max_kv_len exceeds what the block table can address"
     assert _strides_ok(k_pool) and _strides_ok(v_pool), "pools need 16-byte aligned token rows"
-    return (_lib.DTYPES[q.dtype], B > MAX_ROWS, not _strides_ok(q),
+    return (dev.index, load().mi_cache_attend, _lib.DTYPES[q.dtype], B > MAX_ROWS, not _strides_ok(q),
             block_table.stride(0) if B > 1 else width,
             (groups, B, total_q, Hq, Hkv, max_kv_len, d, block_size, k_pool.shape[0] // block_size),
             _strides(q), _strides(k_pool), _strides_of(q.shape, _contig(q.shape)),
