@@ -30,7 +30,8 @@
 // TFLOP/s.  A call costs about 10 us beside its steps: launch 2, plan 1.5, first loads and queries 2.5, the
 // parts' way out 2, the merge 3 to 4.  Replayed, 12 heads of 2 kv heads: 2 rows of 100 keys 10.4 us, 16
 // branches of 2,048 keys 15.2 (each row's keys read for it alone: 17), 40 rows in 9 groups (52 MB of keys) 21.5
-// (39), 8 rows of 50 to 150 new tokens over 5,000 keys 58 (78), 64 branches of 31,000 keys 39 (283).
+// (39), 8 rows of 90 to 150 new tokens over 5,000 keys and up to 900 of their own 58 (78), 64 branches of
+// 31,000 keys 39 (283).
 #include "cache_ops.h"
 
 #include <type_traits>
