@@ -1061,7 +1061,9 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
     Mn = fmaxf(Mn, M);
     const float Mu = Mn == -INFINITY ? 0.f : Mn;
     const float old = exp2_fast((M - Mu) * c);
-    const float f = exp2_fast((m - Mu) * c);
+    // A part that saw no key (l is 0) doesn't count: its O may be anything.  One whose scores are NaN has a
+    // maximum of -inf like it, but an l of NaN, and counts, whatever the others weigh.
+    const float f = l == 0.f ? -1.f : exp2_fast((m - Mu) * c);
     float ls = l * f;
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
@@ -1074,8 +1076,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
       for (int k = 0; k < kFlight; ++k) {
         const int j = j0 + kHalves * k + apart;
         const float wt = __shfl(f, (lane & ~(kLanes - 1)) | (j & (kLanes - 1)));
-        // a part that weighs nothing (that saw no key) doesn't count: its O may be anything
-        const bool live = j < batch && wt != 0.f;
+        const bool live = j < batch && !(wt < 0.f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = live ? __builtin_fmaf(x[k][e], wt, acc[e]) : acc[e];
       }
@@ -1095,12 +1096,12 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += sums[j][lane & 31][e];
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   *reinterpret_cast<u32x2*>(p.o + (int64_t)token * p.o_st + (int64_t)h * p.o_sh + d) =
       u32x2{E::pack2(acc[0] * inv, acc[1] * inv), E::pack2(acc[2] * inv, acc[3] * inv)};
   if (p.lse && (lane & 31) == 0)
     p.lse[h * p.l_sh + token * p.l_st] =
-        L > 0.f ? (M * c + __builtin_log2f(L)) * kLn2 : -INFINITY;
+        L == 0.f ? -INFINITY : (M * c + __builtin_log2f(L)) * kLn2;
 }
 
 // From this many pairs on, half a wave merges each (fewer leave most of the device idle, and have more parts
