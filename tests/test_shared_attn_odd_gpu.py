@@ -1,5 +1,5 @@
 """Attention over shared blocks (csrc/shared_attn.hip) where values are NaN or inf in places that a query
-sees.
+sees, and over key ranges long enough that a worker refills what it knows of their blocks.
 
 A score that is NaN, or a value that is, makes the query's output NaN, whichever part of its keys it lies in
 (the prefix, its own keys, one worker's share of either) and whatever that part weighs; the other
@@ -11,7 +11,7 @@ import torch
 
 from conftest import announce
 from kernels.fa2 import fa2_paged
-from test_shared_attn_gpu import Batch
+from test_shared_attn_gpu import DT, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,42 @@ def test_odd_values_in_a_part_that_weighs_nothing(what, value):
         assert value == math.inf or out[:, :6, 64].isnan().all()
         assert out[:, :6, :64].isfinite().all() and out[:, :6, 65:].isfinite().all()
     assert out[:, 6:].isfinite().all() and lse[6:].isfinite().all()
+
+
+def test_long_shares_of_wide_ranges():
+    """A work-group that walks more than 64 steps of 128 keys finds the next 64 steps' blocks: 2,731 tokens of
+    one row are 129 tiles of each kv head, 258 items of 97 steps each, about one for each work-group.
+
+    Up to 97 * 64 products of a lane's stream are summed in fp32: off by 97 * 64 * 2^-24 < 2^-11 A."""
+    announce("shared attention, wide shares of more than 64 steps")
+    b = Batch([(1, 0)], [12300], [2731], seed=24)
+    b.bound = lambda o, A: Batch.bound(b, o, A) + 2.0 ** -11 * A
+    out, lse = b.call(return_lse=True)
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_long_shares_of_narrow_ranges(dtype):
+    """A wave that walks more than 16 units of 64 keys finds the next 32 steps' block ids: 64 rows of 36,000
+    to 37,000 own keys, one kv head, are 36,000 units and more over at most 2,048 waves."""
+    announce(f"shared attention, narrow shares of more than 16 units, {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(25)
+    b = Batch([(2, 16)], [20, 30], [1, 1], heads=(4, 1), dtype=dtype, seed=25)
+    kv = [36000 + 13 * i for i in range(64)]
+    held = [-(-n // 16) for n in kv]
+    ids = torch.randperm(sum(held), generator=torch.Generator().manual_seed(1)).tolist()
+    b.tables, at = [], 0
+    for n in held:
+        b.tables.append(ids[at:at + n])
+        at += n
+    width = max(held)
+    b.table = torch.tensor([t + [-1] * (width - len(t)) for t in b.tables], dtype=torch.int32,
+                           device="cuda")
+    b.kv, b.new, b.cu = kv, [1] * 64, list(range(65))
+    b.pool = torch.randn(2, sum(held) * 16, 1, 128, generator=g, device="cuda").to(DT[dtype])
+    b.q = torch.randn(64, 4, 128, generator=g, device="cuda").to(DT[dtype])
+    b.lens, b.cu_q = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (kv, b.cu))
+    b.cu_rows = torch.zeros(1, dtype=torch.int32, device="cuda")
+    b.prefix = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out, lse = b.call(return_lse=True)
+    b.check(out, lse)
