@@ -95,22 +95,19 @@ class Engine:
 
         What conv holds in the cache they share (KVCache.fork), all but the history's last token, whose
         logits their first sample needs, provided that blocks and sequence slots for them can be had by
-        evicting idle conversations; otherwise they start without cache, and their first prompt
-        is their whole history."""
+        evicting idle conversations; otherwise nobody is evicted, they start without cache, and
+        their first prompt is their whole history."""
         forks = [Conversation(ids=list(conv.ids), eos_id=conv.eos_id) for _ in range(n)]
         if conv.seq is not None and n > 0:
             held = min(self.cache.length(conv.seq), len(conv.ids) - 1)
             blocks = n if held % self.cache.block_size else 0
-            busy = {id(j.conv) for j in self.active} | {id(conv)}
-
-            def short():
-                return (self.cache.free_block_count() < blocks
-                        or self.cache.free_slot_count() < n)
-            while short():
-                idle = [c for c in self.resident if id(c) not in busy]
-                if not idle:
-                    return forks
-                self._evict(idle[0])
+            idle = self._idle_beside(conv)
+            if (self.cache.free_block_count() + self.cache.reclaimable([c.seq for c in idle]) < blocks
+                    or self.cache.free_slot_count() + len(idle) < n):
+                return forks
+            while (self.cache.free_block_count() < blocks
+                   or self.cache.free_slot_count() < n):
+                idle.remove(self._evict_one(idle, self.cache.free_slot_count() < n))
             for child, seq in zip(forks, self.cache.fork(conv.seq, n, held)):
                 child.seq = seq
                 self._touch(child)
@@ -201,21 +198,37 @@ class Engine:
         if conv in self.resident:
             self.resident.remove(conv)
 
+    def _idle_beside(self, conv):
+        """The conversations holding cache that neither decode nor are conv, least recently used first."""
+        busy = {id(j.conv) for j in self.active} | {id(conv)}
+        return [c for c in self.resident if id(c) not in busy]
+
+    def _evict_one(self, idle, slot):
+        """Evict the least recently used of `idle`, where blocks are short (and no slot) the first that
+        holds some alone, if one does: of branches that share all theirs, none gives any back by itself.
+        Returns it."""
+        conv = idle[0]
+        if not slot:
+            conv = next((c for c in idle if self.cache.reclaimable([c.seq])), conv)
+        self._evict(conv)
+        return conv
+
     def _make_room(self, job):
         """Evict idle conversations, least recently used first, until the job's reservation fits
         in free blocks (chat.py:128-146) and, for a conversation without cache, a sequence slot is
         free."""
-        busy = {id(j.conv) for j in self.active} | {id(job.conv)}
+        idle = self._idle_beside(job.conv)
+
+        def no_slot():
+            return job.conv.seq is None and self.cache.free_slot_count() == 0
 
         def short():
             return (self.cache.blocks_needed(job.conv.seq, self._reserve_len(job))
-                    > self.cache.free_block_count()
-                    or (job.conv.seq is None and self.cache.free_slot_count() == 0))
+                    > self.cache.free_block_count()) or no_slot()
         while short():
-            idle = [c for c in self.resident if id(c) not in busy]
             if not idle:
                 return False
-            self._evict(idle[0])
+            idle.remove(self._evict_one(idle, no_slot()))
         return True
 
     def _touch(self, conv):
