@@ -61,6 +61,14 @@ class Job:
     prefill: list = None   # mixed mode: prompt tokens waiting for the next step
 
 
+def _drop(items, item):
+    """Take item itself out of a list, if it is there (== would compare histories)."""
+    for i, x in enumerate(items):
+        if x is item:
+            del items[i]
+            return
+
+
 class Engine:
     def __init__(self, model, cache, *, max_reply_tokens=512, temperature=1.0, sep_ids=(198,),
                  seed=0, decode_graphs=None, mixed_prefill=False, max_step_tokens=16384):
@@ -107,7 +115,7 @@ class Engine:
                 return forks
             while (self.cache.free_block_count() < blocks
                    or self.cache.free_slot_count() < n):
-                idle.remove(self._evict_one(idle, self.cache.free_slot_count() < n))
+                _drop(idle, self._evict_one(idle, self.cache.free_slot_count() < n))
             for child, seq in zip(forks, self.cache.fork(conv.seq, n, held)):
                 child.seq = seq
                 self._touch(child)
@@ -127,7 +135,7 @@ class Engine:
             return self._tick_mixed()
         for job in list(self.deferred):
             if self._make_room(job):
-                self.deferred.remove(job)
+                _drop(self.deferred, job)
                 self._admit(job)
         if not self.active and not self.deferred:
             if self.queue:  # the reference blocks on its queue here
@@ -155,14 +163,14 @@ class Engine:
 
         for job in list(self.deferred):
             if fits(job) and self._make_room(job):
-                self.deferred.remove(job)
+                _drop(self.deferred, job)
                 admit(job)
         if self.active or not self.deferred:
             while self.queue and fits(self.queue[0]):
                 job = self.queue.popleft()
                 before = len(self.deferred)
                 self._try_admit_or_defer(job)
-                if job in self.active:
+                if any(j is job for j in self.active):
                     budget[0] -= len(job.prefill)
                 elif len(self.deferred) > before:
                     break
@@ -195,8 +203,7 @@ class Engine:
     def _evict(self, conv):
         self.cache.free(conv.seq)
         conv.seq = None
-        if conv in self.resident:
-            self.resident.remove(conv)
+        _drop(self.resident, conv)
 
     def _idle_beside(self, conv):
         """The conversations holding cache that neither decode nor are conv, least recently used first."""
@@ -228,12 +235,11 @@ class Engine:
         while short():
             if not idle:
                 return False
-            idle.remove(self._evict_one(idle, no_slot()))
+            _drop(idle, self._evict_one(idle, no_slot()))
         return True
 
     def _touch(self, conv):
-        if conv in self.resident:
-            self.resident.remove(conv)
+        _drop(self.resident, conv)
         self.resident.append(conv)
 
     def _try_admit_or_defer(self, job):
@@ -273,7 +279,7 @@ class Engine:
         self.cache.trim(conv.seq)
         self._touch(conv)
         job.t_done = time.perf_counter()
-        self.active.remove(job)
+        _drop(self.active, job)
         self.finished.append(job)
 
     def _process(self):

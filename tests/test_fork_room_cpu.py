@@ -81,3 +81,26 @@ def test_branches_go_where_only_all_of_them_help():
     job = eng.submit(Conversation(), list(range(80)), 2)    # 6 of 7 blocks
     eng.run_until_idle()
     assert len(job.generated) == 2 and all(c.seq is None for c in branches)
+
+
+def test_conversations_are_told_apart_without_comparing_histories():
+    """Branches have long equal histories: finding one among the others looks at none of them."""
+    class Ids(list):
+        def __eq__(self, other):
+            raise AssertionError("histories compared")
+        __hash__ = None
+
+    eng = engine(20)
+    conv = idle(eng, 48)
+    convs = eng.fork(conv, 3) + [conv]
+    for c in convs:
+        c.ids = Ids(c.ids)
+    eng._touch(convs[1])
+    assert [id(c) for c in eng.resident] == [id(convs[i]) for i in (3, 0, 2, 1)]
+    more = eng.fork(convs[2], 2)
+    eng.release(convs[0])
+    assert [id(c) for c in eng.resident] == [id(c) for c in (convs[3], convs[2], convs[1], *more)]
+    eng.active = [eng.submit(c, [7], 2) for c in (convs[2], convs[1])]
+    last = eng.active[1]
+    eng._finish(last)
+    assert len(eng.active) == 1 and eng.active[0].conv is convs[2] and eng.finished[-1] is last
