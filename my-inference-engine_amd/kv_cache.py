@@ -169,7 +169,9 @@ class KVCache:
         self._next_seq = 0
         self._holders = [0] * num_blocks   # sequences that hold each block
         self._extra = 0                    # holders beyond a block's first, over all blocks
-        self._path = {}                    # seq id -> its place among its forks (see order)
+        # The tree of forks, for order(): a sequence's parent and its forks.  A freed sequence stays while
+        # at least two of its branches live, so there are fewer of those than sequences.
+        self._above, self._below = {}, {}
         self.device_tables = self.device.type == "cuda" if device_tables is None else device_tables
         # Blocks one sequence may hold.  With device tables this is the width of a table row: the
         # pool, capped at the default context length, so the tables do not grow with the square
@@ -212,7 +214,7 @@ class KVCache:
             self.dev_lens[slot:slot + 1].zero_()
         return seq
 
-    def _new_seq(self):
+    def _new_seq(self, parent=None):
         if not self._free_slots:
             raise RuntimeError(f"all {self.max_seqs} sequence slots are in use")
         seq = self._next_seq
@@ -220,13 +222,27 @@ class KVCache:
         self._block_tables[seq] = []
         self._lengths[seq] = 0
         self.slot[seq] = self._free_slots.pop()
-        self._path[seq] = (seq,)
+        self._above[seq], self._below[seq] = parent, set()
+        if parent is not None:
+            self._below[parent].add(seq)
         return seq
 
     def free(self, seq):
         self._release(self._block_tables.pop(seq))
-        del self._lengths[seq], self._path[seq]
+        del self._lengths[seq]
         self._free_slots.append(self.slot.pop(seq))
+        self._prune(seq)
+
+    def _prune(self, node):
+        """Take a freed sequence that joins no two branches out of the tree of forks."""
+        while node is not None and node not in self._lengths and len(self._below[node]) < 2:
+            above, below = self._above.pop(node), self._below.pop(node)
+            if above is not None:
+                self._below[above].remove(node)
+                self._below[above] |= below
+            for child in below:
+                self._above[child] = above
+            node = above       # it may have joined this branch and one more
 
     def _take(self, n):
         """n free blocks, now held once each."""
@@ -292,8 +308,7 @@ class KVCache:
         fresh = self._take(need)
         forks = []
         for i in range(n):
-            child = self._new_seq()
-            self._path[child] = self._path[seq] + (child,)
+            child = self._new_seq(seq)
             self._block_tables[child] = table[:whole] + fresh[i:i + 1]
             self._lengths[child] = length
             forks.append(child)
@@ -368,11 +383,18 @@ class KVCache:
         were forked from.  Sequences that share nothing keep their order."""
         if not self._extra:
             return list(range(len(seqs)))
-        first = {}
+        paths = {None: ()}     # from the root of its tree to a sequence
+        first, keys = {}, []   # where each tree begins; a row's place
         for i, s in enumerate(seqs):
-            first.setdefault(self._path[s][0], i)
-        return sorted(range(len(seqs)), key=lambda i: (first[self._path[seqs[i]][0]],
-                                                       self._path[seqs[i]]))
+            todo, at = [], s
+            while at not in paths:
+                todo.append(at)
+                at = self._above[at]
+            path = paths[at]
+            for at in reversed(todo):
+                path = paths[at] = path + (at,)
+            keys.append((first.setdefault(path[0], i), path))
+        return sorted(range(len(seqs)), key=keys.__getitem__)
 
     def shared_groups(self, seqs):
         """(cu_rows, prefix tokens) of neighbouring rows that hold the same first blocks, or None if a
