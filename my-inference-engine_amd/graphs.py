@@ -20,13 +20,22 @@ nothing written to the cache, zeros from attention), whose logits are ignored.
 
 Steps whose rows share enough of their blocks (KVCache.shared_groups, device tables only) replay
 another graph of the bucket, whose attention reads them once; which rows share what comes up with the
-slots and ids.  It is captured when the first such step comes.
+slots and ids.  It is captured by capture_shared(), or when the first such step comes: two steps and a
+capture in the middle of serving, and device memory for its intermediates (51 MB of workspace and more).  A
+step for which that memory cannot be had replays the bucket's ordinary graph, which computes the same.
 """
 import numpy as np
 import torch
 
 from kernels.meta import step_metadata
 from kv_cache import SharedRows, StepMeta
+
+
+def _out_of_memory(error):
+    """Whether memory that could not be had is behind an error (ending a capture may raise another)."""
+    while error is not None and not isinstance(error, torch.OutOfMemoryError):
+        error = error.__context__
+    return error is not None
 
 
 class DecodeGraphs:
@@ -38,6 +47,7 @@ class DecodeGraphs:
         self.buckets = sorted(buckets)
         self.graphs = {}
         self.shared_graphs = {}     # by bucket, as they are needed
+        self._no_shared = set()     # buckets whose sharing graph found no memory
         # One capture stream for all buckets, alive as long as the graphs: the kernels' workspace
         # is kept per stream, and a stream handle recycled by torch's pool while these graphs
         # exist would hand their workspace to unrelated calls.
@@ -54,6 +64,28 @@ class DecodeGraphs:
             if b >= n:
                 return b
         raise ValueError(f"batch of {n} rows is larger than the largest captured bucket")
+
+    def capture_shared(self, rows=None):
+        """Capture the sharing graph of a bucket (default: of all that may replay one) now, so that no step
+        has to.  Raises if there is no memory for it."""
+        for bucket in self.buckets if rows is None else [self._bucket(rows)]:
+            if self._may_share(bucket) and bucket not in self.shared_graphs:
+                self._capture(bucket, shared=True)
+                self._no_shared.discard(bucket)
+
+    def _may_share(self, rows):
+        return self.cache.device_tables and rows <= self.cache.SHARED_MAX_ROWS   # (padding rows count)
+
+    def _shared_ready(self, rows):
+        """Whether the bucket's sharing graph is there or can be captured."""
+        if rows not in self.shared_graphs and rows not in self._no_shared:
+            try:
+                self.capture_shared(rows)
+            except RuntimeError as error:
+                if not _out_of_memory(error):
+                    raise
+                self._no_shared.add(rows)
+        return rows in self.shared_graphs
 
     def _capture(self, rows, shared=False):
         dev, W, bs = self.cache.device, self.W, self.cache.block_size
@@ -120,10 +152,9 @@ class DecodeGraphs:
         n = len(seqs)
         rows = self._bucket(n)
         cache = self.cache
-        sharing = cache.device_tables and rows <= cache.SHARED_MAX_ROWS   # (padding rows count)
-        groups = cache.shared_groups(seqs) if sharing else None
-        if groups is not None and rows not in self.shared_graphs:
-            self._capture(rows, shared=True)
+        groups = cache.shared_groups(seqs) if self._may_share(rows) else None
+        if groups is not None and not self._shared_ready(rows):
+            groups = None
         graph, logits, bufs, copied = (self.graphs if groups is None else self.shared_graphs)[rows]
         copied.synchronize()             # the previous upload from these host buffers is done
         if cache.device_tables:
