@@ -143,16 +143,14 @@ class KVCache:
     # Default cap of one sequence's length: Qwen2.5's context window.
     DEFAULT_MAX_TOKENS_PER_SEQ = 32768
     DEFAULT_MAX_SEQS = 4096
-    # K and V bytes that a step would read again in a layer, from which its attention reads the
-    # shared blocks once; with less to save the plain kernels' smaller fixed cost wins.  One new
-    # token, us shared / plain: 16 rows over 1,024 shared keys of 2 heads (15 MB) 14.6 / 12.2, over 2,048
-    # (30 MB) 15.0 / 15.1; 4 rows over 4,096 keys of 4 heads (24 MB) 14.3 / 17.0, of 8 (48 MB) 14.7 /
-    # 20.5; 8 rows over 4,096 of 2 (28 MB) 15.0 / 16.6; 64 rows over 512 of 2 (31 MB) 16.9 / 14.6, over 1,024
-    # of 8 (252 MB) 21.8 / 35.0, over 31,000 of 2 (1.9 GB) 39 / 283.
-    SHARED_BYTES = 24 << 20
-    # New tokens of a row up to which that holds: with more, its own tiles are full and the work is
-    # bound by the matrix products (8 rows over 4,096 keys of 8 heads: 8 new tokens 29 / 52, 32 43 / 52,
-    # 64 63 / 55).
+    # K and V bytes that a step would read again in a layer, from which its attention reads the shared
+    # blocks once (sharing_pays has what else counts).  With less to save the plain kernels' smaller
+    # fixed cost wins.  us of a layer's attention shared / plain, K and V not in the caches, one new token:
+    # 16 rows over 1,024 shared keys of 2 heads (16 MB) 15.2 / 13.7, over 2,048 (31 MB) 15.5 / 17.0; 4 rows over 4,096
+    # of 4 (25 MB) 14.6 / 17.4, of 8 (50 MB) 16.6 / 22.5; 64 rows over 31,000 of 2 (2.0 GB) 38 / 251.
+    SHARED_BYTES = 20 << 20
+    # New tokens of a row up to which it may pay: with more its own tiles are full, and sharing saves no
+    # matrix products.
     SHARED_MAX_NEW = 32
     SHARED_MAX_ROWS = 512     # rows of a call of the kernel
 
@@ -398,10 +396,14 @@ class KVCache:
 
     def shared_groups(self, seqs):
         """(cu_rows, prefix tokens) of neighbouring rows that hold the same first blocks, or None if a
-        step over these rows would gain too little by reading them once."""
+        step of one token a row would gain too little by reading them once."""
+        groups = self._groups(seqs)
+        return groups if groups is not None and self.sharing_pays(seqs, groups) else None
+
+    def _groups(self, seqs):
         if not self._extra or not 2 <= len(seqs) <= self.SHARED_MAX_ROWS:
             return None
-        cu, prefix, saved = [0], [], 0
+        cu, prefix = [0], []
         rows, blocks = 1, 0       # of the group being formed
         tables = [self._block_tables[s] for s in seqs]
         for a, b in zip(tables, tables[1:]):
@@ -411,32 +413,68 @@ class KVCache:
             if joined and rows * joined >= (rows - 1) * blocks:
                 rows, blocks = rows + 1, joined
                 continue
-            saved += (rows - 1) * blocks
             cu.append(cu[-1] + rows)
             prefix.append(blocks * self.block_size)
             rows, blocks = 1, 0
-        saved += (rows - 1) * blocks
         cu.append(cu[-1] + rows)
         prefix.append(blocks * self.block_size)
-        block = 2 * self.block_size * self.buf.shape[3] * self.buf.shape[4] * self.buf.element_size()
-        return (cu, prefix) if saved * block >= self.SHARED_BYTES else None
+        return cu, prefix
 
-    def _shared_rows(self, seqs, counts, cu_q=None):
-        """The SharedRows of a step over `seqs`, or None; cu_q if they are on the device already."""
+    def sharing_pays(self, seqs, groups, new_tokens=None, splits=False, walk=0):
+        """Whether a step over `seqs` gains by reading what `groups` (cu_rows, prefix tokens) share once:
+        whether the bytes it would read again outweigh what the shared kernel costs more.  That grows with
+
+          the bytes that remain: it reads them at 5.4 TB/s, the plain decode kernel at 5.9
+          the rows: each has two parts to merge.  64 rows over 512 shared keys of 2 heads (33 MB saved)
+            take 17.6 us, plain 16.1; 256 rows of 500 keys, four of which share 16,384 more, 61.5 / 52.4
+          new_tokens (of all rows, default one each) beyond one a row: more pairs of each, 16 rows of up
+            to 16 over 512 keys of 8 heads 26.0 / 20.6
+          the tokens of a row where the plain kernel would cut its keys into pieces (splits: a step of
+            equal rows, few enough for it): 8 rows of 8 over 8,192 keys of 2 heads 25.9 / 22.5
+
+        and falls with the keys that a row of several tokens has (walk) where it does not cut them: there
+        one work-group walks them all (the same 8,192 keys under 32 rows 37.0 / 210.2), which the shared
+        kernel deals out.  All in proportion to SHARED_BYTES.  Of 1,373 measured steps with up to 32 new
+        tokens a row the rule sends 918 to the kernel, four of which are slower there by more than 5 %."""
+        cu, prefix = groups
+        rows = len(seqs)
+        more = 0 if new_tokens is None else new_tokens - rows
+        token = 2 * self.buf.shape[3] * self.buf.shape[4] * self.buf.element_size()
+        saved = sum((b - a - 1) * p for a, b, p in zip(cu, cu[1:], prefix))
+        rest = sum(self._lengths[s] for s in seqs) + rows + more - saved
+        cost = 1 + rest * token / (480 << 20) + rows / 52 + more / 110
+        if splits:
+            cost += 0.75 * more / rows
+        else:
+            cost = max(cost - walk / 700, 0.3)   # (0.3: none that saves less was measured)
+        return saved * token >= self.SHARED_BYTES * cost
+
+    def _shared_rows(self, seqs, counts, cu_q=None, query_heads=None):
+        """The SharedRows of a step over `seqs`, or None; cu_q if they are on the device already (a packed
+        step)."""
         if not self._extra or self.device.type != "cuda":
             return None
         rows = 0      # the leading ones with few new tokens
         while rows < len(seqs) and counts[rows] <= self.SHARED_MAX_NEW:
             rows += 1
-        groups = self.shared_groups(seqs[:rows])
+        seqs, counts = seqs[:rows], counts[:rows]
+        if max(counts, default=1) == 1:
+            groups = self.shared_groups(seqs)
+        else:
+            groups = self._groups(seqs)
+            # fa2_paged cuts the keys of a step of equal rows that leave compute units without work
+            splits = cu_q is None and (query_heads or 1) * rows <= 256
+            walk = max(self._lengths[s] + c for s, c in zip(seqs, counts) if c > 1)
+            if groups is not None and not self.sharing_pays(seqs, groups, sum(counts), splits, walk):
+                groups = None
         if groups is None:
             return None
         cu, prefix = groups
         g = len(prefix)
-        offsets = [] if cu_q is not None else np.concatenate([[0], np.cumsum(counts[:rows])])
+        offsets = [] if cu_q is not None else np.concatenate([[0], np.cumsum(counts)])
         up = self._upload(cu, prefix, offsets)
         return SharedRows(rows=rows, cu_q=up[2 * g + 1:] if cu_q is None else cu_q[:rows + 1],
-                          cu_rows=up[:g + 1], prefix_lens=up[g + 1:2 * g + 1], max_q=max(counts[:rows]))
+                          cu_rows=up[:g + 1], prefix_lens=up[g + 1:2 * g + 1], max_q=max(counts))
 
     def _upload(self, *parts):
         """Lists of numbers (or of rows of them) as one flat int32 tensor on the device."""
@@ -494,9 +532,11 @@ class KVCache:
         sm[B:] = -1
         return host, starts, W
 
-    def prepare(self, seqs, T):
+    def prepare(self, seqs, T, query_heads=None):
+        """The metadata of a step that appends T tokens to each of seqs.  query_heads: the model's, which
+        decide with T > 1 from how much on shared blocks are read once (unknown: from more)."""
         if self.device_tables:
-            return self._prepare_device(seqs, [T] * len(seqs), packed=False)
+            return self._prepare_device(seqs, [T] * len(seqs), packed=False, query_heads=query_heads)
         B = len(seqs)
         host, starts, W = self.pack_step(seqs, T)
         tables = [self._block_tables[s] for s in seqs]
@@ -511,7 +551,7 @@ class KVCache:
             block_table=dev[2 * B:2 * B + B * W].view(B, W),
             slot_mapping=dev[2 * B + B * W:].long(),
             slot_mapping32=dev[2 * B + B * W:],
-            tables=[list(t) for t in tables], shared=self._shared_rows(seqs, [T] * B))
+            tables=[list(t) for t in tables], shared=self._shared_rows(seqs, [T] * B, None, query_heads))
 
     def prepare_packed(self, seqs, counts):
         """Grow the rows' tables for counts[b] new tokens each and build a PackedMeta with one
@@ -558,7 +598,7 @@ class KVCache:
             block_table=dev[o + 2 * N + B:].view(B, W), tables=[list(t) for t in tables],
             shared=self._shared_rows(seqs, counts, dev[:B + 1]))
 
-    def _prepare_device(self, seqs, counts, packed):
+    def _prepare_device(self, seqs, counts, packed, query_heads=None):
         """The device-table path of prepare / prepare_packed: one pinned copy of the rows' slots
         (and packed offsets), one metadata launch; tables and lengths never leave the device."""
         from kernels.meta import step_metadata
@@ -587,7 +627,7 @@ class KVCache:
             return StepMeta(starts=starts, T=counts[0], block_size=bs, starts_dev=o_starts,
                             kv_lens=o_kv, slot_mapping=None, block_table=o_bt,
                             slot_mapping32=o_slots, tables=tables,
-                            shared=self._shared_rows(seqs, counts))
+                            shared=self._shared_rows(seqs, counts, None, query_heads))
         n_single = 0
         while n_single < B and counts[n_single] == 1:
             n_single += 1

@@ -345,7 +345,7 @@ class Qwen2ForCausalLM(nn.Module):
         """input_ids [B, T] appended to cache sequences `seqs`; returns last-position logits
         [B, 1, vocab] (model.py:157-207)."""
         _, T = input_ids.shape
-        meta = cache.prepare(seqs, T)
+        meta = cache.prepare(seqs, T, self.cfg.num_heads)
         logits = self.forward_meta(input_ids, cache, meta)
         cache.advance(seqs, T)
         return logits
