@@ -178,10 +178,10 @@ def fork_rows(pool, tables, lens, children, block_size):
     plan = _PLANS.get(key)
     if plan is None:
         plan = _plan(key, _fork_plan, pool, tables, lens, children, block_size)
-    device, fn, shape, table, n_seqs, n = plan
-    if n:
+    device, fn, shape, table, n_seqs, parts = plan
+    for first, n in parts:
         call(device, fn, pool.data_ptr(), *shape, tables.data_ptr(), *table, lens.data_ptr(), n_seqs,
-              children.data_ptr(), n)
+              children.data_ptr() + 16 * first, n)
 
 
 def _fork_plan(pool, tables, lens, children, block_size):
@@ -190,9 +190,10 @@ def _fork_plan(pool, tables, lens, children, block_size):
     stride, width, n_seqs = _table(tables, pool.device)
     _ids(lens, "lens", (n_seqs,), pool.device)
     _ids(children, "children", (None, 4), pool.device)
+    n = children.shape[0] if n_seqs else 0
     return (pool.device.index, load().mi_cache_fork_rows,
             (step, blocks, planes, block_size, size // block_size), (stride, width), n_seqs,
-            children.shape[0] if n_seqs else 0)
+            _parts(n, planes, size, n) if n else [])
 
 
 def move_blocks(pool, tables, rows, pairs, new_ids, block_size):
