@@ -313,14 +313,19 @@ class KVCache:
         for b in table[:whole]:
             self._holders[b] += n
         self._extra += n * whole
-        if self.device_tables:
-            from kernels.blocks import fork_rows
-            slot = self.slot[seq]
-            rows = [[slot, self.slot[c], length, fresh[i] if rest else -1]
-                    for i, c in enumerate(forks)]
-            fork_rows(self.buf, self.dev_tables, self.dev_lens, self._upload(rows).view(n, 4), bs)
-        elif rest:
-            self._copy([(table[whole], b) for b in fresh])
+        try:
+            if self.device_tables:
+                from kernels.blocks import fork_rows
+                slot = self.slot[seq]
+                rows = [[slot, self.slot[c], length, fresh[i] if rest else -1]
+                        for i, c in enumerate(forks)]
+                fork_rows(self.buf, self.dev_tables, self.dev_lens, self._upload(rows).view(n, 4), bs)
+            elif rest:
+                self._copy([(table[whole], b) for b in fresh])
+        except Exception:
+            for child in forks:
+                self.free(child)
+            raise
         return forks
 
     def copy_from(self, other, seq):
@@ -334,14 +339,14 @@ class KVCache:
         mine = self.alloc()
         try:
             self.ensure_capacity(mine, length)
-        except RuntimeError:
+            self._copy(list(zip(other._block_tables[seq], self._block_tables[mine])), other)
+            if self.device_tables:
+                slot = self.slot[mine]
+                self.dev_lens[slot:slot + 1].fill_(length)
+        except Exception:
             self.free(mine)
             raise
         self._lengths[mine] = length
-        self._copy(list(zip(other._block_tables[seq], self._block_tables[mine])), other)
-        if self.device_tables:
-            slot = self.slot[mine]
-            self.dev_lens[slot:slot + 1].fill_(length)
         return mine
 
     def compact(self):
@@ -351,16 +356,10 @@ class KVCache:
         src = [b for b in range(used, self.num_blocks) if self._holders[b]]
         dst = [b for b in range(used) if not self._holders[b]]
         new_ids = list(range(self.num_blocks))
-        for a, b in zip(src, dst):
-            new_ids[a] = b
-            self._holders[b], self._holders[a] = self._holders[a], 0
-        self._free_blocks = list(range(self.num_blocks - 1, used - 1, -1))
-        if not src:
-            return used
-        for table in self._block_tables.values():
-            table[:] = [new_ids[b] for b in table]
         pairs = list(zip(src, dst))
-        if self.device_tables:
+        for a, b in pairs:
+            new_ids[a] = b
+        if pairs and self.device_tables:
             from kernels.blocks import move_blocks
             rows = [(self.slot[s], len(t)) for s, t in self._block_tables.items() if t]
             ids = self._upload(pairs + rows, new_ids)
@@ -369,6 +368,13 @@ class KVCache:
                         self.block_size)
         else:
             self._copy(pairs)
+        # (the books follow what was moved)
+        for a, b in pairs:
+            self._holders[b], self._holders[a] = self._holders[a], 0
+        if pairs:
+            for table in self._block_tables.values():
+                table[:] = [new_ids[b] for b in table]
+        self._free_blocks = list(range(self.num_blocks - 1, used - 1, -1))
         return used
 
     def reclaimable(self, seqs):
