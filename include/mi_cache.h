@@ -79,7 +79,8 @@ MI_CACHE_API int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t n
  *
  * q, o [cu_seqlens_q[batch]][heads_q][128] with strides (token, head), pools [slots][heads_kv][128]
  * with strides (slot, head), lse strides (head, token).  total_q: the tokens of q, at least
- * cu_seqlens_q[batch].  At most 512 rows and 2^25 (token, head) pairs, n_groups <= batch.  workspace:
+ * cu_seqlens_q[batch].  At most 512 rows, 2^25 (token, head) pairs and
+ * max_kv_len 2^31 - 8193, n_groups <= batch.  workspace:
  * mi_cache_attend_workspace_size bytes, 16-byte aligned, contents arbitrary; not shared by calls that
  * may overlap in time.
  */

@@ -231,6 +231,9 @@ int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool, const void
   if (n_groups < 0 || n_groups > batch)
     return fail(kInvalid, "n_groups %d: 0 to batch (%d)", n_groups, batch);
   if (max_kv_len < 0) return fail(kInvalid, "max_kv_len %d < 0", max_kv_len);
+  // a step ends up to 128 keys behind the last one; positions are 32-bit
+  if (max_kv_len > INT32_MAX - 8192)
+    return fail(kUnsupported, "max_kv_len %d: at most 2^31 - 8193", max_kv_len);
   if (block_size < 16 || (block_size & (block_size - 1)))
     return fail(kUnsupported, "block_size %d is not a power of two >= 16", block_size);
   if (num_blocks < 0) return fail(kInvalid, "num_blocks %d < 0", num_blocks);
