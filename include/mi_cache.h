@@ -46,8 +46,8 @@ MI_CACHE_API int mi_cache_copy_blocks(const void* src, int64_t src_plane_bytes,
  *   tables[child][0, w) = tables[parent][0, w), seq_lens[child] = L, and where r > 0
  *   tables[child][w] = new block, whose first r tokens in every plane become those of the parent's
  *   block w.  (Where r == 0 the new block is not looked at.)
- * A child whose slots, length or blocks are out of range, or whose two slots are the same, is skipped
- * whole.  No child slot or new block may occur twice, and no child slot may be a parent slot.
+ * A child whose slots, length, new block or copied block are out of range, or whose two slots are the
+ * same, is skipped whole (the entries of whole blocks are copied as they stand).  No child slot or new block may occur twice, and no child slot may be a parent slot.
  */
 MI_CACHE_API int mi_cache_fork_rows(void* pool, int64_t plane_bytes, int32_t num_blocks,
                                     int32_t planes, int32_t block_size, int64_t token_bytes,
@@ -72,17 +72,18 @@ MI_CACHE_API int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t n
  * mi_fa2_fwd_paged_varlen (head_dim 128; bf16 0, fp16 1; bottom-right causal; a query that sees no key
  * gives 0 and an lse of -inf; keys at or past kv_lens are never read as data), and the groups:
  * cu_rows [n_groups + 1], prefix_lens [n_groups]: rows [cu_rows[g], cu_rows[g + 1]) hold the same
- * first prefix_lens[g] tokens, which are read once for all of them, through the table of the group's
- * first row.  A prefix is used as far as every query of its group sees it and the first row holds it;
+ * first prefix_lens[g] tokens, which are read for all of them together, through the table of the group's
+ * first row.  A prefix is used as far as every query of its group sees it and the first row holds it, and
+ * where that costs less than the rows by themselves (not where each has tiles of queries of its own);
  * what is left of it, and a row of no group, is read through the row's own table.  Empty groups may
  * stand anywhere; where groups overlap, a row can only be in the one that begins last before it.
+ * A query that sees a NaN, in a score or a value, gets NaN.
  *
  * q, o [cu_seqlens_q[batch]][heads_q][128] with strides (token, head), pools [slots][heads_kv][128]
  * with strides (slot, head), lse strides (head, token).  total_q: the tokens of q, at least
- * cu_seqlens_q[batch].  At most 512 rows, 2^25 (token, head) pairs and
- * max_kv_len 2^31 - 8193, n_groups <= batch.  workspace:
- * mi_cache_attend_workspace_size bytes, 16-byte aligned, contents arbitrary; not shared by calls that
- * may overlap in time.
+ * cu_seqlens_q[batch].  At most 512 rows, 2^25 (token, head) pairs and a max_kv_len of 2^31 - 8193;
+ * n_groups <= batch.  workspace: mi_cache_attend_workspace_size bytes, 16-byte aligned, contents
+ * arbitrary; not shared by calls that may overlap in time.
  */
 MI_CACHE_API size_t mi_cache_attend_workspace_size(int32_t total_q, int32_t heads_q);
 MI_CACHE_API int mi_cache_attend(int32_t dtype, const void* q, const void* k_pool,

@@ -11,7 +11,9 @@ constexpr int kBoThreads = 256;
 constexpr int kBoPiece = 16384;  // bytes of a block per work-group
 
 // bytes [0, n) of src to dst by the work-group, U at a time, four loads of a thread in flight.  What is
-// written is not read again soon (non-temporal); NT: nor is what is read.
+// written goes past the caches (non-temporal): blocks copied or moved are not read soon.  (A fork's started
+// block is, by the child's next step: at most 8 KB a child and plane with the engine's blocks, from the last-level
+// cache or memory.)  NT: what is read goes past them too.
 template <typename U, bool NT>
 __device__ __forceinline__ void copy_span(uint8_t* dst, const uint8_t* src, int n) {
   constexpr int kFlight = 4;

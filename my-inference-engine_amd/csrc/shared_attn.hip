@@ -6,6 +6,8 @@
 // So the keys are cut by who holds them: the prefix of a group of rows (one range for all the group's
 // queries) and each row's keys behind it.  All query heads of a kv head read the same keys, so a
 // range's queries are its (token, head) pairs: column p of a tile is token p / group, head p % group.
+// A prefix that costs more that way than every row by itself (rows whose own pairs fill tiles: sharing saves
+// them no matrix products) is not shared (shared_keys).
 //
 // Ranges, and the work.  Range s < B is the prefix of the group that row s leads, range B + b row b's
 // own keys.  A range of up to 32 pairs is narrow: its items (kv head) are walked by single waves, 64
@@ -28,10 +30,13 @@
 // What bounds it.  A wide step takes about 4,300 cycles, of which the MFMAs are 2,048 on each SIMD and LDS is
 // busy for 2,560 (3,700 without the loads); with all CUs at it 2.3 us at the 1.83 GHz they then hold, 930
 // TFLOP/s.  A call costs about 10 us beside its steps: launch 2, plan 1.5, first loads and queries 2.5, the
-// parts' way out 2, the merge 3 to 4.  Replayed, 12 heads of 2 kv heads: 2 rows of 100 keys 10.4 us, 16
-// branches of 2,048 keys 15.2 (each row's keys read for it alone: 17), 40 rows in 9 groups (52 MB of keys) 21.5
-// (39), 8 rows of 90 to 150 new tokens over 5,000 keys and up to 900 of their own 58 (78), 64 branches of
-// 31,000 keys 39 (283).
+// parts' way out 2, the merge 3 to 4.  Replayed at the clock of steady work, keys in the caches, 12 heads of 2
+// kv heads: 2 rows of 100 keys 10.2 us (each row's keys read for it alone by the paged kernels: 6.6), 16 branches
+// of 2,048 keys 15.0 (14.8; from memory 15.5 and 17.0), 40 rows in 9 groups (52 MB of keys) 20.8 (36.6), 12 rows of
+// 1 to 17 new tokens over 3,001 keys 23.3 (41.5), 64 branches of 31,000 keys 38 (267), 8 rows of 90 to 150 new tokens
+// over 5,000 keys and up to 900 of their own 54 (73): these share nothing, and gain by keys dealt out evenly.
+// A prefix of several tiles is fetched into the L2s by each of them (64 branches of 31,000 keys: three tiles, 131
+// MB, of which 65 are distinct; an XCD's share is less than one of the tiles, so they do not meet in its L2).
 #include "cache_ops.h"
 
 #include <type_traits>
@@ -50,8 +55,8 @@ constexpr int kShWideCost = 4, kShNarrowCost = 1;
 constexpr int kShMergeCost = 4;   // of one more wide part for each pair, in the merge
 constexpr int kShNarrowWeight = 7;
 // Narrow shares go to as many work-groups as there is room for, a wave each, then a second wave of each: 64 keys
-// that a wave has to itself arrive sooner than with seven more of its CU's (2 rows of 100 keys 11.1 -> 10.4 us,
-// drawn rows 14.6 -> 12.3 and 12.9 -> 10.8).  From kShSpread shares for each work-group on a wave takes kShEach, so that
+// that a wave has to itself arrive sooner than with seven more of its CU's (2 rows of 100 keys 11.1 -> 10.4
+// us).  From kShSpread shares for each work-group on a wave takes kShEach, so that
 // an item leaves fewer parts (40 rows in 9 groups, 52 MB, 24.6 -> 21.5 us; two each 22.7), or more where
 // eight waves of each do not do, and no more waves than that takes (172 rows of 34 groups 30.9 -> 29.6).
 constexpr int kShSpread = 4, kShEach = 3;
@@ -441,6 +446,9 @@ __device__ __forceinline__ void hide(f32x16& s, int lim) {
 //   p = 2^(c (s - m)): the difference first, so that scores of any size keep their weights.  The
 // reference m may lag the true maximum while no p of the lane exceeds 2^8, as in the prefill kernel.
 // The first keys of a walk (fresh) have no reference yet.
+//   P is rounded to the 16-bit type, as the MFMA takes it and as the other attention kernels here do; the
+// sum is of the rounded values, so that the weights still add up to one.  In bf16 the output is then 0.0021 to
+// 0.0023 of its size off from 64 bits, 0.0017 with P in 32 bits (the rounding of the output alone).
 template <typename E, int N>
 __device__ __forceinline__ void softmax(float c, ShState& st, const f32x16 (&s)[N], u32x4 (&pb)[2 * N],
                                         bool fresh) {
@@ -904,8 +912,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   const int W1 = min(W - W3, N1);
 
   if ((int)blockIdx.x < W1) {
-    // work-group w runs on XCD w % 8: XCD x takes the x-th contiguous share of the work, so that tiles of one
-    // range meet in its L2
+    // work-group w runs on XCD w % 8: XCD x takes the x-th contiguous share of the work, so that its L2 holds what
+    // its share reads.  (Tiles of one range meet in an L2 only if the share holds more than one of them.)
     const int x = blockIdx.x & 7, wg = x * (W1 >> 3) + min(x, W1 & 7) + ((int)blockIdx.x >> 3);
     const ShDeal deal = make_deal(N1, W1);
     int u = first_of(deal, wg);

@@ -2,8 +2,8 @@
 (csrc/shared_attn.hip, through libmi_cache.so, the C ABI in include/mi_cache.h).
 
 `fa2_paged_shared` is `fa2_paged_varlen` for a step some of whose rows are branches of one history
-(KVCache.fork): it takes the groups of rows that share blocks and reads the shared ones once for
-a group's rows, where the reference (and fa2_paged, fa2_paged_varlen) reads every row's keys for
+(KVCache.fork): it takes the groups of rows that share blocks and reads the shared ones for all of
+a group's rows together, where the reference (and fa2_paged, fa2_paged_varlen) reads every row's keys for
 that row alone (model.py:97,103).  No CPU path: CPU tensors are rejected.
 """
 import math
@@ -32,13 +32,15 @@ def fa2_paged_shared(q, k_pool, v_pool, cu_seqlens_q, block_table, kv_lens, max_
     cu_rows      [G + 1] int32, prefix_lens [G] int32, G <= rows: rows [cu_rows[g], cu_rows[g+1])
                  hold the same first prefix_lens[g] tokens (rows of no group share nothing).  They are
                  read through the table of the group's first row, as far as every query of the group
-                 sees them.
+                 sees them and where that costs less than the rows by themselves.
     is_causal    bottom-right aligned per row (query i of row b sees keys <= i + kv_len - T_b)
     out          optional [total_q, Hq, 128] output (any token/head strides); tokens of no row keep
                  what they hold
     More than 512 rows go to fa2_paged_varlen, which reads every row's keys for that row alone.
-    Worth it from tens of MB of K and V that the rows would read again (KVCache.SHARED_BYTES has both sides'
-    times); with more than a few tens of new tokens a row fa2_paged_varlen is faster.
+    Worth it from tens of MB of K and V that the rows would read again (KVCache.sharing_pays has both
+    sides' times).  Rows of more than a few tens of new tokens have full tiles of their own, and sharing saves
+    them nothing: fa2_paged_varlen is faster (64 rows of up to 150 over 512 keys of 4 kv heads 66 us, here 107),
+    but for few rows over long keys, which it does not cut (8 of 150 over 5,000 of 2 heads 73, here 54).
     Returns O [total_q, Hq, 128] (and the fp32 LSE [Hq, total_q] if return_lse).
     """
     # plain values only: the plan is looked up by them
