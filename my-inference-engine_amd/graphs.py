@@ -134,10 +134,12 @@ class DecodeGraphs:
                     torch.zeros(rows, 1, dtype=torch.long).pin_memory())
         side = self._side
         side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side), torch.no_grad():
-            for _ in range(2):                       # allocations and workspaces happen here
-                step()
-        torch.cuda.current_stream(dev).wait_stream(side)
+        try:
+            with torch.cuda.stream(side), torch.no_grad():
+                for _ in range(2):                   # allocations and workspaces happen here
+                    step()
+        finally:      # a step that fails frees the buffers, which the work before it may still use
+            torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph), torch.no_grad():

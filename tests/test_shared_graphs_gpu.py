@@ -91,6 +91,33 @@ def test_other_errors_are_raised(monkeypatch):
     assert lengths == [cache.length(s) for s in seqs]
 
 
+def test_a_capture_that_fails_is_waited_for(monkeypatch):
+    """A warm-up step that runs out of memory leaves the one before it running on the capture stream, over
+    buffers that are free then: what follows on this stream waits for it."""
+    model, cache, seqs, g = start()
+    graphs = DecodeGraphs(model, cache, buckets=(4,))
+    waits, run, calls = [], model.forward_meta, []
+
+    wait = torch.cuda.Stream.wait_stream
+
+    def noted(self, other):
+        waits.append(other)
+        wait(self, other)
+    monkeypatch.setattr(torch.cuda.Stream, "wait_stream", noted)
+
+    def second_fails(*args):
+        calls.append(args)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no memory")
+        return run(*args)
+    monkeypatch.setattr(model, "forward_meta", second_fails)
+    with pytest.raises(torch.OutOfMemoryError):
+        graphs.capture_shared()
+    assert len(calls) == 2 and waits[-1] == graphs._side
+    monkeypatch.undo()
+    steps(model, cache, seqs, graphs, g)
+
+
 def test_host_tables_capture_none():
     model, _ = make("cuda", torch.bfloat16)
     cache = KVCache(100, 16, "cuda", torch.bfloat16, SMALL.num_layers, SMALL.num_kv_heads,
