@@ -77,7 +77,7 @@ MI_CACHE_API int mi_cache_move_blocks(void* pool, int64_t plane_bytes, int32_t n
  * where that costs less than the rows by themselves (not where each has tiles of queries of its own);
  * what is left of it, and a row of no group, is read through the row's own table.  Empty groups may
  * stand anywhere; where groups overlap, a row can only be in the one that begins last before it.
- * A query that sees a NaN, in a score or a value, gets NaN.
+ * A NaN that a query sees shows: a score's in all of its o and in its lse, a value's in that dim.
  *
  * q, o [cu_seqlens_q[batch]][heads_q][128] with strides (token, head), pools [slots][heads_kv][128]
  * with strides (slot, head), lse strides (head, token).  total_q: the tokens of q, at least
