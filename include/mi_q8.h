@@ -1,0 +1,116 @@
+/*
+ * C ABI of libmi_q8.so: the projections of a decoder layer in 8-bit integers on MI355X (gfx950), with
+ * the norm, activation, bias and residual around them.
+ *
+ * The reference has no 8-bit path: these stand for its nn.Linear calls (model.py:81-84,107,112-120,
+ * 204-207) with the RMSNorm before (model.py:49-55) and the residual add after them (model.py:128-138)
+ * in a model whose projections are held in 8 bits.
+ *
+ * Rows in 8 bits.  A row v of n numbers is held as n int8 and one fp32 scale:
+ *   scale = max(max |v|, 2^-100) / 127,   value = round_half_even(v / scale), at most 127 in size.
+ * A row that holds an infinity or a NaN has scale NaN (and zeros), so that whatever is computed from
+ * it is NaN.  values: [rows][mi_q8_row_bytes(n)], 16-byte aligned, zeros from n on.
+ *
+ * Weights in 8 bits.  int8 [out_features][in_features] and one fp32 scale for each out feature, the
+ * values laid out by mi_q8_pack once.  A gated weight (the gate and up rows of a feed-forward block,
+ * gate rows first) is laid out for mi_q8_mlp and used by nothing else.
+ *
+ * A product is sum_k x[m][k] w[n][k], a whole number in 32 bits (exact, in_features <= 131072), times
+ * the two scales in fp32; bias and residual are added in fp32 and the sum is rounded once.
+ *
+ * Common rules.  dtype: 0 bf16, 1 fp16 (everything that is not int8 or fp32 here).  Row strides are in
+ * elements, at least the row's length, any alignment of rows (rows whose addresses are multiples of 16
+ * bytes are faster).  Sizes: in_features at most 131072, out_features at most 2^24, rows at most 2^21.
+ * All launches are asynchronous on `stream`, allocate nothing and may be captured in a graph.
+ * Workspaces: 16-byte aligned, contents arbitrary, not shared by calls that may overlap in time.
+ *
+ * Status codes as in mi_fa2.h: 0 ok, 1 invalid argument, 2 unsupported, 3 workspace too small,
+ * 4 launch failed; mi_q8_last_error() gives the calling thread's last message.
+ */
+#ifndef MI_Q8_H
+#define MI_Q8_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MI_Q8_API __attribute__((visibility("default")))
+
+MI_Q8_API const char* mi_q8_last_error(void);
+
+/* Bytes of a row of n values: n rounded up to a multiple of 128. */
+MI_Q8_API int64_t mi_q8_row_bytes(int32_t n);
+
+/* Rows x [rows, n] in 8 bits. */
+MI_Q8_API int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values,
+                             float* scale, int32_t rows, int32_t n, void* stream);
+
+/*
+ * r = x + y, rounded (y NULL: r is x, and residual_out is not used); values and scale are the rows of
+ * r * rsqrt(mean(r^2) + eps) * weight in 8 bits, taken in fp32 without a rounding in between.
+ * residual_out may be x or y.
+ */
+MI_Q8_API int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
+                                int64_t y_stride, const void* weight, float eps,
+                                void* residual_out, int64_t residual_stride, void* values,
+                                float* scale, int32_t rows, int32_t n, void* stream);
+
+/* out [rows, n] = values * scale, rounded. */
+MI_Q8_API int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
+                               int64_t out_stride, int32_t rows, int32_t n, void* stream);
+
+/*
+ * A weight's values (int8, rows of in_features, `stride` bytes apart) in the products' layout:
+ * mi_q8_packed_bytes() bytes, 16-byte aligned.  gated: out_features is even, gate rows first.
+ */
+MI_Q8_API size_t mi_q8_packed_bytes(int32_t out_features, int32_t in_features, int32_t gated);
+MI_Q8_API int mi_q8_pack(const void* values, int64_t stride, int32_t out_features,
+                         int32_t in_features, int32_t gated, void* packed, void* stream);
+
+/*
+ * out = [residual +] x W^T [+ bias] of rows already in 8 bits: values, scale [rows] as mi_q8_quantize
+ * leaves them, w packed, w_scale [out_features], bias [out_features] or NULL, residual
+ * [rows, out_features] or NULL (may be out).
+ */
+MI_Q8_API size_t mi_q8_matmul_workspace_size(int32_t rows, int32_t out_features,
+                                             int32_t in_features);
+MI_Q8_API int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
+                           const float* w_scale, const void* bias, const void* residual,
+                           int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
+                           int32_t out_features, int32_t in_features, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
+ * The same of rows x [rows, in] that the call holds in 8 bits itself, as mi_q8_add_rmsnorm does without
+ * y (norm_weight) or as mi_q8_quantize does (norm_weight NULL).  out must not overlap x.
+ */
+MI_Q8_API size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features,
+                                             int32_t in_features);
+MI_Q8_API int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight,
+                           float eps, const void* w, const float* w_scale, const void* bias,
+                           const void* residual, int64_t residual_stride, void* out,
+                           int64_t out_stride, int32_t rows, int32_t out_features,
+                           int32_t in_features, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/*
+ * A gated feed-forward block, out = [residual +] a Wd^T with a = silu(g) * u in fp32, held in 8 bits
+ * for the second product, and (g | u) = [rmsnorm] x Wgu^T: x, out, residual [rows, hidden], gate_up
+ * packed as gated [2 * inter, hidden], down packed [hidden, inter].  out may be x and residual.
+ */
+MI_Q8_API size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter);
+MI_Q8_API int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight,
+                        float eps, const void* gate_up, const float* gate_up_scale,
+                        const void* down, const float* down_scale, const void* residual,
+                        int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
+                        int32_t hidden, int32_t inter, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* MI_Q8_H */

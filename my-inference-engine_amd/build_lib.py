@@ -1,11 +1,13 @@
-"""Build libmi_fa2.so, libmi_model.so and libmi_cache.so (the HIP kernels + C ABIs) in-tree with hipcc for gfx950.
+"""Build libmi_fa2.so, libmi_model.so, libmi_cache.so and libmi_q8.so (the HIP kernels + C ABIs) in-tree with hipcc
+for gfx950.
 
     python my-inference-engine_amd/build_lib.py
 
 Compiles every source of csrc/ in parallel into _build/ and links kernels/libmi_fa2.so (attention,
 sampling, step metadata; loaded by kernels/_lib.py), kernels/libmi_model.so (the projections of
-few rows; loaded by kernels/few_rows.py) and kernels/libmi_cache.so (block operations and attention
-over shared blocks; loaded by kernels/blocks.py).  Always rebuilds (a few seconds per file).
+few rows; loaded by kernels/few_rows.py), kernels/libmi_cache.so (block operations and attention
+over shared blocks; loaded by kernels/blocks.py) and kernels/libmi_q8.so (projections in 8 bits;
+loaded by kernels/q8.py).  Always rebuilds (a few seconds per file).
 """
 import os
 import subprocess
@@ -23,6 +25,7 @@ LIBS = {
           "rope_kv.hip", "sample.hip", "step_meta.hip", "model_ops.hip", "fa2_capi.cpp"],
     PKG / "kernels" / "libmi_model.so": ["linear_rows.hip", "model_capi.cpp"],
     PKG / "kernels" / "libmi_cache.so": ["block_ops.hip", "shared_attn.hip", "cache_capi.cpp"],
+    PKG / "kernels" / "libmi_q8.so": ["q8_quant.hip", "q8_rows.hip", "q8_capi.cpp"],
 }
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

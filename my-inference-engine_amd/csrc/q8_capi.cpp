@@ -1,0 +1,396 @@
+// C ABI of libmi_q8.so: argument checks and launches of the 8-bit projections.  The contract of every
+// entry point is in include/mi_q8.h.
+#include "mi_q8.h"
+
+#include <hip/hip_runtime.h>
+
+#include <atomic>
+#include <cstdarg>
+#include <cstdio>
+
+#include "q8.h"
+
+namespace {
+
+using mi_fa2::Q8Params;
+using mi_fa2::Q8QuantParams;
+using mi_fa2::q8_pad;
+
+enum Status { kOk = 0, kInvalid = 1, kUnsupported = 2, kWorkspace = 3, kLaunch = 4 };
+
+thread_local char g_err[256] = "";
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int ok() {
+  g_err[0] = '\0';
+  return kOk;
+}
+
+int launched(hipError_t err) {
+  if (err != hipSuccess) return fail(kLaunch, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The current device's compute units, read once per device.
+int compute_units(int* out) {
+  static std::atomic<int> known[64];
+  int dev = -1;
+  *out = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err == hipSuccess && dev >= 0 && dev < 64) *out = known[dev].load(std::memory_order_relaxed);
+  if (err == hipSuccess && *out == 0) {
+    err = hipDeviceGetAttribute(out, hipDeviceAttributeMultiprocessorCount, dev);
+    if (err == hipSuccess && dev < 64) known[dev].store(*out, std::memory_order_relaxed);
+  }
+  if (err != hipSuccess || *out <= 0)
+    return fail(kLaunch, "reading the device's CU count failed: %s", hipGetErrorString(err));
+  return kOk;
+}
+
+constexpr int32_t kMaxRows = 1 << 21, kMaxOut = 1 << 24, kMaxK = mi_fa2::kQ8MaxK;
+
+int check_dtype(int32_t dtype) {
+  if (dtype != 0 && dtype != 1)
+    return fail(kUnsupported, "dtype %d is not bf16 (0) or fp16 (1)", dtype);
+  return kOk;
+}
+
+int check_count(const char* name, int64_t n, int64_t least, int64_t most) {
+  if (n < least || n > most)
+    return fail(kInvalid, "%s %lld: %lld to %lld", name, (long long)n, (long long)least,
+                (long long)most);
+  return kOk;
+}
+
+int check_ptr(const char* name, const void* p, int align) {
+  if (!p) return fail(kInvalid, "%s is NULL", name);
+  if (!aligned(p, align)) return fail(kInvalid, "%s is not %d-byte aligned", name, align);
+  return kOk;
+}
+
+// Rows of 16-bit elements.
+int check_rows(const char* name, const void* p, int64_t stride, int64_t width) {
+  if (int rc = check_ptr(name, p, 2)) return rc;
+  if (stride < width || stride >= int64_t(1) << 40)
+    return fail(kInvalid, "%s row stride %lld: at least %lld", name, (long long)stride,
+                (long long)width);
+  return kOk;
+}
+
+// Rows that lanes read and write 16 bytes at a time.
+bool wide(const void* p, int64_t stride, int32_t n) {
+  return !p || (aligned(p, 16) && stride % 8 == 0 && n % 8 == 0);
+}
+bool quads(const void* p, int64_t stride) { return !p || (aligned(p, 8) && stride % 4 == 0); }
+
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+int64_t span(int32_t rows, int64_t stride, int32_t n) { return 2 * ((rows - 1) * stride + n); }
+
+// A workspace's parts, each at a multiple of 256 bytes.
+struct Space {
+  size_t total = 0;
+  size_t take(size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) & ~size_t(255);
+    return at;
+  }
+};
+
+// Rows in 8 bits in a workspace.
+struct RowsSpace {
+  size_t values, scale;
+  RowsSpace(Space& s, int32_t rows, int32_t n)
+      : values(s.take((size_t)rows * q8_pad(n))), scale(s.take((size_t)rows * 4)) {}
+};
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (need == 0) return kOk;
+  if (int rc = check_ptr("workspace", ws, 16)) return rc;
+  if (have < need) return fail(kWorkspace, "workspace of %zu bytes needed, %zu given", need, have);
+  return kOk;
+}
+
+int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t y_stride,
+             const void* norm_weight, float eps, void* r, int64_t r_stride, void* values,
+             float* scale, int32_t rows, int32_t n, void* stream) {
+  Q8QuantParams p{};
+  p.x = x;
+  p.x_st = x_stride;
+  p.y = static_cast<const uint16_t*>(y);
+  p.y_st = y_stride;
+  p.norm_w = static_cast<const uint16_t*>(norm_weight);
+  p.eps = eps;
+  p.r_out = static_cast<uint16_t*>(r);
+  p.r_st = r_stride;
+  p.q = static_cast<int8_t*>(values);
+  p.scale = scale;
+  p.M = rows;
+  p.n = n;
+  p.np = q8_pad(n);
+  p.wide = wide(x, x_stride, n) && wide(y, y_stride, n) && wide(norm_weight, 8, n) &&
+           (!y || wide(r, r_stride, n));
+  return launched(mi_fa2::launch_q8_quant(p, dtype, norm_weight ? mi_fa2::kQ8Norm : mi_fa2::kQ8Plain,
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+
+int matmul(int dtype, const void* values, const float* scale, const void* w, const float* w_scale,
+           const void* bias, const void* res, int64_t res_stride, void* out, int64_t out_stride,
+           int32_t rows, int32_t out_features, int32_t in_features, bool gated, void* stream) {
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  Q8Params p{};
+  p.x = static_cast<const int8_t*>(values);
+  p.x_scale = scale;
+  p.w = static_cast<const int8_t*>(w);
+  p.w_scale = w_scale;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.res = static_cast<const uint16_t*>(res);
+  p.res_st = res_stride;
+  p.out = out;
+  p.out_st = out_stride;
+  p.M = rows;
+  p.N = out_features;
+  p.Kp = q8_pad(in_features);
+  p.panels = mi_fa2::q8_panels(gated ? 2 * out_features : out_features, gated);
+  p.quads = quads(bias, 4) && quads(res, res_stride) && quads(out, out_stride);
+  return launched(
+      mi_fa2::launch_q8_rows(p, dtype, gated, cus, reinterpret_cast<hipStream_t>(stream)));
+}
+
+struct MlpSpace {
+  Space s;
+  RowsSpace x, a;
+  size_t act;
+  int64_t act_stride;
+  MlpSpace(int32_t rows, int32_t hidden, int32_t inter)
+      : x(s, rows, hidden), a(s, rows, inter), act(0), act_stride(((int64_t)inter + 7) / 8 * 8) {
+    act = s.take((size_t)rows * act_stride * 4);
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+const char* mi_q8_last_error(void) { return g_err; }
+
+int64_t mi_q8_row_bytes(int32_t n) { return n <= 0 ? 0 : ((int64_t)n + 127) / 128 * 128; }
+
+int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values, float* scale,
+                   int32_t rows, int32_t n, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("n", n, 1, kMaxK)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows("x", x, x_stride, n)) return rc;
+  if (int rc = check_ptr("values", values, 16)) return rc;
+  if (int rc = check_ptr("scale", scale, 4)) return rc;
+  return quantize(dtype, x, x_stride, nullptr, 0, nullptr, 0.f, nullptr, 0, values, scale, rows, n,
+                  stream);
+}
+
+int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
+                      int64_t y_stride, const void* weight, float eps, void* residual_out,
+                      int64_t residual_stride, void* values, float* scale, int32_t rows, int32_t n,
+                      void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("n", n, 1, kMaxK)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows("x", x, x_stride, n)) return rc;
+  if (y)
+    if (int rc = check_rows("y", y, y_stride, n)) return rc;
+  if (y)
+    if (int rc = check_rows("residual_out", residual_out, residual_stride, n)) return rc;
+  if (int rc = check_ptr("weight", weight, 2)) return rc;
+  if (int rc = check_ptr("values", values, 16)) return rc;
+  if (int rc = check_ptr("scale", scale, 4)) return rc;
+  return quantize(dtype, x, x_stride, y, y_stride, weight, eps, residual_out, residual_stride,
+                  values, scale, rows, n, stream);
+}
+
+int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
+                     int64_t out_stride, int32_t rows, int32_t n, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("n", n, 1, kMaxK)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_ptr("values", values, 16)) return rc;
+  if (int rc = check_ptr("scale", scale, 4)) return rc;
+  if (int rc = check_rows("out", out, out_stride, n)) return rc;
+  mi_fa2::Q8DequantParams p{static_cast<const int8_t*>(values), scale, static_cast<uint16_t*>(out),
+                            out_stride, rows, n, q8_pad(n), wide(out, out_stride, n)};
+  return launched(
+      mi_fa2::launch_q8_dequant(p, dtype, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t mi_q8_packed_bytes(int32_t out_features, int32_t in_features, int32_t gated) {
+  if (out_features <= 0 || in_features <= 0 || out_features > kMaxOut || in_features > kMaxK) return 0;
+  return (size_t)mi_fa2::q8_panels(out_features, gated != 0) * 16 * q8_pad(in_features);
+}
+
+int mi_q8_pack(const void* values, int64_t stride, int32_t out_features, int32_t in_features,
+               int32_t gated, void* packed, void* stream) {
+  if (int rc = check_count("out features", out_features, 1, kMaxOut)) return rc;
+  if (int rc = check_count("in features", in_features, 1, kMaxK)) return rc;
+  if (gated && out_features % 2)
+    return fail(kInvalid, "out features %d of a gated weight: gate and up rows", out_features);
+  if (int rc = check_ptr("values", values, 1)) return rc;
+  if (stride < in_features || stride >= int64_t(1) << 40)
+    return fail(kInvalid, "values row stride %lld: at least %d", (long long)stride, in_features);
+  if (int rc = check_ptr("packed", packed, 16)) return rc;
+  mi_fa2::Q8PackParams p{};
+  p.values = static_cast<const int8_t*>(values);
+  p.st = stride;
+  p.packed = static_cast<int8_t*>(packed);
+  p.N = out_features;
+  p.K = in_features;
+  p.Kp = q8_pad(in_features);
+  p.panels = mi_fa2::q8_panels(out_features, gated != 0);
+  p.gated = gated != 0;
+  p.wide = aligned(values, 16) && stride % 16 == 0;
+  return launched(mi_fa2::launch_q8_pack(p, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t mi_q8_matmul_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
+  (void)rows;
+  (void)out_features;
+  (void)in_features;
+  return 0;
+}
+
+namespace {
+
+int check_product(int32_t rows, int32_t out_features, int32_t in_features) {
+  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("out features", out_features, 1, kMaxOut)) return rc;
+  return check_count("in features", in_features, 1, kMaxK);
+}
+
+int check_operands(const void* w, const float* w_scale, const void* bias, const void* residual,
+                   int64_t residual_stride, void* out, int64_t out_stride, int32_t out_features) {
+  if (int rc = check_ptr("w", w, 16)) return rc;
+  if (int rc = check_ptr("w_scale", w_scale, 4)) return rc;
+  if (bias && !aligned(bias, 2)) return check_ptr("bias", bias, 2);
+  if (residual)
+    if (int rc = check_rows("residual", residual, residual_stride, out_features)) return rc;
+  return check_rows("out", out, out_stride, out_features);
+}
+
+}  // namespace
+
+int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
+                 const float* w_scale, const void* bias, const void* residual,
+                 int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
+                 int32_t out_features, int32_t in_features, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_product(rows, out_features, in_features)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_ptr("values", values, 16)) return rc;
+  if (int rc = check_ptr("scale", scale, 4)) return rc;
+  if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
+                              out_features))
+    return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes,
+                               mi_q8_matmul_workspace_size(rows, out_features, in_features)))
+    return rc;
+  return matmul(dtype, values, scale, w, w_scale, bias, residual, residual_stride, out, out_stride,
+                rows, out_features, in_features, false, stream);
+}
+
+size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
+  if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
+  Space s;
+  RowsSpace r(s, rows, in_features);
+  return s.total;
+}
+
+int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
+                 const void* w, const float* w_scale, const void* bias, const void* residual,
+                 int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
+                 int32_t out_features, int32_t in_features, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_product(rows, out_features, in_features)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows("x", x, x_stride, in_features)) return rc;
+  if (norm_weight && !aligned(norm_weight, 2)) return check_ptr("norm_weight", norm_weight, 2);
+  if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
+                              out_features))
+    return rc;
+  if (overlap(x, span(rows, x_stride, in_features), out, span(rows, out_stride, out_features)))
+    return fail(kInvalid, "out overlaps x");
+  Space s;
+  const RowsSpace r(s, rows, in_features);
+  if (int rc = check_workspace(workspace, workspace_bytes, s.total)) return rc;
+  char* ws = static_cast<char*>(workspace);
+  float* scale = reinterpret_cast<float*>(ws + r.scale);
+  if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0, ws + r.values,
+                        scale, rows, in_features, stream))
+    return rc;
+  return matmul(dtype, ws + r.values, scale, w, w_scale, bias, residual, residual_stride, out,
+                out_stride, rows, out_features, in_features, false, stream);
+}
+
+size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter) {
+  if (rows <= 0 || hidden <= 0 || inter <= 0 || hidden > kMaxK || inter > kMaxK) return 0;
+  return MlpSpace(rows, hidden, inter).s.total;
+}
+
+int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
+              const void* gate_up, const float* gate_up_scale, const void* down,
+              const float* down_scale, const void* residual, int64_t residual_stride, void* out,
+              int64_t out_stride, int32_t rows, int32_t hidden, int32_t inter, void* workspace,
+              size_t workspace_bytes, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("hidden", hidden, 1, kMaxK)) return rc;
+  if (int rc = check_count("inter", inter, 1, kMaxK)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows("x", x, x_stride, hidden)) return rc;
+  if (norm_weight && !aligned(norm_weight, 2)) return check_ptr("norm_weight", norm_weight, 2);
+  if (int rc = check_ptr("gate_up", gate_up, 16)) return rc;
+  if (int rc = check_ptr("gate_up_scale", gate_up_scale, 4)) return rc;
+  if (int rc = check_operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride,
+                              hidden))
+    return rc;
+  const MlpSpace sp(rows, hidden, inter);
+  if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
+  char* ws = static_cast<char*>(workspace);
+  float* x_scale = reinterpret_cast<float*>(ws + sp.x.scale);
+  float* a_scale = reinterpret_cast<float*>(ws + sp.a.scale);
+  if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0,
+                        ws + sp.x.values, x_scale, rows, hidden, stream))
+    return rc;
+  if (int rc = matmul(dtype, ws + sp.x.values, x_scale, gate_up, gate_up_scale, nullptr, nullptr, 0,
+                      ws + sp.act, sp.act_stride, rows, inter, hidden, true, stream))
+    return rc;
+  Q8QuantParams q{};
+  q.x = ws + sp.act;
+  q.x_st = sp.act_stride;
+  q.q = reinterpret_cast<int8_t*>(ws + sp.a.values);
+  q.scale = a_scale;
+  q.M = rows;
+  q.n = inter;
+  q.np = q8_pad(inter);
+  if (int rc = launched(mi_fa2::launch_q8_quant(q, dtype, mi_fa2::kQ8Float,
+                                                reinterpret_cast<hipStream_t>(stream))))
+    return rc;
+  return matmul(dtype, ws + sp.a.values, a_scale, down, down_scale, nullptr, residual,
+                residual_stride, out, out_stride, rows, hidden, inter, false, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,276 @@
+"""A decoder layer's projections in 8 bits on the HIP kernels (csrc/q8_quant.hip, csrc/q8_rows.hip, through
+libmi_q8.so, the C ABI in include/mi_q8.h).
+
+  Weight, quantize_weight   a projection's weight in 8 bits, one scale for each out feature
+  quantize, add_rmsnorm     rows of activations in 8 bits, one scale each (Rows)
+  linear                    [residual +] ([rmsnorm] x) W^T [+ bias]
+  mlp                       [residual +] SwiGLU feed-forward block of [rmsnorm] x
+
+They stand beside kernels.few_rows and kernels.model_ops for a model whose projections are held in 8 bits
+(Qwen2ForCausalLM.quantize_), and take any number of rows.  The reference has no such path; what surrounds the
+products is its model.py:49-55,81-84,107,112-138,204-207.
+
+A row of n numbers v is held as round(v / scale) with scale = max|v| / 127; a row with an infinity or a NaN has
+scale NaN, and so is everything computed from it.  Products are whole numbers, exact in 32 bits; scales, bias and
+residual are applied in fp32 and the result is rounded once.  No CPU path and no fallback: a missing library or a
+call that the kernels do not take raises.
+"""
+import ctypes
+import os
+from pathlib import Path
+
+import torch
+
+from . import _lib
+from .fa2 import _MEMO_MAX
+
+LIB_PATH = Path(os.environ.get("MI_Q8_LIB", Path(__file__).resolve().parent / "libmi_q8.so"))
+
+MAX_ROWS = 1 << 21
+MAX_IN = 131072      # 128 * 127 * in stays below 2^31
+MAX_OUT = 1 << 24
+
+_p, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_sz = ctypes.c_size_t
+# name -> (restype, argtypes); mirrors include/mi_q8.h
+SIGNATURES = {
+    "mi_q8_last_error": (ctypes.c_char_p, []),
+    "mi_q8_row_bytes": (_i64, [_i32]),
+    "mi_q8_quantize": (_i32, [_i32, _p, _i64, _p, _p, _i32, _i32, _p]),
+    "mi_q8_add_rmsnorm": (_i32, [_i32, _p, _i64, _p, _i64, _p, _f32, _p, _i64, _p, _p, _i32, _i32,
+                                 _p]),
+    "mi_q8_dequantize": (_i32, [_i32, _p, _p, _p, _i64, _i32, _i32, _p]),
+    "mi_q8_packed_bytes": (_sz, [_i32, _i32, _i32]),
+    "mi_q8_pack": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _p]),
+    "mi_q8_matmul_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "mi_q8_matmul": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32, _p, _sz,
+                            _p]),
+    "mi_q8_linear_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "mi_q8_linear": (_i32, [_i32, _p, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32,
+                            _i32, _p, _sz, _p]),
+    "mi_q8_mlp_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "mi_q8_mlp": (_i32, [_i32, _p, _i64, _p, _f32, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32,
+                         _i32, _p, _sz, _p]),
+}
+
+_library = None
+
+
+def load():
+    """Load libmi_q8.so once; raise if it is missing."""
+    global _library
+    if _library is None:
+        if not LIB_PATH.exists():
+            raise ImportError(
+                f"{LIB_PATH} not found: build it with `python my-inference-engine_amd/build_lib.py`")
+        lib = ctypes.CDLL(str(LIB_PATH))
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+        _library = lib
+    return _library
+
+
+def check(status):
+    if status != _lib.OK:
+        raise _lib.MiFa2Error(f"libmi_q8 status {status}: {load().mi_q8_last_error().decode()}")
+
+
+def call(device, fn, *args):
+    """fn(*args, stream) on the device's current stream; raises what it reports."""
+    if device == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+        return
+    with _lib.on_device(torch.device("cuda", device)) as stream:
+        check(fn(*args, stream))
+
+
+def padded(n):
+    """Bytes of a row of n values in 8 bits."""
+    return -(-n // 128) * 128
+
+
+class Weight:
+    """A projection's weight in 8 bits: values [out, in] int8 and scale [out] fp32 (weight = values *
+    scale[:, None]), laid out for the kernels once.  gated: the gate and up rows of a feed-forward block,
+    gate rows first, which only `mlp` takes.  The values are copied, the scale is kept as it is."""
+    __slots__ = ("data", "scale", "out_features", "in_features", "gated")
+
+    def __init__(self, values, scale, gated=False):
+        assert values.is_cuda and values.dtype == torch.int8 and values.dim() == 2, \
+            "values: an int8 GPU tensor [out, in]"
+        n, k = values.shape
+        assert 1 <= n <= MAX_OUT and 1 <= k <= MAX_IN, \
+            f"a weight of 1 to {MAX_OUT} out features and 1 to {MAX_IN} in features"
+        assert values.stride(1) == 1 or k == 1, "values: unit column stride"
+        assert scale.device == values.device and scale.dtype == torch.float32, \
+            f"scale: fp32 on {values.device}"
+        assert scale.shape == (n,) and scale.is_contiguous(), f"scale: contiguous, of {n}"
+        self.gated = bool(gated)
+        assert not (self.gated and n % 2), "a gated weight has as many gate as up rows"
+        self.out_features, self.in_features, self.scale = n, k, scale
+        lib = load()
+        self.data = torch.empty(lib.mi_q8_packed_bytes(n, k, self.gated), dtype=torch.int8,
+                                device=values.device)
+        call(values.device.index, lib.mi_q8_pack, values.data_ptr(),
+             values.stride(0) if n > 1 else k, n, k, self.gated, self.data.data_ptr())
+
+    @property
+    def device(self):
+        return self.scale.device
+
+
+def quantize_weight(weight, gated=False):
+    """weight [out, in] (bf16 or fp16) in 8 bits, every row by its largest magnitude."""
+    rows = quantize(weight)
+    return Weight(rows.values[:, :rows.n], rows.scale, gated)
+
+
+class Rows:
+    """Rows in 8 bits: values [rows, in rounded up to 128] int8 (zeros from n on), scale [rows] fp32, n the
+    row's length and dtype the type of the rows that they stand for."""
+    __slots__ = ("values", "scale", "n", "dtype")
+
+    def __init__(self, values, scale, n, dtype):
+        self.values, self.scale, self.n, self.dtype = values, scale, n, dtype
+
+    def dequantize(self, out=None):
+        """values * scale [rows, n] in dtype."""
+        v = self.values
+        R, dev = v.shape[0], v.device
+        if out is None:
+            out = torch.empty((R, self.n), device=dev, dtype=self.dtype)
+        op, os_ = _rows(out, "out", self.dtype, dev)
+        assert out.shape == (R, self.n), f"out: [{R}, {self.n}]"
+        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[self.dtype], v.data_ptr(),
+             self.scale.data_ptr(), op, os_, R, self.n)
+        return out
+
+
+def _rows(t, name, dtype, device):
+    """(address, row stride) of [rows, n] with unit column stride."""
+    assert t.device == device and t.dtype == dtype, f"{name}: a {dtype} tensor on {device}"
+    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), \
+        f"{name}: [rows, n] with unit column stride"
+    # one row: its stride is never used, and torch may report any value there
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t, name, n, dtype, device):
+    assert t.device == device and t.dtype == dtype and t.shape == (n,) and t.is_contiguous(), \
+        f"{name}: contiguous {dtype} of {n} on {device}"
+    return t.data_ptr()
+
+
+def _input(x):
+    assert x.is_cuda and x.dtype in _lib.DTYPES, "x: a bf16 / fp16 GPU tensor"
+    assert x.dim() == 2 and 1 <= x.shape[1] <= MAX_IN and x.shape[0] <= MAX_ROWS, \
+        f"x: [rows, n], at most {MAX_ROWS} rows of 1 to {MAX_IN}"
+    return x.dtype, x.device
+
+
+def _empty_rows(R, n, dtype, dev):
+    return Rows(torch.empty((R, padded(n)), dtype=torch.int8, device=dev),
+                torch.empty(R, dtype=torch.float32, device=dev), n, dtype)
+
+
+def quantize(x):
+    """Rows x [rows, n] in 8 bits."""
+    dt, dev = _input(x)
+    R, n = x.shape
+    xp, xs = _rows(x, "x", dt, dev)
+    out = _empty_rows(R, n, dt, dev)
+    call(dev.index, load().mi_q8_quantize, _lib.DTYPES[dt], xp, xs, out.values.data_ptr(),
+         out.scale.data_ptr(), R, n)
+    return out
+
+
+def add_rmsnorm(x, weight, eps, y=None, residual_out=None):
+    """x [rows, n] (+ y) -> (r, Rows): r = x + y rounded (x itself when y is None), and weight * rmsnorm(r)
+    in 8 bits, with no rounding to 16 bits in between.  residual_out may be x or y (in place)."""
+    dt, dev = _input(x)
+    R, n = x.shape
+    xp, xs = _rows(x, "x", dt, dev)
+    yp, ys, r, rp, rs = None, 0, x, None, 0
+    if y is not None:
+        yp, ys = _rows(y, "y", dt, dev)
+        assert y.shape == x.shape, "y: x's shape"
+        r = torch.empty((R, n), device=dev, dtype=dt) if residual_out is None else residual_out
+        rp, rs = _rows(r, "residual_out", dt, dev)
+        assert r.shape == x.shape, "residual_out: x's shape"
+    else:
+        assert residual_out is None, "residual_out goes with y"
+    out = _empty_rows(R, n, dt, dev)
+    call(dev.index, load().mi_q8_add_rmsnorm, _lib.DTYPES[dt], xp, xs, yp, ys,
+         _vector(weight, "weight", n, dt, dev), float(eps), rp, rs, out.values.data_ptr(),
+         out.scale.data_ptr(), R, n)
+    return r, out
+
+
+def _out(out, residual, R, N, dt, dev):
+    if out is None:
+        out = torch.empty((R, N), device=dev, dtype=dt)
+    op, os_ = _rows(out, "out", dt, dev)
+    assert out.shape == (R, N), f"out: [{R}, {N}]"
+    rp, rs = None, 0
+    if residual is not None:
+        rp, rs = _rows(residual, "residual", dt, dev)
+        assert residual.shape == (R, N), f"residual: [{R}, {N}]"
+    return out, op, os_, rp, rs
+
+
+def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
+    """[residual +] x W^T [+ bias] -> [rows, out]: x [rows, in] (bf16 or fp16; with norm_weight RMS-normalised
+    first) or Rows, w a Weight.  residual may be `out` (in place); out must not overlap x."""
+    assert type(w) is Weight and not w.gated, "w: a Weight that is not gated"
+    N, K = w.out_features, w.in_features
+    lib = load()
+    if type(x) is Rows:
+        assert norm_weight is None, "rows in 8 bits are normalised already"
+        dt, dev, R = x.dtype, x.values.device, x.values.shape[0]
+        assert x.n == K and w.device == dev, f"x: rows of {K} on {w.device}"
+        out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
+        ws = torch.empty(lib.mi_q8_matmul_workspace_size(R, N, K), dtype=torch.uint8, device=dev)
+        call(dev.index, lib.mi_q8_matmul, _lib.DTYPES[dt], x.values.data_ptr(), x.scale.data_ptr(),
+             w.data.data_ptr(), w.scale.data_ptr(),
+             _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N,
+             K, ws.data_ptr(), ws.numel())
+        return out
+    dt, dev = _input(x)
+    R = x.shape[0]
+    assert x.shape[1] == K and w.device == dev, f"x: rows of {K} on {w.device}"
+    xp, xs = _rows(x, "x", dt, dev)
+    out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
+    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
+    ws = torch.empty(lib.mi_q8_linear_workspace_size(R, N, K), dtype=torch.uint8, device=dev)
+    call(dev.index, lib.mi_q8_linear, _lib.DTYPES[dt], xp, xs,
+         _vector(norm_weight, "norm_weight", K, dt, dev) if norm_weight is not None else None,
+         float(eps), w.data.data_ptr(), w.scale.data_ptr(),
+         _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N, K,
+         ws.data_ptr(), ws.numel())
+    return out
+
+
+def mlp(x, gate_up, down, residual=None, norm_weight=None, eps=0.0, out=None):
+    """[residual +] (silu(g) * u) Wd^T with (g | u) = [rmsnorm] x Wgu^T -> [rows, hidden]: x [rows, hidden],
+    gate_up a gated Weight [2 * inter, hidden], down a Weight [hidden, inter].  The activation is held in 8 bits
+    too, every row by its largest magnitude.  out may be residual and x."""
+    assert type(gate_up) is Weight and gate_up.gated, "gate_up: a gated Weight"
+    assert type(down) is Weight and not down.gated, "down: a Weight that is not gated"
+    dt, dev = _input(x)
+    R, H = x.shape
+    inter = down.in_features
+    assert gate_up.in_features == H and down.out_features == H, f"weights of hidden size {H}"
+    assert gate_up.out_features == 2 * inter, f"gate_up of {2 * inter} rows"
+    assert gate_up.device == dev and down.device == dev, f"weights on {dev}"
+    lib = load()
+    xp, xs = _rows(x, "x", dt, dev)
+    out, op, os_, rp, rs = _out(out, residual, R, H, dt, dev)
+    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
+    ws = torch.empty(lib.mi_q8_mlp_workspace_size(R, H, inter), dtype=torch.uint8, device=dev)
+    call(dev.index, lib.mi_q8_mlp, _lib.DTYPES[dt], xp, xs,
+         _vector(norm_weight, "norm_weight", H, dt, dev) if norm_weight is not None else None,
+         float(eps), gate_up.data.data_ptr(), gate_up.scale.data_ptr(), down.data.data_ptr(),
+         down.scale.data_ptr(), rp, rs, op, os_, R, H, inter, ws.data_ptr(), ws.numel())
+    return out

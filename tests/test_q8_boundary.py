@@ -1,0 +1,154 @@
+"""CPU checks of libmi_q8.so: it exports exactly what include/mi_q8.h declares and refuses bad arguments
+before touching the GPU, and so do the Python wrappers.  No kernel is launched here."""
+import re
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+from kernels import q8
+from oracle import q8 as o8
+
+HEADER = ROOT / "include" / "mi_q8.h"
+
+
+def declared_symbols():
+    return sorted(set(re.findall(r"MI_Q8_API\s+[\w\s\*]+?\b(mi_q8_\w+)\s*\(", HEADER.read_text())))
+
+
+def test_library_exports_exactly_the_declared_symbols():
+    names = declared_symbols()
+    out = subprocess.run(["nm", "-D", "--defined-only", str(q8.LIB_PATH)], capture_output=True,
+                         text=True, check=True).stdout
+    assert sorted(line.split()[-1] for line in out.splitlines() if " T " in line) == names
+    assert set(names) == set(q8.SIGNATURES)
+    q8.load()
+
+
+def last():
+    return q8.load().mi_q8_last_error().decode()
+
+
+def _quantize(**over):
+    a = dict(dtype=0, x=16, xs=64, values=16, scale=16, rows=3, n=64)
+    a.update(over)
+    return q8.load().mi_q8_quantize(*a.values(), None)
+
+
+def _norm(**over):
+    a = dict(dtype=0, x=16, xs=64, y=16, ys=64, weight=16, eps=1e-6, r=16, rs=64, values=16, scale=16,
+             rows=3, n=64)
+    a.update(over)
+    return q8.load().mi_q8_add_rmsnorm(*a.values(), None)
+
+
+def _dequantize(**over):
+    a = dict(dtype=0, values=16, scale=16, out=16, os=64, rows=3, n=64)
+    a.update(over)
+    return q8.load().mi_q8_dequantize(*a.values(), None)
+
+
+def _pack(**over):
+    a = dict(values=16, stride=64, n=48, k=64, gated=0, packed=16)
+    a.update(over)
+    return q8.load().mi_q8_pack(*a.values(), None)
+
+
+def _matmul(**over):
+    a = dict(dtype=0, values=16, scale=16, w=16, ws=16, bias=None, res=None, rs=0, out=1 << 30, os=48,
+             rows=3, n=48, k=64, space=16, size=1 << 30)
+    a.update(over)
+    return q8.load().mi_q8_matmul(*a.values(), None)
+
+
+def _linear(**over):
+    a = dict(dtype=0, x=16, xs=64, norm=None, eps=0.0, w=16, ws=16, bias=None, res=None, rs=0,
+             out=1 << 30, os=48, rows=3, n=48, k=64, space=16, size=1 << 30)
+    a.update(over)
+    return q8.load().mi_q8_linear(*a.values(), None)
+
+
+def _mlp(**over):
+    a = dict(dtype=0, x=16, xs=64, norm=None, eps=0.0, gu=16, gus=16, down=16, downs=16, res=None,
+             rs=0, out=1 << 30, os=64, rows=3, hidden=64, inter=96, space=16, size=1 << 30)
+    a.update(over)
+    return q8.load().mi_q8_mlp(*a.values(), None)
+
+
+@pytest.mark.parametrize("call,over,status,msg", [
+    (f, o, s, m) for f in (_quantize, _norm, _dequantize) for o, s, m in [
+        (dict(dtype=2), 2, "dtype"), (dict(rows=-1), 1, "rows"), (dict(rows=(1 << 21) + 1), 1, "rows"),
+        (dict(n=0), 1, "n 0"), (dict(n=131073), 1, "131072"), (dict(values=None), 1, "values is NULL"),
+        (dict(values=24), 1, "16-byte"), (dict(scale=None), 1, "scale is NULL"),
+        (dict(scale=18), 1, "4-byte")]] + [
+    (_quantize, dict(x=None), 1, "x is NULL"), (_quantize, dict(xs=63), 1, "x row stride"),
+    (_quantize, dict(x=17), 1, "2-byte"), (_norm, dict(x=None), 1, "x is NULL"),
+    (_norm, dict(ys=10), 1, "y row stride"), (_norm, dict(r=None), 1, "residual_out is NULL"),
+    (_norm, dict(rs=1), 1, "residual_out row stride"), (_norm, dict(weight=None), 1, "weight is NULL"),
+    (_dequantize, dict(out=None), 1, "out is NULL"), (_dequantize, dict(os=9), 1, "out row stride"),
+    (_pack, dict(n=0), 1, "out features"), (_pack, dict(k=0), 1, "in features"),
+    (_pack, dict(k=131073, stride=131073), 1, "in features"), (_pack, dict(stride=63), 1, "stride"),
+    (_pack, dict(values=None), 1, "values is NULL"), (_pack, dict(packed=8), 1, "16-byte"),
+    (_pack, dict(n=(1 << 24) + 1), 1, "out features"), (_pack, dict(n=47, gated=1), 1, "gated")] + [
+    (f, o, s, m) for f in (_matmul, _linear) for o, s, m in [
+        (dict(dtype=2), 2, "dtype"), (dict(rows=-1), 1, "rows"), (dict(n=0), 1, "out features"),
+        (dict(k=131073, xs=131073) if f is _linear else dict(k=131073), 1, "in features"),
+        (dict(w=None), 1, "w is NULL"), (dict(w=8), 1, "16-byte"), (dict(ws=None), 1, "w_scale is NULL"),
+        (dict(bias=3), 1, "bias"), (dict(res=16, rs=47), 1, "residual row stride"),
+        (dict(out=None), 1, "out is NULL"), (dict(os=47), 1, "out row stride")]] + [
+    (_matmul, dict(values=None), 1, "values is NULL"), (_matmul, dict(scale=None), 1, "scale is NULL"),
+    (_linear, dict(x=None), 1, "x is NULL"), (_linear, dict(norm=3), 1, "norm_weight"),
+    (_linear, dict(out=16), 1, "overlaps"), (_linear, dict(out=16 + 2 * (2 * 64 + 63)), 1, "overlaps"),
+    (_linear, dict(x=1 << 30, out=(1 << 30) - 2 * (2 * 48 + 47)), 1, "overlaps"),
+    (_linear, dict(rows=300, space=None), 1, "workspace is NULL"),
+    (_linear, dict(rows=300, space=8), 1, "16-byte"), (_linear, dict(rows=300, size=255), 3, "needed"),
+    (_mlp, dict(dtype=7), 2, "dtype"), (_mlp, dict(rows=-2), 1, "rows"), (_mlp, dict(hidden=0), 1, "hidden"),
+    (_mlp, dict(inter=0), 1, "inter"), (_mlp, dict(inter=131073), 1, "inter"),
+    (_mlp, dict(x=None), 1, "x is NULL"), (_mlp, dict(gu=None), 1, "gate_up is NULL"),
+    (_mlp, dict(gus=None), 1, "gate_up_scale is NULL"), (_mlp, dict(down=4), 1, "16-byte"),
+    (_mlp, dict(res=16, rs=0), 1, "residual row stride"), (_mlp, dict(os=63), 1, "out row stride"),
+    (_mlp, dict(space=None), 1, "workspace is NULL"), (_mlp, dict(size=1000), 3, "needed")])
+def test_refusals(call, over, status, msg):
+    assert call(**over) == status
+    assert msg in last()
+
+
+def test_empty_calls_are_no_ops():
+    for call in (_quantize, _norm, _dequantize, _matmul, _linear, _mlp):
+        assert call(rows=0) == 0 and last() == ""
+
+
+def test_sizes():
+    lib = q8.load()
+    for n in (1, 127, 128, 129, 131072):
+        assert lib.mi_q8_row_bytes(n) == q8.padded(n) == -(-n // 128) * 128
+    assert lib.mi_q8_row_bytes(0) == 0
+    for n, k, gated in ((1, 1, 0), (2, 1, 1), (16, 64, 0), (17, 129, 0), (34, 129, 1), (2048, 1536, 1)):
+        want = o8.packed(torch.zeros(n, k, dtype=torch.int8), gated).numel()
+        assert lib.mi_q8_packed_bytes(n, k, gated) == want
+    assert lib.mi_q8_packed_bytes(0, 5, 0) == 0 and lib.mi_q8_packed_bytes(5, 131073, 0) == 0
+    for rows in (300, 5000):
+        # rows in 8 bits and their scales; the feed-forward block's activation in fp32 and 8 bits beside
+        assert lib.mi_q8_linear_workspace_size(rows, 2048, 1001) >= rows * (1024 + 4)
+        assert lib.mi_q8_mlp_workspace_size(rows, 1536, 8960) >= rows * (1536 + 8960 * 5 + 8)
+    assert lib.mi_q8_linear_workspace_size(0, 5, 5) == 0 and lib.mi_q8_mlp_workspace_size(1, 0, 5) == 0
+    # sizes past 32 bits
+    assert lib.mi_q8_mlp_workspace_size(1 << 21, 1536, 8960) > (1 << 21) * 8960 * 5
+    assert lib.mi_q8_packed_bytes(1 << 24, 131072, 0) == 1 << 41
+
+
+def test_wrappers_refuse():
+    x, w = torch.zeros(3, 64, dtype=torch.bfloat16), torch.zeros(16, 64, dtype=torch.int8)
+    with pytest.raises(AssertionError):
+        q8.Weight(w, torch.ones(16))
+    with pytest.raises(AssertionError):
+        q8.quantize_weight(x)
+    with pytest.raises(AssertionError):
+        q8.quantize(x)
+    with pytest.raises(AssertionError):
+        q8.add_rmsnorm(x, x[0], 1e-6)
+    with pytest.raises(AssertionError):
+        q8.linear(x, w)
+    with pytest.raises(AssertionError):
+        q8.mlp(x, w, w)
