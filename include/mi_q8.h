@@ -9,10 +9,12 @@
  * Rows in 8 bits.  A row v of n numbers is held as n int8 and one fp32 scale:
  *   scale = max(max |v|, 2^-100) / 127,   value = round_half_even(v / scale), at most 127 in size.
  * A row that holds an infinity or a NaN has scale NaN (and zeros), so that whatever is computed from
- * it is NaN.  values: [rows][mi_q8_row_bytes(n)], 16-byte aligned, zeros from n on.
+ * it is NaN.  The values are laid out for the products: panels of 16 rows,
+ *   [ceil(rows / 16)][np / 64][4][16 rows][16 values], np = n rounded up to a multiple of 128,
+ * zeros from n on, mi_q8_rows_bytes() bytes, 16-byte aligned; rows past the last keep what they hold.
  *
  * Weights in 8 bits.  int8 [out_features][in_features] and one fp32 scale for each out feature, the
- * values laid out by mi_q8_pack once.  A gated weight (the gate and up rows of a feed-forward block,
+ * values laid out by mi_q8_pack once, as rows are but with zeros past the last.  A gated weight (the gate and up rows of a feed-forward block,
  * gate rows first) is laid out for mi_q8_mlp and used by nothing else.
  *
  * A product is sum_k x[m][k] w[n][k], a whole number in 32 bits (exact, in_features <= 131072), times
@@ -41,8 +43,8 @@ extern "C" {
 
 MI_Q8_API const char* mi_q8_last_error(void);
 
-/* Bytes of a row of n values: n rounded up to a multiple of 128. */
-MI_Q8_API int64_t mi_q8_row_bytes(int32_t n);
+/* Bytes of the values of rows in 8 bits. */
+MI_Q8_API size_t mi_q8_rows_bytes(int32_t rows, int32_t n);
 
 /* Rows x [rows, n] in 8 bits. */
 MI_Q8_API int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values,

@@ -25,7 +25,7 @@ LIBS = {
           "rope_kv.hip", "sample.hip", "step_meta.hip", "model_ops.hip", "fa2_capi.cpp"],
     PKG / "kernels" / "libmi_model.so": ["linear_rows.hip", "model_capi.cpp"],
     PKG / "kernels" / "libmi_cache.so": ["block_ops.hip", "shared_attn.hip", "cache_capi.cpp"],
-    PKG / "kernels" / "libmi_q8.so": ["q8_quant.hip", "q8_rows.hip", "q8_capi.cpp"],
+    PKG / "kernels" / "libmi_q8.so": ["q8_quant.hip", "q8_rows.hip", "q8_gemm.hip", "q8_capi.cpp"],
 }
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

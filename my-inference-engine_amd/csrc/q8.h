@@ -1,27 +1,62 @@
-// Parameters of the 8-bit projections (q8_quant.hip, q8_rows.hip).
+// Parameters of the 8-bit projections (q8_quant.hip, q8_rows.hip, q8_gemm.hip).
 //
-// Layouts.  Rows in 8 bits: [rows][Kp] int8, Kp = K rounded up to 128, zeros from K on, one fp32 scale
-// a row.  Weights in 8 bits: panels of 16 rows, [panel][Kp / 64][4][16 rows][16 bytes]: lane (n, g) of
-// a wave reads the 16 bytes of row n, k = 64 s + 16 g .. + 15, the A operand of
-// v_mfma_i32_16x16x64_i8, and a wave's load is 1 KB in one run.  Rows past the last are zeros.  A
-// plain panel is rows 16 p .. 16 p + 15; a gated one is gate rows 8 p .. + 7 and the up rows of the
-// same features.
+// Layouts.  Rows of activations and of weights are held alike, in panels of 16 rows, [panel][Kp / 64][4][16
+// rows][16 bytes], Kp = K rounded up to 128, zeros from K on: lane (n, g) of a wave reads the 16 bytes of
+// row n, k = 64 s + 16 g .. + 15, an operand of v_mfma_i32_16x16x64_i8, and a wave's load is 1 KB in one
+// run (rows as they are would have neighbouring lanes 16 rows apart: a product of 64 tokens by 1536 x
+// 8960 24.5 us, in panels 10.7).  One fp32 scale a row.  A gated weight's panel is gate rows 8 p .. + 7 and the
+// up rows of the same features.  Rows past a weight's last are zeros; those past the last token are
+// whatever was there, and only reach results that nobody keeps.
 #pragma once
 
 #include "fa2_common.h"
+#include "q8_rule.h"
 
 namespace mi_fa2 {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));   // at any float
 
 constexpr int kQ8Pad = 128;
 constexpr float kQ8Least = 0x1p-100f;   // a row's largest magnitude counts as at least this
 constexpr int kQ8MaxK = 131072;   // 128 * 127 * K stays below 2^31
 
 __host__ __device__ constexpr int q8_pad(int n) { return (n + kQ8Pad - 1) / kQ8Pad * kQ8Pad; }
+// Byte of row `row`, k = 8 c (c: a chunk of 8).
+__host__ __device__ constexpr int64_t q8_at(int64_t row, int c, int np) {
+  return (row >> 4) * 16 * np + (int64_t)(c >> 3) * 1024 + ((c >> 1) & 3) * 256 + (row & 15) * 16 + (c & 1) * 8;
+}
 __host__ __device__ constexpr int q8_panels(int out, bool gated) {
   return gated ? (out / 2 + 7) / 8 : (out + 15) / 16;
+}
+
+// A row's way to 8 bits: its largest magnitude as the bits of |v|, whose order as whole numbers is that of
+// the magnitudes, with infinity and NaN above all.
+struct Q8Factor {
+  float most, f;   // 127 / most; a row with an infinity or a NaN: 0
+  bool bad;
+};
+__device__ __forceinline__ Q8Factor q8_factor(uint32_t top) {
+  Q8Factor r;
+  r.bad = top >= 0x7f800000u;
+  r.most = fmaxf(__uint_as_float(top), kQ8Least);
+  r.f = r.bad ? 0.f : 127.f / r.most;
+  return r;
+}
+// inv: what every value is multiplied by beside.
+__device__ __forceinline__ float q8_scale(const Q8Factor& r, float inv) {
+  return r.bad ? __builtin_nanf("") : r.most * inv / 127.f;
+}
+// Four values, lowest byte first.  v f is rounded to the nearest whole number, ties to even, by the
+// addition of 1.5 * 2^23, whose last place is 1: its low byte is the number's (two's complement).
+__device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, const Q8Factor& r) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t i = __float_as_uint(__builtin_fmaf(a, r.f, kMagic)), j = __float_as_uint(__builtin_fmaf(b, r.f, kMagic));
+  const uint32_t k = __float_as_uint(__builtin_fmaf(c, r.f, kMagic)), l = __float_as_uint(__builtin_fmaf(d, r.f, kMagic));
+  // v_perm_b32 selects bytes of {second word, first word}: bytes 0 of both, then the halves
+  const uint32_t lo = perm_b32(j, i, 0x0c0c0400u), hi = perm_b32(l, k, 0x0c0c0400u);
+  return r.bad ? 0u : lo | hi << 16;
 }
 
 // Rows to 8 bits, and back.
@@ -34,13 +69,18 @@ struct Q8QuantParams {
   float eps;
   uint16_t* r_out;        // x + y, with y
   int64_t r_st;
-  int8_t* q;              // [M][np]
+  int8_t* q;              // panels of np
   float* scale;           // [M]
   int32_t M, n, np;
   int32_t wide;           // every row and the norm's weight allow 16-byte accesses
+  uint32_t* zero;         // counters this launch zeroes for the next one
+  int32_t n_zero;
+  int32_t spread;         // work-groups are dealt so that a panel's rows share an XCD
 };
-enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2 };
+enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2, kQ8Rows = 3 };
 hipError_t launch_q8_quant(const Q8QuantParams& p, int dtype, int source, hipStream_t stream);
+
+hipError_t launch_q8_zero(uint32_t* p, int n, hipStream_t stream);
 
 struct Q8DequantParams {
   const int8_t* q;
@@ -61,8 +101,11 @@ hipError_t launch_q8_pack(const Q8PackParams& p, hipStream_t stream);
 
 // A product.
 struct Q8Params {
-  const int8_t* x;        // [M][Kp]
-  const float* x_scale;   // [M]
+  const void* x;          // panels of Kp, or (few rows) [M][x_st] 16-bit rows to be brought to 8 bits
+  int64_t x_st;
+  const uint16_t* norm_w; // [K]: their norm's weight
+  float eps;
+  const float* x_scale;   // [M] of rows in 8 bits
   const int8_t* w;        // packed
   const float* w_scale;   // [N] (gated: [2 N], gate first)
   const uint16_t* bias;   // [N] or NULL
@@ -70,10 +113,19 @@ struct Q8Params {
   int64_t res_st;
   void* out;              // [M][out_st] 16-bit; gated: the activation in fp32
   int64_t out_st;
-  int32_t M, N, Kp;       // N: out features (gated: of the activation)
+  int32_t M, N, K, Kp;    // N: out features (gated: of the activation)
   int32_t panels;
-  int32_t quads;          // out, residual and bias allow accesses of 4 elements
+  int32_t wide;           // out and residual allow accesses of 8 elements, bias of 4
+  // splits > 1: work-groups that share a tile's K, their sums and the tiles' arrival counts (zero at
+  // launch)
+  int32_t splits;
+  uint64_t* part;
+  uint32_t* count;
+  uint32_t* zero;         // counters a few-row launch zeroes for the next one
+  int32_t n_zero;
 };
-hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int n_cus, hipStream_t stream);
+hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
+                          hipStream_t stream);
+hipError_t launch_q8_gemm(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream);
 
 }  // namespace mi_fa2

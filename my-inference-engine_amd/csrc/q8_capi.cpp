@@ -90,7 +90,6 @@ int check_rows(const char* name, const void* p, int64_t stride, int64_t width) {
 bool wide(const void* p, int64_t stride, int32_t n) {
   return !p || (aligned(p, 16) && stride % 8 == 0 && n % 8 == 0);
 }
-bool quads(const void* p, int64_t stride) { return !p || (aligned(p, 8) && stride % 4 == 0); }
 
 bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
@@ -112,7 +111,19 @@ struct Space {
 struct RowsSpace {
   size_t values, scale;
   RowsSpace(Space& s, int32_t rows, int32_t n)
-      : values(s.take((size_t)rows * q8_pad(n))), scale(s.take((size_t)rows * 4)) {}
+      : values(s.take((size_t)(((int64_t)rows + 15) / 16 * 16) * q8_pad(n))), scale(s.take((size_t)rows * 4)) {}
+};
+
+// What a product needs beside its rows: the sums of shares of K and the tiles' arrival counts.
+struct ProductSpace {
+  mi_fa2::Q8Plan plan;
+  size_t part, count;
+  ProductSpace(Space& s, int32_t rows, int32_t out_features, int32_t in_features, bool gated)
+      : plan(mi_fa2::q8_plan(rows, mi_fa2::q8_panels(gated ? 2 * out_features : out_features, gated),
+                             q8_pad(in_features))),
+        part(s.take(plan.part)), count(s.take(plan.count)) {}
+  uint32_t* counts(char* ws) const { return plan.count ? reinterpret_cast<uint32_t*>(ws + count) : nullptr; }
+  int32_t n_counts() const { return (int32_t)(plan.count / 4); }
 };
 
 int check_workspace(const void* ws, size_t have, size_t need) {
@@ -124,7 +135,7 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 
 int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t y_stride,
              const void* norm_weight, float eps, void* r, int64_t r_stride, void* values,
-             float* scale, int32_t rows, int32_t n, void* stream) {
+             float* scale, int32_t rows, int32_t n, uint32_t* zero, int32_t n_zero, void* stream) {
   Q8QuantParams p{};
   p.x = x;
   p.x_st = x_stride;
@@ -139,20 +150,19 @@ int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t 
   p.M = rows;
   p.n = n;
   p.np = q8_pad(n);
+  p.zero = zero;
+  p.n_zero = n_zero;
   p.wide = wide(x, x_stride, n) && wide(y, y_stride, n) && wide(norm_weight, 8, n) &&
            (!y || wide(r, r_stride, n));
   return launched(mi_fa2::launch_q8_quant(p, dtype, norm_weight ? mi_fa2::kQ8Norm : mi_fa2::kQ8Plain,
                                           reinterpret_cast<hipStream_t>(stream)));
 }
 
-int matmul(int dtype, const void* values, const float* scale, const void* w, const float* w_scale,
-           const void* bias, const void* res, int64_t res_stride, void* out, int64_t out_stride,
-           int32_t rows, int32_t out_features, int32_t in_features, bool gated, void* stream) {
-  int cus = 0;
-  if (int rc = compute_units(&cus)) return rc;
+// A product's operands but for its rows.
+Q8Params operands(const void* w, const float* w_scale, const void* bias, const void* res,
+                  int64_t res_stride, void* out, int64_t out_stride, int32_t rows,
+                  int32_t out_features, int32_t in_features, bool gated) {
   Q8Params p{};
-  p.x = static_cast<const int8_t*>(values);
-  p.x_scale = scale;
   p.w = static_cast<const int8_t*>(w);
   p.w_scale = w_scale;
   p.bias = static_cast<const uint16_t*>(bias);
@@ -162,20 +172,72 @@ int matmul(int dtype, const void* values, const float* scale, const void* w, con
   p.out_st = out_stride;
   p.M = rows;
   p.N = out_features;
+  p.K = in_features;
   p.Kp = q8_pad(in_features);
   p.panels = mi_fa2::q8_panels(gated ? 2 * out_features : out_features, gated);
-  p.quads = quads(bias, 4) && quads(res, res_stride) && quads(out, out_stride);
-  return launched(
-      mi_fa2::launch_q8_rows(p, dtype, gated, cus, reinterpret_cast<hipStream_t>(stream)));
+  p.wide = out_features % 8 == 0 && wide(res, res_stride, 8) && wide(out, out_stride, 8) &&
+           (!bias || aligned(bias, 8));
+  return p;
 }
+
+// The product of rows in 8 bits.
+int product(Q8Params p, int dtype, bool gated, const void* values, const float* scale,
+            const ProductSpace& sp, char* ws, void* stream) {
+  p.x = values;
+  p.x_scale = scale;
+  p.splits = sp.plan.splits;
+  p.part = reinterpret_cast<uint64_t*>(ws + sp.part);
+  p.count = sp.counts(ws);
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (sp.plan.np) return launched(mi_fa2::launch_q8_gemm(p, sp.plan, dtype, gated, st));
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  return launched(mi_fa2::launch_q8_rows(p, dtype, gated, mi_fa2::kQ8Rows, cus, st));
+}
+
+// The product of 16-bit rows, brought to 8 bits in the same launch where the few-row kernel does that,
+// else before it in the workspace.
+bool fused(const void* x, int64_t x_stride, const void* norm_weight, int32_t rows, int32_t in) {
+  return rows <= mi_fa2::kQ8FusedMax && q8_pad(in) <= mi_fa2::kQ8KeepK && x_stride < 1 << 23 &&
+         wide(x, x_stride, in) && wide(norm_weight, 8, in);
+}
+int product_of(Q8Params p, int dtype, bool gated, const void* x, int64_t x_stride,
+               const void* norm_weight, float eps, const RowsSpace& r, const ProductSpace& sp,
+               char* ws, void* stream) {
+  if (fused(x, x_stride, norm_weight, p.M, p.K)) {
+    p.x = x;
+    p.x_st = x_stride;
+    p.norm_w = static_cast<const uint16_t*>(norm_weight);
+    p.eps = eps;
+    int cus = 0;
+    if (int rc = compute_units(&cus)) return rc;
+    return launched(mi_fa2::launch_q8_rows(p, dtype, gated, norm_weight ? mi_fa2::kQ8Norm : mi_fa2::kQ8Plain,
+                                           cus, reinterpret_cast<hipStream_t>(stream)));
+  }
+  float* scale = reinterpret_cast<float*>(ws + r.scale);
+  if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0, ws + r.values,
+                        scale, p.M, p.K, sp.counts(ws), sp.n_counts(), stream))
+    return rc;
+  return product(p, dtype, gated, ws + r.values, scale, sp, ws, stream);
+}
+
+struct LinearSpace {
+  Space s;
+  RowsSpace x;
+  ProductSpace product;
+  LinearSpace(int32_t rows, int32_t out_features, int32_t in_features)
+      : x(s, rows, in_features), product(s, rows, out_features, in_features, false) {}
+};
 
 struct MlpSpace {
   Space s;
   RowsSpace x, a;
+  ProductSpace gate_up, down;
   size_t act;
   int64_t act_stride;
   MlpSpace(int32_t rows, int32_t hidden, int32_t inter)
-      : x(s, rows, hidden), a(s, rows, inter), act(0), act_stride(((int64_t)inter + 7) / 8 * 8) {
+      : x(s, rows, hidden), a(s, rows, inter), gate_up(s, rows, inter, hidden, true),
+        down(s, rows, hidden, inter, false), act(0), act_stride(((int64_t)inter + 7) / 8 * 8) {
     act = s.take((size_t)rows * act_stride * 4);
   }
 };
@@ -186,7 +248,10 @@ extern "C" {
 
 const char* mi_q8_last_error(void) { return g_err; }
 
-int64_t mi_q8_row_bytes(int32_t n) { return n <= 0 ? 0 : ((int64_t)n + 127) / 128 * 128; }
+size_t mi_q8_rows_bytes(int32_t rows, int32_t n) {
+  if (rows <= 0 || n <= 0 || rows > kMaxRows || n > kMaxK) return 0;
+  return (size_t)((rows + 15) / 16 * 16) * q8_pad(n);
+}
 
 int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values, float* scale,
                    int32_t rows, int32_t n, void* stream) {
@@ -198,7 +263,7 @@ int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values,
   if (int rc = check_ptr("values", values, 16)) return rc;
   if (int rc = check_ptr("scale", scale, 4)) return rc;
   return quantize(dtype, x, x_stride, nullptr, 0, nullptr, 0.f, nullptr, 0, values, scale, rows, n,
-                  stream);
+                  nullptr, 0, stream);
 }
 
 int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
@@ -218,7 +283,7 @@ int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void
   if (int rc = check_ptr("values", values, 16)) return rc;
   if (int rc = check_ptr("scale", scale, 4)) return rc;
   return quantize(dtype, x, x_stride, y, y_stride, weight, eps, residual_out, residual_stride,
-                  values, scale, rows, n, stream);
+                  values, scale, rows, n, nullptr, 0, stream);
 }
 
 int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
@@ -265,10 +330,10 @@ int mi_q8_pack(const void* values, int64_t stride, int32_t out_features, int32_t
 }
 
 size_t mi_q8_matmul_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
-  (void)rows;
-  (void)out_features;
-  (void)in_features;
-  return 0;
+  if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
+  Space s;
+  ProductSpace(s, rows, out_features, in_features, false);
+  return s.total;
 }
 
 namespace {
@@ -304,18 +369,22 @@ int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const vo
   if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
                               out_features))
     return rc;
-  if (int rc = check_workspace(workspace, workspace_bytes,
-                               mi_q8_matmul_workspace_size(rows, out_features, in_features)))
-    return rc;
-  return matmul(dtype, values, scale, w, w_scale, bias, residual, residual_stride, out, out_stride,
-                rows, out_features, in_features, false, stream);
+  Space s;
+  const ProductSpace sp(s, rows, out_features, in_features, false);
+  if (int rc = check_workspace(workspace, workspace_bytes, s.total)) return rc;
+  char* ws = static_cast<char*>(workspace);
+  if (sp.n_counts())
+    if (int rc = launched(mi_fa2::launch_q8_zero(sp.counts(ws), sp.n_counts(),
+                                                 reinterpret_cast<hipStream_t>(stream))))
+      return rc;
+  return product(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
+                          out_features, in_features, false),
+                 dtype, false, values, scale, sp, ws, stream);
 }
 
 size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
   if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
-  Space s;
-  RowsSpace r(s, rows, in_features);
-  return s.total;
+  return LinearSpace(rows, out_features, in_features).s.total;
 }
 
 int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
@@ -333,16 +402,12 @@ int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* nor
     return rc;
   if (overlap(x, span(rows, x_stride, in_features), out, span(rows, out_stride, out_features)))
     return fail(kInvalid, "out overlaps x");
-  Space s;
-  const RowsSpace r(s, rows, in_features);
-  if (int rc = check_workspace(workspace, workspace_bytes, s.total)) return rc;
-  char* ws = static_cast<char*>(workspace);
-  float* scale = reinterpret_cast<float*>(ws + r.scale);
-  if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0, ws + r.values,
-                        scale, rows, in_features, stream))
-    return rc;
-  return matmul(dtype, ws + r.values, scale, w, w_scale, bias, residual, residual_stride, out,
-                out_stride, rows, out_features, in_features, false, stream);
+  const LinearSpace sp(rows, out_features, in_features);
+  if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
+  return product_of(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
+                             out_features, in_features, false),
+                    dtype, false, x, x_stride, norm_weight, eps, sp.x, sp.product,
+                    static_cast<char*>(workspace), stream);
 }
 
 size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter) {
@@ -370,13 +435,10 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
   const MlpSpace sp(rows, hidden, inter);
   if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
   char* ws = static_cast<char*>(workspace);
-  float* x_scale = reinterpret_cast<float*>(ws + sp.x.scale);
   float* a_scale = reinterpret_cast<float*>(ws + sp.a.scale);
-  if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0,
-                        ws + sp.x.values, x_scale, rows, hidden, stream))
-    return rc;
-  if (int rc = matmul(dtype, ws + sp.x.values, x_scale, gate_up, gate_up_scale, nullptr, nullptr, 0,
-                      ws + sp.act, sp.act_stride, rows, inter, hidden, true, stream))
+  if (int rc = product_of(operands(gate_up, gate_up_scale, nullptr, nullptr, 0, ws + sp.act,
+                                   sp.act_stride, rows, inter, hidden, true),
+                          dtype, true, x, x_stride, norm_weight, eps, sp.x, sp.gate_up, ws, stream))
     return rc;
   Q8QuantParams q{};
   q.x = ws + sp.act;
@@ -386,11 +448,14 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
   q.M = rows;
   q.n = inter;
   q.np = q8_pad(inter);
+  q.zero = sp.down.counts(ws);
+  q.n_zero = sp.down.n_counts();
   if (int rc = launched(mi_fa2::launch_q8_quant(q, dtype, mi_fa2::kQ8Float,
                                                 reinterpret_cast<hipStream_t>(stream))))
     return rc;
-  return matmul(dtype, ws + sp.a.values, a_scale, down, down_scale, nullptr, residual,
-                residual_stride, out, out_stride, rows, hidden, inter, false, stream);
+  return product(operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride,
+                          rows, hidden, inter, false),
+                 dtype, false, ws + sp.a.values, a_scale, sp.down, ws, stream);
 }
 
 }  // extern "C"

@@ -8,9 +8,6 @@
 // one reduction brings sum(r^2) and max|r w| together, and inv only enters the scale.  Nothing is
 // rounded to 16 bits on the way from r to the value: a value next to a border between two whole
 // numbers would change by a whole step (a hundredth of the row's largest) for it.
-//
-// The largest magnitude is kept as the bits of |v|, whose order as whole numbers is that of the
-// magnitudes, with infinity and NaN above all: a row that holds either is found by its maximum.
 #include "q8.h"
 
 #include <algorithm>
@@ -47,9 +44,19 @@ __device__ __forceinline__ void load8(const uint16_t* row, int c, int n, float (
 template <typename E, int SRC, bool WIDE, int T, int PER>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8QuantParams p) {
   constexpr int kRows = T < 256 ? 256 / T : 1;
+  if (p.zero && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.n_zero; i += blockDim.x) p.zero[i] = 0;
+  // Work-group b runs on XCD b % 8.  Where there are many, all of a panel's rows go to one, whose L2
+  // then joins their 16-byte pieces into whole lines.
+  constexpr int kPer = 16 / kRows;   // work-groups a panel
+  int at = blockIdx.x;
+  if (p.spread) {
+    const int i = at >> 3;
+    at = ((i / kPer) * 8 + (at & 7)) * kPer + i % kPer;
+  }
   const int tid = threadIdx.x % T;
-  const int row = blockIdx.x * kRows + threadIdx.x / T;
-  if (kRows > 1 && row >= p.M) return;   // (T = 64: whole waves, and no barrier below)
+  const int row = at * kRows + threadIdx.x / T;
+  if (row >= p.M) return;   // (T = 64: whole waves, and no barrier below)
   const int chunks = p.np / 8;
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + (int64_t)row * p.x_st;
   const float* xf = static_cast<const float*>(p.x) + (int64_t)row * p.x_st;
@@ -135,23 +142,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
       top = max(top, part_t[u]);
     }
   }
-  const bool bad = top >= 0x7f800000u;
-  const float most = fmaxf(__uint_as_float(top), kQ8Least);
-  const float f = bad ? 0.f : 127.f / most;
-  if (tid == 0) {
-    const float inv = SRC == kQ8Norm ? rsqrtf(ss / (float)p.n + p.eps) : 1.f;
-    p.scale[row] = bad ? __builtin_nanf("") : most * inv / 127.f;
-  }
-  int8_t* q = p.q + (int64_t)row * p.np;
+  const Q8Factor f = q8_factor(top);
+  if (tid == 0)
+    p.scale[row] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.n + p.eps) : 1.f);
   const auto store = [&](int c, const float (&v)[8]) {
-    u32x2 o = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (NaN times 0 is NaN; a bad row's values are zeros)
-      const int i = bad ? 0 : (int)rintf(v[e] * f);
-      o[e / 4] |= (uint32_t)(i & 0xff) << (8 * (e & 3));
-    }
-    *reinterpret_cast<u32x2*>(q + 8 * c) = o;
+    const u32x2 o = {q8_pack4(v[0], v[1], v[2], v[3], f), q8_pack4(v[4], v[5], v[6], v[7], f)};
+    *reinterpret_cast<u32x2*>(p.q + q8_at(row, c, p.np)) = o;
   };
   if constexpr (PER > 0) {
 #pragma unroll
@@ -168,13 +164,16 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
 namespace {
 
 template <typename E, int SRC, bool WIDE>
-hipError_t launch_quant_t(const Q8QuantParams& p, hipStream_t stream) {
+hipError_t launch_quant_t(Q8QuantParams p, hipStream_t stream) {
+  p.spread = p.M > 128;
+  // (in whole rounds of the 8 XCDs' panels)
+  const int rows = p.spread ? (p.M + 127) / 128 * 128 : p.M;
   if (p.np <= 64 * 4 * 8)
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 64, 4>), dim3((p.M + 3) / 4), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 64, 4>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
   else if (p.np <= 256 * 8 * 8)
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 256, 8>), dim3(p.M), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 256, 8>), dim3(rows), dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 1024, 0>), dim3(p.M), dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 1024, 0>), dim3(rows), dim3(1024), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -199,7 +198,7 @@ __global__ __launch_bounds__(256) void q8_dequant_kernel(const Q8DequantParams p
   const int64_t total = (int64_t)p.M * per_row;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int row = (int)(i / per_row), c = (int)(i - (int64_t)row * per_row);
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p.q + (int64_t)row * p.np + 8 * c);
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p.q + q8_at(row, c, p.np));
     const float s = p.scale[row];
     float v[8];
 #pragma unroll
@@ -257,6 +256,16 @@ __global__ __launch_bounds__(256) void q8_pack_kernel(const Q8PackParams p) {
     }
     *reinterpret_cast<u32x4*>(p.packed + 16 * i) = o;
   }
+}
+
+// Arrival counts of a product whose rows come in 8 bits.
+__global__ __launch_bounds__(256) void q8_zero_kernel(uint32_t* p, int n) {
+  for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
+}
+
+hipError_t launch_q8_zero(uint32_t* p, int n, hipStream_t stream) {
+  hipLaunchKernelGGL(q8_zero_kernel, dim3(1), dim3(256), 0, stream, p, n);
+  return hipGetLastError();
 }
 
 hipError_t launch_q8_pack(const Q8PackParams& p, hipStream_t stream) {

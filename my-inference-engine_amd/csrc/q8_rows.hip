@@ -1,8 +1,20 @@
-// Products of rows in 8 bits with a packed 8-bit weight: out[M][N] = x[M][K] W[N][K]^T.
+// Products of few rows in 8 bits with a packed 8-bit weight: out[M][N] = x[M][K] W[N][K]^T for the tokens
+// of a decode step, with the rows' norm and their way to 8 bits in the same launch.
 //
-// A tile is one panel of W (16 rows) by 16 MT tokens; the 8 waves of a work-group split K, and W goes from
-// memory straight into v_mfma_i32_16x16x64_i8 as its A operand, x as the B operand.  Sums are whole
-// numbers in 32 bits, so their order does not matter.
+// At these sizes a product is one pass over its weight, so the kernel is built to keep as much of W in
+// flight as the chip can hold:
+//   * A tile is NP panels of W (16 rows each).  A work-group's 8 waves split K; W goes from memory
+//     straight into v_mfma_i32_16x16x64_i8 as its A operand, a kilobyte in one run each load, and the
+//     next tile's load goes out as soon as this one's has been used.  x is the B operand, 16 tokens per
+//     MFMA, MT of them.
+//   * For K <= 2048 (KEEP) a wave's share of x stays in registers for all tiles; behind that x is read
+//     along with W.
+//   * Sums are whole numbers in 32 bits.  The waves' meet in LDS and are added by one wave, another
+//     from tile to tile, while the others go on.
+//   * Loads go through buffer resources: tokens past M, steps past a wave's share and tiles past a
+//     work-group's read as zeros, with no branch around the loads.
+// Rows that are not in 8 bits yet (SRC) are brought there first, two by each wave, and pass through LDS into
+// the operands' order, while the first weights are on their way.
 #include "q8.h"
 
 #include <algorithm>
@@ -10,73 +22,204 @@
 namespace mi_fa2 {
 
 namespace {
-constexpr int kQrWaves = 8, kQrThreads = 64 * kQrWaves;
-}
 
-template <typename E, int MT, bool GATED>
-__global__ __launch_bounds__(kQrThreads) void q8_rows_kernel(const Q8Params p) {
-  __shared__ i32x4 red[kQrWaves][MT][64];
+constexpr int kQrWaves = 8, kQrThreads = 64 * kQrWaves;
+constexpr int kQrNone = 0x7ffffff0;   // a byte offset past every resource: reads zeros
+
+}  // namespace
+
+// SRC: kQ8Plain, kQ8Norm: x is 16-bit rows; kQ8Rows: rows in 8 bits.  NS: steps of K (64) a wave takes at a
+// time.
+template <typename E, int MT, int NP, int NS, bool GATED, int SRC, bool KEEP>
+__global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p) {
+  static_assert(SRC == kQ8Rows || (KEEP && MT == 1), "rows come to 8 bits once, 16 of them");
+  constexpr int U = NP * MT;
+  constexpr int kPiece = 256 + 16;   // 16 rows' 16 bytes in LDS; the gap keeps a row's pieces off one bank
+  __shared__ i32x4 red[2][kQrWaves][U][64];
+  __shared__ float row_scale[16 * MT];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int panel = blockIdx.x;
-  const int m0 = blockIdx.y * 16 * MT;
+  // counters the next launch uses
+  if (p.zero && blockIdx.x == 0)
+    for (int i = tid; i < p.n_zero; i += kQrThreads) p.zero[i] = 0;
+
   const int steps = p.Kp >> 6;
   const int lo = wave * steps / kQrWaves, hi = (wave + 1) * steps / kQrWaves;
+  const int chunks = KEEP ? 1 : max(1, (hi - lo + NS - 1) / NS);
+  const int tiles = (p.panels + NP - 1) / NP;
 
-  const int8_t* w = p.w + (int64_t)panel * 16 * p.Kp;
-  const int rows = min(16 * MT, p.M - m0);
-  const __amdgpu_buffer_rsrc_t wr = make_rsrc(w, 16 * p.Kp);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x + (int64_t)m0 * p.Kp, rows * p.Kp);
-  i32x4 acc[MT];
+  // Step i of chunk c of tile t, panel u.
+  const auto load_w = [&](int t, int c, int u, int i) -> i32x4 {
+    const int panel = t * NP + u, s = lo + c * NS + i;
+    const bool live = panel < p.panels;
+    const __amdgpu_buffer_rsrc_t r =
+        make_rsrc(p.w + (int64_t)(live ? panel : 0) * 16 * p.Kp, live ? 16 * p.Kp : 0);
+    return __builtin_bit_cast(i32x4, ld16_buf(r, s < hi ? s * 1024 + lane * 16 : kQrNone));
+  };
+  // x: 16 tokens a panel
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, SRC == kQ8Rows ? (p.M + 15) / 16 * 16 * p.Kp : 0);
+  const auto load_x = [&](int c, int j, int i) -> i32x4 {
+    const int s = lo + c * NS + i;
+    return __builtin_bit_cast(i32x4, ld16_buf(xr, s < hi ? j * 16 * p.Kp + s * 1024 + lane * 16 : kQrNone));
+  };
+
+  i32x4 x[NS][MT], w[NP][NS];
+  constexpr int kChunks = kQ8KeepK / 8 / 64;   // of 8 elements, a lane's share of a row
+  u32x4 raw[SRC == kQ8Rows ? 1 : 2][kChunks], nw[kChunks];
+  if constexpr (SRC == kQ8Rows) {
 #pragma unroll
-  for (int j = 0; j < MT; ++j) acc[j] = i32x4{0, 0, 0, 0};
-  for (int s = lo; s < hi; ++s) {
-    const i32x4 a = __builtin_bit_cast(i32x4, ld16_buf(wr, s * 1024 + lane * 16));
+    for (int i = 0; i < NS; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const i32x4 b = __builtin_bit_cast(i32x4, ld16_buf(xr, (16 * j + n) * p.Kp + s * 64 + g * 16));
-      acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc[j], 0, 0, 0);
+      for (int j = 0; j < MT; ++j) x[i][j] = load_x(0, j, i);
+  } else {
+    // rows `wave` and `wave` + 8
+    const __amdgpu_buffer_rsrc_t rr = make_rsrc(p.x, (int)(((int64_t)(p.M - 1) * p.x_st + p.K) * 2));
+    const __amdgpu_buffer_rsrc_t nr = make_rsrc(p.norm_w, SRC == kQ8Norm ? p.K * 2 : 0);
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = lane + 64 * k;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int m = wave + 8 * h;
+        raw[h][k] = ld16_buf(rr, m < p.M && 8 * c < p.K ? m * (int)p.x_st * 2 + c * 16 : kQrNone);
+      }
+      if constexpr (SRC == kQ8Norm) nw[k] = ld16_buf(nr, c * 16);
     }
   }
 #pragma unroll
-  for (int j = 0; j < MT; ++j) red[wave][j][lane] = acc[j];
-  __syncthreads();
-  for (int j = wave; j < MT; j += kQrWaves) {
-    i32x4 s = red[0][j][lane];
+  for (int u = 0; u < NP; ++u)
 #pragma unroll
-    for (int u = 1; u < kQrWaves; ++u) s += red[u][j][lane];
-    const int m = m0 + 16 * j + n;
-    const bool live = m < p.M;
-    const float xs = p.x_scale[live ? m : m0];
-    float v[4];
-    if constexpr (GATED) {
-      const int f = 8 * panel + 4 * (g & 1);
-      float u[4];
+    for (int i = 0; i < NS; ++i) w[u][i] = load_w(blockIdx.x, 0, u, i);
+
+  if constexpr (SRC != kQ8Rows) {
+    __shared__ __attribute__((aligned(16))) char pieces[kQ8KeepK / 16 * kPiece];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float ws = f + r < p.N ? p.w_scale[(g < 2 ? 0 : p.N) + f + r] : 0.f;
-        v[r] = (float)s[r] * xs * ws;
-        u[r] = __shfl_xor(v[r], 32);
+    for (int h = 0; h < 2; ++h) {
+      const int m = wave + 8 * h;
+      if (m >= p.M) break;
+      float v[kChunks][8], ss = 0.f;
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float a = e & 1 ? E::hi(raw[h][k][e / 2]) : E::lo(raw[h][k][e / 2]);
+          if constexpr (SRC == kQ8Norm) {
+            ss = __builtin_fmaf(a, a, ss);
+            a *= e & 1 ? E::hi(nw[k][e / 2]) : E::lo(nw[k][e / 2]);
+          }
+          v[k][e] = a;
+          top = max(top, __float_as_uint(a) & 0x7fffffffu);
+        }
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) {
+        if (SRC == kQ8Norm) ss += __shfl_xor(ss, d);
+        top = max(top, (uint32_t)__shfl_xor((int)top, d));
       }
-      if (g >= 2 || !live || f >= p.N) continue;
+      const Q8Factor f = q8_factor(top);
+      if (lane == 0)
+        row_scale[m] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.K + p.eps) : 1.f);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * u[r];
-      // (the rows are padded to whole groups)
-      *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
-          f32x4{v[0], v[1], v[2], v[3]};
-    } else {
-      const int f = 16 * panel + 4 * g;
-      if (!live || f >= p.N) continue;
-      const uint16_t* res = p.res ? p.res + (int64_t)m * p.res_st + f : nullptr;
-      uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
+      for (int k = 0; k < kChunks; ++k) {
+        const int c = lane + 64 * k;
+        if (8 * c < p.Kp)
+          *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
+              u32x2{q8_pack4(v[k][0], v[k][1], v[k][2], v[k][3], f),
+                    q8_pack4(v[k][4], v[k][5], v[k][6], v[k][7], f)};
+      }
+    }
+    __syncthreads();
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (f + r >= p.N) break;
-        float t = (float)s[r] * xs * p.w_scale[f + r];
-        if (p.bias) t += E::lo(p.bias[f + r]);
-        if (res) t += E::lo(res[r]);
-        out[r] = (uint16_t)(E::pack2(t, 0.f) & 0xffffu);
+    for (int i = 0; i < NS; ++i)
+      x[i][0] = *reinterpret_cast<const i32x4*>(pieces + (min(lo + i, steps - 1) * 4 + g) * kPiece + n * 16);
+  } else if (tid < 16 * MT) {
+    row_scale[tid] = tid < p.M ? p.x_scale[tid] : 0.f;
+  }
+
+  int it = 0;
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++it) {
+    i32x4 acc[NP][MT];
+#pragma unroll
+    for (int u = 0; u < NP; ++u)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[u][j] = i32x4{0, 0, 0, 0};
+    for (int c = 0; c < chunks; ++c) {
+      const bool more = c + 1 < chunks;
+      const int nt = more ? t : t + gridDim.x, nc = more ? c + 1 : 0;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+            acc[u][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], x[i][j], acc[u][j], 0, 0, 0);
+          w[u][i] = load_w(nt, nc, u, i);
+        }
+        if constexpr (!KEEP)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) x[i][j] = load_x(nc, j, i);
+      }
+    }
+    // The waves' sums: lane (n, g) holds rows 4g .. 4g + 3 of a panel for token 16 j + n.  One barrier
+    // per tile: the other buffer's readers are past it when they meet this one.
+#pragma unroll
+    for (int u = 0; u < NP; ++u)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) red[it & 1][wave][u * MT + j][lane] = acc[u][j];
+    __syncthreads();
+    for (int u = 0; u < U; ++u) {
+      if (((it * U + u) & (kQrWaves - 1)) != wave) continue;
+      i32x4 s = red[it & 1][0][u][lane];
+#pragma unroll
+      for (int v = 1; v < kQrWaves; ++v) s += red[it & 1][v][u][lane];
+      const int panel = t * NP + u / MT, m = 16 * (u % MT) + n;
+      const bool live = m < p.M;
+      const float xs = row_scale[m];
+      float v[4];
+      if constexpr (GATED) {
+        const int f = 8 * panel + 4 * (g & 1);
+        float up[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float ws = f + r < p.N ? p.w_scale[(g < 2 ? 0 : p.N) + f + r] : 0.f;
+          v[r] = (float)s[r] * xs * ws;
+          up[r] = __shfl_xor(v[r], 32);
+        }
+        if (g >= 2 || !live || f >= p.N) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * up[r];
+        // (the rows are padded to whole groups)
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
+            f32x4{v[0], v[1], v[2], v[3]};
+      } else {
+        const int f = 16 * panel + 4 * g;
+        if (!live || f >= p.N) continue;
+        const uint16_t* res = p.res ? p.res + (int64_t)m * p.res_st + f : nullptr;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
+        if (p.wide) {
+          const f32x4 ws = *reinterpret_cast<const f32x4_4*>(p.w_scale + f);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
+          if (p.bias) {
+            const u32x2 b = *reinterpret_cast<const u32x2*>(p.bias + f);
+            v[0] += E::lo(b[0]), v[1] += E::hi(b[0]), v[2] += E::lo(b[1]), v[3] += E::hi(b[1]);
+          }
+          if (res) {
+            const u32x2 b = *reinterpret_cast<const u32x2*>(res);
+            v[0] += E::lo(b[0]), v[1] += E::hi(b[0]), v[2] += E::lo(b[1]), v[3] += E::hi(b[1]);
+          }
+          *reinterpret_cast<u32x2*>(out) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+          continue;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (f + r >= p.N) break;
+          float o = (float)s[r] * xs * p.w_scale[f + r];
+          if (p.bias) o += E::lo(p.bias[f + r]);
+          if (res) o += E::lo(res[r]);
+          out[r] = (uint16_t)(E::pack2(o, 0.f) & 0xffffu);
+        }
       }
     }
   }
@@ -84,25 +227,46 @@ __global__ __launch_bounds__(kQrThreads) void q8_rows_kernel(const Q8Params p) {
 
 namespace {
 
-template <typename E, bool GATED>
-hipError_t launch_rows_e(const Q8Params& p, hipStream_t stream) {
-  const int mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-  const dim3 grid(p.panels, (p.M + 16 * mt - 1) / (16 * mt));
-  if (mt == 1)
-    hipLaunchKernelGGL((q8_rows_kernel<E, 1, GATED>), grid, dim3(kQrThreads), 0, stream, p);
-  else if (mt == 2)
-    hipLaunchKernelGGL((q8_rows_kernel<E, 2, GATED>), grid, dim3(kQrThreads), 0, stream, p);
+template <typename E, int MT, int NP, bool GATED, int SRC>
+hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
+  if (p.Kp <= kQ8KeepK)
+    hipLaunchKernelGGL((q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true>), dim3(grid), dim3(kQrThreads), 0,
+                       stream, p);
+  else if constexpr (SRC == kQ8Rows)
+    hipLaunchKernelGGL((q8_rows_kernel<E, MT, NP, MT == 1 ? 9 : 6, GATED, SRC, false>), dim3(grid),
+                       dim3(kQrThreads), 0, stream, p);
   else
-    hipLaunchKernelGGL((q8_rows_kernel<E, 4, GATED>), grid, dim3(kQrThreads), 0, stream, p);
+    return hipErrorInvalidValue;
   return hipGetLastError();
+}
+
+template <typename E, bool GATED, int SRC>
+hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
+  const int grid = std::min(p.panels, n_cus);
+  if constexpr (SRC == kQ8Rows) {
+    if (p.M > 32) return launch_rows_k<E, 4, 1, GATED, SRC>(p, grid, stream);
+    if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
+  }
+  if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
+  return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);
+}
+
+template <typename E, bool GATED>
+hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t stream) {
+  if (source == kQ8Plain) return launch_rows_m<E, GATED, kQ8Plain>(p, n_cus, stream);
+  if (source == kQ8Norm) return launch_rows_m<E, GATED, kQ8Norm>(p, n_cus, stream);
+  return launch_rows_m<E, GATED, kQ8Rows>(p, n_cus, stream);
 }
 
 }  // namespace
 
-hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int n_cus, hipStream_t stream) {
-  (void)n_cus;
-  if (gated) return launch_rows_e<BF16, true>(p, stream);
-  return dtype == 0 ? launch_rows_e<BF16, false>(p, stream) : launch_rows_e<FP16, false>(p, stream);
+hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
+                          hipStream_t stream) {
+  if (gated)
+    return dtype == 0 ? launch_rows_s<BF16, true>(p, source, n_cus, stream)
+                      : launch_rows_s<FP16, true>(p, source, n_cus, stream);
+  return dtype == 0 ? launch_rows_s<BF16, false>(p, source, n_cus, stream)
+                    : launch_rows_s<FP16, false>(p, source, n_cus, stream);
 }
 
 }  // namespace mi_fa2

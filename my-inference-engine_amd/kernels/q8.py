@@ -35,7 +35,7 @@ _sz = ctypes.c_size_t
 # name -> (restype, argtypes); mirrors include/mi_q8.h
 SIGNATURES = {
     "mi_q8_last_error": (ctypes.c_char_p, []),
-    "mi_q8_row_bytes": (_i64, [_i32]),
+    "mi_q8_rows_bytes": (_sz, [_i32, _i32]),
     "mi_q8_quantize": (_i32, [_i32, _p, _i64, _p, _p, _i32, _i32, _p]),
     "mi_q8_add_rmsnorm": (_i32, [_i32, _p, _i64, _p, _i64, _p, _f32, _p, _i64, _p, _p, _i32, _i32,
                                  _p]),
@@ -86,9 +86,9 @@ def call(device, fn, *args):
         check(fn(*args, stream))
 
 
-def padded(n):
-    """Bytes of a row of n values in 8 bits."""
-    return -(-n // 128) * 128
+def rows_bytes(rows, n):
+    """Bytes of the values of rows in 8 bits: panels of 16 rows, n rounded up to 128."""
+    return -(-rows // 16) * 16 * (-(-n // 128) * 128)
 
 
 class Weight:
@@ -124,26 +124,33 @@ class Weight:
 def quantize_weight(weight, gated=False):
     """weight [out, in] (bf16 or fp16) in 8 bits, every row by its largest magnitude."""
     rows = quantize(weight)
-    return Weight(rows.values[:, :rows.n], rows.scale, gated)
+    return Weight(rows.values, rows.scale, gated)
 
 
 class Rows:
-    """Rows in 8 bits: values [rows, in rounded up to 128] int8 (zeros from n on), scale [rows] fp32, n the
-    row's length and dtype the type of the rows that they stand for."""
-    __slots__ = ("values", "scale", "n", "dtype")
+    """Rows in 8 bits as the kernels read them: data (their values, in panels of 16 rows: `values` has them as
+    [rows, n]), scale [rows] fp32, n the row's length and dtype the type of the rows that they stand for."""
+    __slots__ = ("data", "scale", "n", "dtype")
 
-    def __init__(self, values, scale, n, dtype):
-        self.values, self.scale, self.n, self.dtype = values, scale, n, dtype
+    def __init__(self, data, scale, n, dtype):
+        self.data, self.scale, self.n, self.dtype = data, scale, n, dtype
+
+    @property
+    def values(self):
+        """[rows, n] int8."""
+        R = self.scale.shape[0]
+        np = -(-self.n // 128) * 128
+        whole = self.data.view(-1, np // 64, 4, 16, 16).permute(0, 3, 1, 2, 4)
+        return whole.reshape(-1, np)[:R, :self.n].contiguous()
 
     def dequantize(self, out=None):
         """values * scale [rows, n] in dtype."""
-        v = self.values
-        R, dev = v.shape[0], v.device
+        R, dev = self.scale.shape[0], self.scale.device
         if out is None:
             out = torch.empty((R, self.n), device=dev, dtype=self.dtype)
         op, os_ = _rows(out, "out", self.dtype, dev)
         assert out.shape == (R, self.n), f"out: [{R}, {self.n}]"
-        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[self.dtype], v.data_ptr(),
+        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[self.dtype], self.data.data_ptr(),
              self.scale.data_ptr(), op, os_, R, self.n)
         return out
 
@@ -171,7 +178,7 @@ def _input(x):
 
 
 def _empty_rows(R, n, dtype, dev):
-    return Rows(torch.empty((R, padded(n)), dtype=torch.int8, device=dev),
+    return Rows(torch.empty(rows_bytes(R, n), dtype=torch.int8, device=dev),
                 torch.empty(R, dtype=torch.float32, device=dev), n, dtype)
 
 
@@ -181,7 +188,7 @@ def quantize(x):
     R, n = x.shape
     xp, xs = _rows(x, "x", dt, dev)
     out = _empty_rows(R, n, dt, dev)
-    call(dev.index, load().mi_q8_quantize, _lib.DTYPES[dt], xp, xs, out.values.data_ptr(),
+    call(dev.index, load().mi_q8_quantize, _lib.DTYPES[dt], xp, xs, out.data.data_ptr(),
          out.scale.data_ptr(), R, n)
     return out
 
@@ -203,7 +210,7 @@ def add_rmsnorm(x, weight, eps, y=None, residual_out=None):
         assert residual_out is None, "residual_out goes with y"
     out = _empty_rows(R, n, dt, dev)
     call(dev.index, load().mi_q8_add_rmsnorm, _lib.DTYPES[dt], xp, xs, yp, ys,
-         _vector(weight, "weight", n, dt, dev), float(eps), rp, rs, out.values.data_ptr(),
+         _vector(weight, "weight", n, dt, dev), float(eps), rp, rs, out.data.data_ptr(),
          out.scale.data_ptr(), R, n)
     return r, out
 
@@ -228,11 +235,11 @@ def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
     lib = load()
     if type(x) is Rows:
         assert norm_weight is None, "rows in 8 bits are normalised already"
-        dt, dev, R = x.dtype, x.values.device, x.values.shape[0]
+        dt, dev, R = x.dtype, x.scale.device, x.scale.shape[0]
         assert x.n == K and w.device == dev, f"x: rows of {K} on {w.device}"
         out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
         ws = torch.empty(lib.mi_q8_matmul_workspace_size(R, N, K), dtype=torch.uint8, device=dev)
-        call(dev.index, lib.mi_q8_matmul, _lib.DTYPES[dt], x.values.data_ptr(), x.scale.data_ptr(),
+        call(dev.index, lib.mi_q8_matmul, _lib.DTYPES[dt], x.data.data_ptr(), x.scale.data_ptr(),
              w.data.data_ptr(), w.scale.data_ptr(),
              _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N,
              K, ws.data_ptr(), ws.numel())

@@ -121,9 +121,9 @@ def test_empty_calls_are_no_ops():
 
 def test_sizes():
     lib = q8.load()
-    for n in (1, 127, 128, 129, 131072):
-        assert lib.mi_q8_row_bytes(n) == q8.padded(n) == -(-n // 128) * 128
-    assert lib.mi_q8_row_bytes(0) == 0
+    for rows, n in ((1, 1), (16, 127), (17, 128), (33, 129), (1 << 21, 131072)):
+        assert lib.mi_q8_rows_bytes(rows, n) == q8.rows_bytes(rows, n) == -(-rows // 16) * 16 * (-(-n // 128) * 128)
+    assert lib.mi_q8_rows_bytes(0, 5) == lib.mi_q8_rows_bytes(5, 0) == 0
     for n, k, gated in ((1, 1, 0), (2, 1, 1), (16, 64, 0), (17, 129, 0), (34, 129, 1), (2048, 1536, 1)):
         want = o8.packed(torch.zeros(n, k, dtype=torch.int8), gated).numel()
         assert lib.mi_q8_packed_bytes(n, k, gated) == want

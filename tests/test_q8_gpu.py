@@ -49,9 +49,12 @@ def check_rows(got, v, scale_tol=SCALE):
     """got: Rows; v: what they stand for, in 64 bits."""
     ratio, scale = o8.quantize(v)
     values = got.values.cpu()
-    n = v.shape[1]
-    assert got.n == n and values.shape == (v.shape[0], q8.padded(n))
-    assert not values[:, n:].any(), "what lies behind a row is zeros"
+    R, n = v.shape
+    assert got.n == n and values.shape == (R, n) and got.data.numel() == q8.rows_bytes(R, n)
+    behind = torch.arange(-(-n // 128) * 128).view(-1, 4, 1, 16) >= n
+    live = (torch.arange(-(-R // 16) * 16) < R).view(-1, 1, 1, 16, 1)
+    panels = got.data.cpu().view(-1, behind.shape[0], 4, 16, 16)
+    assert not (panels.bool() & behind & live).any(), "what lies behind a row is zeros"
     fine = torch.isfinite(scale)
     assert torch.equal(torch.isnan(got.scale.cpu()), ~fine)
     assert not values[~fine].any()
@@ -61,7 +64,7 @@ def check_rows(got, v, scale_tol=SCALE):
     assert (far <= 0.5 + VALUE).all(), far.max()
 
 
-SIZES = [(1, 1), (3, 7), (2, 64), (5, 128), (4, 1000), (1, 1536), (130, 1536), (70, 2048), (3, 2049),
+SIZES = [(1, 1), (3, 7), (2, 64), (5, 128), (4, 1000), (1, 1536), (130, 1536), (300, 640), (70, 2048), (3, 2049),
          (9, 4864), (2, 8960), (2, 16384), (3, 16385), (1, 40008)]
 
 
@@ -77,7 +80,7 @@ def test_quantize(rows, n, dtype):
         again = q8.quantize(strided(x, pad, at))
         assert torch.equal(again.values, got.values) and torch.equal(again.scale, got.scale)
     back = got.dequantize()
-    want = got.values[:, :n].double() * got.scale.double()[:, None]
+    want = got.values.double() * got.scale.double()[:, None]
     assert back.dtype == dtype
     assert ((back.double() - want).abs() <= (half(dtype) + 2 * U) * want.abs() + least(dtype)).all()
     into = strided(torch.zeros(rows, n, dtype=dtype), 3, 1)
@@ -126,15 +129,16 @@ def test_rows_of_nothing_and_of_no_number(n, dtype):
     x[7] *= -1
     got = q8.quantize(x.to(DEV))
     check_rows(got, x, 2 * U)
-    assert not got.values[0].any() and (got.values[5, :n] == 127).all()
-    assert got.values[6, n - 1] == -127 and (got.values[7, :n] == -127).all()
+    assert not got.values[0].any() and (got.values[5] == 127).all()
+    assert got.values[6, n - 1] == -127 and (got.values[7] == -127).all()
     w = torch.ones(n, dtype=dtype, device=DEV)
     _, got = q8.add_rmsnorm(x.to(DEV), w, 1e-6)
     bad = torch.isnan(got.scale.cpu())
     # the largest bf16's square is past fp32: its mean is infinite and the row is zero times a number
     assert bad[2:5].all() and not bad[[0, 1, 6, 7, 8]].any()
     assert not got.values[:1].any() and got.scale[0] >= 0
-    check_rows(q8.Rows(got.values[6:], got.scale[6:], n, dtype), o8.rmsnorm(x[6:], w.cpu(), 1e-6))
+    _, got = q8.add_rmsnorm(x[6:].to(DEV), w, 1e-6)
+    check_rows(got, o8.rmsnorm(x[6:], w.cpu(), 1e-6))
 
 
 def test_ties_go_to_the_even_number():
@@ -144,7 +148,7 @@ def test_ties_go_to_the_even_number():
     x[0, 0], x[0, -1] = -63.5 * 2, 63.5 * 2
     got = q8.quantize(x.to(DEV))
     assert got.scale.item() == 1.0
-    assert torch.equal(got.values[0, :n].cpu().double(), torch.round(x[0].double()))
+    assert torch.equal(got.values[0].cpu().double(), torch.round(x[0].double()))
 
 
 @pytest.mark.parametrize("gated", [False, True])
@@ -171,7 +175,7 @@ def weight_of(g, n, k, gated=False):
 def check_product(out, rows, values, scale, bias, residual, extra=0.0):
     """out against the product of Rows; extra: what each entry may be off beside."""
     dt = out.dtype
-    q, xs = rows.values[:, :rows.n].cpu(), rows.scale.cpu()
+    q, xs = rows.values.cpu(), rows.scale.cpu()
     want = o8.product(q, xs, values, scale)
     size = want.abs()
     for t in (bias, residual):
@@ -239,7 +243,7 @@ def mlp_bounds(rows, gate_up, gate_up_scale, down, down_scale):
     """The block's second product in 64 bits from its first rows, and how far it may be off: whole steps of
     values next to a border, the first product's 8 U + 2 SCALE and what an exponential (8 U) and |g|
     make of it in the activation."""
-    q, xs = rows.values[:, :rows.n].cpu(), rows.scale.cpu()
+    q, xs = rows.values.cpu(), rows.scale.cpu()
     both = o8.product(q, xs, gate_up, gate_up_scale)
     gate, up = both.chunk(2, 1)
     act = o8.silu_mul(gate, up)
@@ -290,7 +294,9 @@ def test_mlp(m, hidden, inter, dtype):
     for pad, at in ((8, 8), (3, 1)):
         view = strided(x, pad, at)
         assert q8.mlp(view, gate_up, down, residual=view, norm_weight=nd, eps=1e-6, out=view) is view
-        assert torch.equal(view, out)
+        # (rows that lie otherwise may have their squares summed in another order: the scale moves in its
+        # last places, within SCALE, and activations next to a border by a step, which check() counts)
+        check(view, rows, x)
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
@@ -321,7 +327,7 @@ def test_quantized_weight_is_a_row_for_each_feature():
     got = q8.quantize_weight(w.to(DEV))
     rows = q8.quantize(w.to(DEV))
     check_rows(rows, w, 2 * U)
-    assert torch.equal(got.data.cpu(), o8.packed(rows.values[:, :200].cpu()).flatten())
+    assert torch.equal(got.data.cpu(), o8.packed(rows.values.cpu()).flatten())
     assert torch.equal(got.scale, rows.scale)
 
 
@@ -330,7 +336,7 @@ def test_no_rows():
     x = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
     _, _, w = weight_of(g, 64, 64)
     _, _, gu = weight_of(g, 128, 64, gated=True)
-    assert q8.quantize(x).values.shape == (0, 128)
+    assert q8.quantize(x).values.shape == (0, 64)
     assert q8.linear(x, w).shape == (0, 64) and q8.linear(q8.quantize(x), w).shape == (0, 64)
     assert q8.mlp(x, gu, w).shape == (0, 64)
     assert q8.add_rmsnorm(x, x.new_ones(64), 1e-6)[1].dequantize().shape == (0, 64)
