@@ -77,13 +77,10 @@ MI_Q8_API int mi_q8_pack(const void* values, int64_t stride, int32_t out_feature
  * leaves them, w packed, w_scale [out_features], bias [out_features] or NULL, residual
  * [rows, out_features] or NULL (may be out).
  */
-MI_Q8_API size_t mi_q8_matmul_workspace_size(int32_t rows, int32_t out_features,
-                                             int32_t in_features);
 MI_Q8_API int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
                            const float* w_scale, const void* bias, const void* residual,
                            int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                           int32_t out_features, int32_t in_features, void* workspace,
-                           size_t workspace_bytes, void* stream);
+                           int32_t out_features, int32_t in_features, void* stream);
 
 /*
  * The same of rows x [rows, in] that the call holds in 8 bits itself, as mi_q8_add_rmsnorm does without

@@ -59,6 +59,24 @@ __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d,
   return r.bad ? 0u : lo | hi << 16;
 }
 
+// A sum with its scales, and what is added to that: each rounded by itself, so that every kernel and every
+// alignment gives the same number.
+__device__ __forceinline__ float q8_scaled(int s, float x_scale, float w_scale) {
+#pragma clang fp contract(off)
+  return (float)s * x_scale * w_scale;
+}
+__device__ __forceinline__ float q8_plus(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
+template <typename E>
+__device__ __forceinline__ void add4(float (&v)[4], u32x2 b) {
+  v[0] = q8_plus(v[0], E::lo(b[0]));
+  v[1] = q8_plus(v[1], E::hi(b[0]));
+  v[2] = q8_plus(v[2], E::lo(b[1]));
+  v[3] = q8_plus(v[3], E::hi(b[1]));
+}
+
 // Rows to 8 bits, and back.
 struct Q8QuantParams {
   const void* x;          // [M][x_st] 16-bit, or fp32
@@ -73,14 +91,10 @@ struct Q8QuantParams {
   float* scale;           // [M]
   int32_t M, n, np;
   int32_t wide;           // every row and the norm's weight allow 16-byte accesses
-  uint32_t* zero;         // counters this launch zeroes for the next one
-  int32_t n_zero;
   int32_t spread;         // work-groups are dealt so that a panel's rows share an XCD
 };
 enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2, kQ8Rows = 3 };
 hipError_t launch_q8_quant(const Q8QuantParams& p, int dtype, int source, hipStream_t stream);
-
-hipError_t launch_q8_zero(uint32_t* p, int n, hipStream_t stream);
 
 struct Q8DequantParams {
   const int8_t* q;
@@ -116,16 +130,10 @@ struct Q8Params {
   int32_t M, N, K, Kp;    // N: out features (gated: of the activation)
   int32_t panels;
   int32_t wide;           // out and residual allow accesses of 8 elements, bias of 4
-  // splits > 1: work-groups that share a tile's K, their sums and the tiles' arrival counts (zero at
-  // launch)
-  int32_t splits;
-  uint64_t* part;
-  uint32_t* count;
-  uint32_t* zero;         // counters a few-row launch zeroes for the next one
-  int32_t n_zero;
 };
 hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
                           hipStream_t stream);
+hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream);
 hipError_t launch_q8_gemm(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream);
 
 }  // namespace mi_fa2

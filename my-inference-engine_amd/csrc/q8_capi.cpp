@@ -114,18 +114,6 @@ struct RowsSpace {
       : values(s.take((size_t)(((int64_t)rows + 15) / 16 * 16) * q8_pad(n))), scale(s.take((size_t)rows * 4)) {}
 };
 
-// What a product needs beside its rows: the sums of shares of K and the tiles' arrival counts.
-struct ProductSpace {
-  mi_fa2::Q8Plan plan;
-  size_t part, count;
-  ProductSpace(Space& s, int32_t rows, int32_t out_features, int32_t in_features, bool gated)
-      : plan(mi_fa2::q8_plan(rows, mi_fa2::q8_panels(gated ? 2 * out_features : out_features, gated),
-                             q8_pad(in_features))),
-        part(s.take(plan.part)), count(s.take(plan.count)) {}
-  uint32_t* counts(char* ws) const { return plan.count ? reinterpret_cast<uint32_t*>(ws + count) : nullptr; }
-  int32_t n_counts() const { return (int32_t)(plan.count / 4); }
-};
-
 int check_workspace(const void* ws, size_t have, size_t need) {
   if (need == 0) return kOk;
   if (int rc = check_ptr("workspace", ws, 16)) return rc;
@@ -135,7 +123,7 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 
 int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t y_stride,
              const void* norm_weight, float eps, void* r, int64_t r_stride, void* values,
-             float* scale, int32_t rows, int32_t n, uint32_t* zero, int32_t n_zero, void* stream) {
+             float* scale, int32_t rows, int32_t n, void* stream) {
   Q8QuantParams p{};
   p.x = x;
   p.x_st = x_stride;
@@ -150,8 +138,6 @@ int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t 
   p.M = rows;
   p.n = n;
   p.np = q8_pad(n);
-  p.zero = zero;
-  p.n_zero = n_zero;
   p.wide = wide(x, x_stride, n) && wide(y, y_stride, n) && wide(norm_weight, 8, n) &&
            (!y || wide(r, r_stride, n));
   return launched(mi_fa2::launch_q8_quant(p, dtype, norm_weight ? mi_fa2::kQ8Norm : mi_fa2::kQ8Plain,
@@ -181,15 +167,17 @@ Q8Params operands(const void* w, const float* w_scale, const void* bias, const v
 }
 
 // The product of rows in 8 bits.
-int product(Q8Params p, int dtype, bool gated, const void* values, const float* scale,
-            const ProductSpace& sp, char* ws, void* stream) {
+int product(Q8Params p, int dtype, bool gated, const void* values, const float* scale, void* stream) {
   p.x = values;
   p.x_scale = scale;
-  p.splits = sp.plan.splits;
-  p.part = reinterpret_cast<uint64_t*>(ws + sp.part);
-  p.count = sp.counts(ws);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (sp.plan.np) return launched(mi_fa2::launch_q8_gemm(p, sp.plan, dtype, gated, st));
+  const mi_fa2::Q8Plan plan = mi_fa2::q8_plan(p.M, p.panels, p.Kp);
+  switch (plan.kernel) {
+    case mi_fa2::kQ8Tile32:
+    case mi_fa2::kQ8Tile64: return launched(mi_fa2::launch_q8_tile(p, plan, dtype, gated, st));
+    case mi_fa2::kQ8Gemm64:
+    case mi_fa2::kQ8Gemm128: return launched(mi_fa2::launch_q8_gemm(p, plan, dtype, gated, st));
+  }
   int cus = 0;
   if (int rc = compute_units(&cus)) return rc;
   return launched(mi_fa2::launch_q8_rows(p, dtype, gated, mi_fa2::kQ8Rows, cus, st));
@@ -202,8 +190,7 @@ bool fused(const void* x, int64_t x_stride, const void* norm_weight, int32_t row
          wide(x, x_stride, in) && wide(norm_weight, 8, in);
 }
 int product_of(Q8Params p, int dtype, bool gated, const void* x, int64_t x_stride,
-               const void* norm_weight, float eps, const RowsSpace& r, const ProductSpace& sp,
-               char* ws, void* stream) {
+               const void* norm_weight, float eps, const RowsSpace& r, char* ws, void* stream) {
   if (fused(x, x_stride, norm_weight, p.M, p.K)) {
     p.x = x;
     p.x_st = x_stride;
@@ -216,28 +203,24 @@ int product_of(Q8Params p, int dtype, bool gated, const void* x, int64_t x_strid
   }
   float* scale = reinterpret_cast<float*>(ws + r.scale);
   if (int rc = quantize(dtype, x, x_stride, nullptr, 0, norm_weight, eps, nullptr, 0, ws + r.values,
-                        scale, p.M, p.K, sp.counts(ws), sp.n_counts(), stream))
+                        scale, p.M, p.K, stream))
     return rc;
-  return product(p, dtype, gated, ws + r.values, scale, sp, ws, stream);
+  return product(p, dtype, gated, ws + r.values, scale, stream);
 }
 
 struct LinearSpace {
   Space s;
   RowsSpace x;
-  ProductSpace product;
-  LinearSpace(int32_t rows, int32_t out_features, int32_t in_features)
-      : x(s, rows, in_features), product(s, rows, out_features, in_features, false) {}
+  LinearSpace(int32_t rows, int32_t in_features) : x(s, rows, in_features) {}
 };
 
 struct MlpSpace {
   Space s;
   RowsSpace x, a;
-  ProductSpace gate_up, down;
   size_t act;
   int64_t act_stride;
   MlpSpace(int32_t rows, int32_t hidden, int32_t inter)
-      : x(s, rows, hidden), a(s, rows, inter), gate_up(s, rows, inter, hidden, true),
-        down(s, rows, hidden, inter, false), act(0), act_stride(((int64_t)inter + 7) / 8 * 8) {
+      : x(s, rows, hidden), a(s, rows, inter), act(0), act_stride(((int64_t)inter + 7) / 8 * 8) {
     act = s.take((size_t)rows * act_stride * 4);
   }
 };
@@ -263,7 +246,7 @@ int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values,
   if (int rc = check_ptr("values", values, 16)) return rc;
   if (int rc = check_ptr("scale", scale, 4)) return rc;
   return quantize(dtype, x, x_stride, nullptr, 0, nullptr, 0.f, nullptr, 0, values, scale, rows, n,
-                  nullptr, 0, stream);
+                  stream);
 }
 
 int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
@@ -283,7 +266,7 @@ int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void
   if (int rc = check_ptr("values", values, 16)) return rc;
   if (int rc = check_ptr("scale", scale, 4)) return rc;
   return quantize(dtype, x, x_stride, y, y_stride, weight, eps, residual_out, residual_stride,
-                  values, scale, rows, n, nullptr, 0, stream);
+                  values, scale, rows, n, stream);
 }
 
 int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
@@ -329,13 +312,6 @@ int mi_q8_pack(const void* values, int64_t stride, int32_t out_features, int32_t
   return launched(mi_fa2::launch_q8_pack(p, reinterpret_cast<hipStream_t>(stream)));
 }
 
-size_t mi_q8_matmul_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
-  if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
-  Space s;
-  ProductSpace(s, rows, out_features, in_features, false);
-  return s.total;
-}
-
 namespace {
 
 int check_product(int32_t rows, int32_t out_features, int32_t in_features) {
@@ -359,8 +335,7 @@ int check_operands(const void* w, const float* w_scale, const void* bias, const 
 int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
                  const float* w_scale, const void* bias, const void* residual,
                  int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                 int32_t out_features, int32_t in_features, void* workspace,
-                 size_t workspace_bytes, void* stream) {
+                 int32_t out_features, int32_t in_features, void* stream) {
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_product(rows, out_features, in_features)) return rc;
   if (rows == 0) return ok();
@@ -369,22 +344,14 @@ int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const vo
   if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
                               out_features))
     return rc;
-  Space s;
-  const ProductSpace sp(s, rows, out_features, in_features, false);
-  if (int rc = check_workspace(workspace, workspace_bytes, s.total)) return rc;
-  char* ws = static_cast<char*>(workspace);
-  if (sp.n_counts())
-    if (int rc = launched(mi_fa2::launch_q8_zero(sp.counts(ws), sp.n_counts(),
-                                                 reinterpret_cast<hipStream_t>(stream))))
-      return rc;
   return product(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
                           out_features, in_features, false),
-                 dtype, false, values, scale, sp, ws, stream);
+                 dtype, false, values, scale, stream);
 }
 
 size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
   if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
-  return LinearSpace(rows, out_features, in_features).s.total;
+  return LinearSpace(rows, in_features).s.total;
 }
 
 int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
@@ -402,12 +369,12 @@ int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* nor
     return rc;
   if (overlap(x, span(rows, x_stride, in_features), out, span(rows, out_stride, out_features)))
     return fail(kInvalid, "out overlaps x");
-  const LinearSpace sp(rows, out_features, in_features);
+  const LinearSpace sp(rows, in_features);
   if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
   return product_of(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
                              out_features, in_features, false),
-                    dtype, false, x, x_stride, norm_weight, eps, sp.x, sp.product,
-                    static_cast<char*>(workspace), stream);
+                    dtype, false, x, x_stride, norm_weight, eps, sp.x, static_cast<char*>(workspace),
+                    stream);
 }
 
 size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter) {
@@ -438,7 +405,7 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
   float* a_scale = reinterpret_cast<float*>(ws + sp.a.scale);
   if (int rc = product_of(operands(gate_up, gate_up_scale, nullptr, nullptr, 0, ws + sp.act,
                                    sp.act_stride, rows, inter, hidden, true),
-                          dtype, true, x, x_stride, norm_weight, eps, sp.x, sp.gate_up, ws, stream))
+                          dtype, true, x, x_stride, norm_weight, eps, sp.x, ws, stream))
     return rc;
   Q8QuantParams q{};
   q.x = ws + sp.act;
@@ -448,14 +415,12 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
   q.M = rows;
   q.n = inter;
   q.np = q8_pad(inter);
-  q.zero = sp.down.counts(ws);
-  q.n_zero = sp.down.n_counts();
   if (int rc = launched(mi_fa2::launch_q8_quant(q, dtype, mi_fa2::kQ8Float,
                                                 reinterpret_cast<hipStream_t>(stream))))
     return rc;
   return product(operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride,
                           rows, hidden, inter, false),
-                 dtype, false, ws + sp.a.values, a_scale, sp.down, ws, stream);
+                 dtype, false, ws + sp.a.values, a_scale, stream);
 }
 
 }  // extern "C"

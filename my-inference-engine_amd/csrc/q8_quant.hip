@@ -44,8 +44,6 @@ __device__ __forceinline__ void load8(const uint16_t* row, int c, int n, float (
 template <typename E, int SRC, bool WIDE, int T, int PER>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8QuantParams p) {
   constexpr int kRows = T < 256 ? 256 / T : 1;
-  if (p.zero && blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.n_zero; i += blockDim.x) p.zero[i] = 0;
   // Work-group b runs on XCD b % 8.  Where there are many, all of a panel's rows go to one, whose L2
   // then joins their 16-byte pieces into whole lines.
   constexpr int kPer = 16 / kRows;   // work-groups a panel
@@ -256,16 +254,6 @@ __global__ __launch_bounds__(256) void q8_pack_kernel(const Q8PackParams p) {
     }
     *reinterpret_cast<u32x4*>(p.packed + 16 * i) = o;
   }
-}
-
-// Arrival counts of a product whose rows come in 8 bits.
-__global__ __launch_bounds__(256) void q8_zero_kernel(uint32_t* p, int n) {
-  for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
-}
-
-hipError_t launch_q8_zero(uint32_t* p, int n, hipStream_t stream) {
-  hipLaunchKernelGGL(q8_zero_kernel, dim3(1), dim3(256), 0, stream, p, n);
-  return hipGetLastError();
 }
 
 hipError_t launch_q8_pack(const Q8PackParams& p, hipStream_t stream) {

@@ -26,6 +26,52 @@ namespace {
 constexpr int kQrWaves = 8, kQrThreads = 64 * kQrWaves;
 constexpr int kQrNone = 0x7ffffff0;   // a byte offset past every resource: reads zeros
 
+// The sums s of rows 4g .. 4g + 3 of a panel with token m, whose scale is xs, on their way out.  All lanes of
+// the wave call it.
+template <typename E, bool GATED>
+__device__ __forceinline__ void finish(const Q8Params& p, int panel, int m, int g, float xs, i32x4 s) {
+  const bool live = m < p.M;
+  float v[4];
+  if constexpr (GATED) {
+    const int f = 8 * panel + 4 * (g & 1);
+    float up[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float ws = f + r < p.N ? p.w_scale[(g < 2 ? 0 : p.N) + f + r] : 0.f;
+      v[r] = q8_scaled(s[r], xs, ws);
+      up[r] = __shfl_xor(v[r], 32);
+    }
+    if (g >= 2 || !live || f >= p.N) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * up[r];
+    // (the rows are padded to whole groups)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
+        f32x4{v[0], v[1], v[2], v[3]};
+  } else {
+    const int f = 16 * panel + 4 * g;
+    if (!live || f >= p.N) return;
+    const uint16_t* res = p.res ? p.res + (int64_t)m * p.res_st + f : nullptr;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
+    if (p.wide) {
+      const f32x4 ws = *reinterpret_cast<const f32x4_4*>(p.w_scale + f);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = q8_scaled(s[r], xs, ws[r]);
+      if (p.bias) add4<E>(v, *reinterpret_cast<const u32x2*>(p.bias + f));
+      if (res) add4<E>(v, *reinterpret_cast<const u32x2*>(res));
+      *reinterpret_cast<u32x2*>(out) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+      return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (f + r >= p.N) break;
+      float o = q8_scaled(s[r], xs, p.w_scale[f + r]);
+      if (p.bias) o = q8_plus(o, E::lo(p.bias[f + r]));
+      if (res) o = q8_plus(o, E::lo(res[r]));
+      out[r] = (uint16_t)(E::pack2(o, 0.f) & 0xffffu);
+    }
+  }
+}
+
 }  // namespace
 
 // SRC: kQ8Plain, kQ8Norm: x is 16-bit rows; kQ8Rows: rows in 8 bits.  NS: steps of K (64) a wave takes at a
@@ -40,9 +86,6 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  // counters the next launch uses
-  if (p.zero && blockIdx.x == 0)
-    for (int i = tid; i < p.n_zero; i += kQrThreads) p.zero[i] = 0;
 
   const int steps = p.Kp >> 6;
   const int lo = wave * steps / kQrWaves, hi = (wave + 1) * steps / kQrWaves;
@@ -173,55 +216,69 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
       i32x4 s = red[it & 1][0][u][lane];
 #pragma unroll
       for (int v = 1; v < kQrWaves; ++v) s += red[it & 1][v][u][lane];
-      const int panel = t * NP + u / MT, m = 16 * (u % MT) + n;
-      const bool live = m < p.M;
-      const float xs = row_scale[m];
-      float v[4];
-      if constexpr (GATED) {
-        const int f = 8 * panel + 4 * (g & 1);
-        float up[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float ws = f + r < p.N ? p.w_scale[(g < 2 ? 0 : p.N) + f + r] : 0.f;
-          v[r] = (float)s[r] * xs * ws;
-          up[r] = __shfl_xor(v[r], 32);
-        }
-        if (g >= 2 || !live || f >= p.N) continue;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * up[r];
-        // (the rows are padded to whole groups)
-        *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
-            f32x4{v[0], v[1], v[2], v[3]};
-      } else {
-        const int f = 16 * panel + 4 * g;
-        if (!live || f >= p.N) continue;
-        const uint16_t* res = p.res ? p.res + (int64_t)m * p.res_st + f : nullptr;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
-        if (p.wide) {
-          const f32x4 ws = *reinterpret_cast<const f32x4_4*>(p.w_scale + f);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
-          if (p.bias) {
-            const u32x2 b = *reinterpret_cast<const u32x2*>(p.bias + f);
-            v[0] += E::lo(b[0]), v[1] += E::hi(b[0]), v[2] += E::lo(b[1]), v[3] += E::hi(b[1]);
-          }
-          if (res) {
-            const u32x2 b = *reinterpret_cast<const u32x2*>(res);
-            v[0] += E::lo(b[0]), v[1] += E::hi(b[0]), v[2] += E::lo(b[1]), v[3] += E::hi(b[1]);
-          }
-          *reinterpret_cast<u32x2*>(out) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
-          continue;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (f + r >= p.N) break;
-          float o = (float)s[r] * xs * p.w_scale[f + r];
-          if (p.bias) o += E::lo(p.bias[f + r]);
-          if (res) o += E::lo(res[r]);
-          out[r] = (uint16_t)(E::pack2(o, 0.f) & 0xffffu);
-        }
-      }
+      const int m = 16 * (u % MT) + n;
+      finish<E, GATED>(p, t * NP + u / MT, m, g, row_scale[m], s);
     }
+  }
+}
+
+// A tile of NP panels by 16 MT tokens a work-group, its 8 waves' shares of K each from memory straight into
+// the MFMAs: nothing is shared but the sums, so there is no barrier before the last.
+template <typename E, int MT, int NP, bool GATED>
+__global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p) {
+  constexpr int U = NP * MT, D = 3;
+  __shared__ i32x4 red[kQrWaves][U][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  // work-group b runs on XCD b % 8: an XCD takes a contiguous share of the tiles, all tokens of a few
+  // panels
+  const int total = gridDim.x, mt = (p.M + 16 * MT - 1) / (16 * MT);
+  const int xcd = blockIdx.x & 7, id = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+  const int tn = id / mt, j0 = (id - tn * mt) * MT, panel0 = tn * NP;
+  const int steps = p.Kp >> 6;
+  const int lo = wave * steps / kQrWaves, hi = (wave + 1) * steps / kQrWaves;
+  const __amdgpu_buffer_rsrc_t wr =
+      make_rsrc(p.w + (int64_t)panel0 * 16 * p.Kp, min(NP, p.panels - panel0) * 16 * p.Kp);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(static_cast<const int8_t*>(p.x) + (int64_t)j0 * 16 * p.Kp,
+                                              min(MT, (p.M + 15) / 16 - j0) * 16 * p.Kp);
+  i32x4 w[D][NP], x[D][MT], acc[NP][MT];
+  const auto load = [&](int d, int s) {
+    const int at = s < hi ? s * 1024 + lane * 16 : kQrNone;
+#pragma unroll
+    for (int u = 0; u < NP; ++u)
+      w[d][u] = __builtin_bit_cast(i32x4, ld16_buf(wr, s < hi ? at + u * 16 * p.Kp : kQrNone));
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      x[d][j] = __builtin_bit_cast(i32x4, ld16_buf(xr, s < hi ? at + j * 16 * p.Kp : kQrNone));
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(d, lo + d);
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[u][j] = i32x4{0, 0, 0, 0};
+  for (int s = lo; s < hi; s += D)
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          acc[u][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][u], x[d][j], acc[u][j], 0, 0, 0);
+      load(d, s + d + D);
+    }
+#pragma unroll
+  for (int u = 0; u < NP; ++u)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[wave][u * MT + j][lane] = acc[u][j];
+  __syncthreads();
+  for (int u = wave; u < U; u += kQrWaves) {
+    i32x4 s = red[0][u][lane];
+#pragma unroll
+    for (int v = 1; v < kQrWaves; ++v) s += red[v][u][lane];
+    const int m = (j0 + u % MT) * 16 + n;
+    finish<E, GATED>(p, panel0 + u / MT, m, g, p.x_scale[min(m, p.M - 1)], s);
   }
 }
 
@@ -259,6 +316,21 @@ hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t s
 }
 
 }  // namespace
+
+hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream) {
+  const dim3 grid(plan.tiles), block(kQrThreads);
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p); };
+  if (plan.kernel == kQ8Tile64) {
+    if (gated) go(q8_tile_kernel<BF16, 4, 4, true>);
+    else if (dtype == 0) go(q8_tile_kernel<BF16, 4, 4, false>);
+    else go(q8_tile_kernel<FP16, 4, 4, false>);
+  } else {
+    if (gated) go(q8_tile_kernel<BF16, 2, 4, true>);
+    else if (dtype == 0) go(q8_tile_kernel<BF16, 2, 4, false>);
+    else go(q8_tile_kernel<FP16, 2, 4, false>);
+  }
+  return hipGetLastError();
+}
 
 hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
                           hipStream_t stream) {

@@ -1,7 +1,6 @@
 // Which kernel computes a product in 8 bits, and in what tiles.  No device code: tests ask it on the CPU.
 #pragma once
 
-#include <stddef.h>
 #include <stdint.h>
 #ifdef Q8_TUNE
 #include <cstdlib>
@@ -13,34 +12,42 @@ constexpr int kQ8RowsMax = 64;    // rows that the few-row kernel takes
 constexpr int kQ8KeepK = 2048;    // (padded) in features whose rows it keeps in registers
 constexpr int kQ8FusedMax = 16;   // rows that it brings to 8 bits itself, of at most kQ8KeepK
 
+enum Q8Kernel { kQ8FewRows = 0, kQ8Tile32 = 1, kQ8Tile64 = 2, kQ8Gemm64 = 3, kQ8Gemm128 = 4 };
+
 struct Q8Plan {
-  int32_t np;       // panels of W a tile, 0: the few-row kernel
-  int32_t tm;       // tokens a tile
-  int32_t tiles;
-  int32_t splits;   // work-groups that share a tile's K
-  size_t part;      // bytes of their sums (4 for each number of every tile and share), 0 for one
-  size_t count;     // bytes of their arrival counts
+  int32_t kernel;   // Q8Kernel
+  int32_t tiles;    // work-groups
 };
 
+// The tile kernel (32 or 64 tokens by 64 features, K split over the work-group's waves, straight from
+// memory) hides the most latency but reads x and W once for every tile that needs them: it is taken while
+// its tiles are no more than the 256 CUs.  Behind that the products that share operands through LDS:
+// 64 x 64 tiles until there are enough of 128 x 128 for every CU.  Measured (us, 32 x 64 / 64 x 64 straight from
+// memory, 64 x 64 / 128 x 128 through LDS):
+//   tokens x features x K: 96 x 1536 x 8960 12.1 16.9 22.5 39;  512 x 1536 x 8960 22.3 18.3 22.9 41;
+//   1024 x 1536 x 8960 37.0 35.4 26.9 42;  256 x 2048 x 1536 5.2 6.3 6.4 11;  400 x 2048 x 1536 7.3 6.6 6.6 11;
+//   1024 x 2048 x 1536 13.6 13.1 8.5 12;  4096 x 2048 x 1536 - - 25.7 20.0;  150 x 17920 x 1536 19.4 23.6 13.6
+//   14.8;  512 x 17920 x 1536 48 51 28.2 25.2
 inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
-  Q8Plan p{};
-  p.splits = 1;
-  if (rows <= kQ8RowsMax) return p;
-  const int steps = kp / 64;
-  p.np = 16;
-  p.tm = 128;
+  constexpr int64_t kCus = 256;
+  (void)kp;
+  const auto tiles = [&](int tm, int np) {
+    return (int64_t)((rows + tm - 1) / tm) * ((panels + np - 1) / np);
+  };
 #ifdef Q8_TUNE
-  if (const char* e = getenv("Q8_NP")) { p.np = atoi(e); p.tm = p.np == 4 ? 64 : 128; }
-  if (const char* e = getenv("Q8_SPLITS")) p.splits = atoi(e) < steps ? atoi(e) : steps;
-#endif
-  (void)steps;
-  const int64_t tiles = (int64_t)((rows + p.tm - 1) / p.tm) * ((panels + p.np - 1) / p.np);
-  p.tiles = (int32_t)tiles;
-  if (p.splits > 1) {
-    p.part = (size_t)tiles * p.splits * p.np * 16 * p.tm * 4;
-    p.count = (size_t)tiles * 4;
+  if (getenv("Q8_NP") && (rows > 64 || atoi(getenv("Q8_NP")))) {
+    const int np = atoi(getenv("Q8_NP"));
+    if (np == 1) return {kQ8Tile32, (int32_t)tiles(32, 4)};
+    if (np == 2) return {kQ8Tile64, (int32_t)tiles(64, 4)};
+    if (np == 4) return {kQ8Gemm64, (int32_t)tiles(64, 4)};
+    if (np == 8) return {kQ8Gemm128, (int32_t)tiles(128, 8)};
   }
-  return p;
+#endif
+  if (rows <= kQ8RowsMax) return {kQ8FewRows, 0};
+  if (tiles(32, 4) <= kCus) return {kQ8Tile32, (int32_t)tiles(32, 4)};
+  if (tiles(64, 4) <= kCus) return {kQ8Tile64, (int32_t)tiles(64, 4)};
+  if (tiles(128, 8) < kCus) return {kQ8Gemm64, (int32_t)tiles(64, 4)};
+  return {kQ8Gemm128, (int32_t)tiles(128, 8)};
 }
 
 }  // namespace mi_fa2

@@ -42,9 +42,7 @@ SIGNATURES = {
     "mi_q8_dequantize": (_i32, [_i32, _p, _p, _p, _i64, _i32, _i32, _p]),
     "mi_q8_packed_bytes": (_sz, [_i32, _i32, _i32]),
     "mi_q8_pack": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _p]),
-    "mi_q8_matmul_workspace_size": (_sz, [_i32, _i32, _i32]),
-    "mi_q8_matmul": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32, _p, _sz,
-                            _p]),
+    "mi_q8_matmul": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32, _p]),
     "mi_q8_linear_workspace_size": (_sz, [_i32, _i32, _i32]),
     "mi_q8_linear": (_i32, [_i32, _p, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32,
                             _i32, _p, _sz, _p]),
@@ -238,11 +236,10 @@ def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
         dt, dev, R = x.dtype, x.scale.device, x.scale.shape[0]
         assert x.n == K and w.device == dev, f"x: rows of {K} on {w.device}"
         out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
-        ws = torch.empty(lib.mi_q8_matmul_workspace_size(R, N, K), dtype=torch.uint8, device=dev)
         call(dev.index, lib.mi_q8_matmul, _lib.DTYPES[dt], x.data.data_ptr(), x.scale.data_ptr(),
              w.data.data_ptr(), w.scale.data_ptr(),
              _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N,
-             K, ws.data_ptr(), ws.numel())
+             K)
         return out
     dt, dev = _input(x)
     R = x.shape[0]

@@ -57,7 +57,7 @@ def _pack(**over):
 
 def _matmul(**over):
     a = dict(dtype=0, values=16, scale=16, w=16, ws=16, bias=None, res=None, rs=0, out=1 << 30, os=48,
-             rows=3, n=48, k=64, space=16, size=1 << 30)
+             rows=3, n=48, k=64)
     a.update(over)
     return q8.load().mi_q8_matmul(*a.values(), None)
 
