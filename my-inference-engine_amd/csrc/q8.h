@@ -16,7 +16,9 @@ namespace mi_fa2 {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));   // at any float
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));      // at any float
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));   // at any 16-bit element
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr int kQ8Pad = 128;
 constexpr float kQ8Least = 0x1p-100f;   // a row's largest magnitude counts as at least this
@@ -31,10 +33,34 @@ __host__ __device__ constexpr int q8_panels(int out, bool gated) {
   return gated ? (out / 2 + 7) / 8 : (out + 15) / 16;
 }
 
+// Elements 8c .. 8c + 7 of a row of n 16-bit values at any element, two to a word, zeros past its end.  In steps, so
+// that nothing stands between the loads: q8_load8 (chunks past the end read the last whole one), q8_cut8, and,
+// where n is no multiple of 8, q8_tail8.
+__device__ __forceinline__ u32x4 q8_load8(const uint16_t* row, int c, int n) {
+  return n >= 8 ? *reinterpret_cast<const u32x4_2*>(row + 8 * min(c, (n >> 3) - 1)) : u32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ u32x4 q8_cut8(u32x4 a, int c, int n) {
+  return c < n >> 3 ? a : u32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ u32x4 q8_tail8(u32x4 a, const uint16_t* row, int c, int n) {
+  if (c == n >> 3)
+    for (int e = 0; e < (n & 7); ++e) a[e >> 1] |= (uint32_t)row[8 * c + e] << (16 * (e & 1));
+  return a;
+}
+// The same stored, elements past n left alone.
+__device__ __forceinline__ void q8_store8(uint16_t* row, int c, int n, u32x4 v) {
+  if (8 * c + 8 <= n) {
+    *reinterpret_cast<u32x4_2*>(row + 8 * c) = v;
+  } else {
+    for (int e = 0; e < 7; ++e)
+      if (8 * c + e < n) row[8 * c + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
 // A row's way to 8 bits: its largest magnitude as the bits of |v|, whose order as whole numbers is that of
 // the magnitudes, with infinity and NaN above all.
 struct Q8Factor {
-  float most, f;   // 127 / most; a row with an infinity or a NaN: 0
+  float most, f, rest;   // 127 / most is f + rest; a row with an infinity or a NaN: 0
   bool bad;
 };
 __device__ __forceinline__ Q8Factor q8_factor(uint32_t top) {
@@ -42,6 +68,7 @@ __device__ __forceinline__ Q8Factor q8_factor(uint32_t top) {
   r.bad = top >= 0x7f800000u;
   r.most = fmaxf(__uint_as_float(top), kQ8Least);
   r.f = r.bad ? 0.f : 127.f / r.most;
+  r.rest = r.bad ? 0.f : __builtin_fmaf(-r.f, r.most, 127.f) * (r.f * (1.f / 127.f));
   return r;
 }
 // inv: what every value is multiplied by beside.
@@ -49,14 +76,51 @@ __device__ __forceinline__ float q8_scale(const Q8Factor& r, float inv) {
   return r.bad ? __builtin_nanf("") : r.most * inv / 127.f;
 }
 // Four values, lowest byte first.  v f is rounded to the nearest whole number, ties to even, by the
-// addition of 1.5 * 2^23, whose last place is 1: its low byte is the number's (two's complement).
-__device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, const Q8Factor& r) {
+// addition of 1.5 * 2^23, whose last place is 1: its low byte is the number's (two's complement).  EXACT: for rows
+// as they are, whose values are short numbers and can lie halfway between two whole ones (one row in 128 has a
+// largest magnitude that is a multiple of 127); f alone, rounded, would send them to either side.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t q8_whole(float v, const Q8Factor& r) {
+#pragma clang fp contract(off)
   constexpr float kMagic = 12582912.f;
-  const uint32_t i = __float_as_uint(__builtin_fmaf(a, r.f, kMagic)), j = __float_as_uint(__builtin_fmaf(b, r.f, kMagic));
-  const uint32_t k = __float_as_uint(__builtin_fmaf(c, r.f, kMagic)), l = __float_as_uint(__builtin_fmaf(d, r.f, kMagic));
+  if constexpr (EXACT) {
+    const float y = __builtin_fmaf(v, r.f, v * r.rest);
+    return __float_as_uint(y + kMagic);
+  } else {
+    return __float_as_uint(__builtin_fmaf(v, r.f, kMagic));
+  }
+}
+template <bool EXACT>
+__device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d, const Q8Factor& r) {
   // v_perm_b32 selects bytes of {second word, first word}: bytes 0 of both, then the halves
-  const uint32_t lo = perm_b32(j, i, 0x0c0c0400u), hi = perm_b32(l, k, 0x0c0c0400u);
+  const uint32_t lo = perm_b32(q8_whole<EXACT>(b, r), q8_whole<EXACT>(a, r), 0x0c0c0400u);
+  const uint32_t hi = perm_b32(q8_whole<EXACT>(d, r), q8_whole<EXACT>(c, r), 0x0c0c0400u);
   return r.bad ? 0u : lo | hi << 16;
+}
+
+// A wave's sum and maximum, by DPP: each row of 16 lanes by shifts, then the rows' last lanes along.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t q8_dpp(uint32_t v) {   // 0 where no lane is read
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  const auto add = [&](uint32_t o) { v += __uint_as_float(o); };
+  add(q8_dpp<0x111, 0xf>(__float_as_uint(v)));   // row_shr:1, 2, 4, 8
+  add(q8_dpp<0x112, 0xf>(__float_as_uint(v)));
+  add(q8_dpp<0x114, 0xf>(__float_as_uint(v)));
+  add(q8_dpp<0x118, 0xf>(__float_as_uint(v)));
+  add(q8_dpp<0x142, 0xa>(__float_as_uint(v)));   // row_bcast:15 to rows 1, 3; row_bcast:31 to rows 2, 3
+  add(q8_dpp<0x143, 0xc>(__float_as_uint(v)));
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, q8_dpp<0x111, 0xf>(v));
+  v = max(v, q8_dpp<0x112, 0xf>(v));
+  v = max(v, q8_dpp<0x114, 0xf>(v));
+  v = max(v, q8_dpp<0x118, 0xf>(v));
+  v = max(v, q8_dpp<0x142, 0xa>(v));
+  v = max(v, q8_dpp<0x143, 0xc>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // A sum with its scales, and what is added to that: each rounded by itself, so that every kernel and every
@@ -90,7 +154,6 @@ struct Q8QuantParams {
   int8_t* q;              // panels of np
   float* scale;           // [M]
   int32_t M, n, np;
-  int32_t wide;           // every row and the norm's weight allow 16-byte accesses
   int32_t spread;         // work-groups are dealt so that a panel's rows share an XCD
 };
 enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2, kQ8Rows = 3 };
@@ -101,7 +164,7 @@ struct Q8DequantParams {
   const float* scale;
   uint16_t* out;
   int64_t out_st;
-  int32_t M, n, np, wide;
+  int32_t M, n, np;
 };
 hipError_t launch_q8_dequant(const Q8DequantParams& p, int dtype, hipStream_t stream);
 
@@ -129,7 +192,6 @@ struct Q8Params {
   int64_t out_st;
   int32_t M, N, K, Kp;    // N: out features (gated: of the activation)
   int32_t panels;
-  int32_t wide;           // out and residual allow accesses of 8 elements, bias of 4
 };
 hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
                           hipStream_t stream);

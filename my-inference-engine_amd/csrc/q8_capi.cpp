@@ -86,11 +86,6 @@ int check_rows(const char* name, const void* p, int64_t stride, int64_t width) {
   return kOk;
 }
 
-// Rows that lanes read and write 16 bytes at a time.
-bool wide(const void* p, int64_t stride, int32_t n) {
-  return !p || (aligned(p, 16) && stride % 8 == 0 && n % 8 == 0);
-}
-
 bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
   return x < y + b_bytes && y < x + a_bytes;
@@ -138,8 +133,6 @@ int quantize(int dtype, const void* x, int64_t x_stride, const void* y, int64_t 
   p.M = rows;
   p.n = n;
   p.np = q8_pad(n);
-  p.wide = wide(x, x_stride, n) && wide(y, y_stride, n) && wide(norm_weight, 8, n) &&
-           (!y || wide(r, r_stride, n));
   return launched(mi_fa2::launch_q8_quant(p, dtype, norm_weight ? mi_fa2::kQ8Norm : mi_fa2::kQ8Plain,
                                           reinterpret_cast<hipStream_t>(stream)));
 }
@@ -161,8 +154,6 @@ Q8Params operands(const void* w, const float* w_scale, const void* bias, const v
   p.K = in_features;
   p.Kp = q8_pad(in_features);
   p.panels = mi_fa2::q8_panels(gated ? 2 * out_features : out_features, gated);
-  p.wide = out_features % 8 == 0 && wide(res, res_stride, 8) && wide(out, out_stride, 8) &&
-           (!bias || aligned(bias, 8));
   return p;
 }
 
@@ -185,13 +176,9 @@ int product(Q8Params p, int dtype, bool gated, const void* values, const float* 
 
 // The product of 16-bit rows, brought to 8 bits in the same launch where the few-row kernel does that,
 // else before it in the workspace.
-bool fused(const void* x, int64_t x_stride, const void* norm_weight, int32_t rows, int32_t in) {
-  return rows <= mi_fa2::kQ8FusedMax && q8_pad(in) <= mi_fa2::kQ8KeepK && x_stride < 1 << 23 &&
-         wide(x, x_stride, in) && wide(norm_weight, 8, in);
-}
 int product_of(Q8Params p, int dtype, bool gated, const void* x, int64_t x_stride,
                const void* norm_weight, float eps, const RowsSpace& r, char* ws, void* stream) {
-  if (fused(x, x_stride, norm_weight, p.M, p.K)) {
+  if (p.M <= mi_fa2::kQ8FusedMax && p.Kp <= mi_fa2::kQ8KeepK) {
     p.x = x;
     p.x_st = x_stride;
     p.norm_w = static_cast<const uint16_t*>(norm_weight);
@@ -279,7 +266,7 @@ int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void
   if (int rc = check_ptr("scale", scale, 4)) return rc;
   if (int rc = check_rows("out", out, out_stride, n)) return rc;
   mi_fa2::Q8DequantParams p{static_cast<const int8_t*>(values), scale, static_cast<uint16_t*>(out),
-                            out_stride, rows, n, q8_pad(n), wide(out, out_stride, n)};
+                            out_stride, rows, n, q8_pad(n)};
   return launched(
       mi_fa2::launch_q8_dequant(p, dtype, reinterpret_cast<hipStream_t>(stream)));
 }
@@ -407,6 +394,16 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
                                    sp.act_stride, rows, inter, hidden, true),
                           dtype, true, x, x_stride, norm_weight, eps, sp.x, ws, stream))
     return rc;
+  Q8Params d = operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride, rows, hidden,
+                        inter, false);
+  if (rows <= mi_fa2::kQ8FloatMax && q8_pad(inter) <= mi_fa2::kQ8FloatK) {
+    d.x = ws + sp.act;
+    d.x_st = sp.act_stride;
+    int cus = 0;
+    if (int rc = compute_units(&cus)) return rc;
+    return launched(mi_fa2::launch_q8_rows(d, dtype, false, mi_fa2::kQ8Float, cus,
+                                           reinterpret_cast<hipStream_t>(stream)));
+  }
   Q8QuantParams q{};
   q.x = ws + sp.act;
   q.x_st = sp.act_stride;
@@ -418,9 +415,7 @@ int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_w
   if (int rc = launched(mi_fa2::launch_q8_quant(q, dtype, mi_fa2::kQ8Float,
                                                 reinterpret_cast<hipStream_t>(stream))))
     return rc;
-  return product(operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride,
-                          rows, hidden, inter, false),
-                 dtype, false, ws + sp.a.values, a_scale, stream);
+  return product(d, dtype, false, ws + sp.a.values, a_scale, stream);
 }
 
 }  // extern "C"

@@ -40,9 +40,6 @@ __device__ __forceinline__ void wait_loads_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <typename E>
-__device__ __forceinline__ uint16_t round16(float x) { return (uint16_t)(E::pack2(x, 0.f) & 0xffffu); }
-
 }  // namespace
 
 template <typename E, int NP, int TM, int WN, int ST, bool GATED>
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
         *reinterpret_cast<f32x4*>(out + t * p.out_st + 4 * c) =
             *reinterpret_cast<const f32x4*>(lds + t * kRow + c * 16);
     }
-  } else if (p.wide) {
+  } else {
     constexpr int kPieces = NP * 2;   // of 16 bytes a row
     uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m0 * p.out_st + panel0 * 16;
     const int c = tid % kPieces, n_left = p.N - panel0 * 16;
@@ -198,8 +195,11 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
 #pragma unroll
       for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
         const int t = (tid + e * kQgThreads) / kPieces;
-        if (m0 + t < p.M && 8 * c < n_left)
-          *reinterpret_cast<u32x4*>(lds + t * kRow + c * 16) = ld16(res + t * p.res_st + 8 * c);
+        if (m0 + t < p.M && 8 * c < n_left) {
+          u32x4 v = q8_cut8(q8_load8(res + t * p.res_st, c, n_left), c, n_left);
+          if (n_left & 7) v = q8_tail8(v, res + t * p.res_st, c, n_left);
+          *reinterpret_cast<u32x4*>(lds + t * kRow + c * 16) = v;
+        }
       }
       __syncthreads();
     }
@@ -210,7 +210,13 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
         const int n = w_first + 32 * i + 8 * q;
         const f32x4 ws = *reinterpret_cast<const f32x4*>(w_scale + n);
         u32x2 bias = {0, 0};
-        if (p.bias) bias = *reinterpret_cast<const u32x2*>(p.bias + min(panel0 * 16 + n, p.N - 4));
+        if (p.bias) {
+          if (n + 4 <= n_left)
+            bias = *reinterpret_cast<const u32x2_2*>(p.bias + panel0 * 16 + n);
+          else
+            for (int r = 0; r < n_left - n; ++r)
+              bias[r >> 1] |= (uint32_t)p.bias[panel0 * 16 + n + r] << (16 * (r & 1));
+        }
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
           const int t = wm * TJ * 32 + j * 32 + r32;
@@ -228,29 +234,12 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
 #pragma unroll
     for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
       const int t = (tid + e * kQgThreads) / kPieces;
-      if (m0 + t < p.M && 8 * c < n_left)
-        __builtin_nontemporal_store(*reinterpret_cast<const u32x4*>(lds + t * kRow + c * 16),
-                                    reinterpret_cast<u32x4*>(out + t * p.out_st + 8 * c));
-    }
-  } else {
-    // rows that 16-byte accesses do not fit: element by element
-    uint16_t* out = static_cast<uint16_t*>(p.out);
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int m = m0 + wm * TJ * 32 + j * 32 + r32;
-      if (m >= p.M) continue;
-      const float xs = x_scale[m - m0];
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int w = w_first + 32 * i + 8 * (e / 4) + e % 4, n = panel0 * 16 + w;
-          if (n >= p.N) continue;
-          float v = q8_scaled(acc[i][j][e], xs, w_scale[w]);
-          if (p.bias) v = q8_plus(v, E::lo(p.bias[n]));
-          if (p.res) v = q8_plus(v, E::lo(p.res[(int64_t)m * p.res_st + n]));
-          out[(int64_t)m * p.out_st + n] = round16<E>(v);
-        }
+      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + t * kRow + c * 16);
+      if (m0 + t >= p.M) break;
+      if (8 * c + 8 <= n_left)
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_2*>(out + t * p.out_st + 8 * c));
+      else
+        q8_store8(out + t * p.out_st, c, n_left, v);
     }
   }
 }

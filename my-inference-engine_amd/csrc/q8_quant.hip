@@ -17,23 +17,11 @@ namespace mi_fa2 {
 namespace {
 
 template <typename E>
-__device__ __forceinline__ float q8_f(uint16_t x) { return E::lo(x); }
-template <typename E>
-__device__ __forceinline__ uint16_t q8_r(float x) { return (uint16_t)(E::pack2(x, 0.f) & 0xffffu); }
-
-// Elements 8c .. 8c + 7 of a row of n 16-bit values, zeros past its end.
-template <typename E, bool WIDE>
-__device__ __forceinline__ void load8(const uint16_t* row, int c, int n, float (&v)[8]) {
-  if (WIDE) {   // n is a multiple of 8
-    const u32x4 a = 8 * c < n ? ld16(row + 8 * c) : u32x4{0, 0, 0, 0};
+__device__ __forceinline__ void unpack8(u32x4 a, float (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = E::lo(a[e]);
-      v[2 * e + 1] = E::hi(a[e]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < n ? q8_f<E>(row[8 * c + e]) : 0.f;
+  for (int e = 0; e < 4; ++e) {
+    v[2 * e] = E::lo(a[e]);
+    v[2 * e + 1] = E::hi(a[e]);
   }
 }
 
@@ -41,7 +29,7 @@ __device__ __forceinline__ void load8(const uint16_t* row, int c, int n, float (
 
 // T threads take a row, PER chunks of 8 elements each in registers; PER = 0: any length, the row is
 // read twice.
-template <typename E, int SRC, bool WIDE, int T, int PER>
+template <typename E, int SRC, int T, int PER>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8QuantParams p) {
   constexpr int kRows = T < 256 ? 256 / T : 1;
   // Work-group b runs on XCD b % 8.  Where there are many, all of a panel's rows go to one, whose L2
@@ -56,51 +44,66 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
   const int row = at * kRows + threadIdx.x / T;
   if (row >= p.M) return;   // (T = 64: whole waves, and no barrier below)
   const int chunks = p.np / 8;
-  const uint16_t* x = static_cast<const uint16_t*>(p.x) + (int64_t)row * p.x_st;
-  const float* xf = static_cast<const float*>(p.x) + (int64_t)row * p.x_st;
-  const uint16_t* y = SRC == kQ8Norm && p.y ? p.y + (int64_t)row * p.y_st : nullptr;
-  uint16_t* r_out = SRC == kQ8Norm && p.y ? p.r_out + (int64_t)row * p.r_st : nullptr;
+  // A row is a wave's or a work-group's: its address is uniform.
+  const int64_t urow = __builtin_amdgcn_readfirstlane(row);
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + urow * p.x_st;
+  const __amdgpu_buffer_rsrc_t xf = make_rsrc(static_cast<const float*>(p.x) + urow * p.x_st, SRC == kQ8Float ? p.n * 4 : 0);
+  const bool add = SRC == kQ8Norm && p.y;
+  const uint16_t* y = add ? p.y + urow * p.y_st : nullptr;
+  uint16_t* r = add ? p.r_out + urow * p.r_st : nullptr;
 
   float ss = 0.f;
   uint32_t top = 0;
-  // chunk c of what is held in 8 bits (the norm's factor apart); `first`: counted, and r written
-  const auto load = [&](int c, float (&v)[8], bool first) {
+  // A chunk as it is loaded, and what of it is held in 8 bits (the norm's factor apart); `first`: counted, and
+  // r written.
+  struct Chunk {
+    u32x4 x[SRC == kQ8Float ? 2 : 1], y, w;
+  };
+  const auto load = [&](int c, bool first) {
+    Chunk k{};
+    if constexpr (SRC == kQ8Float) {   // (zeros past the row's end)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) k.x[h] = ld16_buf(xf, 32 * c + 16 * h);
+    } else {
+      k.x[0] = q8_load8(add && !first ? r : x, c, p.n);   // (the second time r is this thread's own stores)
+      if (add && first) k.y = q8_load8(y, c, p.n);
+      if constexpr (SRC == kQ8Norm) k.w = q8_load8(p.norm_w, c, p.n);
+    }
+    return k;
+  };
+  const auto cut = [&](int c, Chunk& k) {
+    if constexpr (SRC != kQ8Float) {
+      k.x[0] = q8_cut8(k.x[0], c, p.n);
+      k.y = q8_cut8(k.y, c, p.n);
+      k.w = q8_cut8(k.w, c, p.n);
+    }
+  };
+  const auto tail = [&](int c, Chunk& k, bool first) {
+    if constexpr (SRC != kQ8Float) {
+      k.x[0] = q8_tail8(k.x[0], add && !first ? r : x, c, p.n);
+      if (add && first) k.y = q8_tail8(k.y, y, c, p.n);
+      if (SRC == kQ8Norm) k.w = q8_tail8(k.w, p.norm_w, c, p.n);
+    }
+  };
+  const bool odd = SRC != kQ8Float && (p.n & 7);
+  const auto take = [&](int c, const Chunk& k, float (&v)[8], bool first) {
     if constexpr (SRC == kQ8Float) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // the rows are padded to whole chunks
-        const f32x4 a = 8 * c < p.n ? *reinterpret_cast<const f32x4*>(xf + 8 * c + 4 * h)
-                                    : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * h + e] = 8 * c + 4 * h + e < p.n ? a[e] : 0.f;
-      }
+      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(k.x[e / 4][e % 4]);
     } else {
-      load8<E, WIDE>(x, c, p.n, v);
+      unpack8<E>(k.x[0], v);
       if constexpr (SRC == kQ8Norm) {
-        if (y) {
-          if (first) {
-            float b[8];
-            load8<E, WIDE>(y, c, p.n, b);
-            u32x4 o;
+        if (add && first) {
+          float b[8];
+          unpack8<E>(k.y, b);
+          u32x4 o;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[e] = E::pack2(v[2 * e] + b[2 * e], v[2 * e + 1] + b[2 * e + 1]);
-              v[2 * e] = E::lo(o[e]);
-              v[2 * e + 1] = E::hi(o[e]);
-            }
-            if (WIDE) {
-              if (8 * c < p.n) *reinterpret_cast<u32x4*>(r_out + 8 * c) = o;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (8 * c + e < p.n) r_out[8 * c + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
-            }
-          } else {
-            load8<E, WIDE>(r_out, c, p.n, v);   // (this thread's own stores)
-          }
+          for (int e = 0; e < 4; ++e) o[e] = E::pack2(v[2 * e] + b[2 * e], v[2 * e + 1] + b[2 * e + 1]);
+          unpack8<E>(o, v);
+          q8_store8(r, c, p.n, o);
         }
         float w[8];
-        load8<E, WIDE>(p.norm_w, c, p.n, w);
+        unpack8<E>(k.w, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (first) ss = __builtin_fmaf(v[e], v[e], ss);
@@ -115,17 +118,26 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
 
   float kept[PER ? PER : 1][8];
   if constexpr (PER > 0) {
+    Chunk k[PER];
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-      if (tid + k * T < chunks) load(tid + k * T, kept[k], true);
+    for (int i = 0; i < PER; ++i) k[i] = load(tid + i * T, true);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) cut(tid + i * T, k[i]);
+    if (odd)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) tail(tid + i * T, k[i], true);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) take(tid + i * T, k[i], kept[i], true);
   } else {
-    for (int c = tid; c < chunks; c += T) load(c, kept[0], true);
+    for (int c = tid; c < chunks; c += T) {
+      Chunk k = load(c, true);
+      cut(c, k);
+      if (odd) tail(c, k, true);
+      take(c, k, kept[0], true);
+    }
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    if (SRC == kQ8Norm) ss += __shfl_xor(ss, d);
-    top = max(top, (uint32_t)__shfl_xor((int)top, d));
-  }
+  if (SRC == kQ8Norm) ss = wave_sum(ss);
+  top = wave_max(top);
   if constexpr (T > 64) {
     __shared__ float part_s[T / 64];
     __shared__ uint32_t part_t[T / 64];
@@ -144,7 +156,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
   if (tid == 0)
     p.scale[row] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.n + p.eps) : 1.f);
   const auto store = [&](int c, const float (&v)[8]) {
-    const u32x2 o = {q8_pack4(v[0], v[1], v[2], v[3], f), q8_pack4(v[4], v[5], v[6], v[7], f)};
+    const u32x2 o = {q8_pack4<SRC == kQ8Plain>(v[0], v[1], v[2], v[3], f), q8_pack4<SRC == kQ8Plain>(v[4], v[5], v[6], v[7], f)};
     *reinterpret_cast<u32x2*>(p.q + q8_at(row, c, p.np)) = o;
   };
   if constexpr (PER > 0) {
@@ -153,7 +165,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
       if (tid + k * T < chunks) store(tid + k * T, kept[k]);
   } else {
     for (int c = tid; c < chunks; c += T) {
-      load(c, kept[0], false);
+      Chunk k = load(c, false);
+      cut(c, k);
+      if (odd) tail(c, k, false);
+      take(c, k, kept[0], false);
       store(c, kept[0]);
     }
   }
@@ -161,55 +176,54 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
 
 namespace {
 
-template <typename E, int SRC, bool WIDE>
+template <typename E, int SRC, int T, int PER, int LAST>
+void launch_quant_per(const Q8QuantParams& p, dim3 grid, hipStream_t stream) {
+  if constexpr (PER < LAST)
+    if (p.np > T * 8 * PER) return launch_quant_per<E, SRC, T, PER + 1, LAST>(p, grid, stream);
+  hipLaunchKernelGGL((q8_quant_kernel<E, SRC, T, PER>), grid, dim3(T < 256 ? 256 : T), 0, stream, p);
+}
+
+template <typename E, int SRC>
 hipError_t launch_quant_t(Q8QuantParams p, hipStream_t stream) {
   p.spread = p.M > 128;
   // (in whole rounds of the 8 XCDs' panels)
   const int rows = p.spread ? (p.M + 127) / 128 * 128 : p.M;
-  if (p.np <= 64 * 4 * 8)
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 64, 4>), dim3((rows + 3) / 4), dim3(256), 0, stream, p);
-  else if (p.np <= 256 * 8 * 8)
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 256, 8>), dim3(rows), dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((q8_quant_kernel<E, SRC, WIDE, 1024, 0>), dim3(rows), dim3(1024), 0, stream, p);
+  if (p.np <= 64 * 4 * 8) launch_quant_per<E, SRC, 64, 1, 4>(p, dim3((rows + 3) / 4), stream);
+  else if (p.np <= 256 * 8 * 8) launch_quant_per<E, SRC, 256, 2, 8>(p, dim3(rows), stream);
+  else launch_quant_per<E, SRC, 1024, 0, 0>(p, dim3(rows), stream);
   return hipGetLastError();
-}
-
-template <typename E>
-hipError_t launch_quant_e(const Q8QuantParams& p, int source, hipStream_t stream) {
-  if (source == kQ8Norm)
-    return p.wide ? launch_quant_t<E, kQ8Norm, true>(p, stream) : launch_quant_t<E, kQ8Norm, false>(p, stream);
-  return p.wide ? launch_quant_t<E, kQ8Plain, true>(p, stream) : launch_quant_t<E, kQ8Plain, false>(p, stream);
 }
 
 }  // namespace
 
 hipError_t launch_q8_quant(const Q8QuantParams& p, int dtype, int source, hipStream_t stream) {
-  if (source == kQ8Float) return launch_quant_t<BF16, kQ8Float, true>(p, stream);
-  return dtype == 0 ? launch_quant_e<BF16>(p, source, stream) : launch_quant_e<FP16>(p, source, stream);
+  if (source == kQ8Float) return launch_quant_t<BF16, kQ8Float>(p, stream);
+  if (source == kQ8Norm)
+    return dtype == 0 ? launch_quant_t<BF16, kQ8Norm>(p, stream) : launch_quant_t<FP16, kQ8Norm>(p, stream);
+  return dtype == 0 ? launch_quant_t<BF16, kQ8Plain>(p, stream) : launch_quant_t<FP16, kQ8Plain>(p, stream);
 }
 
-// A thread takes 8 values.
+// A thread takes 16 values of one row, a wave 16 rows' 64: it reads 1 KB in one run and writes each row's
+// 128 bytes.
 template <typename E>
 __global__ __launch_bounds__(256) void q8_dequant_kernel(const Q8DequantParams p) {
-  const int per_row = (p.n + 7) / 8;
-  const int64_t total = (int64_t)p.M * per_row;
+  const int per_panel = p.np;   // 16-byte pieces
+  const int64_t total = (int64_t)((p.M + 15) / 16) * per_panel;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int row = (int)(i / per_row), c = (int)(i - (int64_t)row * per_row);
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p.q + q8_at(row, c, p.np));
+    const int64_t panel = i / per_panel;
+    const int at = (int)(i - panel * per_panel);
+    const int64_t row = panel * 16 + (at & 15);
+    if (row >= p.M) continue;
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p.q + 16 * i);
     const float s = p.scale[row];
-    float v[8];
+    float v[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(a[e / 4] >> (8 * (e & 3))) * s;
-    uint16_t* out = p.out + (int64_t)row * p.out_st + 8 * c;
-    if (p.wide) {
-      *reinterpret_cast<u32x4*>(out) = u32x4{E::pack2(v[0], v[1]), E::pack2(v[2], v[3]),
-                                             E::pack2(v[4], v[5]), E::pack2(v[6], v[7])};
-    } else {
+    for (int e = 0; e < 16; ++e) v[e] = (float)(int8_t)(a[e / 4] >> (8 * (e & 3))) * s;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (8 * c + e < p.n) out[e] = q8_r<E>(v[e]);
-    }
+    for (int h = 0; h < 2; ++h)
+      q8_store8(p.out + row * p.out_st, (at >> 4) * 2 + h, p.n,
+                u32x4{E::pack2(v[8 * h], v[8 * h + 1]), E::pack2(v[8 * h + 2], v[8 * h + 3]),
+                      E::pack2(v[8 * h + 4], v[8 * h + 5]), E::pack2(v[8 * h + 6], v[8 * h + 7])});
   }
 }
 
@@ -219,8 +233,7 @@ uint32_t grid_of(int64_t pieces) { return (uint32_t)std::min<int64_t>((pieces + 
 }  // namespace
 
 hipError_t launch_q8_dequant(const Q8DequantParams& p, int dtype, hipStream_t stream) {
-  const int64_t n = (int64_t)p.M * ((p.n + 7) / 8);
-  const dim3 grid(grid_of(n));
+  const dim3 grid(grid_of((int64_t)((p.M + 15) / 16) * p.np));
   if (dtype == 0)
     hipLaunchKernelGGL((q8_dequant_kernel<BF16>), grid, dim3(256), 0, stream, p);
   else

@@ -18,6 +18,7 @@
 #include "q8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mi_fa2 {
 
@@ -26,14 +27,13 @@ namespace {
 constexpr int kQrWaves = 8, kQrThreads = 64 * kQrWaves;
 constexpr int kQrNone = 0x7ffffff0;   // a byte offset past every resource: reads zeros
 
-// The sums s of rows 4g .. 4g + 3 of a panel with token m, whose scale is xs, on their way out.  All lanes of
-// the wave call it.
+// The sums s of four rows of W with token m, whose scale is xs, on their way out: features f .. f + 3
+// (GATED: the gate's in lane groups g = 0, 1, the up rows' in 2, 3).  All lanes of the wave call it.
 template <typename E, bool GATED>
-__device__ __forceinline__ void finish(const Q8Params& p, int panel, int m, int g, float xs, i32x4 s) {
-  const bool live = m < p.M;
+__device__ __forceinline__ void finish(const Q8Params& p, int f, int m, int g, bool live, float xs, i32x4 s) {
+  live = live && m < p.M;
   float v[4];
   if constexpr (GATED) {
-    const int f = 8 * panel + 4 * (g & 1);
     float up[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -48,22 +48,19 @@ __device__ __forceinline__ void finish(const Q8Params& p, int panel, int m, int 
     *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
         f32x4{v[0], v[1], v[2], v[3]};
   } else {
-    const int f = 16 * panel + 4 * g;
     if (!live || f >= p.N) return;
     const uint16_t* res = p.res ? p.res + (int64_t)m * p.res_st + f : nullptr;
     uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
-    if (p.wide) {
+    if (f + 4 <= p.N) {
       const f32x4 ws = *reinterpret_cast<const f32x4_4*>(p.w_scale + f);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = q8_scaled(s[r], xs, ws[r]);
-      if (p.bias) add4<E>(v, *reinterpret_cast<const u32x2*>(p.bias + f));
-      if (res) add4<E>(v, *reinterpret_cast<const u32x2*>(res));
-      *reinterpret_cast<u32x2*>(out) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+      if (p.bias) add4<E>(v, *reinterpret_cast<const u32x2_2*>(p.bias + f));
+      if (res) add4<E>(v, *reinterpret_cast<const u32x2_2*>(res));
+      *reinterpret_cast<u32x2_2*>(out) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
       return;
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (f + r >= p.N) break;
+    for (int r = 0; r < p.N - f; ++r) {
       float o = q8_scaled(s[r], xs, p.w_scale[f + r]);
       if (p.bias) o = q8_plus(o, E::lo(p.bias[f + r]));
       if (res) o = q8_plus(o, E::lo(res[r]));
@@ -74,13 +71,15 @@ __device__ __forceinline__ void finish(const Q8Params& p, int panel, int m, int 
 
 }  // namespace
 
-// SRC: kQ8Plain, kQ8Norm: x is 16-bit rows; kQ8Rows: rows in 8 bits.  NS: steps of K (64) a wave takes at a
-// time.
-template <typename E, int MT, int NP, int NS, bool GATED, int SRC, bool KEEP>
+// SRC: kQ8Plain, kQ8Norm: x is 16-bit rows; kQ8Float: fp32 rows, 4 at most; kQ8Rows: rows in 8 bits.  NS:
+// steps of K (64) a wave takes at a time.  HALF: a tile is half a panel, whose rows fill the operand twice.
+// FT: of fp32 rows, their most.
+template <typename E, int MT, int NP, int NS, bool GATED, int SRC, bool KEEP, bool HALF, int FT = 0>
 __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p) {
-  static_assert(SRC == kQ8Rows || (KEEP && MT == 1), "rows come to 8 bits once, 16 of them");
+  static_assert(SRC == kQ8Rows || MT == 1, "rows come to 8 bits 16 at a time");
+  static_assert(KEEP || SRC == kQ8Rows || SRC == kQ8Float, "");
+  static_assert(!HALF || (NP == 1 && !GATED), "");
   constexpr int U = NP * MT;
-  constexpr int kPiece = 256 + 16;   // 16 rows' 16 bytes in LDS; the gap keeps a row's pieces off one bank
   __shared__ i32x4 red[2][kQrWaves][U][64];
   __shared__ float row_scale[16 * MT];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -90,94 +89,167 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
   const int steps = p.Kp >> 6;
   const int lo = wave * steps / kQrWaves, hi = (wave + 1) * steps / kQrWaves;
   const int chunks = KEEP ? 1 : max(1, (hi - lo + NS - 1) / NS);
-  const int tiles = (p.panels + NP - 1) / NP;
+  const int tiles = HALF ? 2 * p.panels : (p.panels + NP - 1) / NP;
 
   // Step i of chunk c of tile t, panel u.
   const auto load_w = [&](int t, int c, int u, int i) -> i32x4 {
-    const int panel = t * NP + u, s = lo + c * NS + i;
+    const int panel = HALF ? t >> 1 : t * NP + u, s = lo + c * NS + i;
     const bool live = panel < p.panels;
     const __amdgpu_buffer_rsrc_t r =
         make_rsrc(p.w + (int64_t)(live ? panel : 0) * 16 * p.Kp, live ? 16 * p.Kp : 0);
-    return __builtin_bit_cast(i32x4, ld16_buf(r, s < hi ? s * 1024 + lane * 16 : kQrNone));
+    const int at = HALF ? g * 256 + (8 * (t & 1) + (n & 7)) * 16 : lane * 16;
+    return __builtin_bit_cast(i32x4, ld16_buf(r, s < hi ? s * 1024 + at : kQrNone));
   };
-  // x: 16 tokens a panel
+  // Rows in 8 bits: 16 tokens a panel.
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x, SRC == kQ8Rows ? (p.M + 15) / 16 * 16 * p.Kp : 0);
+  // Rows brought to 8 bits here, in LDS: a token's 16 bytes beside those of the others.  The gap keeps a
+  // row's pieces off one bank.
+  constexpr int kTokens = SRC == kQ8Float ? FT : 16, kPiece = kTokens * 16 + 16;
+  constexpr int kMostK = SRC == kQ8Float ? kQ8FloatK : NS * 64 * kQrWaves;
+  __shared__ __attribute__((aligned(16))) char pieces[SRC == kQ8Rows ? 16 : kMostK / 16 * kPiece];
   const auto load_x = [&](int c, int j, int i) -> i32x4 {
     const int s = lo + c * NS + i;
-    return __builtin_bit_cast(i32x4, ld16_buf(xr, s < hi ? j * 16 * p.Kp + s * 1024 + lane * 16 : kQrNone));
+    if constexpr (SRC == kQ8Rows)
+      return __builtin_bit_cast(i32x4, ld16_buf(xr, s < hi ? j * 16 * p.Kp + s * 1024 + lane * 16 : kQrNone));
+    else   // (steps past the share meet weights that are zeros, tokens past the last their own column)
+      return *reinterpret_cast<const i32x4*>(pieces + (min(s, steps - 1) * 4 + g) * kPiece + n % kTokens * 16);
   };
 
   i32x4 x[NS][MT], w[NP][NS];
-  constexpr int kChunks = kQ8KeepK / 8 / 64;   // of 8 elements, a lane's share of a row
-  u32x4 raw[SRC == kQ8Rows ? 1 : 2][kChunks], nw[kChunks];
+  const auto first_w = [&] {
+#pragma unroll
+    for (int u = 0; u < NP; ++u)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) w[u][i] = load_w(blockIdx.x, 0, u, i);
+  };
   if constexpr (SRC == kQ8Rows) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j) x[i][j] = load_x(0, j, i);
-  } else {
-    // rows `wave` and `wave` + 8
-    const __amdgpu_buffer_rsrc_t rr = make_rsrc(p.x, (int)(((int64_t)(p.M - 1) * p.x_st + p.K) * 2));
-    const __amdgpu_buffer_rsrc_t nr = make_rsrc(p.norm_w, SRC == kQ8Norm ? p.K * 2 : 0);
+    first_w();
+    if (tid < 16 * MT) row_scale[tid] = tid < p.M ? p.x_scale[tid] : 0.f;
+  } else if constexpr (SRC == kQ8Float) {
+    // All waves share each row.
+    constexpr int kPer = kQ8FloatK / 8 / kQrThreads;   // chunks of 8 a thread
+    __shared__ uint32_t part[kQrWaves][kTokens];
+    f32x4 v[kTokens][kPer][2];
 #pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      const int c = lane + 64 * k;
+    for (int m = 0; m < kTokens; ++m) {
+      const __amdgpu_buffer_rsrc_t rr = make_rsrc(static_cast<const float*>(p.x) + (int64_t)m * p.x_st,
+                                                  m < p.M ? p.K * 4 : 0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int m = wave + 8 * h;
-        raw[h][k] = ld16_buf(rr, m < p.M && 8 * c < p.K ? m * (int)p.x_st * 2 + c * 16 : kQrNone);
-      }
-      if constexpr (SRC == kQ8Norm) nw[k] = ld16_buf(nr, c * 16);
+      for (int k = 0; k < kPer; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[m][k][h] = __builtin_bit_cast(f32x4, ld16_buf(rr, (tid + k * kQrThreads) * 32 + h * 16));
     }
-  }
+    first_w();
+    uint32_t top[kTokens];
 #pragma unroll
-  for (int u = 0; u < NP; ++u)
+    for (int m = 0; m < kTokens; ++m) {
+      top[m] = 0;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) w[u][i] = load_w(blockIdx.x, 0, u, i);
-
-  if constexpr (SRC != kQ8Rows) {
-    __shared__ __attribute__((aligned(16))) char pieces[kQ8KeepK / 16 * kPiece];
+      for (int k = 0; k < kPer; ++k)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int m = wave + 8 * h;
-      if (m >= p.M) break;
-      float v[kChunks][8], ss = 0.f;
-      uint32_t top = 0;
-#pragma unroll
-      for (int k = 0; k < kChunks; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float a = e & 1 ? E::hi(raw[h][k][e / 2]) : E::lo(raw[h][k][e / 2]);
-          if constexpr (SRC == kQ8Norm) {
-            ss = __builtin_fmaf(a, a, ss);
-            a *= e & 1 ? E::hi(nw[k][e / 2]) : E::lo(nw[k][e / 2]);
-          }
-          v[k][e] = a;
-          top = max(top, __float_as_uint(a) & 0x7fffffffu);
-        }
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) {
-        if (SRC == kQ8Norm) ss += __shfl_xor(ss, d);
-        top = max(top, (uint32_t)__shfl_xor((int)top, d));
-      }
-      const Q8Factor f = q8_factor(top);
-      if (lane == 0)
-        row_scale[m] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.K + p.eps) : 1.f);
-#pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-        const int c = lane + 64 * k;
-        if (8 * c < p.Kp)
-          *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
-              u32x2{q8_pack4(v[k][0], v[k][1], v[k][2], v[k][3], f),
-                    q8_pack4(v[k][4], v[k][5], v[k][6], v[k][7], f)};
-      }
+        for (int e = 0; e < 8; ++e) top[m] = max(top[m], __float_as_uint(v[m][k][e / 4][e % 4]) & 0x7fffffffu);
+      top[m] = wave_max(top[m]);
+      if (lane == 0) part[wave][m] = top[m];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
-      x[i][0] = *reinterpret_cast<const i32x4*>(pieces + (min(lo + i, steps - 1) * 4 + g) * kPiece + n * 16);
-  } else if (tid < 16 * MT) {
-    row_scale[tid] = tid < p.M ? p.x_scale[tid] : 0.f;
+    for (int m = 0; m < kTokens; ++m) {
+#pragma unroll
+      for (int u = 0; u < kQrWaves; ++u) top[m] = max(top[m], part[u][m]);
+      const Q8Factor f = q8_factor(top[m]);
+      if (tid == m) row_scale[m] = q8_scale(f, 1.f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int c = tid + k * kQrThreads;
+        if (8 * c < p.Kp)
+          *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
+              u32x2{q8_pack4<SRC == kQ8Plain>(v[m][k][0][0], v[m][k][0][1], v[m][k][0][2], v[m][k][0][3], f),
+                    q8_pack4<SRC == kQ8Plain>(v[m][k][1][0], v[m][k][1][1], v[m][k][1][2], v[m][k][1][3], f)};
+      }
+    }
+    __syncthreads();
+  } else {
+    // Each wave brings rows `wave` and `wave` + 8 there.
+    constexpr int kChunks = NS;   // of 8 elements, a lane's share of a row of NS * 512
+    u32x4 raw[2][kChunks], nw[kChunks];
+    const uint16_t* x16 = static_cast<const uint16_t*>(p.x);
+    // (with more than 8 rows, rows past the last: the last again, and not kept)
+    if (wave < p.M)
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) raw[0][k] = q8_load8(x16 + wave * p.x_st, lane + 64 * k, p.K);
+    if (p.M > 8)
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+        raw[1][k] = q8_load8(x16 + min(wave + 8, p.M - 1) * p.x_st, lane + 64 * k, p.K);
+    if constexpr (SRC == kQ8Norm)
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) nw[k] = q8_load8(p.norm_w, lane + 64 * k, p.K);
+    first_w();
+    const auto bring = [&](auto rows) {
+      constexpr int R = decltype(rows)::value;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+#pragma unroll
+        for (int h = 0; h < R; ++h) raw[h][k] = q8_cut8(raw[h][k], lane + 64 * k, p.K);
+        if constexpr (SRC == kQ8Norm) nw[k] = q8_cut8(nw[k], lane + 64 * k, p.K);
+      }
+      if (p.K & 7)
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+#pragma unroll
+          for (int h = 0; h < R; ++h)
+            raw[h][k] = q8_tail8(raw[h][k], x16 + min(wave + 8 * h, p.M - 1) * p.x_st, lane + 64 * k, p.K);
+          if constexpr (SRC == kQ8Norm) nw[k] = q8_tail8(nw[k], p.norm_w, lane + 64 * k, p.K);
+        }
+      float v[R][kChunks][8], ss[R];
+      uint32_t top[R];
+#pragma unroll
+      for (int h = 0; h < R; ++h) {
+        ss[h] = 0.f;
+        top[h] = 0;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a = e & 1 ? E::hi(raw[h][k][e / 2]) : E::lo(raw[h][k][e / 2]);
+            if constexpr (SRC == kQ8Norm) {
+              ss[h] = __builtin_fmaf(a, a, ss[h]);
+              a *= e & 1 ? E::hi(nw[k][e / 2]) : E::lo(nw[k][e / 2]);
+            }
+            v[h][k][e] = a;
+            top[h] = max(top[h], __float_as_uint(a) & 0x7fffffffu);
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < R; ++h) {
+        if (SRC == kQ8Norm) ss[h] = wave_sum(ss[h]);
+        top[h] = wave_max(top[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < R; ++h) {
+        const int m = wave + 8 * h;
+        const Q8Factor f = q8_factor(top[h]);
+        if (lane == 0) row_scale[m] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss[h] / (float)p.K + p.eps) : 1.f);
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          const int c = lane + 64 * k;
+          if (8 * c < p.Kp)
+            *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
+                u32x2{q8_pack4<SRC == kQ8Plain>(v[h][k][0], v[h][k][1], v[h][k][2], v[h][k][3], f),
+                      q8_pack4<SRC == kQ8Plain>(v[h][k][4], v[h][k][5], v[h][k][6], v[h][k][7], f)};
+        }
+      }
+    };
+    if (p.M > 8) bring(std::integral_constant<int, 2>{});
+    else if (wave < p.M) bring(std::integral_constant<int, 1>{});
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NS; ++i) x[i][0] = load_x(0, 0, i);
   }
 
   int it = 0;
@@ -192,6 +264,7 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
       const int nt = more ? t : t + gridDim.x, nc = more ? c + 1 : 0;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
+        if constexpr (SRC == kQ8Float) x[i][0] = load_x(c, 0, i);
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
 #pragma unroll
@@ -199,7 +272,7 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
             acc[u][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][i], x[i][j], acc[u][j], 0, 0, 0);
           w[u][i] = load_w(nt, nc, u, i);
         }
-        if constexpr (!KEEP)
+        if constexpr (SRC == kQ8Rows && !KEEP)
 #pragma unroll
           for (int j = 0; j < MT; ++j) x[i][j] = load_x(nc, j, i);
       }
@@ -216,8 +289,9 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
       i32x4 s = red[it & 1][0][u][lane];
 #pragma unroll
       for (int v = 1; v < kQrWaves; ++v) s += red[it & 1][v][u][lane];
-      const int m = 16 * (u % MT) + n;
-      finish<E, GATED>(p, t * NP + u / MT, m, g, row_scale[m], s);
+      const int m = 16 * (u % MT) + n, panel = t * NP + u / MT;
+      const int f = GATED ? 8 * panel + 4 * (g & 1) : HALF ? 8 * t + 4 * (g & 1) : 16 * panel + 4 * g;
+      finish<E, GATED>(p, f, m, g, !HALF || g < 2, row_scale[m], s);
     }
   }
 }
@@ -277,21 +351,30 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p
     i32x4 s = red[0][u][lane];
 #pragma unroll
     for (int v = 1; v < kQrWaves; ++v) s += red[v][u][lane];
-    const int m = (j0 + u % MT) * 16 + n;
-    finish<E, GATED>(p, panel0 + u / MT, m, g, p.x_scale[min(m, p.M - 1)], s);
+    const int m = (j0 + u % MT) * 16 + n, panel = panel0 + u / MT;
+    finish<E, GATED>(p, GATED ? 8 * panel + 4 * (g & 1) : 16 * panel + 4 * g, m, g, true,
+                     p.x_scale[min(m, p.M - 1)], s);
   }
 }
 
 namespace {
 
-template <typename E, int MT, int NP, bool GATED, int SRC>
+template <typename E, int MT, int NP, bool GATED, int SRC, bool HALF = false>
 hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
-  if (p.Kp <= kQ8KeepK)
-    hipLaunchKernelGGL((q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true>), dim3(grid), dim3(kQrThreads), 0,
-                       stream, p);
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kQrThreads), 0, stream, p); };
+  constexpr int kMany = SRC == kQ8Float && HALF ? 18 : MT == 1 ? 9 : 6;
+  if constexpr (SRC == kQ8Float) {
+    if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF, 1>);
+    else go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF, kQ8FloatMax>);
+  }
+  else if (p.Kp <= 1024)
+    go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, HALF>);
+  else if (p.Kp <= 1536)
+    go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, HALF>);
+  else if (p.Kp <= kQ8KeepK)
+    go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, HALF>);
   else if constexpr (SRC == kQ8Rows)
-    hipLaunchKernelGGL((q8_rows_kernel<E, MT, NP, MT == 1 ? 9 : 6, GATED, SRC, false>), dim3(grid),
-                       dim3(kQrThreads), 0, stream, p);
+    go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF>);
   else
     return hipErrorInvalidValue;
   return hipGetLastError();
@@ -304,7 +387,10 @@ hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
     if (p.M > 32) return launch_rows_k<E, 4, 1, GATED, SRC>(p, grid, stream);
     if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
   }
-  if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
+  if constexpr (!GATED)
+    if (2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, true>(p, 2 * p.panels, stream);
+  if constexpr (SRC != kQ8Float)
+    if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
   return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);
 }
 
@@ -312,6 +398,8 @@ template <typename E, bool GATED>
 hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t stream) {
   if (source == kQ8Plain) return launch_rows_m<E, GATED, kQ8Plain>(p, n_cus, stream);
   if (source == kQ8Norm) return launch_rows_m<E, GATED, kQ8Norm>(p, n_cus, stream);
+  if constexpr (!GATED)
+    if (source == kQ8Float) return launch_rows_m<E, GATED, kQ8Float>(p, n_cus, stream);
   return launch_rows_m<E, GATED, kQ8Rows>(p, n_cus, stream);
 }
 

@@ -11,6 +11,7 @@ namespace mi_fa2 {
 constexpr int kQ8RowsMax = 64;    // rows that the few-row kernel takes
 constexpr int kQ8KeepK = 2048;    // (padded) in features whose rows it keeps in registers
 constexpr int kQ8FusedMax = 16;   // rows that it brings to 8 bits itself, of at most kQ8KeepK
+constexpr int kQ8FloatMax = 4, kQ8FloatK = 12288;   // fp32 rows that it does, and their most features
 
 enum Q8Kernel { kQ8FewRows = 0, kQ8Tile32 = 1, kQ8Tile64 = 2, kQ8Gemm64 = 3, kQ8Gemm128 = 4 };
 

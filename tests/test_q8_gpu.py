@@ -141,14 +141,25 @@ def test_rows_of_nothing_and_of_no_number(n, dtype):
     check_rows(got, o8.rmsnorm(x[6:], w.cpu(), 1e-6))
 
 
-def test_ties_go_to_the_even_number():
-    # the largest magnitude is 127 halves: every value is a whole number or one and a half
-    n = 255
-    x = (torch.arange(-127, 128) / 2.0).to(torch.float16)[None]
-    x[0, 0], x[0, -1] = -63.5 * 2, 63.5 * 2
-    got = q8.quantize(x.to(DEV))
-    assert got.scale.item() == 1.0
-    assert torch.equal(got.values[0].cpu().double(), torch.round(x[0].double()))
+@pytest.mark.parametrize("step", [1, 3, 5, 7, 10, 13])
+def test_ties_go_to_the_even_number(step):
+    # every value is a whole number or one and a half, times the scale: exact in fp16, and so is the answer
+    halves = torch.arange(-127, 128).double()
+    x = halves * step / 2.0 ** 7
+    x[0], x[-1] = -127 * step / 2.0 ** 6, 127 * step / 2.0 ** 6
+    assert torch.equal(x.to(torch.float16).double(), x)
+    want = torch.round(halves / 2)
+    want[0], want[-1] = -127, 127
+    x = x.to(torch.float16)[None].to(DEV)
+    got = q8.quantize(x)
+    assert got.scale.item() == step / 2.0 ** 6
+    assert torch.equal(got.values[0].cpu().double(), want)
+    # the same in the launch of a product: a weight of ones in one place each gives the values back
+    eye = torch.eye(256, dtype=torch.int8)[:, :255].contiguous()
+    w = q8.Weight(eye.to(DEV), torch.full((256,), 2.0 ** 6 / step, device=DEV))
+    for rows in (x, x.repeat(40, 1)):
+        out = q8.linear(rows, w).cpu().double()
+        assert torch.equal(out[:, :255], want.expand(len(rows), -1))
 
 
 @pytest.mark.parametrize("gated", [False, True])
