@@ -55,10 +55,20 @@ MI_Q8_API int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, voi
  * r * rsqrt(mean(r^2) + eps) * weight in 8 bits, taken in fp32 without a rounding in between.
  * residual_out may be x or y.
  */
-MI_Q8_API int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
-                                int64_t y_stride, const void* weight, float eps,
-                                void* residual_out, int64_t residual_stride, void* values,
-                                float* scale, int32_t rows, int32_t n, void* stream);
+typedef struct mi_q8_norm_args {
+  const void* x;
+  int64_t x_stride;
+  const void* y;
+  int64_t y_stride;
+  const void* weight;
+  void* residual_out;
+  int64_t residual_stride;
+  void* values;
+  float* scale;
+  int32_t dtype, rows, n;
+  float eps;
+} mi_q8_norm_args;
+MI_Q8_API int mi_q8_add_rmsnorm(const mi_q8_norm_args* args, void* stream);
 
 /* out [rows, n] = values * scale, rounded. */
 MI_Q8_API int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
@@ -73,40 +83,59 @@ MI_Q8_API int mi_q8_pack(const void* values, int64_t stride, int32_t out_feature
                          int32_t in_features, int32_t gated, void* packed, void* stream);
 
 /*
- * out = [residual +] x W^T [+ bias] of rows already in 8 bits: values, scale [rows] as mi_q8_quantize
- * leaves them, w packed, w_scale [out_features], bias [out_features] or NULL, residual
+ * out = [residual +] x W^T [+ bias]: w packed, w_scale [out_features], bias [out_features] or NULL, residual
  * [rows, out_features] or NULL (may be out).
+ *
+ * x_scale NULL: x is 16-bit rows [rows, in_features], which the call brings to 8 bits itself, as
+ * mi_q8_add_rmsnorm does without y (norm_weight) or as mi_q8_quantize does (norm_weight NULL); out must not
+ * overlap x; workspace: mi_q8_linear_workspace_size() bytes (0 for few rows: none is looked at).
+ * Otherwise x and x_scale are rows already in 8 bits as those leave them; x_stride, norm_weight, eps and the
+ * workspace are not used.
  */
-MI_Q8_API int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
-                           const float* w_scale, const void* bias, const void* residual,
-                           int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                           int32_t out_features, int32_t in_features, void* stream);
-
-/*
- * The same of rows x [rows, in] that the call holds in 8 bits itself, as mi_q8_add_rmsnorm does without
- * y (norm_weight) or as mi_q8_quantize does (norm_weight NULL).  out must not overlap x.
- */
-MI_Q8_API size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features,
-                                             int32_t in_features);
-MI_Q8_API int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight,
-                           float eps, const void* w, const float* w_scale, const void* bias,
-                           const void* residual, int64_t residual_stride, void* out,
-                           int64_t out_stride, int32_t rows, int32_t out_features,
-                           int32_t in_features, void* workspace, size_t workspace_bytes,
-                           void* stream);
+typedef struct mi_q8_linear_args {
+  const void* x;
+  int64_t x_stride;
+  const float* x_scale;
+  const void* norm_weight;
+  const void* w;
+  const float* w_scale;
+  const void* bias;
+  const void* residual;
+  int64_t residual_stride;
+  void* out;
+  int64_t out_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t dtype, rows, out_features, in_features;
+  float eps;
+} mi_q8_linear_args;
+MI_Q8_API size_t mi_q8_linear_workspace_size(int32_t rows, int32_t in_features);
+MI_Q8_API int mi_q8_linear(const mi_q8_linear_args* args, void* stream);
 
 /*
  * A gated feed-forward block, out = [residual +] a Wd^T with a = silu(g) * u in fp32, held in 8 bits
  * for the second product, and (g | u) = [rmsnorm] x Wgu^T: x, out, residual [rows, hidden], gate_up
  * packed as gated [2 * inter, hidden], down packed [hidden, inter].  out may be x and residual.
  */
+typedef struct mi_q8_mlp_args {
+  const void* x;
+  int64_t x_stride;
+  const void* norm_weight;
+  const void* gate_up;
+  const float* gate_up_scale;
+  const void* down;
+  const float* down_scale;
+  const void* residual;
+  int64_t residual_stride;
+  void* out;
+  int64_t out_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t dtype, rows, hidden, inter;
+  float eps;
+} mi_q8_mlp_args;
 MI_Q8_API size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter);
-MI_Q8_API int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight,
-                        float eps, const void* gate_up, const float* gate_up_scale,
-                        const void* down, const float* down_scale, const void* residual,
-                        int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                        int32_t hidden, int32_t inter, void* workspace, size_t workspace_bytes,
-                        void* stream);
+MI_Q8_API int mi_q8_mlp(const mi_q8_mlp_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -86,6 +86,18 @@ int check_rows(const char* name, const void* p, int64_t stride, int64_t width) {
   return kOk;
 }
 
+int check_weight(const char* name, const void* w, const float* scale) {
+  if (int rc = check_ptr(name, w, 16)) return rc;
+  if (!scale || !aligned(scale, 4)) return fail(kInvalid, "%s_scale is %s", name, scale ? "not 4-byte aligned" : "NULL");
+  return kOk;
+}
+
+int check_out(const void* residual, int64_t residual_stride, void* out, int64_t out_stride, int32_t n) {
+  if (residual)
+    if (int rc = check_rows("residual", residual, residual_stride, n)) return rc;
+  return check_rows("out", out, out_stride, n);
+}
+
 bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
   return x < y + b_bytes && y < x + a_bytes;
@@ -176,9 +188,12 @@ int product(Q8Params p, int dtype, bool gated, const void* values, const float* 
 
 // The product of 16-bit rows, brought to 8 bits in the same launch where the few-row kernel does that,
 // else before it in the workspace.
+bool fused(int32_t rows, int32_t in) {
+  return rows <= mi_fa2::kQ8FusedMax && q8_pad(in) <= mi_fa2::kQ8KeepK;
+}
 int product_of(Q8Params p, int dtype, bool gated, const void* x, int64_t x_stride,
                const void* norm_weight, float eps, const RowsSpace& r, char* ws, void* stream) {
-  if (p.M <= mi_fa2::kQ8FusedMax && p.Kp <= mi_fa2::kQ8KeepK) {
+  if (fused(p.M, p.K)) {
     p.x = x;
     p.x_st = x_stride;
     p.norm_w = static_cast<const uint16_t*>(norm_weight);
@@ -236,24 +251,23 @@ int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, void* values,
                   stream);
 }
 
-int mi_q8_add_rmsnorm(int32_t dtype, const void* x, int64_t x_stride, const void* y,
-                      int64_t y_stride, const void* weight, float eps, void* residual_out,
-                      int64_t residual_stride, void* values, float* scale, int32_t rows, int32_t n,
-                      void* stream) {
-  if (int rc = check_dtype(dtype)) return rc;
-  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
-  if (int rc = check_count("n", n, 1, kMaxK)) return rc;
-  if (rows == 0) return ok();
-  if (int rc = check_rows("x", x, x_stride, n)) return rc;
-  if (y)
-    if (int rc = check_rows("y", y, y_stride, n)) return rc;
-  if (y)
-    if (int rc = check_rows("residual_out", residual_out, residual_stride, n)) return rc;
-  if (int rc = check_ptr("weight", weight, 2)) return rc;
-  if (int rc = check_ptr("values", values, 16)) return rc;
-  if (int rc = check_ptr("scale", scale, 4)) return rc;
-  return quantize(dtype, x, x_stride, y, y_stride, weight, eps, residual_out, residual_stride,
-                  values, scale, rows, n, stream);
+int mi_q8_add_rmsnorm(const mi_q8_norm_args* args, void* stream) {
+  if (!args) return fail(kInvalid, "args is NULL");
+  const mi_q8_norm_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (int rc = check_count("rows", a.rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("n", a.n, 1, kMaxK)) return rc;
+  if (a.rows == 0) return ok();
+  if (int rc = check_rows("x", a.x, a.x_stride, a.n)) return rc;
+  if (a.y) {
+    if (int rc = check_rows("y", a.y, a.y_stride, a.n)) return rc;
+    if (int rc = check_rows("residual_out", a.residual_out, a.residual_stride, a.n)) return rc;
+  }
+  if (int rc = check_ptr("weight", a.weight, 2)) return rc;
+  if (int rc = check_ptr("values", a.values, 16)) return rc;
+  if (int rc = check_ptr("scale", a.scale, 4)) return rc;
+  return quantize(a.dtype, a.x, a.x_stride, a.y, a.y_stride, a.weight, a.eps, a.residual_out,
+                  a.residual_stride, a.values, a.scale, a.rows, a.n, stream);
 }
 
 int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
@@ -299,69 +313,43 @@ int mi_q8_pack(const void* values, int64_t stride, int32_t out_features, int32_t
   return launched(mi_fa2::launch_q8_pack(p, reinterpret_cast<hipStream_t>(stream)));
 }
 
-namespace {
-
-int check_product(int32_t rows, int32_t out_features, int32_t in_features) {
-  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
-  if (int rc = check_count("out features", out_features, 1, kMaxOut)) return rc;
-  return check_count("in features", in_features, 1, kMaxK);
-}
-
-int check_operands(const void* w, const float* w_scale, const void* bias, const void* residual,
-                   int64_t residual_stride, void* out, int64_t out_stride, int32_t out_features) {
-  if (int rc = check_ptr("w", w, 16)) return rc;
-  if (int rc = check_ptr("w_scale", w_scale, 4)) return rc;
-  if (bias && !aligned(bias, 2)) return check_ptr("bias", bias, 2);
-  if (residual)
-    if (int rc = check_rows("residual", residual, residual_stride, out_features)) return rc;
-  return check_rows("out", out, out_stride, out_features);
-}
-
-}  // namespace
-
-int mi_q8_matmul(int32_t dtype, const void* values, const float* scale, const void* w,
-                 const float* w_scale, const void* bias, const void* residual,
-                 int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                 int32_t out_features, int32_t in_features, void* stream) {
-  if (int rc = check_dtype(dtype)) return rc;
-  if (int rc = check_product(rows, out_features, in_features)) return rc;
-  if (rows == 0) return ok();
-  if (int rc = check_ptr("values", values, 16)) return rc;
-  if (int rc = check_ptr("scale", scale, 4)) return rc;
-  if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
-                              out_features))
-    return rc;
-  return product(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
-                          out_features, in_features, false),
-                 dtype, false, values, scale, stream);
-}
-
-size_t mi_q8_linear_workspace_size(int32_t rows, int32_t out_features, int32_t in_features) {
-  if (rows <= 0 || out_features <= 0 || in_features <= 0 || in_features > kMaxK) return 0;
+size_t mi_q8_linear_workspace_size(int32_t rows, int32_t in_features) {
+  if (rows <= 0 || in_features <= 0 || in_features > kMaxK || fused(rows, in_features)) return 0;
   return LinearSpace(rows, in_features).s.total;
 }
 
-int mi_q8_linear(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
-                 const void* w, const float* w_scale, const void* bias, const void* residual,
-                 int64_t residual_stride, void* out, int64_t out_stride, int32_t rows,
-                 int32_t out_features, int32_t in_features, void* workspace,
-                 size_t workspace_bytes, void* stream) {
-  if (int rc = check_dtype(dtype)) return rc;
-  if (int rc = check_product(rows, out_features, in_features)) return rc;
-  if (rows == 0) return ok();
-  if (int rc = check_rows("x", x, x_stride, in_features)) return rc;
-  if (norm_weight && !aligned(norm_weight, 2)) return check_ptr("norm_weight", norm_weight, 2);
-  if (int rc = check_operands(w, w_scale, bias, residual, residual_stride, out, out_stride,
-                              out_features))
-    return rc;
-  if (overlap(x, span(rows, x_stride, in_features), out, span(rows, out_stride, out_features)))
+int mi_q8_linear(const mi_q8_linear_args* args, void* stream) {
+  if (!args) return fail(kInvalid, "args is NULL");
+  const mi_q8_linear_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (int rc = check_count("rows", a.rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("out features", a.out_features, 1, kMaxOut)) return rc;
+  if (int rc = check_count("in features", a.in_features, 1, kMaxK)) return rc;
+  if (a.rows == 0) return ok();
+  if (a.x_scale) {
+    if (int rc = check_ptr("x", a.x, 16)) return rc;
+    if (int rc = check_ptr("x_scale", a.x_scale, 4)) return rc;
+  } else {
+    if (int rc = check_rows("x", a.x, a.x_stride, a.in_features)) return rc;
+    if (a.norm_weight)
+      if (int rc = check_ptr("norm_weight", a.norm_weight, 2)) return rc;
+  }
+  if (int rc = check_weight("w", a.w, a.w_scale)) return rc;
+  if (a.bias)
+    if (int rc = check_ptr("bias", a.bias, 2)) return rc;
+  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.out_features)) return rc;
+  const Q8Params p = operands(a.w, a.w_scale, a.bias, a.residual, a.residual_stride, a.out, a.out_stride,
+                              a.rows, a.out_features, a.in_features, false);
+  if (a.x_scale) return product(p, a.dtype, false, a.x, a.x_scale, stream);
+  if (overlap(a.x, span(a.rows, a.x_stride, a.in_features), a.out,
+              span(a.rows, a.out_stride, a.out_features)))
     return fail(kInvalid, "out overlaps x");
-  const LinearSpace sp(rows, in_features);
-  if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
-  return product_of(operands(w, w_scale, bias, residual, residual_stride, out, out_stride, rows,
-                             out_features, in_features, false),
-                    dtype, false, x, x_stride, norm_weight, eps, sp.x, static_cast<char*>(workspace),
-                    stream);
+  const LinearSpace sp(a.rows, a.in_features);
+  if (int rc = check_workspace(a.workspace, a.workspace_bytes,
+                               fused(a.rows, a.in_features) ? 0 : sp.s.total))
+    return rc;
+  return product_of(p, a.dtype, false, a.x, a.x_stride, a.norm_weight, a.eps, sp.x,
+                    static_cast<char*>(a.workspace), stream);
 }
 
 size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter) {
@@ -369,53 +357,50 @@ size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter) {
   return MlpSpace(rows, hidden, inter).s.total;
 }
 
-int mi_q8_mlp(int32_t dtype, const void* x, int64_t x_stride, const void* norm_weight, float eps,
-              const void* gate_up, const float* gate_up_scale, const void* down,
-              const float* down_scale, const void* residual, int64_t residual_stride, void* out,
-              int64_t out_stride, int32_t rows, int32_t hidden, int32_t inter, void* workspace,
-              size_t workspace_bytes, void* stream) {
-  if (int rc = check_dtype(dtype)) return rc;
-  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
-  if (int rc = check_count("hidden", hidden, 1, kMaxK)) return rc;
-  if (int rc = check_count("inter", inter, 1, kMaxK)) return rc;
-  if (rows == 0) return ok();
-  if (int rc = check_rows("x", x, x_stride, hidden)) return rc;
-  if (norm_weight && !aligned(norm_weight, 2)) return check_ptr("norm_weight", norm_weight, 2);
-  if (int rc = check_ptr("gate_up", gate_up, 16)) return rc;
-  if (int rc = check_ptr("gate_up_scale", gate_up_scale, 4)) return rc;
-  if (int rc = check_operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride,
-                              hidden))
+int mi_q8_mlp(const mi_q8_mlp_args* args, void* stream) {
+  if (!args) return fail(kInvalid, "args is NULL");
+  const mi_q8_mlp_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (int rc = check_count("rows", a.rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("hidden", a.hidden, 1, kMaxK)) return rc;
+  if (int rc = check_count("inter", a.inter, 1, kMaxK)) return rc;
+  if (a.rows == 0) return ok();
+  if (int rc = check_rows("x", a.x, a.x_stride, a.hidden)) return rc;
+  if (a.norm_weight)
+    if (int rc = check_ptr("norm_weight", a.norm_weight, 2)) return rc;
+  if (int rc = check_weight("gate_up", a.gate_up, a.gate_up_scale)) return rc;
+  if (int rc = check_weight("down", a.down, a.down_scale)) return rc;
+  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.hidden)) return rc;
+  const MlpSpace sp(a.rows, a.hidden, a.inter);
+  if (int rc = check_workspace(a.workspace, a.workspace_bytes, sp.s.total)) return rc;
+  char* ws = static_cast<char*>(a.workspace);
+  if (int rc = product_of(operands(a.gate_up, a.gate_up_scale, nullptr, nullptr, 0, ws + sp.act,
+                                   sp.act_stride, a.rows, a.inter, a.hidden, true),
+                          a.dtype, true, a.x, a.x_stride, a.norm_weight, a.eps, sp.x, ws, stream))
     return rc;
-  const MlpSpace sp(rows, hidden, inter);
-  if (int rc = check_workspace(workspace, workspace_bytes, sp.s.total)) return rc;
-  char* ws = static_cast<char*>(workspace);
-  float* a_scale = reinterpret_cast<float*>(ws + sp.a.scale);
-  if (int rc = product_of(operands(gate_up, gate_up_scale, nullptr, nullptr, 0, ws + sp.act,
-                                   sp.act_stride, rows, inter, hidden, true),
-                          dtype, true, x, x_stride, norm_weight, eps, sp.x, ws, stream))
-    return rc;
-  Q8Params d = operands(down, down_scale, nullptr, residual, residual_stride, out, out_stride, rows, hidden,
-                        inter, false);
-  if (rows <= mi_fa2::kQ8FloatMax && q8_pad(inter) <= mi_fa2::kQ8FloatK) {
+  Q8Params d = operands(a.down, a.down_scale, nullptr, a.residual, a.residual_stride, a.out,
+                        a.out_stride, a.rows, a.hidden, a.inter, false);
+  if (a.rows <= mi_fa2::kQ8FloatMax && d.Kp <= mi_fa2::kQ8FloatK) {
     d.x = ws + sp.act;
     d.x_st = sp.act_stride;
     int cus = 0;
     if (int rc = compute_units(&cus)) return rc;
-    return launched(mi_fa2::launch_q8_rows(d, dtype, false, mi_fa2::kQ8Float, cus,
+    return launched(mi_fa2::launch_q8_rows(d, a.dtype, false, mi_fa2::kQ8Float, cus,
                                            reinterpret_cast<hipStream_t>(stream)));
   }
+  float* a_scale = reinterpret_cast<float*>(ws + sp.a.scale);
   Q8QuantParams q{};
   q.x = ws + sp.act;
   q.x_st = sp.act_stride;
   q.q = reinterpret_cast<int8_t*>(ws + sp.a.values);
   q.scale = a_scale;
-  q.M = rows;
-  q.n = inter;
-  q.np = q8_pad(inter);
-  if (int rc = launched(mi_fa2::launch_q8_quant(q, dtype, mi_fa2::kQ8Float,
+  q.M = a.rows;
+  q.n = a.inter;
+  q.np = q8_pad(a.inter);
+  if (int rc = launched(mi_fa2::launch_q8_quant(q, a.dtype, mi_fa2::kQ8Float,
                                                 reinterpret_cast<hipStream_t>(stream))))
     return rc;
-  return product(d, dtype, false, ws + sp.a.values, a_scale, stream);
+  return product(d, a.dtype, false, ws + sp.a.values, a_scale, stream);
 }
 
 }  // extern "C"

@@ -17,6 +17,7 @@ call that the kernels do not take raises.
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -30,26 +31,26 @@ MAX_ROWS = 1 << 21
 MAX_IN = 131072      # 128 * 127 * in stays below 2^31
 MAX_OUT = 1 << 24
 
-_p, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
-_sz = ctypes.c_size_t
+_p, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+_sz, _args = ctypes.c_size_t, ctypes.c_char_p
 # name -> (restype, argtypes); mirrors include/mi_q8.h
 SIGNATURES = {
     "mi_q8_last_error": (ctypes.c_char_p, []),
     "mi_q8_rows_bytes": (_sz, [_i32, _i32]),
     "mi_q8_quantize": (_i32, [_i32, _p, _i64, _p, _p, _i32, _i32, _p]),
-    "mi_q8_add_rmsnorm": (_i32, [_i32, _p, _i64, _p, _i64, _p, _f32, _p, _i64, _p, _p, _i32, _i32,
-                                 _p]),
+    "mi_q8_add_rmsnorm": (_i32, [_args, _p]),
     "mi_q8_dequantize": (_i32, [_i32, _p, _p, _p, _i64, _i32, _i32, _p]),
     "mi_q8_packed_bytes": (_sz, [_i32, _i32, _i32]),
     "mi_q8_pack": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _p]),
-    "mi_q8_matmul": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32, _p]),
-    "mi_q8_linear_workspace_size": (_sz, [_i32, _i32, _i32]),
-    "mi_q8_linear": (_i32, [_i32, _p, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32,
-                            _i32, _p, _sz, _p]),
+    "mi_q8_linear_workspace_size": (_sz, [_i32, _i32]),
+    "mi_q8_linear": (_i32, [_args, _p]),
     "mi_q8_mlp_workspace_size": (_sz, [_i32, _i32, _i32]),
-    "mi_q8_mlp": (_i32, [_i32, _p, _i64, _p, _f32, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _i32,
-                         _i32, _p, _sz, _p]),
+    "mi_q8_mlp": (_i32, [_args, _p]),
 }
+# the argument structs, packed in one go: a call of 18 arguments costs ctypes 1.9 us, this 0.6
+NORM_ARGS = struct.Struct("@PqPqPPqPPiiif")
+LINEAR_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
+MLP_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
 
 _library = None
 
@@ -93,7 +94,7 @@ class Weight:
     """A projection's weight in 8 bits: values [out, in] int8 and scale [out] fp32 (weight = values *
     scale[:, None]), laid out for the kernels once.  gated: the gate and up rows of a feed-forward block,
     gate rows first, which only `mlp` takes.  The values are copied, the scale is kept as it is."""
-    __slots__ = ("data", "scale", "out_features", "in_features", "gated")
+    __slots__ = ("data", "scale", "out_features", "in_features", "gated", "sig", "data_ptr", "scale_ptr")
 
     def __init__(self, values, scale, gated=False):
         assert values.is_cuda and values.dtype == torch.int8 and values.dim() == 2, \
@@ -113,6 +114,8 @@ class Weight:
                                 device=values.device)
         call(values.device.index, lib.mi_q8_pack, values.data_ptr(),
              values.stride(0) if n > 1 else k, n, k, self.gated, self.data.data_ptr())
+        self.sig = (n, k, self.gated, values.device)
+        self.data_ptr, self.scale_ptr = self.data.data_ptr(), scale.data_ptr()
 
     @property
     def device(self):
@@ -143,13 +146,15 @@ class Rows:
 
     def dequantize(self, out=None):
         """values * scale [rows, n] in dtype."""
-        R, dev = self.scale.shape[0], self.scale.device
+        scale, dt = self.scale, self.dtype
+        R, dev = scale.shape[0], scale.device
         if out is None:
-            out = torch.empty((R, self.n), device=dev, dtype=self.dtype)
-        op, os_ = _rows(out, "out", self.dtype, dev)
-        assert out.shape == (R, self.n), f"out: [{R}, {self.n}]"
-        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[self.dtype], self.data.data_ptr(),
-             self.scale.data_ptr(), op, os_, R, self.n)
+            out, os_ = torch.empty((R, self.n), device=dev, dtype=dt), self.n
+        else:
+            _, os_ = _rows(out, "out", dt, dev)
+            assert out.shape == (R, self.n), f"out: [{R}, {self.n}]"
+        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[dt], self.data.data_ptr(),
+             scale.data_ptr(), out.data_ptr(), os_, R, self.n)
         return out
 
 
@@ -191,90 +196,157 @@ def quantize(x):
     return out
 
 
+# What a call's shapes, strides, types and devices decide, checked once per combination.
+_PLANS = {}
+
+
+def _plan(key, make, *args):
+    if len(_PLANS) >= _MEMO_MAX:
+        _PLANS.clear()
+    got = _PLANS[key] = make(*args)
+    return got
+
+
+def _sig(t):
+    return (t.shape, t.stride(), t.dtype, t.device) if t is not None else None
+
+
 def add_rmsnorm(x, weight, eps, y=None, residual_out=None):
     """x [rows, n] (+ y) -> (r, Rows): r = x + y rounded (x itself when y is None), and weight * rmsnorm(r)
     in 8 bits, with no rounding to 16 bits in between.  residual_out may be x or y (in place)."""
+    key = ("norm", x.shape, x.stride(), x.dtype, x.device, _sig(weight), _sig(y), _sig(residual_out))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _norm_plan, x, weight, y, residual_out)
+    index, fn, code, R, n, nbytes, xs, ys, rs = plan
+    if y is None:
+        r, yp, rp = x, 0, 0
+    else:
+        r = x.new_empty((R, n)) if residual_out is None else residual_out
+        yp, rp = y.data_ptr(), r.data_ptr()
+    dev = x.device
+    data = torch.empty(nbytes, dtype=torch.int8, device=dev)
+    scale = torch.empty(R, dtype=torch.float32, device=dev)
+    call(index, fn, NORM_ARGS.pack(x.data_ptr(), xs, yp, ys, weight.data_ptr(), rp, rs,
+                                   data.data_ptr(), scale.data_ptr(), code, R, n, eps))
+    return r, Rows(data, scale, n, x.dtype)
+
+
+def _norm_plan(x, weight, y, residual_out):
     dt, dev = _input(x)
     R, n = x.shape
-    xp, xs = _rows(x, "x", dt, dev)
-    yp, ys, r, rp, rs = None, 0, x, None, 0
+    _, xs = _rows(x, "x", dt, dev)
+    _vector(weight, "weight", n, dt, dev)
+    ys, rs = 0, n
     if y is not None:
-        yp, ys = _rows(y, "y", dt, dev)
+        _, ys = _rows(y, "y", dt, dev)
         assert y.shape == x.shape, "y: x's shape"
-        r = torch.empty((R, n), device=dev, dtype=dt) if residual_out is None else residual_out
-        rp, rs = _rows(r, "residual_out", dt, dev)
-        assert r.shape == x.shape, "residual_out: x's shape"
+        if residual_out is not None:
+            _, rs = _rows(residual_out, "residual_out", dt, dev)
+            assert residual_out.shape == x.shape, "residual_out: x's shape"
     else:
         assert residual_out is None, "residual_out goes with y"
-    out = _empty_rows(R, n, dt, dev)
-    call(dev.index, load().mi_q8_add_rmsnorm, _lib.DTYPES[dt], xp, xs, yp, ys,
-         _vector(weight, "weight", n, dt, dev), float(eps), rp, rs, out.data.data_ptr(),
-         out.scale.data_ptr(), R, n)
-    return r, out
+    return (dev.index, load().mi_q8_add_rmsnorm, _lib.DTYPES[dt], R, n, rows_bytes(R, n), xs, ys, rs)
 
 
-def _out(out, residual, R, N, dt, dev):
-    if out is None:
-        out = torch.empty((R, N), device=dev, dtype=dt)
-    op, os_ = _rows(out, "out", dt, dev)
-    assert out.shape == (R, N), f"out: [{R}, {N}]"
-    rp, rs = None, 0
+def _ends(out, residual, R, N, dt, dev):
+    """Row strides of out (None: a new one) and residual (or None) [R, N]."""
+    os_, rs = N, 0
+    if out is not None:
+        _, os_ = _rows(out, "out", dt, dev)
+        assert out.shape == (R, N), f"out: [{R}, {N}]"
     if residual is not None:
-        rp, rs = _rows(residual, "residual", dt, dev)
+        _, rs = _rows(residual, "residual", dt, dev)
         assert residual.shape == (R, N), f"residual: [{R}, {N}]"
-    return out, op, os_, rp, rs
+    return os_, rs
 
 
 def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
     """[residual +] x W^T [+ bias] -> [rows, out]: x [rows, in] (bf16 or fp16; with norm_weight RMS-normalised
     first) or Rows, w a Weight.  residual may be `out` (in place); out must not overlap x."""
-    assert type(w) is Weight and not w.gated, "w: a Weight that is not gated"
+    assert type(w) is Weight, "w: a Weight"
+    if type(x) is Rows:
+        assert norm_weight is None, "rows in 8 bits are normalised already"
+        data, scale = x.data, x.scale
+        key = ("rows", x.n, x.dtype, scale.shape, scale.device, w.sig, _sig(bias), _sig(residual), _sig(out))
+    else:
+        data, scale = x, None
+        key = ("linear", x.shape, x.stride(), x.dtype, x.device, w.sig, _sig(bias), _sig(residual), _sig(out),
+               _sig(norm_weight))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _linear_plan, x, w, bias, residual, norm_weight, out)
+    index, fn, code, dt, shape, K, nbytes, xs, rs, os_ = plan
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=data.device)
+    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=data.device) if nbytes else None
+    call(index, fn, LINEAR_ARGS.pack(
+        data.data_ptr(), xs, scale.data_ptr() if scale is not None else 0,
+        norm_weight.data_ptr() if norm_weight is not None else 0, w.data_ptr, w.scale_ptr,
+        bias.data_ptr() if bias is not None else 0, residual.data_ptr() if residual is not None else 0,
+        rs, out.data_ptr(), os_, ws.data_ptr() if nbytes else 0, nbytes, code, *shape, K, eps))
+    return out
+
+
+def _linear_plan(x, w, bias, residual, norm_weight, out):
+    assert not w.gated, "w: a Weight that is not gated"
     N, K = w.out_features, w.in_features
     lib = load()
     if type(x) is Rows:
-        assert norm_weight is None, "rows in 8 bits are normalised already"
         dt, dev, R = x.dtype, x.scale.device, x.scale.shape[0]
         assert x.n == K and w.device == dev, f"x: rows of {K} on {w.device}"
-        out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
-        call(dev.index, lib.mi_q8_matmul, _lib.DTYPES[dt], x.data.data_ptr(), x.scale.data_ptr(),
-             w.data.data_ptr(), w.scale.data_ptr(),
-             _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N,
-             K)
-        return out
-    dt, dev = _input(x)
-    R = x.shape[0]
-    assert x.shape[1] == K and w.device == dev, f"x: rows of {K} on {w.device}"
-    xp, xs = _rows(x, "x", dt, dev)
-    out, op, os_, rp, rs = _out(out, residual, R, N, dt, dev)
-    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
-    ws = torch.empty(lib.mi_q8_linear_workspace_size(R, N, K), dtype=torch.uint8, device=dev)
-    call(dev.index, lib.mi_q8_linear, _lib.DTYPES[dt], xp, xs,
-         _vector(norm_weight, "norm_weight", K, dt, dev) if norm_weight is not None else None,
-         float(eps), w.data.data_ptr(), w.scale.data_ptr(),
-         _vector(bias, "bias", N, dt, dev) if bias is not None else None, rp, rs, op, os_, R, N, K,
-         ws.data_ptr(), ws.numel())
-    return out
+        xs = nbytes = 0
+    else:
+        dt, dev = _input(x)
+        R = x.shape[0]
+        assert x.shape[1] == K and w.device == dev, f"x: rows of {K} on {w.device}"
+        _, xs = _rows(x, "x", dt, dev)
+        nbytes = lib.mi_q8_linear_workspace_size(R, K)
+        if norm_weight is not None:
+            _vector(norm_weight, "norm_weight", K, dt, dev)
+    if bias is not None:
+        _vector(bias, "bias", N, dt, dev)
+    os_, rs = _ends(out, residual, R, N, dt, dev)
+    return (dev.index, lib.mi_q8_linear, _lib.DTYPES[dt], dt, (R, N), K, nbytes, xs, rs, os_)
 
 
 def mlp(x, gate_up, down, residual=None, norm_weight=None, eps=0.0, out=None):
     """[residual +] (silu(g) * u) Wd^T with (g | u) = [rmsnorm] x Wgu^T -> [rows, hidden]: x [rows, hidden],
     gate_up a gated Weight [2 * inter, hidden], down a Weight [hidden, inter].  The activation is held in 8 bits
     too, every row by its largest magnitude.  out may be residual and x."""
-    assert type(gate_up) is Weight and gate_up.gated, "gate_up: a gated Weight"
-    assert type(down) is Weight and not down.gated, "down: a Weight that is not gated"
+    assert type(gate_up) is Weight and type(down) is Weight, "gate_up, down: Weights"
+    key = ("mlp", x.shape, x.stride(), x.dtype, x.device, gate_up.sig, down.sig, _sig(residual),
+           _sig(norm_weight), _sig(out))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _mlp_plan, x, gate_up, down, residual, norm_weight, out)
+    index, fn, code, R, H, inter, nbytes, xs, rs, os_ = plan
+    if out is None:
+        out = x.new_empty((R, H))
+    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    call(index, fn, MLP_ARGS.pack(
+        x.data_ptr(), xs, norm_weight.data_ptr() if norm_weight is not None else 0, gate_up.data_ptr,
+        gate_up.scale_ptr, down.data_ptr, down.scale_ptr,
+        residual.data_ptr() if residual is not None else 0, rs, out.data_ptr(), os_, ws.data_ptr(),
+        nbytes, code, R, H, inter, eps))
+    return out
+
+
+def _mlp_plan(x, gate_up, down, residual, norm_weight, out):
+    assert gate_up.gated, "gate_up: a gated Weight"
+    assert not down.gated, "down: a Weight that is not gated"
     dt, dev = _input(x)
     R, H = x.shape
     inter = down.in_features
     assert gate_up.in_features == H and down.out_features == H, f"weights of hidden size {H}"
     assert gate_up.out_features == 2 * inter, f"gate_up of {2 * inter} rows"
     assert gate_up.device == dev and down.device == dev, f"weights on {dev}"
+    _, xs = _rows(x, "x", dt, dev)
+    if norm_weight is not None:
+        _vector(norm_weight, "norm_weight", H, dt, dev)
+    os_, rs = _ends(out, residual, R, H, dt, dev)
     lib = load()
-    xp, xs = _rows(x, "x", dt, dev)
-    out, op, os_, rp, rs = _out(out, residual, R, H, dt, dev)
-    # every call has its own (from torch's caching allocator, in stream order): nothing is shared
-    ws = torch.empty(lib.mi_q8_mlp_workspace_size(R, H, inter), dtype=torch.uint8, device=dev)
-    call(dev.index, lib.mi_q8_mlp, _lib.DTYPES[dt], xp, xs,
-         _vector(norm_weight, "norm_weight", H, dt, dev) if norm_weight is not None else None,
-         float(eps), gate_up.data.data_ptr(), gate_up.scale.data_ptr(), down.data.data_ptr(),
-         down.scale.data_ptr(), rp, rs, op, os_, R, H, inter, ws.data_ptr(), ws.numel())
-    return out
+    return (dev.index, lib.mi_q8_mlp, _lib.DTYPES[dt], R, H, inter,
+            lib.mi_q8_mlp_workspace_size(R, H, inter), xs, rs, os_)

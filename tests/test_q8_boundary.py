@@ -37,10 +37,10 @@ def _quantize(**over):
 
 
 def _norm(**over):
-    a = dict(dtype=0, x=16, xs=64, y=16, ys=64, weight=16, eps=1e-6, r=16, rs=64, values=16, scale=16,
-             rows=3, n=64)
+    a = dict(x=16, xs=64, y=16, ys=64, weight=16, r=16, rs=64, values=16, scale=16, dtype=0, rows=3, n=64,
+             eps=1e-6)
     a.update(over)
-    return q8.load().mi_q8_add_rmsnorm(*a.values(), None)
+    return q8.load().mi_q8_add_rmsnorm(q8.NORM_ARGS.pack(*(v or 0 for v in a.values())), None)
 
 
 def _dequantize(**over):
@@ -55,25 +55,22 @@ def _pack(**over):
     return q8.load().mi_q8_pack(*a.values(), None)
 
 
-def _matmul(**over):
-    a = dict(dtype=0, values=16, scale=16, w=16, ws=16, bias=None, res=None, rs=0, out=1 << 30, os=48,
-             rows=3, n=48, k=64)
-    a.update(over)
-    return q8.load().mi_q8_matmul(*a.values(), None)
-
-
 def _linear(**over):
-    a = dict(dtype=0, x=16, xs=64, norm=None, eps=0.0, w=16, ws=16, bias=None, res=None, rs=0,
-             out=1 << 30, os=48, rows=3, n=48, k=64, space=16, size=1 << 30)
+    a = dict(x=16, xs=64, scale=None, norm=None, w=16, ws=16, bias=None, res=None, rs=0, out=1 << 30, os=48,
+             space=16, size=1 << 30, dtype=0, rows=3, n=48, k=64, eps=0.0)
     a.update(over)
-    return q8.load().mi_q8_linear(*a.values(), None)
+    return q8.load().mi_q8_linear(q8.LINEAR_ARGS.pack(*(v or 0 for v in a.values())), None)
+
+
+def _matmul(**over):
+    return _linear(**{"scale": 16, **over})
 
 
 def _mlp(**over):
-    a = dict(dtype=0, x=16, xs=64, norm=None, eps=0.0, gu=16, gus=16, down=16, downs=16, res=None,
-             rs=0, out=1 << 30, os=64, rows=3, hidden=64, inter=96, space=16, size=1 << 30)
+    a = dict(x=16, xs=64, norm=None, gu=16, gus=16, down=16, downs=16, res=None, rs=0, out=1 << 30, os=64,
+             space=16, size=1 << 30, dtype=0, rows=3, hidden=64, inter=96, eps=0.0)
     a.update(over)
-    return q8.load().mi_q8_mlp(*a.values(), None)
+    return q8.load().mi_q8_mlp(q8.MLP_ARGS.pack(*(v or 0 for v in a.values())), None)
 
 
 @pytest.mark.parametrize("call,over,status,msg", [
@@ -97,7 +94,8 @@ def _mlp(**over):
         (dict(w=None), 1, "w is NULL"), (dict(w=8), 1, "16-byte"), (dict(ws=None), 1, "w_scale is NULL"),
         (dict(bias=3), 1, "bias"), (dict(res=16, rs=47), 1, "residual row stride"),
         (dict(out=None), 1, "out is NULL"), (dict(os=47), 1, "out row stride")]] + [
-    (_matmul, dict(values=None), 1, "values is NULL"), (_matmul, dict(scale=None), 1, "scale is NULL"),
+    (_matmul, dict(x=None), 1, "x is NULL"), (_matmul, dict(x=24), 1, "16-byte"),
+    (_matmul, dict(scale=18), 1, "x_scale is not 4-byte"),
     (_linear, dict(x=None), 1, "x is NULL"), (_linear, dict(norm=3), 1, "norm_weight"),
     (_linear, dict(out=16), 1, "overlaps"), (_linear, dict(out=16 + 2 * (2 * 64 + 63)), 1, "overlaps"),
     (_linear, dict(x=1 << 30, out=(1 << 30) - 2 * (2 * 48 + 47)), 1, "overlaps"),
@@ -112,6 +110,31 @@ def _mlp(**over):
 def test_refusals(call, over, status, msg):
     assert call(**over) == status
     assert msg in last()
+
+
+def test_arguments_that_are_not_there():
+    for fn in (q8.load().mi_q8_add_rmsnorm, q8.load().mi_q8_linear, q8.load().mi_q8_mlp):
+        assert fn(None, None) == 1 and "args is NULL" in last()
+
+
+STRUCTS = """
+#include <stdio.h>
+#include "mi_q8.h"
+int main() {
+  printf("%zu %zu %zu\\n", sizeof(mi_q8_norm_args), sizeof(mi_q8_linear_args), sizeof(mi_q8_mlp_args));
+  printf("%zu %zu %zu\\n", offsetof(mi_q8_norm_args, eps), offsetof(mi_q8_linear_args, eps),
+         offsetof(mi_q8_mlp_args, eps));
+}
+"""
+
+
+def test_argument_structs_are_the_headers(tmp_path):
+    (tmp_path / "s.c").write_text(STRUCTS)
+    subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    sizes, ends = (list(map(int, line.split())) for line in subprocess.run(
+        [str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.splitlines())
+    for st, size, end in zip((q8.NORM_ARGS, q8.LINEAR_ARGS, q8.MLP_ARGS), sizes, ends):
+        assert st.size == end + 4 and st.size <= size < st.size + 8   # (the struct ends aligned)
 
 
 def test_empty_calls_are_no_ops():
@@ -130,9 +153,9 @@ def test_sizes():
     assert lib.mi_q8_packed_bytes(0, 5, 0) == 0 and lib.mi_q8_packed_bytes(5, 131073, 0) == 0
     for rows in (300, 5000):
         # rows in 8 bits and their scales; the feed-forward block's activation in fp32 and 8 bits beside
-        assert lib.mi_q8_linear_workspace_size(rows, 2048, 1001) >= rows * (1024 + 4)
+        assert lib.mi_q8_linear_workspace_size(rows, 1001) >= rows * (1024 + 4)
         assert lib.mi_q8_mlp_workspace_size(rows, 1536, 8960) >= rows * (1536 + 8960 * 5 + 8)
-    assert lib.mi_q8_linear_workspace_size(0, 5, 5) == 0 and lib.mi_q8_mlp_workspace_size(1, 0, 5) == 0
+    assert lib.mi_q8_linear_workspace_size(0, 5) == 0 and lib.mi_q8_mlp_workspace_size(1, 0, 5) == 0
     # sizes past 32 bits
     assert lib.mi_q8_mlp_workspace_size(1 << 21, 1536, 8960) > (1 << 21) * 8960 * 5
     assert lib.mi_q8_packed_bytes(1 << 24, 131072, 0) == 1 << 41
