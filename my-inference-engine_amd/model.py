@@ -32,6 +32,10 @@ token reaches the logits.  The reference runs each admitted prompt as a forward 
 Rows that share the blocks of one history (KVCache.fork), a step's metadata says which, go to
 kernels.shared.fa2_paged_shared, which reads the shared blocks once.
 
+quantize_() holds the projections in 8 bits, one scale for each out feature, and every product's rows too, one
+scale each (kernels.q8): a step then reads half the weight bytes and its products run at the 8-bit matrix
+rate.  The residual stream, attention and the cache stay in 16 bits.
+
 On CPU tensors the model takes the reference's own fallback (dense read + fp32 SDPA with the
 bottom-right mask, model.py:104-107,181-195), which only the CPU tests of the scheduler use; the
 attention kernels themselves have no CPU path.
@@ -43,7 +47,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
 
-from kernels import few_rows
+from kernels import few_rows, q8
 from kernels.fa2 import fa2_paged, fa2_paged_varlen
 from kernels.model_ops import add_rmsnorm, silu_mul
 from kernels.rope import rope_kv_write
@@ -153,6 +157,20 @@ def sdpa_fallback(q, k, v, starts, n_rep):
     return F.scaled_dot_product_attention(q, k, v, attn_mask=mask)
 
 
+class Linear8(nn.Module):
+    """An nn.Linear whose weight is held in 8 bits (kernels.q8.Weight): what Qwen2ForCausalLM.quantize_ puts in
+    its place.  GPU only; the weight is in no state_dict and follows no .to()."""
+
+    def __init__(self, linear, gated=False):
+        super().__init__()
+        self.weight = q8.quantize_weight(linear.weight.detach(), gated)
+        self.bias = linear.bias
+
+    def forward(self, x):
+        rows = x.reshape(-1, x.shape[-1])
+        return q8.linear(rows, self.weight, bias=self.bias).view(*x.shape[:-1], self.weight.out_features)
+
+
 class Attention(nn.Module):
     def __init__(self, cfg):
         super().__init__()
@@ -210,7 +228,7 @@ class Attention(nn.Module):
     def few_rows_fit(self, x, norm):
         """Whether few_rows_step takes x [tokens, hidden]."""
         qkv, o = self.qkv_proj, self.o_proj
-        return (plain(self, norm, qkv, o) and self.cfg.head_dim == few_rows.HEAD_DIM
+        return (type(qkv) is nn.Linear and plain(self, norm, qkv, o) and self.cfg.head_dim == few_rows.HEAD_DIM
                 and few_rows.linear_fits(x, qkv.weight, norm.weight)
                 and qkv.weight.shape[0] == self.q_size + 2 * self.kv_size
                 and few_rows.bias_fits(qkv.bias, x, qkv.weight.shape[0])
@@ -227,6 +245,18 @@ class Attention(nn.Module):
                               cfg.num_heads, cfg.num_kv_heads)
         a = self._attend(q, B, T, cache, layer, meta).view(n, self.q_size)
         few_rows.linear(a, self.o_proj.weight, residual=res, out=res)
+
+    def q8_step(self, res, norm, shape, cos, sin, cache, layer, meta):
+        """few_rows_step of projections in 8 bits, for any number of tokens."""
+        cfg = self.cfg
+        (B, T, _), n = shape, res.shape[0]
+        qkv = q8.linear(res, self.qkv_proj.weight, bias=self.qkv_proj.bias, norm_weight=norm.weight,
+                        eps=cfg.rms_norm_eps)
+        q = rope_kv_write(qkv, cos[:, 0].reshape(n, cfg.head_dim), sin[:, 0].reshape(n, cfg.head_dim),
+                          meta.slot_mapping32, cache.k_pool(layer), cache.v_pool(layer), cfg.num_heads,
+                          cfg.num_kv_heads)
+        a = self._attend(q, B, T, cache, layer, meta).view(n, self.q_size)
+        q8.linear(a, self.o_proj.weight, residual=res, out=res)
 
     def _attend_packed(self, q, cache, layer, meta):
         """q [N, Hq, d] packed queries of a mixed step -> [N, Hq, d]: the leading one-token rows
@@ -275,6 +305,10 @@ class MLP(nn.Module):
         self.down_proj = nn.Linear(cfg.intermediate_size, cfg.hidden_size, bias=False)
 
     def forward(self, x):
+        if type(self.gate_up_proj) is Linear8:
+            assert plain(self.gate_up_proj, self.down_proj), "the block's projections in 8 bits run as one"
+            rows = x.reshape(-1, x.shape[-1])
+            return q8.mlp(rows, self.gate_up_proj.weight, self.down_proj.weight).view(x.shape)
         if x.is_cuda:
             rows = x.reshape(-1, x.shape[-1])
             if few_rows.mlp_pays(*rows.shape) and self.few_rows_fit(rows):
@@ -290,7 +324,7 @@ class MLP(nn.Module):
     def few_rows_fit(self, x, norm=None):
         """Whether few_rows.mlp does this module's work on x [tokens, hidden] (after `norm`)."""
         gu, down = self.gate_up_proj, self.down_proj
-        if not plain(gu, down, *((self, norm) if norm is not None else ())):
+        if type(gu) is not nn.Linear or not plain(gu, down, *((self, norm) if norm is not None else ())):
             return False
         gw, dw = gu.weight, down.weight
         return (gu.bias is None and down.bias is None and inference(x, gw, dw)
@@ -310,7 +344,7 @@ class Block(nn.Module):
         return x + self.mlp(self.post_attention_layernorm(x))
 
 
-_PLAIN = (nn.Linear, RMSNorm, Attention, MLP, Block)   # what plain() knows
+_PLAIN = (nn.Linear, Linear8, RMSNorm, Attention, MLP, Block)   # what plain() knows
 
 
 class Qwen2ForCausalLM(nn.Module):
@@ -322,6 +356,7 @@ class Qwen2ForCausalLM(nn.Module):
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2).float() / cfg.head_dim))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
+        self.quantized, self.head8 = False, None   # quantize_
 
     @torch.no_grad()
     def init_random(self, std=0.02, seed=0):
@@ -333,6 +368,24 @@ class Qwen2ForCausalLM(nn.Module):
             else:
                 prm.copy_(torch.randn(prm.shape, generator=g, device=prm.device,
                                       dtype=torch.float32).mul_(std).to(prm.dtype))
+        return self
+
+    @torch.no_grad()
+    def quantize_(self, lm_head=False):
+        """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head) in 8
+        bits from now on; their 16-bit weights are let go.  The model is on the GPU, in bf16 or fp16; graphs
+        captured before replay the old weights."""
+        held = [(m, name) for layer in self.layers
+                for m, name in ((layer.self_attn, "qkv_proj"), (layer.self_attn, "o_proj"),
+                                (layer.mlp, "gate_up_proj"), (layer.mlp, "down_proj"))]
+        old = [getattr(m, name) for m, name in held]
+        assert all(type(linear) is nn.Linear and plain(linear) for linear in old), \
+            "projections that are nn.Linear with nothing hooked on"
+        new = [Linear8(linear, name == "gate_up_proj") for (_, name), linear in zip(held, old)]
+        self.head8 = q8.quantize_weight(self.embed_tokens.weight.detach()) if lm_head else None
+        for (m, name), linear in zip(held, new):
+            setattr(m, name, linear)
+        self.quantized = True
         return self
 
     def rope_cos_sin(self, position_ids, dtype):
@@ -367,6 +420,10 @@ class Qwen2ForCausalLM(nn.Module):
         x = self.run_layers(x, cos, sin, cache, meta)
         x, w = x[:, -1:], self.embed_tokens.weight
         rows = x.reshape(-1, x.shape[-1])
+        if (self.head8 is not None and plain(self.norm) and inference(x, w, self.norm.weight)
+                and self._own("lm_head")):
+            return q8.linear(rows, self.head8, norm_weight=self.norm.weight,
+                             eps=self.norm.eps).view(*x.shape[:-1], w.shape[0])
         if (x.is_cuda and rows.shape[0] <= few_rows.MAX_NORM_ROWS and plain(self.norm)
                 and inference(x, w, self.norm.weight)
                 and self._own("lm_head") and few_rows.linear_fits(rows, w, self.norm.weight)):
@@ -381,6 +438,8 @@ class Qwen2ForCausalLM(nn.Module):
     def lm_head(self, x):
         """Tied-embedding logits (model.py:204-207)."""
         w = self.embed_tokens.weight
+        if self.head8 is not None:
+            return q8.linear(x.reshape(-1, x.shape[-1]), self.head8).view(*x.shape[:-1], w.shape[0])
         if x.is_cuda:
             rows = x.reshape(-1, x.shape[-1])
             if (few_rows.linear_pays(rows.shape[0], w) and inference(x, w)
@@ -407,6 +466,13 @@ class Qwen2ForCausalLM(nn.Module):
                 few_rows.mlp(res, mlp.gate_up_proj.weight, mlp.down_proj.weight, residual=res,
                              norm_weight=norm.weight, eps=eps, out=res)
             return res.view(shape)
+        if self._q8_fit(res):
+            for i, layer in enumerate(self.layers):
+                layer.self_attn.q8_step(res, layer.input_layernorm, shape, cos, sin, cache, i, meta)
+                norm, mlp = layer.post_attention_layernorm, layer.mlp
+                q8.mlp(res, mlp.gate_up_proj.weight, mlp.down_proj.weight, residual=res,
+                       norm_weight=norm.weight, eps=eps, out=res)
+            return res.view(shape)
         _, h = add_rmsnorm(res, self.layers[0].input_layernorm.weight, eps)
         for i, layer in enumerate(self.layers):
             a = layer.self_attn(h.view(shape), cos, sin, cache, i, meta).reshape(-1, H)
@@ -427,6 +493,15 @@ class Qwen2ForCausalLM(nn.Module):
                 and all(layer.self_attn.few_rows_fit(res, layer.input_layernorm)
                         and layer.mlp.few_rows_fit(res, layer.post_attention_layernorm)
                         for layer in self.layers))
+
+    def _q8_fit(self, res):
+        """Whether every layer of a step over res [tokens, hidden] runs on the 8-bit kernels' own norms and residual
+        adds."""
+        return (self.quantized
+                and inference(res, *(self.parameters() if torch.is_grad_enabled() else ()))
+                and all(plain(layer.self_attn, layer.input_layernorm, layer.post_attention_layernorm, layer.mlp,
+                              layer.self_attn.qkv_proj, layer.self_attn.o_proj, layer.mlp.gate_up_proj,
+                              layer.mlp.down_proj) for layer in self.layers))
 
     def forward_mixed(self, rows, cache, seqs):
         """One packed step: rows[b] (a list of token ids, at least one) is appended to cache
