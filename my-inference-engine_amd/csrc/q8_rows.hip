@@ -298,9 +298,9 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
 
 // A tile of NP panels by 16 MT tokens a work-group, its 8 waves' shares of K each from memory straight into
 // the MFMAs: nothing is shared but the sums, so there is no barrier before the last.
-template <typename E, int MT, int NP, bool GATED>
+template <typename E, int MT, int NP, int D, bool GATED>
 __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p) {
-  constexpr int U = NP * MT, D = 3;
+  constexpr int U = NP * MT;
   __shared__ i32x4 red[kQrWaves][U][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -373,7 +373,7 @@ hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
     go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, HALF>);
   else if (p.Kp <= kQ8KeepK)
     go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, HALF>);
-  else if constexpr (SRC == kQ8Rows)
+  else if constexpr (SRC == kQ8Rows && MT < 4)   // (q8_plan: no more than 32 rows of these)
     go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF>);
   else
     return hipErrorInvalidValue;
@@ -408,15 +408,16 @@ hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t s
 hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream) {
   const dim3 grid(plan.tiles), block(kQrThreads);
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p); };
-  if (plan.kernel == kQ8Tile64) {
-    if (gated) go(q8_tile_kernel<BF16, 4, 4, true>);
-    else if (dtype == 0) go(q8_tile_kernel<BF16, 4, 4, false>);
-    else go(q8_tile_kernel<FP16, 4, 4, false>);
-  } else {
-    if (gated) go(q8_tile_kernel<BF16, 2, 4, true>);
-    else if (dtype == 0) go(q8_tile_kernel<BF16, 2, 4, false>);
-    else go(q8_tile_kernel<FP16, 2, 4, false>);
-  }
+  const auto sized = [&](auto type, auto gate) {
+    using E = decltype(type);
+    constexpr bool kGated = decltype(gate)::value;
+    if (plan.kernel == kQ8Tile32x32) go(q8_tile_kernel<E, 2, 2, 4, kGated>);
+    else if (plan.kernel == kQ8Tile32x64) go(q8_tile_kernel<E, 2, 4, 3, kGated>);
+    else go(q8_tile_kernel<E, 4, 4, 3, kGated>);
+  };
+  if (gated) sized(BF16{}, std::true_type{});
+  else if (dtype == 0) sized(BF16{}, std::false_type{});
+  else sized(FP16{}, std::false_type{});
   return hipGetLastError();
 }
 

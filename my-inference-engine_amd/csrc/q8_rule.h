@@ -13,42 +13,59 @@ constexpr int kQ8KeepK = 2048;    // (padded) in features whose rows it keeps in
 constexpr int kQ8FusedMax = 16;   // rows that it brings to 8 bits itself, of at most kQ8KeepK
 constexpr int kQ8FloatMax = 4, kQ8FloatK = 12288;   // fp32 rows that it does, and their most features
 
-enum Q8Kernel { kQ8FewRows = 0, kQ8Tile32 = 1, kQ8Tile64 = 2, kQ8Gemm64 = 3, kQ8Gemm128 = 4 };
+enum Q8Kernel { kQ8FewRows, kQ8Tile32x32, kQ8Tile32x64, kQ8Tile64x64, kQ8Gemm64, kQ8Gemm128 };
 
 struct Q8Plan {
   int32_t kernel;   // Q8Kernel
   int32_t tiles;    // work-groups
 };
 
-// The tile kernel (32 or 64 tokens by 64 features, K split over the work-group's waves, straight from
-// memory) hides the most latency but reads x and W once for every tile that needs them: it is taken while
-// its tiles are no more than the 256 CUs.  Behind that the products that share operands through LDS:
-// 64 x 64 tiles until there are enough of 128 x 128 for every CU.  Measured (us, 32 x 64 / 64 x 64 straight from
-// memory, 64 x 64 / 128 x 128 through LDS):
-//   tokens x features x K: 96 x 1536 x 8960 12.1 16.9 22.5 39;  512 x 1536 x 8960 22.3 18.3 22.9 41;
-//   1024 x 1536 x 8960 37.0 35.4 26.9 42;  256 x 2048 x 1536 5.2 6.3 6.4 11;  400 x 2048 x 1536 7.3 6.6 6.6 11;
-//   1024 x 2048 x 1536 13.6 13.1 8.5 12;  4096 x 2048 x 1536 - - 25.7 20.0;  150 x 17920 x 1536 19.4 23.6 13.6
-//   14.8;  512 x 17920 x 1536 48 51 28.2 25.2
+// Three families.  The few-row kernel streams W once past 16 to 64 tokens.  The tile kernel (32 or 64 tokens by 32
+// or 64 features, K split over the work-group's waves, operands straight from memory) hides the most latency,
+// but reads x and W again for every tile that needs them: it is taken while its tiles are no more than the 256
+// CUs.  Behind both, the products that share operands through LDS: 64 x 64 tiles until there are enough of
+// 128 x 128 for every CU.  Measured (us; few-row, 32 x 32, 32 x 64, 64 x 64 in LDS, 128 x 128 in LDS):
+//   tokens x features x K        few    32x32  32x64  64L    128L
+//   17 x 2048 x 1536             3.5    4.8    5.2    6.0    9.7
+//   32 x 1536 x 8960             7.9    10.0   12.5   22.1   38.4
+//   32 x 6144 x 4096             9.8    7.9    8.9    12.0   20.3
+//   32 x 14336 x 4096            15.8   13.1   12.6   13.2   20.8
+//   64 x 6144 x 2048             7.1    7.8    7.6    8.2    12.8
+//   64 x 9728 x 896              7.1    8.8    7.8    5.3    8.1
+//   64 x 17920 x 1536            9.7    14.2   11.8   8.8    12.0
+//   64 x 151936 x 1536           67     102    78     55     49
+//   64 x 1536 x 8960             11.3   10.0   12.4   22.2   38.9
+//   150 x 896 x 4864             -      7.7    9.3    13.8   26.6
+//   256 x 1536 x 8960            -      16.7   13.1   22.6   45.3
+//   512 x 17920 x 1536           -      -      48     28.2   25.2
+// (512 x 1536 x 8960: 64 x 64 straight from memory 18.3, through LDS 22.9; 400 x 2048 x 1536 6.6 both.)
 inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
   constexpr int64_t kCus = 256;
-  (void)kp;
-  const auto tiles = [&](int tm, int np) {
-    return (int64_t)((rows + tm - 1) / tm) * ((panels + np - 1) / np);
+  const auto plan = [&](Q8Kernel kernel, int tm, int np) {
+    return Q8Plan{kernel, (int32_t)((int64_t)((rows + tm - 1) / tm) * ((panels + np - 1) / np))};
   };
+  const Q8Plan t32x32 = plan(kQ8Tile32x32, 32, 2), t32x64 = plan(kQ8Tile32x64, 32, 4),
+               t64x64 = plan(kQ8Tile64x64, 64, 4), g64 = plan(kQ8Gemm64, 64, 4),
+               g128 = plan(kQ8Gemm128, 128, 8);
 #ifdef Q8_TUNE
-  if (getenv("Q8_NP") && (rows > 64 || atoi(getenv("Q8_NP")))) {
+  if (getenv("Q8_NP")) {
     const int np = atoi(getenv("Q8_NP"));
-    if (np == 1) return {kQ8Tile32, (int32_t)tiles(32, 4)};
-    if (np == 2) return {kQ8Tile64, (int32_t)tiles(64, 4)};
-    if (np == 4) return {kQ8Gemm64, (int32_t)tiles(64, 4)};
-    if (np == 8) return {kQ8Gemm128, (int32_t)tiles(128, 8)};
+    if (np == 1) return t32x32;
+    if (np == 2) return t32x64;
+    if (np == 3) return t64x64;
+    if (np == 4) return g64;
+    if (np == 8) return g128;
   }
 #endif
-  if (rows <= kQ8RowsMax) return {kQ8FewRows, 0};
-  if (tiles(32, 4) <= kCus) return {kQ8Tile32, (int32_t)tiles(32, 4)};
-  if (tiles(64, 4) <= kCus) return {kQ8Tile64, (int32_t)tiles(64, 4)};
-  if (tiles(128, 8) < kCus) return {kQ8Gemm64, (int32_t)tiles(64, 4)};
-  return {kQ8Gemm128, (int32_t)tiles(128, 8)};
+  const bool keep = kp <= kQ8KeepK;
+  if (rows <= 16) return {kQ8FewRows, 0};
+  if (rows <= kQ8RowsMax && (keep ? panels <= 512 : rows <= 32 && panels < 256)) return {kQ8FewRows, 0};
+  if (rows > kQ8RowsMax || !keep) {
+    if (t32x32.tiles <= kCus) return t32x32;
+    if (t32x64.tiles <= kCus) return t32x64;
+    if (t64x64.tiles <= kCus && !keep) return t64x64;
+  }
+  return g128.tiles < kCus ? g64 : g128;
 }
 
 }  // namespace mi_fa2

@@ -205,7 +205,8 @@ def check_product(out, rows, values, scale, bias, residual, extra=0.0):
 PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96), (16, 1536, 1536), (17, 100, 640),
             (31, 777, 1001), (33, 130, 200), (48, 64, 8960), (64, 2048, 1536), (65, 33, 300),
             (100, 128, 256), (127, 250, 128), (129, 257, 1000), (150, 896, 4864), (200, 1024, 64),
-            (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72)]
+            (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
+            (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -271,7 +272,7 @@ def mlp_bounds(rows, gate_up, gate_up_scale, down, down_scale):
 
 MLPS = [(1, 1536, 8960), (1, 64, 8), (2, 100, 36), (16, 1536, 8960), (5, 128, 17), (17, 896, 4864),
         (33, 300, 500), (64, 256, 1000), (65, 512, 1024), (150, 896, 4864), (260, 640, 1531),
-        (515, 256, 768)]
+        (515, 256, 768), (130, 512, 1100), (400, 2176, 750), (40, 64, 4201), (600, 128, 3500)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
