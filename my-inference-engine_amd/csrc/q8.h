@@ -76,9 +76,10 @@ __device__ __forceinline__ float q8_scale(const Q8Factor& r, float inv) {
   return r.bad ? __builtin_nanf("") : r.most * inv / 127.f;
 }
 // Four values, lowest byte first.  v f is rounded to the nearest whole number, ties to even, by the
-// addition of 1.5 * 2^23, whose last place is 1: its low byte is the number's (two's complement).  EXACT: for rows
-// as they are, whose values are short numbers and can lie halfway between two whole ones (one row in 128 has a
-// largest magnitude that is a multiple of 127); f alone, rounded, would send them to either side.
+// addition of 1.5 * 2^23, whose last place is 1: its low byte is the number's (two's complement).  EXACT: for 16-bit
+// rows and their products with a norm's weight, which are short numbers and can lie halfway between two whole ones
+// (one row in 128 has a largest magnitude that is a multiple of 127; 4 of 89,600 values of a drawn fp16 case); f
+// alone, rounded, would send those to either side.
 template <bool EXACT>
 __device__ __forceinline__ uint32_t q8_whole(float v, const Q8Factor& r) {
 #pragma clang fp contract(off)

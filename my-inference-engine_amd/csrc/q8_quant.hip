@@ -156,7 +156,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
   if (tid == 0)
     p.scale[row] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.n + p.eps) : 1.f);
   const auto store = [&](int c, const float (&v)[8]) {
-    const u32x2 o = {q8_pack4<SRC == kQ8Plain>(v[0], v[1], v[2], v[3], f), q8_pack4<SRC == kQ8Plain>(v[4], v[5], v[6], v[7], f)};
+    const u32x2 o = {q8_pack4<SRC != kQ8Float>(v[0], v[1], v[2], v[3], f), q8_pack4<SRC != kQ8Float>(v[4], v[5], v[6], v[7], f)};
     *reinterpret_cast<u32x2*>(p.q + q8_at(row, c, p.np)) = o;
   };
   if constexpr (PER > 0) {

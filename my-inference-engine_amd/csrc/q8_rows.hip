@@ -168,8 +168,8 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
         const int c = tid + k * kQrThreads;
         if (8 * c < p.Kp)
           *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
-              u32x2{q8_pack4<SRC == kQ8Plain>(v[m][k][0][0], v[m][k][0][1], v[m][k][0][2], v[m][k][0][3], f),
-                    q8_pack4<SRC == kQ8Plain>(v[m][k][1][0], v[m][k][1][1], v[m][k][1][2], v[m][k][1][3], f)};
+              u32x2{q8_pack4<SRC != kQ8Float>(v[m][k][0][0], v[m][k][0][1], v[m][k][0][2], v[m][k][0][3], f),
+                    q8_pack4<SRC != kQ8Float>(v[m][k][1][0], v[m][k][1][1], v[m][k][1][2], v[m][k][1][3], f)};
       }
     }
     __syncthreads();
@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
           const int c = lane + 64 * k;
           if (8 * c < p.Kp)
             *reinterpret_cast<u32x2*>(pieces + (c >> 1) * kPiece + m * 16 + (c & 1) * 8) =
-                u32x2{q8_pack4<SRC == kQ8Plain>(v[h][k][0], v[h][k][1], v[h][k][2], v[h][k][3], f),
-                      q8_pack4<SRC == kQ8Plain>(v[h][k][4], v[h][k][5], v[h][k][6], v[h][k][7], f)};
+                u32x2{q8_pack4<SRC != kQ8Float>(v[h][k][0], v[h][k][1], v[h][k][2], v[h][k][3], f),
+                      q8_pack4<SRC != kQ8Float>(v[h][k][4], v[h][k][5], v[h][k][6], v[h][k][7], f)};
         }
       }
     };

@@ -154,12 +154,18 @@ def test_ties_go_to_the_even_number(step):
     got = q8.quantize(x)
     assert got.scale.item() == step / 2.0 ** 6
     assert torch.equal(got.values[0].cpu().double(), want)
+    # normalised, by a weight of one
+    one = torch.ones(255, dtype=torch.float16, device=DEV)
+    _, normed = q8.add_rmsnorm(x, one, 1e-6)
+    assert torch.equal(normed.values[0].cpu().double(), want)
     # the same in the launch of a product: a weight of ones in one place each gives the values back
     eye = torch.eye(256, dtype=torch.int8)[:, :255].contiguous()
     w = q8.Weight(eye.to(DEV), torch.full((256,), 2.0 ** 6 / step, device=DEV))
     for rows in (x, x.repeat(40, 1)):
         out = q8.linear(rows, w).cpu().double()
         assert torch.equal(out[:, :255], want.expand(len(rows), -1))
+        out = q8.linear(rows, w, norm_weight=one, eps=1e-6)
+        assert torch.equal(out, q8.linear(q8.add_rmsnorm(rows, one, 1e-6)[1], w))
 
 
 @pytest.mark.parametrize("gated", [False, True])
