@@ -137,6 +137,35 @@ typedef struct mi_q8_mlp_args {
 MI_Q8_API size_t mi_q8_mlp_workspace_size(int32_t rows, int32_t hidden, int32_t inter);
 MI_Q8_API int mi_q8_mlp(const mi_q8_mlp_args* args, void* stream);
 
+/*
+ * The q/k/v projection of a decode step's few rows with what surrounds it, mi_model_qkv_rope's contract on a
+ * weight in 8 bits: (q | k | v) = rmsnorm(x) W^T + bias, rounded, w packed [(heads_q + 2 heads_kv) * 128,
+ * hidden]; rotated q to q_out [rows, heads_q * 128], rotated k and v to the cache slot of each token (a slot
+ * outside [0, num_slots) writes nothing).  rows <= 16, hidden <= 2048; cos, sin [rows, 128]; k_pool, v_pool
+ * [num_slots, heads_kv, 128] with these slot and head strides in elements.  Bitwise mi_q8_linear and
+ * mi_fa2_rope_kv_write.
+ */
+typedef struct mi_q8_qkv_rope_args {
+  const void* x;
+  int64_t x_stride;
+  const void* norm_weight;
+  const void* w;
+  const float* w_scale;
+  const void* bias;
+  const void* cos;
+  const void* sin;
+  int64_t cs_stride;
+  const int32_t* slot_mapping;
+  void* q_out;
+  int64_t q_stride;
+  void* k_pool;
+  void* v_pool;
+  int64_t pool_slot_stride, pool_head_stride;
+  int32_t dtype, rows, hidden, heads_q, heads_kv, num_slots;
+  float eps;
+} mi_q8_qkv_rope_args;
+MI_Q8_API int mi_q8_qkv_rope(const mi_q8_qkv_rope_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -193,9 +193,20 @@ struct Q8Params {
   int64_t out_st;
   int32_t M, N, K, Kp;    // N: out features (gated: of the activation)
   int32_t panels;
+  // q/k/v with what follows (few rows): rotary tables [M][cs_st], 128 used, each token's cache slot, one
+  // layer of the pools; out is the rotated q
+  const uint16_t* cos;
+  const uint16_t* sin;
+  int64_t cs_st;
+  const int32_t* slots;
+  uint16_t* k_pool;
+  uint16_t* v_pool;
+  int64_t pool_st, pool_sh;
+  int32_t num_slots, Hq, Hkv;
 };
 hipError_t launch_q8_rows(const Q8Params& p, int dtype, bool gated, int source, int n_cus,
                           hipStream_t stream);
+hipError_t launch_q8_qkv_rope(const Q8Params& p, int dtype, int n_cus, hipStream_t stream);
 hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream);
 hipError_t launch_q8_gemm(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream);
 

@@ -404,4 +404,53 @@ int mi_q8_mlp(const mi_q8_mlp_args* args, void* stream) {
   return product(d, a.dtype, false, ws + sp.a.values, a_scale, stream);
 }
 
+int mi_q8_qkv_rope(const mi_q8_qkv_rope_args* args, void* stream) {
+  if (!args) return fail(kInvalid, "args is NULL");
+  const mi_q8_qkv_rope_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (int rc = check_count("rows", a.rows, 0, mi_fa2::kQ8FusedMax)) return rc;
+  if (int rc = check_count("hidden", a.hidden, 1, mi_fa2::kQ8KeepK)) return rc;
+  if (int rc = check_count("heads_q", a.heads_q, 1, 4096)) return rc;
+  if (int rc = check_count("heads_kv", a.heads_kv, 1, 4096)) return rc;
+  if (int rc = check_count("num_slots", a.num_slots, 0, INT32_MAX)) return rc;
+  if (a.rows == 0) return ok();
+  const int d = mi_fa2::kHeadDim;
+  if (int rc = check_rows("x", a.x, a.x_stride, a.hidden)) return rc;
+  if (int rc = check_ptr("norm_weight", a.norm_weight, 2)) return rc;
+  if (int rc = check_weight("w", a.w, a.w_scale)) return rc;
+  if (a.bias)
+    if (int rc = check_ptr("bias", a.bias, 2)) return rc;
+  if (int rc = check_rows("cos", a.cos, a.cs_stride, d)) return rc;
+  if (int rc = check_rows("sin", a.sin, a.cs_stride, d)) return rc;
+  if (int rc = check_ptr("slot_mapping", a.slot_mapping, 4)) return rc;
+  if (int rc = check_rows("q_out", a.q_out, a.q_stride, (int64_t)a.heads_q * d)) return rc;
+  if (int rc = check_ptr("k_pool", a.k_pool, 2)) return rc;
+  if (int rc = check_ptr("v_pool", a.v_pool, 2)) return rc;
+  if (a.pool_slot_stride < d || a.pool_head_stride < d)
+    return fail(kInvalid, "pool strides %lld, %lld: at least %d", (long long)a.pool_slot_stride,
+                (long long)a.pool_head_stride, d);
+  if (overlap(a.x, span(a.rows, a.x_stride, a.hidden), a.q_out, span(a.rows, a.q_stride, a.heads_q * d)))
+    return fail(kInvalid, "q_out overlaps x");
+  Q8Params p = operands(a.w, a.w_scale, a.bias, nullptr, 0, a.q_out, a.q_stride, a.rows,
+                        (a.heads_q + 2 * a.heads_kv) * d, a.hidden, false);
+  p.x = a.x;
+  p.x_st = a.x_stride;
+  p.norm_w = static_cast<const uint16_t*>(a.norm_weight);
+  p.eps = a.eps;
+  p.cos = static_cast<const uint16_t*>(a.cos);
+  p.sin = static_cast<const uint16_t*>(a.sin);
+  p.cs_st = a.cs_stride;
+  p.slots = a.slot_mapping;
+  p.k_pool = static_cast<uint16_t*>(a.k_pool);
+  p.v_pool = static_cast<uint16_t*>(a.v_pool);
+  p.pool_st = a.pool_slot_stride;
+  p.pool_sh = a.pool_head_stride;
+  p.num_slots = a.num_slots;
+  p.Hq = a.heads_q;
+  p.Hkv = a.heads_kv;
+  int cus = 0;
+  if (int rc = compute_units(&cus)) return rc;
+  return launched(mi_fa2::launch_q8_qkv_rope(p, a.dtype, cus, reinterpret_cast<hipStream_t>(stream)));
+}
+
 }  // extern "C"

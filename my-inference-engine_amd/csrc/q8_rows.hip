@@ -69,16 +69,68 @@ __device__ __forceinline__ void finish(const Q8Params& p, int f, int m, int g, b
   }
 }
 
+// A value rounded to the tensor type.
+template <typename E>
+__device__ __forceinline__ float rounded(float x) { return E::lo(E::pack2(x, 0.f) & 0xffffu); }
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// The sums of a rotation tile (kQrPairs) with token m: dims d .. d + 3 of a head, the lower halves of the
+// pairs in lane groups g = 0, 1, the upper in 2, 3.  The projection is rounded, rotated (rounded where the
+// model's separate tensor operations round: model.py:58-65) and goes to q or to the token's cache slot.
+template <typename E>
+__device__ __forceinline__ void finish_rope(const Q8Params& p, int tile, int m, int g, float xs, i32x4 s) {
+  const int head = tile >> 3, d = 8 * (tile & 7) + 4 * (g & 1) + 64 * (g >> 1), f = head * kHeadDim + d;
+  const f32x4 ws = *reinterpret_cast<const f32x4_4*>(p.w_scale + f);
+  float o[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = q8_scaled(s[r], xs, ws[r]);
+  if (p.bias) add4<E>(o, *reinterpret_cast<const u32x2_2*>(p.bias + f));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = rounded<E>(o[r]);
+  const bool live = m < p.M;
+  if (head < p.Hq + p.Hkv) {
+    const int64_t at = (int64_t)(live ? m : 0) * p.cs_st + d;
+    const u32x2 cv = *reinterpret_cast<const u32x2_2*>(p.cos + at), sv = *reinterpret_cast<const u32x2_2*>(p.sin + at);
+    float other[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) other[r] = __shfl_xor(o[r], 32);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      // d < 64: x[d] cos[d] - x[d + 64] sin[d];  d >= 64: x[d] cos[d] + x[d - 64] sin[d]
+      const float c = r & 1 ? E::hi(cv[r / 2]) : E::lo(cv[r / 2]), n = r & 1 ? E::hi(sv[r / 2]) : E::lo(sv[r / 2]);
+      o[r] = q8_plus(rounded<E>(times(o[r], c)), rounded<E>(times(g < 2 ? -other[r] : other[r], n)));
+    }
+  }
+  if (!live) return;
+  uint16_t* dst;
+  if (head < p.Hq) {
+    dst = static_cast<uint16_t*>(p.out) + (int64_t)m * p.out_st + f;
+  } else {
+    const int slot = p.slots[m];
+    if ((unsigned)slot >= (unsigned)p.num_slots) return;   // padding row
+    const int h = head - p.Hq;
+    dst = (h < p.Hkv ? p.k_pool + h * p.pool_sh : p.v_pool + (h - p.Hkv) * p.pool_sh) + slot * p.pool_st + d;
+  }
+  *reinterpret_cast<u32x2_2*>(dst) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+}
+
+// What a tile's 16 rows of W are: panels; half a panel, whose rows fill the operand twice; the 8 + 8 rows of 8
+// rotation pairs of a head of 128.
+enum RowsTile { kQrPanels, kQrHalf, kQrPairs };
+
 }  // namespace
 
 // SRC: kQ8Plain, kQ8Norm: x is 16-bit rows; kQ8Float: fp32 rows, 4 at most; kQ8Rows: rows in 8 bits.  NS:
-// steps of K (64) a wave takes at a time.  HALF: a tile is half a panel, whose rows fill the operand twice.
+// steps of K (64) a wave takes at a time.
 // FT: of fp32 rows, their most.
-template <typename E, int MT, int NP, int NS, bool GATED, int SRC, bool KEEP, bool HALF, int FT = 0>
+template <typename E, int MT, int NP, int NS, bool GATED, int SRC, bool KEEP, RowsTile TILE, int FT = 0>
 __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p) {
   static_assert(SRC == kQ8Rows || MT == 1, "rows come to 8 bits 16 at a time");
   static_assert(KEEP || SRC == kQ8Rows || SRC == kQ8Float, "");
-  static_assert(!HALF || (NP == 1 && !GATED), "");
+  static_assert(TILE == kQrPanels || (NP == 1 && !GATED), "");
   constexpr int U = NP * MT;
   __shared__ i32x4 red[2][kQrWaves][U][64];
   __shared__ float row_scale[16 * MT];
@@ -89,15 +141,19 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
   const int steps = p.Kp >> 6;
   const int lo = wave * steps / kQrWaves, hi = (wave + 1) * steps / kQrWaves;
   const int chunks = KEEP ? 1 : max(1, (hi - lo + NS - 1) / NS);
-  const int tiles = HALF ? 2 * p.panels : (p.panels + NP - 1) / NP;
+  const int tiles = TILE == kQrHalf ? 2 * p.panels : (p.panels + NP - 1) / NP;
 
   // Step i of chunk c of tile t, panel u.
   const auto load_w = [&](int t, int c, int u, int i) -> i32x4 {
-    const int panel = HALF ? t >> 1 : t * NP + u, s = lo + c * NS + i;
-    const bool live = panel < p.panels;
+    const int s = lo + c * NS + i;
+    // (rotation pairs: rows 8 (t % 8) .. + 7 of the head's 128, and those 64, four panels, on)
+    const int panel = TILE == kQrHalf ? t >> 1 : TILE == kQrPairs ? (t >> 3) * 8 + ((t & 7) >> 1) : t * NP + u;
+    const bool live = TILE == kQrPairs ? t < tiles : panel < p.panels;
+    constexpr int kPanels = TILE == kQrPairs ? 5 : 1;
     const __amdgpu_buffer_rsrc_t r =
-        make_rsrc(p.w + (int64_t)(live ? panel : 0) * 16 * p.Kp, live ? 16 * p.Kp : 0);
-    const int at = HALF ? g * 256 + (8 * (t & 1) + (n & 7)) * 16 : lane * 16;
+        make_rsrc(p.w + (int64_t)(live ? panel : 0) * 16 * p.Kp, live ? kPanels * 16 * p.Kp : 0);
+    const int at = (TILE == kQrPanels ? lane * 16 : g * 256 + (8 * (t & 1) + (n & 7)) * 16) +
+                   (TILE == kQrPairs && n >= 8 ? 64 * p.Kp : 0);
     return __builtin_bit_cast(i32x4, ld16_buf(r, s < hi ? s * 1024 + at : kQrNone));
   };
   // Rows in 8 bits: 16 tokens a panel.
@@ -192,6 +248,7 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
     first_w();
     const auto bring = [&](auto rows) {
       constexpr int R = decltype(rows)::value;
+      if (p.K != kChunks * 512)
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
 #pragma unroll
@@ -290,8 +347,13 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
 #pragma unroll
       for (int v = 1; v < kQrWaves; ++v) s += red[it & 1][v][u][lane];
       const int m = 16 * (u % MT) + n, panel = t * NP + u / MT;
-      const int f = GATED ? 8 * panel + 4 * (g & 1) : HALF ? 8 * t + 4 * (g & 1) : 16 * panel + 4 * g;
-      finish<E, GATED>(p, f, m, g, !HALF || g < 2, row_scale[m], s);
+      if constexpr (TILE == kQrPairs) {
+        finish_rope<E>(p, t, m, g, row_scale[m], s);
+      } else {
+        constexpr bool kHalf = TILE == kQrHalf;
+        const int f = GATED ? 8 * panel + 4 * (g & 1) : kHalf ? 8 * t + 4 * (g & 1) : 16 * panel + 4 * g;
+        finish<E, GATED>(p, f, m, g, !kHalf || g < 2, row_scale[m], s);
+      }
     }
   }
 }
@@ -359,22 +421,22 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p
 
 namespace {
 
-template <typename E, int MT, int NP, bool GATED, int SRC, bool HALF = false>
+template <typename E, int MT, int NP, bool GATED, int SRC, RowsTile TILE = kQrPanels>
 hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kQrThreads), 0, stream, p); };
-  constexpr int kMany = SRC == kQ8Float && HALF ? 18 : MT == 1 ? 9 : 6;
+  constexpr int kMany = SRC == kQ8Float && TILE == kQrHalf ? 18 : MT == 1 ? 9 : 6;
   if constexpr (SRC == kQ8Float) {
-    if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF, 1>);
-    else go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF, kQ8FloatMax>);
+    if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, 1>);
+    else go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, kQ8FloatMax>);
   }
   else if (p.Kp <= 1024)
-    go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, HALF>);
+    go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, TILE>);
   else if (p.Kp <= 1536)
-    go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, HALF>);
+    go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, TILE>);
   else if (p.Kp <= kQ8KeepK)
-    go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, HALF>);
+    go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, TILE>);
   else if constexpr (SRC == kQ8Rows && MT < 4)   // (q8_plan: no more than 32 rows of these)
-    go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, HALF>);
+    go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
   else
     return hipErrorInvalidValue;
   return hipGetLastError();
@@ -388,7 +450,7 @@ hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
     if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
   }
   if constexpr (!GATED)
-    if (2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, true>(p, 2 * p.panels, stream);
+    if (2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, 2 * p.panels, stream);
   if constexpr (SRC != kQ8Float)
     if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
   return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);
@@ -404,6 +466,12 @@ hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t s
 }
 
 }  // namespace
+
+hipError_t launch_q8_qkv_rope(const Q8Params& p, int dtype, int n_cus, hipStream_t stream) {
+  const int grid = std::min(p.panels, n_cus);
+  return dtype == 0 ? launch_rows_k<BF16, 1, 1, false, kQ8Norm, kQrPairs>(p, grid, stream)
+                    : launch_rows_k<FP16, 1, 1, false, kQ8Norm, kQrPairs>(p, grid, stream);
+}
 
 hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream) {
   const dim3 grid(plan.tiles), block(kQrThreads);

@@ -5,6 +5,7 @@ libmi_q8.so, the C ABI in include/mi_q8.h).
   quantize, add_rmsnorm     rows of activations in 8 bits, one scale each (Rows)
   linear                    [residual +] ([rmsnorm] x) W^T [+ bias]
   mlp                       [residual +] SwiGLU feed-forward block of [rmsnorm] x
+  qkv_rope                  rmsnorm, q/k/v projection, rotary embedding and the paged cache write
 
 They stand beside kernels.few_rows and kernels.model_ops for a model whose projections are held in 8 bits
 (Qwen2ForCausalLM.quantize_), and take any number of rows.  The reference has no such path; what surrounds the
@@ -24,12 +25,14 @@ import torch
 
 from . import _lib
 from .fa2 import _MEMO_MAX
+from .rope import HEAD_DIM, rope_kv_write
 
 LIB_PATH = Path(os.environ.get("MI_Q8_LIB", Path(__file__).resolve().parent / "libmi_q8.so"))
 
 MAX_ROWS = 1 << 21
 MAX_IN = 131072      # 128 * 127 * in stays below 2^31
 MAX_OUT = 1 << 24
+FUSED_ROWS, FUSED_IN = 16, 2048   # of qkv_rope in one launch
 
 _p, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 _sz, _args = ctypes.c_size_t, ctypes.c_char_p
@@ -46,10 +49,12 @@ SIGNATURES = {
     "mi_q8_linear": (_i32, [_args, _p]),
     "mi_q8_mlp_workspace_size": (_sz, [_i32, _i32, _i32]),
     "mi_q8_mlp": (_i32, [_args, _p]),
+    "mi_q8_qkv_rope": (_i32, [_args, _p]),
 }
 # the argument structs, packed in one go: a call of 18 arguments costs ctypes 1.9 us, this 0.6
 NORM_ARGS = struct.Struct("@PqPqPPqPPiiif")
 LINEAR_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
+QKV_ARGS = struct.Struct("@PqPPPPPPqPPqPPqqiiiiiif")
 MLP_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
 
 _library = None
@@ -350,3 +355,54 @@ def _mlp_plan(x, gate_up, down, residual, norm_weight, out):
     lib = load()
     return (dev.index, lib.mi_q8_mlp, _lib.DTYPES[dt], R, H, inter,
             lib.mi_q8_mlp_workspace_size(R, H, inter), xs, rs, os_)
+
+
+def qkv_rope(x, norm_weight, eps, w, bias, cos, sin, slot_mapping, k_pool, v_pool, heads_q, heads_kv):
+    """x [rows, hidden], w a Weight [(heads_q + 2 heads_kv) * 128, hidden], cos/sin [rows, 128], slot_mapping
+    [rows] int32, k_pool/v_pool [slots, heads_kv, 128] (one layer of KVCache.buf).  Returns the rotated queries
+    [rows, heads_q * 128]; k and v go to the rows' cache slots (a slot outside the pool: nowhere).  Up to 16 rows
+    of a hidden size up to 2048 in one launch, more through `linear` and rope_kv_write (whose rows of cos and sin
+    lie at multiples of 16 bytes), bitwise the same."""
+    assert type(w) is Weight, "w: a Weight"
+    rows, hidden = x.shape
+    if rows > FUSED_ROWS or hidden > FUSED_IN:
+        qkv = linear(x, w, bias=bias, norm_weight=norm_weight, eps=eps)
+        return rope_kv_write(qkv, cos, sin, slot_mapping, k_pool, v_pool, heads_q, heads_kv)
+    key = ("qkv", x.shape, x.stride(), x.dtype, x.device, w.sig, _sig(norm_weight), _sig(bias), _sig(cos),
+           _sig(sin), _sig(slot_mapping), _sig(k_pool), _sig(v_pool), heads_q, heads_kv)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(key, _qkv_plan, x, w, norm_weight, bias, cos, sin, slot_mapping, k_pool, v_pool, heads_q,
+                     heads_kv)
+    index, fn, code, xs, cs, pool_strides, slots, width = plan
+    q = x.new_empty((rows, width))
+    call(index, fn, QKV_ARGS.pack(
+        x.data_ptr(), xs, norm_weight.data_ptr(), w.data_ptr, w.scale_ptr,
+        bias.data_ptr() if bias is not None else 0, cos.data_ptr(), sin.data_ptr(), cs,
+        slot_mapping.data_ptr(), q.data_ptr(), width, k_pool.data_ptr(), v_pool.data_ptr(), *pool_strides,
+        code, rows, hidden, heads_q, heads_kv, slots, eps))
+    return q
+
+
+def _qkv_plan(x, w, norm_weight, bias, cos, sin, slot_mapping, k_pool, v_pool, heads_q, heads_kv):
+    dt, dev = _input(x)
+    R, H = x.shape
+    assert not w.gated and w.device == dev, f"w: a Weight on {dev} that is not gated"
+    n_out = (heads_q + 2 * heads_kv) * HEAD_DIM
+    assert w.in_features == H and w.out_features == n_out, f"w: [{n_out}, {H}]"
+    _, xs = _rows(x, "x", dt, dev)
+    _vector(norm_weight, "norm_weight", H, dt, dev)
+    if bias is not None:
+        _vector(bias, "bias", n_out, dt, dev)
+    _, cs = _rows(cos, "cos", dt, dev)
+    assert cos.shape == (R, HEAD_DIM) and sin.shape == (R, HEAD_DIM) and _rows(sin, "sin", dt, dev)[1] == cs, \
+        f"cos, sin: [{R}, {HEAD_DIM}], alike"
+    assert slot_mapping.device == dev and slot_mapping.dtype == torch.int32 and slot_mapping.shape == (R,) \
+        and slot_mapping.is_contiguous(), f"slot_mapping: contiguous int32 of {R} on {dev}"
+    for pool, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+        assert pool.device == dev and pool.dtype == dt and pool.dim() == 3 and pool.stride(2) == 1, \
+            f"{name}: a {dt} [slots, heads_kv, {HEAD_DIM}] on {dev}"
+        assert pool.shape[1:] == (heads_kv, HEAD_DIM), f"{name}: [slots, {heads_kv}, {HEAD_DIM}]"
+    assert k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride(), "pools of one shape and strides"
+    return (dev.index, load().mi_q8_qkv_rope, _lib.DTYPES[dt], xs, cs, k_pool.stride()[:2], k_pool.shape[0],
+            heads_q * HEAD_DIM)

@@ -250,11 +250,10 @@ class Attention(nn.Module):
         """few_rows_step of projections in 8 bits, for any number of tokens."""
         cfg = self.cfg
         (B, T, _), n = shape, res.shape[0]
-        qkv = q8.linear(res, self.qkv_proj.weight, bias=self.qkv_proj.bias, norm_weight=norm.weight,
-                        eps=cfg.rms_norm_eps)
-        q = rope_kv_write(qkv, cos[:, 0].reshape(n, cfg.head_dim), sin[:, 0].reshape(n, cfg.head_dim),
-                          meta.slot_mapping32, cache.k_pool(layer), cache.v_pool(layer), cfg.num_heads,
-                          cfg.num_kv_heads)
+        q = q8.qkv_rope(res, norm.weight, cfg.rms_norm_eps, self.qkv_proj.weight, self.qkv_proj.bias,
+                        cos[:, 0].reshape(n, cfg.head_dim), sin[:, 0].reshape(n, cfg.head_dim),
+                        meta.slot_mapping32, cache.k_pool(layer), cache.v_pool(layer), cfg.num_heads,
+                        cfg.num_kv_heads)
         a = self._attend(q, B, T, cache, layer, meta).view(n, self.q_size)
         q8.linear(a, self.o_proj.weight, residual=res, out=res)
 

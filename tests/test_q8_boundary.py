@@ -73,6 +73,14 @@ def _mlp(**over):
     return q8.load().mi_q8_mlp(q8.MLP_ARGS.pack(*(v or 0 for v in a.values())), None)
 
 
+def _qkv(**over):
+    a = dict(x=16, xs=64, norm=16, w=16, ws=16, bias=None, cos=16, sin=16, cs=128, slots=16, q=1 << 30, qs=256,
+             k=16, v=16, ps=128, ph=128, dtype=0, rows=3, hidden=64, heads_q=2, heads_kv=1, num_slots=32,
+             eps=0.0)
+    a.update(over)
+    return q8.load().mi_q8_qkv_rope(q8.QKV_ARGS.pack(*(v or 0 for v in a.values())), None)
+
+
 @pytest.mark.parametrize("call,over,status,msg", [
     (f, o, s, m) for f in (_quantize, _norm, _dequantize) for o, s, m in [
         (dict(dtype=2), 2, "dtype"), (dict(rows=-1), 1, "rows"), (dict(rows=(1 << 21) + 1), 1, "rows"),
@@ -101,6 +109,14 @@ def _mlp(**over):
     (_linear, dict(x=1 << 30, out=(1 << 30) - 2 * (2 * 48 + 47)), 1, "overlaps"),
     (_linear, dict(rows=300, space=None), 1, "workspace is NULL"),
     (_linear, dict(rows=300, space=8), 1, "16-byte"), (_linear, dict(rows=300, size=255), 3, "needed"),
+    (_qkv, dict(dtype=3), 2, "dtype"), (_qkv, dict(rows=17), 1, "rows"), (_qkv, dict(hidden=2049, xs=2049), 1, "hidden"),
+    (_qkv, dict(heads_q=0), 1, "heads_q"), (_qkv, dict(heads_kv=5000), 1, "heads_kv"),
+    (_qkv, dict(num_slots=-1), 1, "num_slots"), (_qkv, dict(x=None), 1, "x is NULL"),
+    (_qkv, dict(norm=None), 1, "norm_weight is NULL"), (_qkv, dict(w=8), 1, "16-byte"),
+    (_qkv, dict(ws=None), 1, "w_scale is NULL"), (_qkv, dict(bias=5), 1, "bias"), (_qkv, dict(cs=127), 1, "cos row"),
+    (_qkv, dict(sin=None), 1, "sin is NULL"), (_qkv, dict(slots=None), 1, "slot_mapping is NULL"),
+    (_qkv, dict(qs=255), 1, "q_out row"), (_qkv, dict(k=None), 1, "k_pool is NULL"),
+    (_qkv, dict(ps=100), 1, "pool strides"), (_qkv, dict(q=16), 1, "q_out overlaps"),
     (_mlp, dict(dtype=7), 2, "dtype"), (_mlp, dict(rows=-2), 1, "rows"), (_mlp, dict(hidden=0), 1, "hidden"),
     (_mlp, dict(inter=0), 1, "inter"), (_mlp, dict(inter=131073), 1, "inter"),
     (_mlp, dict(x=None), 1, "x is NULL"), (_mlp, dict(gu=None), 1, "gate_up is NULL"),
@@ -113,7 +129,8 @@ def test_refusals(call, over, status, msg):
 
 
 def test_arguments_that_are_not_there():
-    for fn in (q8.load().mi_q8_add_rmsnorm, q8.load().mi_q8_linear, q8.load().mi_q8_mlp):
+    lib = q8.load()
+    for fn in (lib.mi_q8_add_rmsnorm, lib.mi_q8_linear, lib.mi_q8_mlp, lib.mi_q8_qkv_rope):
         assert fn(None, None) == 1 and "args is NULL" in last()
 
 
@@ -121,9 +138,10 @@ STRUCTS = """
 #include <stdio.h>
 #include "mi_q8.h"
 int main() {
-  printf("%zu %zu %zu\\n", sizeof(mi_q8_norm_args), sizeof(mi_q8_linear_args), sizeof(mi_q8_mlp_args));
-  printf("%zu %zu %zu\\n", offsetof(mi_q8_norm_args, eps), offsetof(mi_q8_linear_args, eps),
-         offsetof(mi_q8_mlp_args, eps));
+  printf("%zu %zu %zu %zu\\n", sizeof(mi_q8_norm_args), sizeof(mi_q8_linear_args), sizeof(mi_q8_mlp_args),
+         sizeof(mi_q8_qkv_rope_args));
+  printf("%zu %zu %zu %zu\\n", offsetof(mi_q8_norm_args, eps), offsetof(mi_q8_linear_args, eps),
+         offsetof(mi_q8_mlp_args, eps), offsetof(mi_q8_qkv_rope_args, eps));
 }
 """
 
@@ -133,12 +151,12 @@ def test_argument_structs_are_the_headers(tmp_path):
     subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
     sizes, ends = (list(map(int, line.split())) for line in subprocess.run(
         [str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.splitlines())
-    for st, size, end in zip((q8.NORM_ARGS, q8.LINEAR_ARGS, q8.MLP_ARGS), sizes, ends):
+    for st, size, end in zip((q8.NORM_ARGS, q8.LINEAR_ARGS, q8.MLP_ARGS, q8.QKV_ARGS), sizes, ends):
         assert st.size == end + 4 and st.size <= size < st.size + 8   # (the struct ends aligned)
 
 
 def test_empty_calls_are_no_ops():
-    for call in (_quantize, _norm, _dequantize, _matmul, _linear, _mlp):
+    for call in (_quantize, _norm, _dequantize, _matmul, _linear, _mlp, _qkv):
         assert call(rows=0) == 0 and last() == ""
 
 

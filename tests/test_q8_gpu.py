@@ -15,6 +15,7 @@ import torch
 
 from conftest import announce
 from kernels import q8
+from kernels.rope import rope_kv_write
 from oracle import q8 as o8
 
 pytestmark = pytest.mark.gpu
@@ -315,6 +316,36 @@ def test_mlp(m, hidden, inter, dtype):
         # (rows that lie otherwise may have their squares summed in another order: the scale moves in its
         # last places, within SCALE, and activations next to a border by a step, which check() counts)
         check(view, rows, x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,hidden,heads", [(1, 1536, (12, 2)), (16, 1536, (12, 2)), (9, 896, (14, 2)), (5, 1001, (1, 1)),
+                                            (16, 2048, (40, 8)), (3, 64, (3, 3)), (17, 256, (4, 1)),
+                                            (2, 2049, (2, 1))])
+def test_qkv_rope_is_the_separate_launches(m, hidden, heads, dtype):
+    announce(f"qkv_rope {m} x {hidden} {heads} {dtype}")
+    g = torch.Generator().manual_seed(m + hidden)
+    hq, hkv = heads
+    _, _, w = weight_of(g, (hq + 2 * hkv) * 128, hidden)
+    x = rows_of(g, dtype, m, hidden, 0.3)
+    norm = (1 + 0.2 * torch.randn(hidden, generator=g)).to(dtype).to(DEV)
+    angle = torch.rand(m, 64, generator=g).repeat(1, 2) * 6.28
+    bias = torch.randn(w.out_features, generator=g).to(dtype).to(DEV)
+    slots = torch.randperm(40, generator=g)[:m].to(torch.int32)
+    if m > 2:
+        slots[1], slots[m // 2] = -1, 40      # nowhere
+    slots = slots.to(DEV)
+    cos16, sin16 = angle.cos().to(dtype), angle.sin().to(dtype)
+    one_launch = m <= q8.FUSED_ROWS and hidden <= q8.FUSED_IN
+    pad, at = (5, 3) if one_launch else (8, 8)     # (rope_kv_write takes rows at multiples of 16 bytes)
+    for xd, cos, sin, b in ((x.to(DEV), cos16.to(DEV), sin16.to(DEV), bias),
+                            (strided(x, 3, 1), strided(cos16, pad, at), strided(sin16, pad, at), None)):
+        pools = [torch.full((2, 2, 40, hkv, 128), 3.0, dtype=dtype, device=DEV) for _ in range(2)]
+        got = q8.qkv_rope(xd, norm, 1e-6, w, b, cos, sin, slots, pools[0][1, 0], pools[0][1, 1], hq, hkv)
+        qkv = q8.linear(xd, w, bias=b, norm_weight=norm, eps=1e-6)
+        want = rope_kv_write(qkv, cos16.to(DEV), sin16.to(DEV), slots,
+                             pools[1][1, 0], pools[1][1, 1], hq, hkv)
+        assert torch.equal(got, want) and torch.equal(*pools)
 
 
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
