@@ -33,19 +33,28 @@ __host__ __device__ constexpr int q8_panels(int out, bool gated) {
   return gated ? (out / 2 + 7) / 8 : (out + 15) / 16;
 }
 
-// Elements 8c .. 8c + 7 of a row of n 16-bit values at any element, two to a word, zeros past its end.  In steps, so
-// that nothing stands between the loads: q8_load8 (chunks past the end read the last whole one), q8_cut8, and,
-// where n is no multiple of 8, q8_tail8.
+// Elements 8c .. 8c + 7 of a row of n 16-bit values at any element, two to a word, zeros past its end.  In two steps, so
+// that nothing stands between the loads: q8_load8 (chunks past the last whole one read the row's last 8 elements)
+// and q8_cut8.
 __device__ __forceinline__ u32x4 q8_load8(const uint16_t* row, int c, int n) {
-  return n >= 8 ? *reinterpret_cast<const u32x4_2*>(row + 8 * min(c, (n >> 3) - 1)) : u32x4{0, 0, 0, 0};
+  if (n >= 8) return *reinterpret_cast<const u32x4_2*>(row + (c < n >> 3 ? 8 * c : n - 8));
+  u32x4 a = {0, 0, 0, 0};
+  if (c == 0)
+    for (int e = 0; e < n; ++e) a[e >> 1] |= (uint32_t)row[e] << (16 * (e & 1));
+  return a;
 }
 __device__ __forceinline__ u32x4 q8_cut8(u32x4 a, int c, int n) {
-  return c < n >> 3 ? a : u32x4{0, 0, 0, 0};
-}
-__device__ __forceinline__ u32x4 q8_tail8(u32x4 a, const uint16_t* row, int c, int n) {
-  if (c == n >> 3)
-    for (int e = 0; e < (n & 7); ++e) a[e >> 1] |= (uint32_t)row[8 * c + e] << (16 * (e & 1));
-  return a;
+  if (n < 8) return a;
+  u32x4 tail = {0, 0, 0, 0};
+  if (n & 7) {   // the last n % 8 of the 8 elements, from the first place on
+    const int by = 8 - (n & 7);
+    tail = by & 4 ? u32x4{a[2], a[3], 0, 0} : a;
+    if (by & 2) tail = u32x4{tail[1], tail[2], tail[3], 0};
+    if (by & 1)
+      tail = u32x4{tail[0] >> 16 | tail[1] << 16, tail[1] >> 16 | tail[2] << 16, tail[2] >> 16 | tail[3] << 16,
+                   tail[3] >> 16};
+  }
+  return c < n >> 3 ? a : c == n >> 3 ? tail : u32x4{0, 0, 0, 0};
 }
 // The same stored, elements past n left alone.
 __device__ __forceinline__ void q8_store8(uint16_t* row, int c, int n, u32x4 v) {

@@ -196,8 +196,7 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
       for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
         const int t = (tid + e * kQgThreads) / kPieces;
         if (m0 + t < p.M && 8 * c < n_left) {
-          u32x4 v = q8_cut8(q8_load8(res + t * p.res_st, c, n_left), c, n_left);
-          if (n_left & 7) v = q8_tail8(v, res + t * p.res_st, c, n_left);
+          const u32x4 v = q8_cut8(q8_load8(res + t * p.res_st, c, n_left), c, n_left);
           *reinterpret_cast<u32x4*>(lds + t * kRow + c * 16) = v;
         }
       }

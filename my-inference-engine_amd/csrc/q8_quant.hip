@@ -78,14 +78,6 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
       k.w = q8_cut8(k.w, c, p.n);
     }
   };
-  const auto tail = [&](int c, Chunk& k, bool first) {
-    if constexpr (SRC != kQ8Float) {
-      k.x[0] = q8_tail8(k.x[0], add && !first ? r : x, c, p.n);
-      if (add && first) k.y = q8_tail8(k.y, y, c, p.n);
-      if (SRC == kQ8Norm) k.w = q8_tail8(k.w, p.norm_w, c, p.n);
-    }
-  };
-  const bool odd = SRC != kQ8Float && (p.n & 7);
   const auto take = [&](int c, const Chunk& k, float (&v)[8], bool first) {
     if constexpr (SRC == kQ8Float) {
 #pragma unroll
@@ -121,18 +113,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
     Chunk k[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) k[i] = load(tid + i * T, true);
+    if (p.n != PER * T * 8)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) cut(tid + i * T, k[i]);
-    if (odd)
-#pragma unroll
-      for (int i = 0; i < PER; ++i) tail(tid + i * T, k[i], true);
+      for (int i = 0; i < PER; ++i) cut(tid + i * T, k[i]);
 #pragma unroll
     for (int i = 0; i < PER; ++i) take(tid + i * T, k[i], kept[i], true);
   } else {
     for (int c = tid; c < chunks; c += T) {
       Chunk k = load(c, true);
       cut(c, k);
-      if (odd) tail(c, k, true);
       take(c, k, kept[0], true);
     }
   }
@@ -167,7 +156,6 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
     for (int c = tid; c < chunks; c += T) {
       Chunk k = load(c, false);
       cut(c, k);
-      if (odd) tail(c, k, false);
       take(c, k, kept[0], false);
       store(c, kept[0]);
     }
@@ -189,6 +177,7 @@ hipError_t launch_quant_t(Q8QuantParams p, hipStream_t stream) {
   // (in whole rounds of the 8 XCDs' panels)
   const int rows = p.spread ? (p.M + 127) / 128 * 128 : p.M;
   if (p.np <= 64 * 4 * 8) launch_quant_per<E, SRC, 64, 1, 4>(p, dim3((rows + 3) / 4), stream);
+  else if (p.M <= 64 && p.np <= 1024 * 8 * 4) launch_quant_per<E, SRC, 1024, 1, 4>(p, dim3(rows), stream);
   else if (p.np <= 256 * 8 * 8) launch_quant_per<E, SRC, 256, 2, 8>(p, dim3(rows), stream);
   else launch_quant_per<E, SRC, 1024, 0, 0>(p, dim3(rows), stream);
   return hipGetLastError();

@@ -250,18 +250,10 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
       constexpr int R = decltype(rows)::value;
       if (p.K != kChunks * 512)
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-#pragma unroll
-        for (int h = 0; h < R; ++h) raw[h][k] = q8_cut8(raw[h][k], lane + 64 * k, p.K);
-        if constexpr (SRC == kQ8Norm) nw[k] = q8_cut8(nw[k], lane + 64 * k, p.K);
-      }
-      if (p.K & 7)
-#pragma unroll
         for (int k = 0; k < kChunks; ++k) {
 #pragma unroll
-          for (int h = 0; h < R; ++h)
-            raw[h][k] = q8_tail8(raw[h][k], x16 + min(wave + 8 * h, p.M - 1) * p.x_st, lane + 64 * k, p.K);
-          if constexpr (SRC == kQ8Norm) nw[k] = q8_tail8(nw[k], p.norm_w, lane + 64 * k, p.K);
+          for (int h = 0; h < R; ++h) raw[h][k] = q8_cut8(raw[h][k], lane + 64 * k, p.K);
+          if constexpr (SRC == kQ8Norm) nw[k] = q8_cut8(nw[k], lane + 64 * k, p.K);
         }
       float v[R][kChunks][8], ss[R];
       uint32_t top[R];

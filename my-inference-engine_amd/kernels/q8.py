@@ -12,7 +12,7 @@ They stand beside kernels.few_rows and kernels.model_ops for a model whose proje
 products is its model.py:49-55,81-84,107,112-138,204-207.
 
 A row of n numbers v is held as round(v / scale) with scale = max|v| / 127; a row with an infinity or a NaN has
-scale NaN, and so is everything computed from it.  Products are whole numbers, exact in 32 bits; scales, bias and
+scale NaN, and so is everything computed from it.  Inference only: no gradient is recorded.  Products are whole numbers, exact in 32 bits; scales, bias and
 residual are applied in fp32 and the result is rounded once.  No CPU path and no fallback: a missing library or a
 call that the kernels do not take raises.
 """
@@ -99,7 +99,7 @@ class Weight:
     """A projection's weight in 8 bits: values [out, in] int8 and scale [out] fp32 (weight = values *
     scale[:, None]), laid out for the kernels once.  gated: the gate and up rows of a feed-forward block,
     gate rows first, which only `mlp` takes.  The values are copied, the scale is kept as it is."""
-    __slots__ = ("data", "scale", "out_features", "in_features", "gated", "sig", "data_ptr", "scale_ptr")
+    __slots__ = ("data", "scale", "out_features", "in_features", "gated", "sig")
 
     def __init__(self, values, scale, gated=False):
         assert values.is_cuda and values.dtype == torch.int8 and values.dim() == 2, \
@@ -111,20 +111,30 @@ class Weight:
         assert scale.device == values.device and scale.dtype == torch.float32, \
             f"scale: fp32 on {values.device}"
         assert scale.shape == (n,) and scale.is_contiguous(), f"scale: contiguous, of {n}"
-        self.gated = bool(gated)
-        assert not (self.gated and n % 2), "a gated weight has as many gate as up rows"
-        self.out_features, self.in_features, self.scale = n, k, scale
+        gated = bool(gated)
+        assert not (gated and n % 2), "a gated weight has as many gate as up rows"
         lib = load()
-        self.data = torch.empty(lib.mi_q8_packed_bytes(n, k, self.gated), dtype=torch.int8,
-                                device=values.device)
+        data = torch.empty(lib.mi_q8_packed_bytes(n, k, gated), dtype=torch.int8, device=values.device)
         call(values.device.index, lib.mi_q8_pack, values.data_ptr(),
-             values.stride(0) if n > 1 else k, n, k, self.gated, self.data.data_ptr())
-        self.sig = (n, k, self.gated, values.device)
-        self.data_ptr, self.scale_ptr = self.data.data_ptr(), scale.data_ptr()
+             values.stride(0) if n > 1 else k, n, k, gated, data.data_ptr())
+        self._hold(data, scale, n, k, gated)
+
+    def _hold(self, data, scale, n, k, gated):
+        self.data, self.scale, self.out_features, self.in_features, self.gated = data, scale, n, k, gated
+        self.sig = (n, k, gated, scale.device)   # what a call's plan depends on
+
+    def __reduce__(self):   # copied and saved as its two tensors, wherever those come back
+        return _held, (self.data, self.scale, self.out_features, self.in_features, self.gated)
 
     @property
     def device(self):
         return self.scale.device
+
+
+def _held(*parts):
+    w = object.__new__(Weight)
+    w._hold(*parts)
+    return w
 
 
 def quantize_weight(weight, gated=False):
@@ -288,7 +298,7 @@ def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=data.device) if nbytes else None
     call(index, fn, LINEAR_ARGS.pack(
         data.data_ptr(), xs, scale.data_ptr() if scale is not None else 0,
-        norm_weight.data_ptr() if norm_weight is not None else 0, w.data_ptr, w.scale_ptr,
+        norm_weight.data_ptr() if norm_weight is not None else 0, w.data.data_ptr(), w.scale.data_ptr(),
         bias.data_ptr() if bias is not None else 0, residual.data_ptr() if residual is not None else 0,
         rs, out.data_ptr(), os_, ws.data_ptr() if nbytes else 0, nbytes, code, *shape, K, eps))
     return out
@@ -332,8 +342,8 @@ def mlp(x, gate_up, down, residual=None, norm_weight=None, eps=0.0, out=None):
     # every call has its own (from torch's caching allocator, in stream order): nothing is shared
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     call(index, fn, MLP_ARGS.pack(
-        x.data_ptr(), xs, norm_weight.data_ptr() if norm_weight is not None else 0, gate_up.data_ptr,
-        gate_up.scale_ptr, down.data_ptr, down.scale_ptr,
+        x.data_ptr(), xs, norm_weight.data_ptr() if norm_weight is not None else 0, gate_up.data.data_ptr(),
+        gate_up.scale.data_ptr(), down.data.data_ptr(), down.scale.data_ptr(),
         residual.data_ptr() if residual is not None else 0, rs, out.data_ptr(), os_, ws.data_ptr(),
         nbytes, code, R, H, inter, eps))
     return out
@@ -377,7 +387,7 @@ def qkv_rope(x, norm_weight, eps, w, bias, cos, sin, slot_mapping, k_pool, v_poo
     index, fn, code, xs, cs, pool_strides, slots, width = plan
     q = x.new_empty((rows, width))
     call(index, fn, QKV_ARGS.pack(
-        x.data_ptr(), xs, norm_weight.data_ptr(), w.data_ptr, w.scale_ptr,
+        x.data_ptr(), xs, norm_weight.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(),
         bias.data_ptr() if bias is not None else 0, cos.data_ptr(), sin.data_ptr(), cs,
         slot_mapping.data_ptr(), q.data_ptr(), width, k_pool.data_ptr(), v_pool.data_ptr(), *pool_strides,
         code, rows, hidden, heads_q, heads_kv, slots, eps))

@@ -372,8 +372,8 @@ class Qwen2ForCausalLM(nn.Module):
     @torch.no_grad()
     def quantize_(self, lm_head=False):
         """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head) in 8
-        bits from now on; their 16-bit weights are let go.  The model is on the GPU, in bf16 or fp16; graphs
-        captured before replay the old weights."""
+        bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit weights are let go: capture decode
+        graphs after this, those captured before read memory that is no longer theirs."""
         held = [(m, name) for layer in self.layers
                 for m, name in ((layer.self_attn, "qkv_proj"), (layer.self_attn, "o_proj"),
                                 (layer.mlp, "gate_up_proj"), (layer.mlp, "down_proj"))]

@@ -10,6 +10,8 @@ Tolerances.  U = 2^-24 is half a step of fp32, relative; H = finfo(t).eps / 2 th
   product the whole number rounded to fp32, two factors (each scale exact, or 60 U off), bias and residual:
           8 U of the magnitudes added, then H of the result (or half the least positive number)
 """
+import copy
+
 import pytest
 import torch
 
@@ -378,6 +380,22 @@ def test_quantized_weight_is_a_row_for_each_feature():
     check_rows(rows, w, 2 * U)
     assert torch.equal(got.data.cpu(), o8.packed(rows.values.cpu()).flatten())
     assert torch.equal(got.scale, rows.scale)
+
+
+def test_a_weight_copied_and_saved(tmp_path):
+    g = torch.Generator().manual_seed(6)
+    _, _, w = weight_of(g, 48, 200)
+    x = rows_of(g, torch.bfloat16, 3, 200).to(DEV)
+    want = q8.linear(x, w)
+    other = copy.deepcopy(w)
+    assert other.data.data_ptr() != w.data.data_ptr() and other.scale.data_ptr() != w.scale.data_ptr()
+    torch.save(w, tmp_path / "w.pt")
+    loaded = torch.load(tmp_path / "w.pt", weights_only=False)
+    on_cpu = torch.load(tmp_path / "w.pt", weights_only=False, map_location="cpu")
+    del w
+    assert torch.equal(q8.linear(x, other), want) and torch.equal(q8.linear(x, loaded), want)
+    with pytest.raises(AssertionError):
+        q8.linear(x, on_cpu)
 
 
 def test_no_rows():
