@@ -43,7 +43,7 @@ __device__ __forceinline__ void wait_loads_and_barrier() {
 }  // namespace
 
 template <typename E, int NP, int TM, int WN, int ST, bool GATED>
-__global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p) {
+__global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
   constexpr int WM = kQgWaves / WN;
   constexpr int TI = NP * 16 / WN / 32, TJ = TM / WM / 32;
   constexpr int kStage = NP * 1024 + TM * 64;
@@ -51,9 +51,10 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
   // the tile on its way out: rows of tokens, 16-bit results or fp32 activations (half as many)
   constexpr int kRow = NP * 16 * 2 + 16;
   constexpr int kTile = ST * kStage > TM * kRow ? ST * kStage : TM * kRow;
-  __shared__ __attribute__((aligned(1024))) char lds[kTile + (NP * 16 + TM) * 4];
+  __shared__ __attribute__((aligned(1024))) char lds[kTile + (2 * NP * 16 + TM) * 4];
   float* w_scale = reinterpret_cast<float*>(lds + kTile);   // of the tile's rows of W and tokens
   float* x_scale = w_scale + NP * 16;
+  float* bias = x_scale + TM;   // in fp32
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % WN, wm = wave / WN;
@@ -152,8 +153,8 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
 
   // Results.  Lane l holds token l % 32 of each 32 x 32 block and rows 8 (r / 4) + 4 (l / 32) + r % 4 of W.
   const int w_first = wn * TI * 32 + 4 * kc;   // of block i, quad q: + 32 i + 8 q
-  __syncthreads();
   if constexpr (GATED) {
+    __syncthreads();
     // quads 0 and 2 are gate rows, 1 and 3 the up rows of the same features
     constexpr int kPieces = NP * 2;   // of 16 bytes a row
     const int f0 = panel0 * 8;
@@ -190,32 +191,30 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
     constexpr int kPieces = NP * 2;   // of 16 bytes a row
     uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m0 * p.out_st + panel0 * 16;
     const int c = tid % kPieces, n_left = p.N - panel0 * 16;
+    uint16_t my_bias = 0;
+    if (p.bias && tid < NP * 16 && tid < n_left) my_bias = p.bias[panel0 * 16 + tid];
     if (p.res) {
-      const uint16_t* res = p.res + (int64_t)m0 * p.res_st + panel0 * 16;
+      // the residual takes its place in LDS, where the sums then meet it
+      constexpr int kEach = TM * kPieces / kQgThreads;
+      u32x4 res[kEach];
 #pragma unroll
-      for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
-        const int t = (tid + e * kQgThreads) / kPieces;
-        if (m0 + t < p.M && 8 * c < n_left) {
-          const u32x4 v = q8_cut8(q8_load8(res + t * p.res_st, c, n_left), c, n_left);
-          *reinterpret_cast<u32x4*>(lds + t * kRow + c * 16) = v;
-        }
+      for (int e = 0; e < kEach; ++e) {
+        const int m = min(m0 + (tid + e * kQgThreads) / kPieces, p.M - 1);
+        res[e] = q8_load8(p.res + m * p.res_st + panel0 * 16, c, n_left);
       }
       __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        *reinterpret_cast<u32x4*>(lds + (tid + e * kQgThreads) / kPieces * kRow + c * 16) = q8_cut8(res[e], c, n_left);
     }
+    if (tid < NP * 16) bias[tid] = E::lo(my_bias);
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < TI; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = w_first + 32 * i + 8 * q;
-        const f32x4 ws = *reinterpret_cast<const f32x4*>(w_scale + n);
-        u32x2 bias = {0, 0};
-        if (p.bias) {
-          if (n + 4 <= n_left)
-            bias = *reinterpret_cast<const u32x2_2*>(p.bias + panel0 * 16 + n);
-          else
-            for (int r = 0; r < n_left - n; ++r)
-              bias[r >> 1] |= (uint32_t)p.bias[panel0 * 16 + n + r] << (16 * (r & 1));
-        }
+        const f32x4 ws = *reinterpret_cast<const f32x4*>(w_scale + n), bs = *reinterpret_cast<const f32x4*>(bias + n);
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
           const int t = wm * TJ * 32 + j * 32 + r32;
@@ -223,8 +222,10 @@ __global__ __launch_bounds__(kQgThreads, 2) void q8_gemm_kernel(const Q8Params p
           u32x2* at = reinterpret_cast<u32x2*>(lds + t * kRow + n * 2);
           float v[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = q8_scaled(acc[i][j][4 * q + r], xs, ws[r]);
-          if (p.bias) add4<E>(v, bias);
+          for (int r = 0; r < 4; ++r) {
+            v[r] = q8_scaled(acc[i][j][4 * q + r], xs, ws[r]);
+            if (p.bias) v[r] = q8_plus(v[r], bs[r]);
+          }
           if (p.res) add4<E>(v, *at);
           *at = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
         }
