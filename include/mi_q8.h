@@ -22,7 +22,7 @@
  *
  * Common rules.  dtype: 0 bf16, 1 fp16 (everything that is not int8 or fp32 here).  Row strides are in
  * elements, at least the row's length, any alignment of rows (rows whose addresses are multiples of 16
- * bytes are faster).  Sizes: in_features at most 131072, out_features at most 2^24, rows at most 2^21.
+ * bytes are faster).  Rows of one stride may be columns of one tensor.  Sizes: in_features at most 131072, out_features at most 2^24, rows at most 2^21.
  * All launches are asynchronous on `stream`, allocate nothing and may be captured in a graph.
  * Workspaces: 16-byte aligned, contents arbitrary, not shared by calls that may overlap in time.
  *
@@ -53,7 +53,7 @@ MI_Q8_API int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, voi
 /*
  * r = x + y, rounded (y NULL: r is x, and residual_out is not used); values and scale are the rows of
  * r * rsqrt(mean(r^2) + eps) * weight in 8 bits, taken in fp32 without a rounding in between.
- * residual_out may be x or y.
+ * residual_out may be x or y, and shares nothing with them otherwise.
  */
 typedef struct mi_q8_norm_args {
   const void* x;
@@ -84,7 +84,7 @@ MI_Q8_API int mi_q8_pack(const void* values, int64_t stride, int32_t out_feature
 
 /*
  * out = [residual +] x W^T [+ bias]: w packed, w_scale [out_features], bias [out_features] or NULL, residual
- * [rows, out_features] or NULL (may be out).
+ * [rows, out_features] or NULL (may be out, and shares nothing with it otherwise).
  *
  * x_scale NULL: x is 16-bit rows [rows, in_features], which the call brings to 8 bits itself, as
  * mi_q8_add_rmsnorm does without y (norm_weight) or as mi_q8_quantize does (norm_weight NULL); out must not
@@ -115,7 +115,8 @@ MI_Q8_API int mi_q8_linear(const mi_q8_linear_args* args, void* stream);
 /*
  * A gated feed-forward block, out = [residual +] a Wd^T with a = silu(g) * u in fp32, held in 8 bits
  * for the second product, and (g | u) = [rmsnorm] x Wgu^T: x, out, residual [rows, hidden], gate_up
- * packed as gated [2 * inter, hidden], down packed [hidden, inter].  out may be x and residual.
+ * packed as gated [2 * inter, hidden], down packed [hidden, inter].  out may be x, and
+ * residual (and shares nothing with it otherwise).
  */
 typedef struct mi_q8_mlp_args {
   const void* x;

@@ -7,6 +7,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 #include "q8.h"
 
@@ -92,17 +93,40 @@ int check_weight(const char* name, const void* w, const float* scale) {
   return kOk;
 }
 
-int check_out(const void* residual, int64_t residual_stride, void* out, int64_t out_stride, int32_t n) {
-  if (residual)
-    if (int rc = check_rows("residual", residual, residual_stride, n)) return rc;
-  return check_rows("out", out, out_stride, n);
+// 16-bit rows as a call's arguments describe them.
+struct View {
+  const void* at;
+  int64_t stride;
+  int64_t n;
+};
+
+// Whether two views of `rows` rows share an element.  Of one stride: exactly (columns of one tensor do not).
+// Else by their extents.
+bool overlap(int64_t rows, View a, View b) {
+  const int64_t d = ((intptr_t)b.at - (intptr_t)a.at) / 2;   // elements from a to b
+  if (d >= (rows - 1) * a.stride + a.n || -d >= (rows - 1) * b.stride + b.n) return false;
+  const int64_t s = a.stride;
+  if (rows == 1 || s != b.stride) return true;
+  int64_t q = d / s, e = d % s;   // b's row j begins e elements into a's row q + j
+  if (e < 0) --q, e += s;
+  return (e < a.n && std::abs(q) < rows) || (e + b.n > s && std::abs(q + 1) < rows);
 }
 
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-  const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
-  return x < y + b_bytes && y < x + a_bytes;
+// `out` is `in` itself or shares nothing with it.
+int check_in_place(const char* in_name, const char* out_name, int64_t rows, View in, View out) {
+  if (in.at == out.at && (rows == 1 || in.stride == out.stride)) return kOk;
+  if (!overlap(rows, in, out)) return kOk;
+  return fail(kInvalid, "%s overlaps %s, and is not the same rows", out_name, in_name);
 }
-int64_t span(int32_t rows, int64_t stride, int32_t n) { return 2 * ((rows - 1) * stride + n); }
+
+int check_out(const void* residual, int64_t residual_stride, void* out, int64_t out_stride, int64_t rows,
+              int32_t n) {
+  if (residual)
+    if (int rc = check_rows("residual", residual, residual_stride, n)) return rc;
+  if (int rc = check_rows("out", out, out_stride, n)) return rc;
+  if (!residual) return kOk;
+  return check_in_place("residual", "out", rows, {residual, residual_stride, n}, {out, out_stride, n});
+}
 
 // A workspace's parts, each at a multiple of 256 bytes.
 struct Space {
@@ -263,6 +287,9 @@ int mi_q8_add_rmsnorm(const mi_q8_norm_args* args, void* stream) {
   if (a.y) {
     if (int rc = check_rows("y", a.y, a.y_stride, a.n)) return rc;
     if (int rc = check_rows("residual_out", a.residual_out, a.residual_stride, a.n)) return rc;
+    const View r{a.residual_out, a.residual_stride, a.n};
+    if (int rc = check_in_place("x", "residual_out", a.rows, {a.x, a.x_stride, a.n}, r)) return rc;
+    if (int rc = check_in_place("y", "residual_out", a.rows, {a.y, a.y_stride, a.n}, r)) return rc;
   }
   if (int rc = check_ptr("weight", a.weight, 2)) return rc;
   if (int rc = check_ptr("values", a.values, 16)) return rc;
@@ -338,12 +365,11 @@ int mi_q8_linear(const mi_q8_linear_args* args, void* stream) {
   if (int rc = check_weight("w", a.w, a.w_scale)) return rc;
   if (a.bias)
     if (int rc = check_ptr("bias", a.bias, 2)) return rc;
-  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.out_features)) return rc;
+  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.rows, a.out_features)) return rc;
   const Q8Params p = operands(a.w, a.w_scale, a.bias, a.residual, a.residual_stride, a.out, a.out_stride,
                               a.rows, a.out_features, a.in_features, false);
   if (a.x_scale) return product(p, a.dtype, false, a.x, a.x_scale, stream);
-  if (overlap(a.x, span(a.rows, a.x_stride, a.in_features), a.out,
-              span(a.rows, a.out_stride, a.out_features)))
+  if (overlap(a.rows, {a.x, a.x_stride, a.in_features}, {a.out, a.out_stride, a.out_features}))
     return fail(kInvalid, "out overlaps x");
   const LinearSpace sp(a.rows, a.in_features);
   if (int rc = check_workspace(a.workspace, a.workspace_bytes,
@@ -371,7 +397,7 @@ int mi_q8_mlp(const mi_q8_mlp_args* args, void* stream) {
     if (int rc = check_ptr("norm_weight", a.norm_weight, 2)) return rc;
   if (int rc = check_weight("gate_up", a.gate_up, a.gate_up_scale)) return rc;
   if (int rc = check_weight("down", a.down, a.down_scale)) return rc;
-  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.hidden)) return rc;
+  if (int rc = check_out(a.residual, a.residual_stride, a.out, a.out_stride, a.rows, a.hidden)) return rc;
   const MlpSpace sp(a.rows, a.hidden, a.inter);
   if (int rc = check_workspace(a.workspace, a.workspace_bytes, sp.s.total)) return rc;
   char* ws = static_cast<char*>(a.workspace);
@@ -429,7 +455,7 @@ int mi_q8_qkv_rope(const mi_q8_qkv_rope_args* args, void* stream) {
   if (a.pool_slot_stride < d || a.pool_head_stride < d)
     return fail(kInvalid, "pool strides %lld, %lld: at least %d", (long long)a.pool_slot_stride,
                 (long long)a.pool_head_stride, d);
-  if (overlap(a.x, span(a.rows, a.x_stride, a.hidden), a.q_out, span(a.rows, a.q_stride, a.heads_q * d)))
+  if (overlap(a.rows, {a.x, a.x_stride, a.hidden}, {a.q_out, a.q_stride, a.heads_q * d}))
     return fail(kInvalid, "q_out overlaps x");
   Q8Params p = operands(a.w, a.w_scale, a.bias, nullptr, 0, a.q_out, a.q_stride, a.rows,
                         (a.heads_q + 2 * a.heads_kv) * d, a.hidden, false);

@@ -278,7 +278,7 @@ def _ends(out, residual, R, N, dt, dev):
 
 def linear(x, w, bias=None, residual=None, norm_weight=None, eps=0.0, out=None):
     """[residual +] x W^T [+ bias] -> [rows, out]: x [rows, in] (bf16 or fp16; with norm_weight RMS-normalised
-    first) or Rows, w a Weight.  residual may be `out` (in place); out must not overlap x."""
+    first) or Rows, w a Weight.  residual may be `out` (in place); out shares nothing with x."""
     assert type(w) is Weight, "w: a Weight"
     if type(x) is Rows:
         assert norm_weight is None, "rows in 8 bits are normalised already"

@@ -107,6 +107,21 @@ def _qkv(**over):
     (_linear, dict(x=None), 1, "x is NULL"), (_linear, dict(norm=3), 1, "norm_weight"),
     (_linear, dict(out=16), 1, "overlaps"), (_linear, dict(out=16 + 2 * (2 * 64 + 63)), 1, "overlaps"),
     (_linear, dict(x=1 << 30, out=(1 << 30) - 2 * (2 * 48 + 47)), 1, "overlaps"),
+    # (x: 3 rows of 64 in a stride of 160; out: 48 columns one before its end, or running into its next row)
+    (_linear, dict(x=1024, xs=160, out=1024 + 2 * 63, os=160), 1, "overlaps x"),
+    (_linear, dict(x=1024, xs=160, out=1024 + 2 * (160 + 113), os=160), 1, "overlaps x"),
+    (_linear, dict(x=1024, xs=160, out=1024 - 2 * 47, os=160), 1, "overlaps x"),
+    (_linear, dict(x=1024, xs=160, out=1024 + 2 * (320 + 63), os=160), 1, "overlaps x"),
+    (_matmul, dict(res=1 << 30, rs=56, os=48), 1, "out overlaps residual"),
+    (_matmul, dict(res=(1 << 30) + 2, rs=48), 1, "out overlaps residual"),
+    (_mlp, dict(res=(1 << 30) - 2 * (2 * 64 + 63), rs=64), 1, "out overlaps residual"),
+    (_norm, dict(r=18), 1, "residual_out overlaps x"), (_norm, dict(x=4096, r=18), 1, "residual_out overlaps y"),
+    (_norm, dict(r=16, rs=80), 1, "residual_out overlaps x"),
+    # columns of one tensor: past that check, to the workspace's
+    *((_linear, dict(rows=300, x=4096, xs=160, out=4096 + 2 * at, os=160, space=None), 1, "workspace is NULL")
+      for at in (64, 112, -48, -96, 160 * 299 + 64, -160 * 299 - 48)),
+    *((_linear, dict(rows=300, res=(1 << 30) + at, rs=96, os=96, space=None), 1, "workspace is NULL")
+      for at in (0, 96, -96)),
     (_linear, dict(rows=300, space=None), 1, "workspace is NULL"),
     (_linear, dict(rows=300, space=8), 1, "16-byte"), (_linear, dict(rows=300, size=255), 3, "needed"),
     (_qkv, dict(dtype=3), 2, "dtype"), (_qkv, dict(rows=17), 1, "rows"), (_qkv, dict(hidden=2049, xs=2049), 1, "hidden"),

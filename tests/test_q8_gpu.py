@@ -215,7 +215,8 @@ PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96),
             (31, 777, 1001), (33, 130, 200), (48, 64, 8960), (64, 2048, 1536), (65, 33, 300),
             (100, 128, 256), (127, 250, 128), (129, 257, 1000), (150, 896, 4864), (200, 1024, 64),
             (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
-            (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200)]
+            (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200),
+            (3, 66000, 70), (2, 65553, 2100)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -380,6 +381,68 @@ def test_quantized_weight_is_a_row_for_each_feature():
     check_rows(rows, w, 2 * U)
     assert torch.equal(got.data.cpu(), o8.packed(rows.values.cpu()).flatten())
     assert torch.equal(got.scale, rows.scale)
+
+
+def test_past_two_gigabytes():
+    """Rows, weights and results that lie more than 2^31 bytes in: the last ones against calls of their own."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n, k, few = 270000, 8192, 37
+    announce("rows past 2^31 bytes")
+    x = torch.randn(n, k, generator=g, device=DEV, dtype=torch.bfloat16)
+    small = q8.quantize_weight(torch.randn(48, k, generator=g, device=DEV, dtype=torch.bfloat16))
+    rows, last = q8.quantize(x), q8.quantize(x[-few:].clone())
+    assert torch.equal(rows.scale[-few:], last.scale)
+    assert torch.equal(rows.dequantize()[-few:], last.dequantize())
+    assert torch.equal(q8.linear(rows, small)[-few:], q8.linear(last, small))
+    del rows
+    announce("weights past 2^31 bytes")
+    big, end = q8.quantize_weight(x), q8.quantize_weight(x[-16 * 3:].clone())
+    for m in (1, 20, 70, 300):
+        y = torch.randn(m, k, generator=g, device=DEV, dtype=torch.bfloat16)
+        assert torch.equal(q8.linear(y, big)[:, -48:], q8.linear(y, end))
+
+
+def test_results_and_activations_past_two_gigabytes():
+    g = torch.Generator(device=DEV).manual_seed(6)
+    m, few = 300000, 5
+    announce("results past 2^31 bytes")
+    x = torch.randn(m, 64, generator=g, device=DEV, dtype=torch.bfloat16)
+    w = q8.quantize_weight(torch.randn(4096, 64, generator=g, device=DEV, dtype=torch.bfloat16))
+    assert torch.equal(q8.linear(x, w)[-few:], q8.linear(x[-few:].clone(), w))
+    announce("activations past 2^31 bytes")
+    gu = torch.randn(4096, 64, generator=g, device=DEV, dtype=torch.bfloat16)
+    down = torch.randn(64, 2048, generator=g, device=DEV, dtype=torch.bfloat16)
+    gate_up, down = q8.quantize_weight(gu, gated=True), q8.quantize_weight(down)
+    # (as many rows as take the same kernels)
+    some = x[-20000:].clone()
+    assert torch.equal(q8.mlp(x, gate_up, down)[-few:], q8.mlp(some, gate_up, down)[-few:])
+
+
+@pytest.mark.parametrize("m", [3, 17, 40, 70])
+def test_rows_far_apart(m):
+    """x, residual and out with rows 2^30 elements or so apart."""
+    g = torch.Generator(device=DEV).manual_seed(m)
+    k, n, stride = 256, 300, 2 ** 32 // m + 8
+    announce(f"rows far apart {m}")
+    buf = torch.empty(m * stride, device=DEV, dtype=torch.bfloat16)
+
+    def far(at, width):
+        return torch.as_strided(buf, (m, width), (stride, 1), at)
+
+    x, res = (torch.randn(m, c, generator=g, device=DEV, dtype=torch.bfloat16) for c in (k, n))
+    far(0, k).copy_(x)
+    far(1000, n).copy_(res)
+    norm = torch.randn(k, generator=g, device=DEV, dtype=torch.bfloat16)
+    w = q8.quantize_weight(torch.randn(n, k, generator=g, device=DEV, dtype=torch.bfloat16))
+    for nw in (None, norm):
+        kw = {} if nw is None else dict(norm_weight=nw, eps=1e-6)
+        got = q8.linear(far(0, k), w, residual=far(1000, n), out=far(2000, n), **kw)
+        assert torch.equal(got, q8.linear(x, w, residual=res, **kw))
+    assert torch.equal(far(1000, n), res) and torch.equal(far(0, k), x)
+    r, rows = q8.add_rmsnorm(far(0, k), norm, 1e-6, y=far(1000, k), residual_out=far(3000, k))
+    want_r, want = q8.add_rmsnorm(x, norm, 1e-6, y=far(1000, k).contiguous())
+    assert torch.equal(r, want_r) and torch.equal(rows.scale, want.scale)
+    assert torch.equal(rows.values, want.values)
 
 
 def test_a_weight_copied_and_saved(tmp_path):
