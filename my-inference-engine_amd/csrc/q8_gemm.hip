@@ -1,4 +1,25 @@
 // Products of many rows in 8 bits with a packed 8-bit weight: out[M][N] = x[M][K] W[N][K]^T.
+//
+// A work-group of 4 waves computes TM tokens by NP panels (128 x 128, a wave 64 x 64; or 64 x 64, a wave
+// 32 x 32) with v_mfma_i32_32x32x32_i8.  W is the A operand, so a lane's four sums in a row are four
+// features of one token.  Both operands come in panels (q8.h): a stage of 64 of K is NP + TM / 16 loads of 1 KB
+// straight into LDS, and a 32 x 32 operand is read out of two panels' kilobytes, 16 lanes in a run, with no two
+// on a bank.  ST stages are in flight.  A stage's operands are read during the MFMAs of the stage before, behind
+// one barrier a stage; the loads ST stages ahead follow between the second half of the MFMAs (reads, then
+// MFMAs, then loads, without that: 6001 x 6144 x 4096 153-159 us where this took 148-152).
+// Results: the tile's scales wait in LDS, loaded with the first stage; the sums are scaled, meet bias and
+// residual in fp32, and leave through LDS as whole rows, past the caches (143 -> 121 us for 4001 x 17920 x 1536
+// against stores that stay in the L2).  GATED: quads of gate and up rows of the same features lie in one lane,
+// silu(g) u leaves in fp32: in bfloat16 the values between half the row's largest and the largest lie half a
+// step of the 8 bits apart, so one in eight of them would move by a whole step.
+//
+// Measured (rows in 8 bits, launches in a graph, two cards): 8192^3 490-531 us (2.07-2.24 POP/s; the library's
+// int8 product 2.06 on the first), 6001 x 6144 x 4096 144-154 us (the library's 180), 4001 x 17920 x 1536
+// 122-132, 4001 x 1536 x 8960 60-64, 4096 x 2048 x 1536 17.4-20.1 (the library's 25.0).  What bounds the long ones is power: the MFMAs alone run at 3.8 POP/s, here a stage of
+// three work-groups takes 900 cycles for 768 of MFMAs, at 1.4 GHz; the same launch on zeros runs at 1.9 GHz and
+// 3.1 POP/s.  128 x 256 tiles move a quarter less and are no faster (8192^3 495 and 505 us, 4001 x 1536 x 8960
+// 61 and 64).  K of 1536 is only 24 stages: there a tile's start and its results show (without the stores
+// 4001 x 17920 x 1536 took 119 us for 121, 4096 x 2048 x 1536 18.2 for 20.1).
 #include "q8.h"
 
 #include <algorithm>
@@ -42,6 +63,7 @@ __device__ __forceinline__ void wait_loads_and_barrier() {
 
 }  // namespace
 
+// WN of the waves stand side by side along W.  Three work-groups a CU (135 registers) for 128 x 128.
 template <typename E, int NP, int TM, int WN, int ST, bool GATED>
 __global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
   constexpr int WM = kQgWaves / WN;

@@ -15,6 +15,15 @@
 //     work-group's read as zeros, with no branch around the loads.
 // Rows that are not in 8 bits yet (SRC) are brought there first, two by each wave, and pass through LDS into
 // the operands' order, while the first weights are on their way.
+//
+// Bound by the weight stream and a launch's fixed cost.  Measured (bf16, launches in a graph, weights in the
+// last-level cache; one token and 16): 2048 x 1536 with norm 3.5 and 5.0 us, rows in 8 bits already 2.6;
+// 17920 x 1536 8.3 and 10.1, 7.5 (3.6 TB/s); 151936 x 1536 41.1 and 45.7, 39.5 (5.9 TB/s; a large copy moves
+// 5.2).  Weights from memory: 17920 x 1536 9.9 and 11.4.  The norm of 16 rows costs 2.3 us here, where every
+// work-group does it over; a launch of its own costs 3.1.
+// Two tiles in flight a work-group instead of one: 17920 x 1536 by one token 7.3 -> 8.0 us, the feed-forward
+// block of 16 tokens with weights from memory 24.1 -> 23.6.
+// The tile kernel at the end of the file is for the sizes q8_rule.h says.
 #include "q8.h"
 
 #include <algorithm>
@@ -351,7 +360,9 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
 }
 
 // A tile of NP panels by 16 MT tokens a work-group, its 8 waves' shares of K each from memory straight into
-// the MFMAs: nothing is shared but the sums, so there is no barrier before the last.
+// the MFMAs, D steps ahead: nothing is shared but the sums, so there is no barrier before the last.  A step is
+// (NP + MT) KB for NP MT MFMAs of 16 cycles: bound by the 64 bytes a CU's vector cache gives a cycle, and by
+// latency where there are few steps.  64 x 1536 x 8960 9.5-10.0 us (1.4 TB/s of weights), 150 x 896 x 4864 7.1-7.7.
 template <typename E, int MT, int NP, int D, bool GATED>
 __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p) {
   constexpr int U = NP * MT;
@@ -416,6 +427,8 @@ namespace {
 template <typename E, int MT, int NP, bool GATED, int SRC, RowsTile TILE = kQrPanels>
 hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kQrThreads), 0, stream, p); };
+  // Steps a wave has in flight where x does not stay: one token's half tiles of 1536 x 8960 take all 18 at once
+  // (the feed-forward block 17.1 -> 15.4 us); with rows in 8 bits beside them 9 (6.0 us, 18: 7.1).
   constexpr int kMany = SRC == kQ8Float && TILE == kQrHalf ? 18 : MT == 1 ? 9 : 6;
   if constexpr (SRC == kQ8Float) {
     if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, 1>);
@@ -441,8 +454,10 @@ hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
     if (p.M > 32) return launch_rows_k<E, 4, 1, GATED, SRC>(p, grid, stream);
     if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
   }
+  // Few panels: half a panel a work-group (1536 x 8960 by one token 6.4 -> 5.8 us).
   if constexpr (!GATED)
     if (2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, 2 * p.panels, stream);
+  // Very many: four panels between two barriers.
   if constexpr (SRC != kQ8Float)
     if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
   return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);

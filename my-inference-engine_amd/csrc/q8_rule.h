@@ -2,9 +2,6 @@
 #pragma once
 
 #include <stdint.h>
-#ifdef Q8_TUNE
-#include <cstdlib>
-#endif
 
 namespace mi_fa2 {
 
@@ -47,16 +44,6 @@ inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
   const Q8Plan t32x32 = plan(kQ8Tile32x32, 32, 2), t32x64 = plan(kQ8Tile32x64, 32, 4),
                t64x64 = plan(kQ8Tile64x64, 64, 4), g64 = plan(kQ8Gemm64, 64, 4),
                g128 = plan(kQ8Gemm128, 128, 8);
-#ifdef Q8_TUNE
-  if (getenv("Q8_NP")) {
-    const int np = atoi(getenv("Q8_NP"));
-    if (np == 1) return t32x32;
-    if (np == 2) return t32x64;
-    if (np == 3) return t64x64;
-    if (np == 4) return g64;
-    if (np == 8) return g128;
-  }
-#endif
   const bool keep = kp <= kQ8KeepK;
   if (rows <= 16) return {kQ8FewRows, 0};
   if (rows <= kQ8RowsMax && (keep ? panels <= 512 : rows <= 32 && panels < 256)) return {kQ8FewRows, 0};
