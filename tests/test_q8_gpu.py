@@ -461,6 +461,31 @@ def test_a_weight_copied_and_saved(tmp_path):
         q8.linear(x, on_cpu)
 
 
+def test_rows_made_of_their_tensors(tmp_path):
+    """Rows put together by hand, copied and saved; tensors that do not belong together are refused."""
+    g = torch.Generator().manual_seed(8)
+    _, _, w = weight_of(g, 48, 200)
+    rows = q8.quantize(rows_of(g, torch.float16, 19, 200).to(DEV))
+    want = q8.linear(rows, w)
+    torch.save(rows, tmp_path / "rows.pt")
+    made = q8.Rows(rows.data.clone(), rows.scale.clone(), 200, torch.float16)
+    for other in (made, copy.deepcopy(rows), torch.load(tmp_path / "rows.pt", weights_only=False)):
+        assert other.data.data_ptr() != rows.data.data_ptr()
+        assert torch.equal(q8.linear(other, w), want) and torch.equal(other.dequantize(), rows.dequantize())
+    ok = dict(data=rows.data, scale=rows.scale, n=200, dtype=torch.float16)
+    for wrong in (dict(data=rows.data[:-1]), dict(data=rows.data[::2]), dict(data=rows.data.view(torch.uint8)),
+                  dict(data=rows.data.cpu()), dict(scale=rows.scale.cpu()), dict(scale=rows.scale[:3]),
+                  dict(scale=rows.scale.double()), dict(scale=rows.scale.view(19, 1)), dict(n=0), dict(n=300),
+                  dict(dtype=torch.float32)):
+        with pytest.raises(AssertionError):
+            q8.Rows(**{**ok, **wrong})
+
+
+def test_a_weight_keeps_its_own_tensors_only():
+    w = q8.quantize_weight(torch.randn(64, 640, device=DEV, dtype=torch.bfloat16))
+    assert w.data.untyped_storage().nbytes() == 64 * 640 and w.scale.untyped_storage().nbytes() == 64 * 4
+
+
 def test_no_rows():
     g = torch.Generator().manual_seed(0)
     x = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
