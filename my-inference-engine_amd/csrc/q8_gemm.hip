@@ -63,9 +63,11 @@ __device__ __forceinline__ void wait_loads_and_barrier() {
 
 }  // namespace
 
-// WN of the waves stand side by side along W.  Three work-groups a CU (135 registers) for 128 x 128.
+// WN of the waves stand side by side along W.  A CU holds three work-groups of 128 x 128 (135 registers), two of
+// the larger tiles; fewer hide less (128 x 128 with a fourth stage, and so with two: 150 -> 186 us for 6001 x 6144 x
+// 4096; 128 x 192 with a fourth, and so with one: 137 -> 222).
 template <typename E, int NP, int TM, int WN, int ST, bool GATED>
-__global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
+__global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
   constexpr int WM = kQgWaves / WN;
   constexpr int TI = NP * 16 / WN / 32, TJ = TM / WM / 32;
   constexpr int kStage = NP * 1024 + TM * 64;
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(co
     float* out = static_cast<float*>(p.out) + (int64_t)m0 * p.out_st + f0;
 #pragma unroll
     for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
-      const int t = (tid + e * kQgThreads) / kPieces, c = tid % kPieces;
+      const int t = (tid + e * kQgThreads) / kPieces, c = (tid + e * kQgThreads) % kPieces;
       if (m0 + t < p.M && f0 + 4 * c < p.N)
         *reinterpret_cast<f32x4*>(out + t * p.out_st + 4 * c) =
             *reinterpret_cast<const f32x4*>(lds + t * kRow + c * 16);
@@ -212,22 +214,27 @@ __global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(co
   } else {
     constexpr int kPieces = NP * 2;   // of 16 bytes a row
     uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m0 * p.out_st + panel0 * 16;
-    const int c = tid % kPieces, n_left = p.N - panel0 * 16;
+    const int n_left = p.N - panel0 * 16;
     uint16_t my_bias = 0;
     if (p.bias && tid < NP * 16 && tid < n_left) my_bias = p.bias[panel0 * 16 + tid];
     if (p.res) {
       // the residual takes its place in LDS, where the sums then meet it
-      constexpr int kEach = TM * kPieces / kQgThreads;
-      u32x4 res[kEach];
+      constexpr int kEach = TM * kPieces / kQgThreads, kBatch = kEach > 12 ? kEach / 2 : kEach;
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int m = min(m0 + (tid + e * kQgThreads) / kPieces, p.M - 1);
-        res[e] = q8_load8(p.res + m * p.res_st + panel0 * 16, c, n_left);
+      for (int first = 0; first < kEach; first += kBatch) {
+        u32x4 res[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const int at = tid + (first + e) * kQgThreads, m = min(m0 + at / kPieces, p.M - 1);
+          res[e] = q8_load8(p.res + m * p.res_st + panel0 * 16, at % kPieces, n_left);
+        }
+        if (first == 0) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const int at = tid + (first + e) * kQgThreads, c = at % kPieces;
+          *reinterpret_cast<u32x4*>(lds + at / kPieces * kRow + c * 16) = q8_cut8(res[e], c, n_left);
+        }
       }
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        *reinterpret_cast<u32x4*>(lds + (tid + e * kQgThreads) / kPieces * kRow + c * 16) = q8_cut8(res[e], c, n_left);
     }
     if (tid < NP * 16) bias[tid] = E::lo(my_bias);
     __syncthreads();
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(kQgThreads, NP == 8 ? 3 : 4) void q8_gemm_kernel(co
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
-      const int t = (tid + e * kQgThreads) / kPieces;
+      const int t = (tid + e * kQgThreads) / kPieces, c = (tid + e * kQgThreads) % kPieces;
       const u32x4 v = *reinterpret_cast<const u32x4*>(lds + t * kRow + c * 16);
       if (m0 + t >= p.M) break;
       if (8 * c + 8 <= n_left)
@@ -270,11 +277,17 @@ namespace {
 
 template <typename E, bool GATED>
 hipError_t launch_gemm_e(const Q8Params& p, const Q8Plan& plan, hipStream_t stream) {
-  const dim3 grid(plan.tiles), block(kQgThreads);
-  if (plan.kernel == kQ8Gemm128)
-    hipLaunchKernelGGL((q8_gemm_kernel<E, 8, 128, 2, 3, GATED>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((q8_gemm_kernel<E, 4, 64, 2, 4, GATED>), grid, block, 0, stream, p);
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(plan.tiles), dim3(kQgThreads), 0, stream, p);
+  };
+  if (plan.kernel == kQ8Gemm64) go(q8_gemm_kernel<E, 4, 64, 2, 4, GATED>);
+  else if (plan.kernel == kQ8Gemm128) go(q8_gemm_kernel<E, 8, 128, 2, 3, GATED>);
+  else if constexpr (!GATED) {
+    if (plan.kernel == kQ8Gemm128x192) go(q8_gemm_kernel<E, 12, 128, 2, 3, false>);
+    else if (plan.kernel == kQ8Gemm192x128) go(q8_gemm_kernel<E, 8, 192, 2, 3, false>);
+    else if (plan.kernel == kQ8Gemm128x256) go(q8_gemm_kernel<E, 16, 128, 2, 3, false>);
+    else go(q8_gemm_kernel<E, 12, 192, 2, 3, false>);
+  }
   return hipGetLastError();
 }
 

@@ -10,7 +10,11 @@ constexpr int kQ8KeepK = 2048;    // (padded) in features whose rows it keeps in
 constexpr int kQ8FusedMax = 16;   // rows that it brings to 8 bits itself, of at most kQ8KeepK
 constexpr int kQ8FloatMax = 4, kQ8FloatK = 12288;   // fp32 rows that it does, and their most features
 
-enum Q8Kernel { kQ8FewRows, kQ8Tile32x32, kQ8Tile32x64, kQ8Tile64x64, kQ8Gemm64, kQ8Gemm128 };
+// (tokens by features)
+enum Q8Kernel {
+  kQ8FewRows, kQ8Tile32x32, kQ8Tile32x64, kQ8Tile64x64, kQ8Gemm64, kQ8Gemm128, kQ8Gemm128x192, kQ8Gemm192x128,
+  kQ8Gemm128x256, kQ8Gemm192x192
+};
 
 struct Q8Plan {
   int32_t kernel;   // Q8Kernel
@@ -21,7 +25,7 @@ struct Q8Plan {
 // or 64 features, K split over the work-group's waves, operands straight from memory) hides the most latency,
 // but reads x and W again for every tile that needs them: it is taken while its tiles are no more than the 256
 // CUs.  Behind both, the products that share operands through LDS: 64 x 64 tiles until there are enough of
-// 128 x 128 for every CU.  Measured (us; few-row, 32 x 32, 32 x 64, 64 x 64 in LDS, 128 x 128 in LDS):
+// 128 x 128 for every CU, then the tile below.  Measured (us; few-row, 32 x 32, 32 x 64, 64 x 64 in LDS, 128 x 128 in LDS):
 //   tokens x features x K        few    32x32  32x64  64L    128L
 //   17 x 2048 x 1536             3.5    4.8    5.2    6.0    9.7
 //   32 x 1536 x 8960             7.9    10.0   12.5   22.1   38.4
@@ -36,7 +40,25 @@ struct Q8Plan {
 //   256 x 1536 x 8960            -      16.7   13.1   22.6   45.3
 //   512 x 17920 x 1536           -      -      48     28.2   25.2
 // (512 x 1536 x 8960: 64 x 64 straight from memory 18.3, through LDS 22.9; 400 x 2048 x 1536 6.6 both.)
-inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
+//
+// Of the large tiles the one whose work for the CU with the most tiles is least: rounds of 256 tiles, times the tile's
+// area, times 0.9 at one and a half and 0.84 at twice 128 x 128 and more, which read each operand for more
+// products; one round alone counts 1.2 times, with nothing beside a work-group to hide its waits.  Over 22 shapes
+// from 512 x 17920 x 1536 to 8192^3 that is 0.3% behind the best tile of each, 128 x 128 always 6.8%:
+//   tokens x features x K        128x128  128x192  192x128  128x256  192x192
+//   512 x 17920 x 1536           20.7     20.5     19.4     23.9     27.7
+//   2048 x 17920 x 1536          62.0     60.8     65.9     62.9     67.3
+//   4096 x 2048 x 1536           16.1     20.3     18.2     18.2     21.0
+//   4001 x 1536 x 8960           58.5     52.9     52.8     55.6     57.9
+//   16384 x 1536 x 8960          214      199      230      189      193
+//   1024 x 6144 x 4096           29.4     27.1     36.0     29.4     31.5
+//   6001 x 6144 x 4096           144      137      137      141      131
+//   3000 x 4096 x 14336          164      205      153      163      179
+//   4096 x 4096 x 4096           67.2     67.8     67.2     62.1     66.4
+//   8192 x 8192 x 8192           487      473      460      441      458
+// The gated product leaves twice the bytes and an exponential a result: there larger tiles gained nothing (a block of
+// 4,001 x 1536 x 8960 220 us with 128 x 128 and with 128 x 192, 224 with 128 x 256).
+inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp, bool gated) {
   constexpr int64_t kCus = 256;
   const auto plan = [&](Q8Kernel kernel, int tm, int np) {
     return Q8Plan{kernel, (int32_t)((int64_t)((rows + tm - 1) / tm) * ((panels + np - 1) / np))};
@@ -52,7 +74,21 @@ inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
     if (t32x64.tiles <= kCus) return t32x64;
     if (t64x64.tiles <= kCus && !keep) return t64x64;
   }
-  return g128.tiles < kCus ? g64 : g128;
+  if (g128.tiles < kCus) return g64;
+  Q8Plan best = g128;
+  int64_t least = INT64_MAX;
+  const auto consider = [&](Q8Kernel kernel, int tm, int np, int weight) {
+    const Q8Plan t = plan(kernel, tm, np);
+    const int64_t rounds = (t.tiles + kCus - 1) / kCus, cost = rounds * weight * (rounds == 1 ? 6 : 5);
+    if (cost < least) least = cost, best = t;
+  };
+  consider(kQ8Gemm128, 128, 8, 100);
+  if (gated) return best;
+  consider(kQ8Gemm128x192, 128, 12, 135);
+  consider(kQ8Gemm192x128, 192, 8, 135);
+  consider(kQ8Gemm128x256, 128, 16, 168);
+  consider(kQ8Gemm192x192, 192, 12, 189);
+  return best;
 }
 
 }  // namespace mi_fa2

@@ -216,7 +216,8 @@ PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96),
             (100, 128, 256), (127, 250, 128), (129, 257, 1000), (150, 896, 4864), (200, 1024, 64),
             (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
             (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200),
-            (3, 66000, 70), (2, 65553, 2100)]
+            (3, 66000, 70), (2, 65553, 2100), (151, 16383, 72), (262, 16323, 600), (644, 16598, 70),
+            (517, 13074, 300)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
