@@ -198,7 +198,7 @@ int product(Q8Params p, int dtype, bool gated, const void* values, const float* 
   p.x = values;
   p.x_scale = scale;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const mi_fa2::Q8Plan plan = mi_fa2::q8_plan(p.M, p.panels, p.Kp, gated);
+  const mi_fa2::Q8Plan plan = mi_fa2::q8_plan(p.M, p.panels, p.Kp);
   switch (plan.kernel) {
     case mi_fa2::kQ8Tile32x32:
     case mi_fa2::kQ8Tile32x64:

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) v
           for (int r = 0; r < 4; ++r) {
             const float g = q8_scaled(acc[i][j][8 * h + r], xs, gs[r]);
             const float u = q8_scaled(acc[i][j][8 * h + 4 + r], xs, us[r]);
-            o[r] = g / (1.f + expf(-g)) * u;
+            o[r] = q8_silu_mul(g, u);
           }
           *reinterpret_cast<f32x4*>(lds + t * kRow + (wn * TI * 16 + 4 * kc + 16 * i + 8 * h) * 4) = o;
         }
@@ -282,12 +282,10 @@ hipError_t launch_gemm_e(const Q8Params& p, const Q8Plan& plan, hipStream_t stre
   };
   if (plan.kernel == kQ8Gemm64) go(q8_gemm_kernel<E, 4, 64, 2, 4, GATED>);
   else if (plan.kernel == kQ8Gemm128) go(q8_gemm_kernel<E, 8, 128, 2, 3, GATED>);
-  else if constexpr (!GATED) {
-    if (plan.kernel == kQ8Gemm128x192) go(q8_gemm_kernel<E, 12, 128, 2, 3, false>);
-    else if (plan.kernel == kQ8Gemm192x128) go(q8_gemm_kernel<E, 8, 192, 2, 3, false>);
-    else if (plan.kernel == kQ8Gemm128x256) go(q8_gemm_kernel<E, 16, 128, 2, 3, false>);
-    else go(q8_gemm_kernel<E, 12, 192, 2, 3, false>);
-  }
+  else if (plan.kernel == kQ8Gemm128x192) go(q8_gemm_kernel<E, 12, 128, 2, 3, GATED>);
+  else if (plan.kernel == kQ8Gemm192x128) go(q8_gemm_kernel<E, 8, 192, 2, 3, GATED>);
+  else if (plan.kernel == kQ8Gemm192x192) go(q8_gemm_kernel<E, 12, 192, 2, 3, GATED>);
+  else go(q8_gemm_kernel<E, 16, 128, 2, 3, GATED>);
   return hipGetLastError();
 }
 

@@ -52,7 +52,7 @@ __device__ __forceinline__ void finish(const Q8Params& p, int f, int m, int g, b
     }
     if (g >= 2 || !live || f >= p.N) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = v[r] / (1.f + expf(-v[r])) * up[r];
+    for (int r = 0; r < 4; ++r) v[r] = q8_silu_mul(v[r], up[r]);
     // (the rows are padded to whole groups)
     *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + (int64_t)m * p.out_st + f) =
         f32x4{v[0], v[1], v[2], v[3]};

@@ -56,9 +56,11 @@ struct Q8Plan {
 //   3000 x 4096 x 14336          164      205      153      163      179
 //   4096 x 4096 x 4096           67.2     67.8     67.2     62.1     66.4
 //   8192 x 8192 x 8192           487      473      460      441      458
-// The gated product leaves twice the bytes and an exponential a result: there larger tiles gained nothing (a block of
-// 4,001 x 1536 x 8960 220 us with 128 x 128 and with 128 x 192, 224 with 128 x 256).
-inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp, bool gated) {
+// The gated product likewise, a block's three launches (tokens x hidden x inner size):
+//   4001 x 1536 x 8960           243      237      228      227      219
+//   1024 x 1536 x 8960           76.9     75.8     80.5     79.2     81.1
+//   2048 x 4096 x 14336          399      395      392      374      382
+inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
   constexpr int64_t kCus = 256;
   const auto plan = [&](Q8Kernel kernel, int tm, int np) {
     return Q8Plan{kernel, (int32_t)((int64_t)((rows + tm - 1) / tm) * ((panels + np - 1) / np))};
@@ -83,11 +85,10 @@ inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp, bool gated) {
     if (cost < least) least = cost, best = t;
   };
   consider(kQ8Gemm128, 128, 8, 100);
-  if (gated) return best;
-  consider(kQ8Gemm128x192, 128, 12, 135);
   consider(kQ8Gemm192x128, 192, 8, 135);
-  consider(kQ8Gemm128x256, 128, 16, 168);
+  consider(kQ8Gemm128x192, 128, 12, 135);
   consider(kQ8Gemm192x192, 192, 12, 189);
+  consider(kQ8Gemm128x256, 128, 16, 168);
   return best;
 }
 

@@ -19,18 +19,18 @@ SHAPE = {T32X32: (32, 32), T32X64: (32, 64), T64X64: (64, 64), G64: (64, 64), G1
 def _library():
     with tempfile.TemporaryDirectory() as tmp:
         fn = rules(Path(tmp), "q8_rule.h", """
-int plan(int rows, int panels, int kp, int gated, int* tiles) {
-  const mi_fa2::Q8Plan p = mi_fa2::q8_plan(rows, panels, kp, gated != 0);
+int plan(int rows, int panels, int kp, int* tiles) {
+  const mi_fa2::Q8Plan p = mi_fa2::q8_plan(rows, panels, kp);
   *tiles = p.tiles;
   return p.kernel;
 }""").plan
-    fn.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(ctypes.c_int)]
+    fn.argtypes = [ctypes.c_int] * 3 + [ctypes.POINTER(ctypes.c_int)]
     return fn
 
 
-def plan(rows, features, k, gated=False):
+def plan(rows, features, k):
     tiles = ctypes.c_int()
-    kernel = _library()(rows, -(-features // 16), -(-k // 128) * 128, gated, ctypes.byref(tiles))
+    kernel = _library()(rows, -(-features // 16), -(-k // 128) * 128, ctypes.byref(tiles))
     return kernel, tiles.value
 
 
@@ -39,8 +39,8 @@ def plan(rows, features, k, gated=False):
     (64, 6144, 2048, FEW), (32, 1536, 8960, FEW), (32, 6144, 4096, T32X32), (32, 14336, 4096, T32X64),
     (33, 1536, 8960, T32X32), (64, 6144, 4096, T32X64), (64, 9728, 896, G64), (64, 17920, 1536, G64),
     (17, 151936, 1536, G128), (150, 896, 4864, T32X32), (256, 1536, 8960, T32X64),
-    (512, 1536, 8960, T64X64), (400, 2048, 1536, G64), (512, 17920, 1536, G128X192),
-    (4096, 2048, 1536, G128), (2048, 17920, 1536, G128X192), (4001, 1536, 8960, G128X192),
+    (512, 1536, 8960, T64X64), (400, 2048, 1536, G64), (512, 17920, 1536, G192X128),
+    (4096, 2048, 1536, G128), (2048, 17920, 1536, G128X192), (4001, 1536, 8960, G192X128), (4096, 1536, 8960, G128X192),
     (16384, 1536, 8960, G128X256), (6001, 6144, 4096, G192X192), (3000, 4096, 14336, G192X128),
     (8192, 8192, 8192, G128X256), (1, 1, 1, FEW), (65, 1, 1, T32X32)])
 def test_kernels(rows, features, k, kernel):
@@ -61,4 +61,4 @@ def test_work_groups_cover_every_result():
 
 def test_the_gpu_tests_reach_every_kernel():
     assert {plan(*size)[0] for size in test_q8_gpu.PRODUCTS} == set(range(10))
-    assert {plan(m, 2 * inter, hidden, True)[0] for m, hidden, inter in test_q8_gpu.MLPS} == set(range(6))
+    assert {plan(m, 2 * inter, hidden)[0] for m, hidden, inter in test_q8_gpu.MLPS} == set(range(10))
