@@ -71,8 +71,14 @@ typedef struct mi_q8_norm_args {
 MI_Q8_API int mi_q8_add_rmsnorm(const mi_q8_norm_args* args, void* stream);
 
 /* out [rows, n] = values * scale, rounded. */
-MI_Q8_API int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
-                               int64_t out_stride, int32_t rows, int32_t n, void* stream);
+typedef struct mi_q8_dequantize_args {
+  const void* values;
+  const float* scale;
+  void* out;
+  int64_t out_stride;
+  int32_t dtype, rows, n;
+} mi_q8_dequantize_args;
+MI_Q8_API int mi_q8_dequantize(const mi_q8_dequantize_args* args, void* stream);
 
 /*
  * A weight's values (int8, rows of in_features, `stride` bytes apart) in the products' layout:

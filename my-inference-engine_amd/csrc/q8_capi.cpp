@@ -302,19 +302,20 @@ int mi_q8_add_rmsnorm(const mi_q8_norm_args* args, void* stream) {
                   a.residual_stride, a.values, a.scale, a.rows, a.n, stream);
 }
 
-int mi_q8_dequantize(int32_t dtype, const void* values, const float* scale, void* out,
-                     int64_t out_stride, int32_t rows, int32_t n, void* stream) {
-  if (int rc = check_dtype(dtype)) return rc;
-  if (int rc = check_count("rows", rows, 0, kMaxRows)) return rc;
-  if (int rc = check_count("n", n, 1, kMaxK)) return rc;
-  if (rows == 0) return ok();
-  if (int rc = check_ptr("values", values, 16)) return rc;
-  if (int rc = check_ptr("scale", scale, 4)) return rc;
-  if (int rc = check_rows("out", out, out_stride, n)) return rc;
-  mi_fa2::Q8DequantParams p{static_cast<const int8_t*>(values), scale, static_cast<uint16_t*>(out),
-                            out_stride, rows, n, q8_pad(n)};
+int mi_q8_dequantize(const mi_q8_dequantize_args* args, void* stream) {
+  if (!args) return fail(kInvalid, "args is NULL");
+  const mi_q8_dequantize_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (int rc = check_count("rows", a.rows, 0, kMaxRows)) return rc;
+  if (int rc = check_count("n", a.n, 1, kMaxK)) return rc;
+  if (a.rows == 0) return ok();
+  if (int rc = check_ptr("values", a.values, 16)) return rc;
+  if (int rc = check_ptr("scale", a.scale, 4)) return rc;
+  if (int rc = check_rows("out", a.out, a.out_stride, a.n)) return rc;
+  mi_fa2::Q8DequantParams p{static_cast<const int8_t*>(a.values), a.scale, static_cast<uint16_t*>(a.out),
+                            a.out_stride, a.rows, a.n, q8_pad(a.n)};
   return launched(
-      mi_fa2::launch_q8_dequant(p, dtype, reinterpret_cast<hipStream_t>(stream)));
+      mi_fa2::launch_q8_dequant(p, a.dtype, reinterpret_cast<hipStream_t>(stream)));
 }
 
 size_t mi_q8_packed_bytes(int32_t out_features, int32_t in_features, int32_t gated) {

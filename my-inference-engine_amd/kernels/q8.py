@@ -42,7 +42,7 @@ SIGNATURES = {
     "mi_q8_rows_bytes": (_sz, [_i32, _i32]),
     "mi_q8_quantize": (_i32, [_i32, _p, _i64, _p, _p, _i32, _i32, _p]),
     "mi_q8_add_rmsnorm": (_i32, [_args, _p]),
-    "mi_q8_dequantize": (_i32, [_i32, _p, _p, _p, _i64, _i32, _i32, _p]),
+    "mi_q8_dequantize": (_i32, [_args, _p]),
     "mi_q8_packed_bytes": (_sz, [_i32, _i32, _i32]),
     "mi_q8_pack": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _p]),
     "mi_q8_linear_workspace_size": (_sz, [_i32, _i32]),
@@ -53,6 +53,7 @@ SIGNATURES = {
 }
 # the argument structs, packed in one go: a call of 18 arguments costs ctypes 1.9 us, this 0.6
 NORM_ARGS = struct.Struct("@PqPqPPqPPiiif")
+DEQUANTIZE_ARGS = struct.Struct("@PPPqiii")
 LINEAR_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
 QKV_ARGS = struct.Struct("@PqPPPPPPqPPqPPqqiiiiiif")
 MLP_ARGS = struct.Struct("@PqPPPPPPqPqPNiiiif")
@@ -178,8 +179,8 @@ class Rows:
         else:
             _, os_ = _rows(out, "out", dt, dev)
             assert out.shape == (R, self.n), f"out: [{R}, {self.n}]"
-        call(dev.index, load().mi_q8_dequantize, _lib.DTYPES[dt], self.data.data_ptr(),
-             scale.data_ptr(), out.data_ptr(), os_, R, self.n)
+        call(dev.index, load().mi_q8_dequantize, DEQUANTIZE_ARGS.pack(
+            self.data.data_ptr(), scale.data_ptr(), out.data_ptr(), os_, _lib.DTYPES[dt], R, self.n))
         return out
 
 

@@ -44,9 +44,9 @@ def _norm(**over):
 
 
 def _dequantize(**over):
-    a = dict(dtype=0, values=16, scale=16, out=16, os=64, rows=3, n=64)
+    a = dict(values=16, scale=16, out=16, os=64, dtype=0, rows=3, n=64)
     a.update(over)
-    return q8.load().mi_q8_dequantize(*a.values(), None)
+    return q8.load().mi_q8_dequantize(q8.DEQUANTIZE_ARGS.pack(*(v or 0 for v in a.values())), None)
 
 
 def _pack(**over):
@@ -145,7 +145,7 @@ def test_refusals(call, over, status, msg):
 
 def test_arguments_that_are_not_there():
     lib = q8.load()
-    for fn in (lib.mi_q8_add_rmsnorm, lib.mi_q8_linear, lib.mi_q8_mlp, lib.mi_q8_qkv_rope):
+    for fn in (lib.mi_q8_add_rmsnorm, lib.mi_q8_dequantize, lib.mi_q8_linear, lib.mi_q8_mlp, lib.mi_q8_qkv_rope):
         assert fn(None, None) == 1 and "args is NULL" in last()
 
 
@@ -153,10 +153,10 @@ STRUCTS = """
 #include <stdio.h>
 #include "mi_q8.h"
 int main() {
-  printf("%zu %zu %zu %zu\\n", sizeof(mi_q8_norm_args), sizeof(mi_q8_linear_args), sizeof(mi_q8_mlp_args),
-         sizeof(mi_q8_qkv_rope_args));
-  printf("%zu %zu %zu %zu\\n", offsetof(mi_q8_norm_args, eps), offsetof(mi_q8_linear_args, eps),
-         offsetof(mi_q8_mlp_args, eps), offsetof(mi_q8_qkv_rope_args, eps));
+  printf("%zu %zu %zu %zu %zu\\n", sizeof(mi_q8_dequantize_args), sizeof(mi_q8_norm_args), sizeof(mi_q8_linear_args),
+         sizeof(mi_q8_mlp_args), sizeof(mi_q8_qkv_rope_args));
+  printf("%zu %zu %zu %zu %zu\\n", offsetof(mi_q8_dequantize_args, n), offsetof(mi_q8_norm_args, eps),
+         offsetof(mi_q8_linear_args, eps), offsetof(mi_q8_mlp_args, eps), offsetof(mi_q8_qkv_rope_args, eps));
 }
 """
 
@@ -166,7 +166,7 @@ def test_argument_structs_are_the_headers(tmp_path):
     subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
     sizes, ends = (list(map(int, line.split())) for line in subprocess.run(
         [str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.splitlines())
-    for st, size, end in zip((q8.NORM_ARGS, q8.LINEAR_ARGS, q8.MLP_ARGS, q8.QKV_ARGS), sizes, ends):
+    for st, size, end in zip((q8.DEQUANTIZE_ARGS, q8.NORM_ARGS, q8.LINEAR_ARGS, q8.MLP_ARGS, q8.QKV_ARGS), sizes, ends):
         assert st.size == end + 4 and st.size <= size < st.size + 8   # (the struct ends aligned)
 
 
