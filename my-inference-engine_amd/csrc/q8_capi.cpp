@@ -200,19 +200,16 @@ int product(Q8Params p, int dtype, bool gated, const void* values, const float* 
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const mi_fa2::Q8Plan plan = mi_fa2::q8_plan(p.M, p.panels, p.Kp);
   switch (plan.kernel) {
+    case mi_fa2::kQ8FewRows: {
+      int cus = 0;
+      if (int rc = compute_units(&cus)) return rc;
+      return launched(mi_fa2::launch_q8_rows(p, dtype, gated, mi_fa2::kQ8Rows, cus, st));
+    }
     case mi_fa2::kQ8Tile32x32:
     case mi_fa2::kQ8Tile32x64:
     case mi_fa2::kQ8Tile64x64: return launched(mi_fa2::launch_q8_tile(p, plan, dtype, gated, st));
-    case mi_fa2::kQ8Gemm64:
-    case mi_fa2::kQ8Gemm128:
-    case mi_fa2::kQ8Gemm128x192:
-    case mi_fa2::kQ8Gemm192x128:
-    case mi_fa2::kQ8Gemm128x256:
-    case mi_fa2::kQ8Gemm192x192: return launched(mi_fa2::launch_q8_gemm(p, plan, dtype, gated, st));
+    default: return launched(mi_fa2::launch_q8_gemm(p, plan, dtype, gated, st));
   }
-  int cus = 0;
-  if (int rc = compute_units(&cus)) return rc;
-  return launched(mi_fa2::launch_q8_rows(p, dtype, gated, mi_fa2::kQ8Rows, cus, st));
 }
 
 // The product of 16-bit rows, brought to 8 bits in the same launch where the few-row kernel does that,

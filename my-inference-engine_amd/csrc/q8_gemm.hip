@@ -1,8 +1,8 @@
 // Products of many rows in 8 bits with a packed 8-bit weight: out[M][N] = x[M][K] W[N][K]^T.
 //
-// A work-group of 4 waves computes TM tokens by NP panels (128 x 128, a wave 64 x 64; or 64 x 64, a wave
-// 32 x 32) with v_mfma_i32_32x32x32_i8.  W is the A operand, so a lane's four sums in a row are four
-// features of one token.  Both operands come in panels (q8.h): a stage of 64 of K is NP + TM / 16 loads of 1 KB
+// A work-group of 4 waves (8) computes TM tokens by NP panels (64 x 64, a wave 32 x 32; 128 x 128, a wave 64 x 64;
+// up to 256 x 256, a wave 64 tokens by 128 features) with v_mfma_i32_32x32x32_i8.  W is the A operand, so a lane's
+// four sums in a row are four features of one token.  Both operands come in panels (q8.h): a stage of 64 of K is NP + TM / 16 loads of 1 KB
 // straight into LDS, and a 32 x 32 operand is read out of two panels' kilobytes, 16 lanes in a run, with no two
 // on a bank.  ST stages are in flight.  A stage's operands are read during the MFMAs of the stage before, behind
 // one barrier a stage; the loads ST stages ahead follow between the second half of the MFMAs (reads, then
@@ -13,13 +13,13 @@
 // silu(g) u leaves in fp32: in bfloat16 the values between half the row's largest and the largest lie half a
 // step of the 8 bits apart, so one in eight of them would move by a whole step.
 //
-// Measured (rows in 8 bits, launches in a graph, two cards): 8192^3 490-531 us (2.07-2.24 POP/s; the library's
-// int8 product 2.06 on the first), 6001 x 6144 x 4096 144-154 us (the library's 180), 4001 x 17920 x 1536
-// 122-132, 4001 x 1536 x 8960 60-64, 4096 x 2048 x 1536 17.4-20.1 (the library's 25.0).  What bounds the long ones is power: the MFMAs alone run at 3.8 POP/s, here a stage of
-// three work-groups takes 900 cycles for 768 of MFMAs, at 1.4 GHz; the same launch on zeros runs at 1.9 GHz and
-// 3.1 POP/s.  128 x 256 tiles move a quarter less and are no faster (8192^3 495 and 505 us, 4001 x 1536 x 8960
-// 61 and 64).  K of 1536 is only 24 stages: there a tile's start and its results show (without the stores
-// 4001 x 17920 x 1536 took 119 us for 121, 4096 x 2048 x 1536 18.2 for 20.1).
+// Measured (rows in 8 bits, launches in a graph, several cards): 8192^3 426-435 us (2.53-2.58 POP/s; the library's
+// int8 product 2.06), 4096^3 60-61, 6001 x 6144 x 4096 130-137 us (the library's 180), 4096 x 17920 x 1536
+// 112-122 (140), 4001 x 1536 x 8960 53-59 (70), 4096 x 2048 x 1536 16.1-20.1 (25.0).  What bounds the long ones is
+// power: the MFMAs alone run at 3.8 POP/s; with 128 x 128 tiles 8192^3 ran at 1.4 GHz (a stage of three work-groups
+// 900 cycles for 768 of MFMAs), and on zeros at 1.9 GHz and 3.1 POP/s.  Larger tiles move fewer bytes for a product
+// (128 x 128 483 us, 128 x 256 441, 256 x 256 426).  K of 1536 is only 24 stages: there a tile's start and its
+// results show (without the stores 4001 x 17920 x 1536 took 119 us for 121, 4096 x 2048 x 1536 18.2 for 20.1).
 #include "q8.h"
 
 #include <algorithm>
@@ -28,7 +28,6 @@ namespace mi_fa2 {
 
 namespace {
 
-constexpr int kQgThreads = 256, kQgWaves = 4;
 
 // lds_dma16 with a wave-uniform byte offset beside the lanes' (which alone are held against `bytes`).
 __device__ __forceinline__ void lds_dma16_at(uint64_t base, uint32_t bytes, uint32_t lds_addr,
@@ -64,14 +63,14 @@ __device__ __forceinline__ void wait_loads_and_barrier() {
 }  // namespace
 
 // WN of the waves stand side by side along W.  A CU holds three work-groups of 128 x 128 (135 registers), two of
-// the larger tiles; fewer hide less (128 x 128 with a fourth stage, and so with two: 150 -> 186 us for 6001 x 6144 x
-// 4096; 128 x 192 with a fourth, and so with one: 137 -> 222).
-template <typename E, int NP, int TM, int WN, int ST, bool GATED>
-__global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
-  constexpr int WM = kQgWaves / WN;
+// the larger tiles, or one of 8 waves (256 x 256: as many waves, a third fewer loads); fewer hide less (6001 x 6144
+// x 4096 with 128 x 128 in four stages, and so two a CU, 150 -> 186 us; with 128 x 192 in four, and so one, 137 -> 222).
+template <typename E, int NP, int TM, int WN, int ST, bool GATED, int WAVES = 4>
+__global__ __launch_bounds__(WAVES * 64, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) void q8_gemm_kernel(const Q8Params p) {
+  constexpr int kThreads = WAVES * 64, WM = WAVES / WN;
   constexpr int TI = NP * 16 / WN / 32, TJ = TM / WM / 32;
   constexpr int kStage = NP * 1024 + TM * 64;
-  constexpr int LW = NP / kQgWaves, LX = TM / 16 / kQgWaves, kLoads = LW + LX;
+  constexpr int LW = NP / WAVES, LX = TM / 16 / WAVES, kLoads = LW + LX;
   // the tile on its way out: rows of tokens, 16-bit results or fp32 activations (half as many)
   constexpr int kRow = NP * 16 * 2 + 16;
   constexpr int kTile = ST * kStage > TM * kRow ? ST * kStage : TM * kRow;
@@ -111,8 +110,9 @@ __global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) v
   }
   const auto load = [&](int i, int s, int buf) {   // one of a stage's kLoads
     const uint32_t at = lds0 + buf * kStage + wave * 1024;
-    if (i < LW) lds_dma16_at(w_base, w_bytes, at + i * 4096, off + i * 64 * p.Kp, s * 1024);
-    else lds_dma16_at(x_base, x_bytes, at + NP * 1024 + (i - LW) * 4096, off + (i - LW) * 64 * p.Kp, s * 1024);
+    if (i < LW) lds_dma16_at(w_base, w_bytes, at + i * WAVES * 1024, off + i * WAVES * 16 * p.Kp, s * 1024);
+    else
+      lds_dma16_at(x_base, x_bytes, at + (NP + (i - LW) * WAVES) * 1024, off + (i - LW) * WAVES * 16 * p.Kp, s * 1024);
   };
 
   i32x16 acc[TI][TJ];
@@ -205,8 +205,8 @@ __global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) v
     __syncthreads();
     float* out = static_cast<float*>(p.out) + (int64_t)m0 * p.out_st + f0;
 #pragma unroll
-    for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
-      const int t = (tid + e * kQgThreads) / kPieces, c = (tid + e * kQgThreads) % kPieces;
+    for (int e = 0; e < TM * kPieces / kThreads; ++e) {
+      const int t = (tid + e * kThreads) / kPieces, c = (tid + e * kThreads) % kPieces;
       if (m0 + t < p.M && f0 + 4 * c < p.N)
         *reinterpret_cast<f32x4*>(out + t * p.out_st + 4 * c) =
             *reinterpret_cast<const f32x4*>(lds + t * kRow + c * 16);
@@ -219,19 +219,19 @@ __global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) v
     if (p.bias && tid < NP * 16 && tid < n_left) my_bias = p.bias[panel0 * 16 + tid];
     if (p.res) {
       // the residual takes its place in LDS, where the sums then meet it
-      constexpr int kEach = TM * kPieces / kQgThreads, kBatch = kEach > 12 ? kEach / 2 : kEach;
+      constexpr int kEach = TM * kPieces / kThreads, kBatch = kEach > 12 ? kEach / 2 : kEach;
 #pragma unroll
       for (int first = 0; first < kEach; first += kBatch) {
         u32x4 res[kBatch];
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
-          const int at = tid + (first + e) * kQgThreads, m = min(m0 + at / kPieces, p.M - 1);
+          const int at = tid + (first + e) * kThreads, m = min(m0 + at / kPieces, p.M - 1);
           res[e] = q8_load8(p.res + m * p.res_st + panel0 * 16, at % kPieces, n_left);
         }
         if (first == 0) __syncthreads();
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
-          const int at = tid + (first + e) * kQgThreads, c = at % kPieces;
+          const int at = tid + (first + e) * kThreads, c = at % kPieces;
           *reinterpret_cast<u32x4*>(lds + at / kPieces * kRow + c * 16) = q8_cut8(res[e], c, n_left);
         }
       }
@@ -261,8 +261,8 @@ __global__ __launch_bounds__(kQgThreads, NP * TM > 1024 ? 2 : NP == 8 ? 3 : 4) v
       }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < TM * kPieces / kQgThreads; ++e) {
-      const int t = (tid + e * kQgThreads) / kPieces, c = (tid + e * kQgThreads) % kPieces;
+    for (int e = 0; e < TM * kPieces / kThreads; ++e) {
+      const int t = (tid + e * kThreads) / kPieces, c = (tid + e * kThreads) % kPieces;
       const u32x4 v = *reinterpret_cast<const u32x4*>(lds + t * kRow + c * 16);
       if (m0 + t >= p.M) break;
       if (8 * c + 8 <= n_left)
@@ -277,15 +277,19 @@ namespace {
 
 template <typename E, bool GATED>
 hipError_t launch_gemm_e(const Q8Params& p, const Q8Plan& plan, hipStream_t stream) {
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(plan.tiles), dim3(kQgThreads), 0, stream, p);
+  const auto go = [&](auto kernel, int threads = 256) {
+    hipLaunchKernelGGL(kernel, dim3(plan.tiles), dim3(threads), 0, stream, p);
   };
-  if (plan.kernel == kQ8Gemm64) go(q8_gemm_kernel<E, 4, 64, 2, 4, GATED>);
-  else if (plan.kernel == kQ8Gemm128) go(q8_gemm_kernel<E, 8, 128, 2, 3, GATED>);
-  else if (plan.kernel == kQ8Gemm128x192) go(q8_gemm_kernel<E, 12, 128, 2, 3, GATED>);
-  else if (plan.kernel == kQ8Gemm192x128) go(q8_gemm_kernel<E, 8, 192, 2, 3, GATED>);
-  else if (plan.kernel == kQ8Gemm192x192) go(q8_gemm_kernel<E, 12, 192, 2, 3, GATED>);
-  else go(q8_gemm_kernel<E, 16, 128, 2, 3, GATED>);
+  switch (plan.kernel) {
+    case kQ8Gemm64: go(q8_gemm_kernel<E, 4, 64, 2, 4, GATED>); break;
+    case kQ8Gemm128: go(q8_gemm_kernel<E, 8, 128, 2, 3, GATED>); break;
+    case kQ8Gemm128x192: go(q8_gemm_kernel<E, 12, 128, 2, 3, GATED>); break;
+    case kQ8Gemm192x128: go(q8_gemm_kernel<E, 8, 192, 2, 3, GATED>); break;
+    case kQ8Gemm128x256: go(q8_gemm_kernel<E, 16, 128, 2, 3, GATED>); break;
+    case kQ8Gemm192x192: go(q8_gemm_kernel<E, 12, 192, 2, 3, GATED>); break;
+    case kQ8Gemm256x256: go(q8_gemm_kernel<E, 16, 256, 2, 4, GATED, 8>, 512); break;
+    default: return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 

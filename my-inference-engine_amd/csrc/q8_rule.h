@@ -13,7 +13,7 @@ constexpr int kQ8FloatMax = 4, kQ8FloatK = 12288;   // fp32 rows that it does, a
 // (tokens by features)
 enum Q8Kernel {
   kQ8FewRows, kQ8Tile32x32, kQ8Tile32x64, kQ8Tile64x64, kQ8Gemm64, kQ8Gemm128, kQ8Gemm128x192, kQ8Gemm192x128,
-  kQ8Gemm128x256, kQ8Gemm192x192
+  kQ8Gemm128x256, kQ8Gemm192x192, kQ8Gemm256x256
 };
 
 struct Q8Plan {
@@ -42,20 +42,23 @@ struct Q8Plan {
 // (512 x 1536 x 8960: 64 x 64 straight from memory 18.3, through LDS 22.9; 400 x 2048 x 1536 6.6 both.)
 //
 // Of the large tiles the one whose work for the CU with the most tiles is least: rounds of 256 tiles, times the tile's
-// area, times 0.9 at one and a half and 0.84 at twice 128 x 128 and more, which read each operand for more
-// products; one round alone counts 1.2 times, with nothing beside a work-group to hide its waits.  Over 22 shapes
-// from 512 x 17920 x 1536 to 8192^3 that is 0.3% behind the best tile of each, 128 x 128 always 6.8%:
-//   tokens x features x K        128x128  128x192  192x128  128x256  192x192
+// area, times 0.9 at one and a half times 128 x 128, 0.84 at twice and 0.81 at four times, which read each operand for
+// more products; a single round of work-groups of four waves counts 1.2 times, with nothing beside them to hide their
+// waits.  Over 22 shapes from 512 x 17920 x 1536 to 8192^3 that is 0.3% behind the best of the first five, 128 x 128
+// always 6.8%:
+//   tokens x features x K        128x128  128x192  192x128  128x256  192x192  256x256
 //   512 x 17920 x 1536           20.7     20.5     19.4     23.9     27.7
 //   2048 x 17920 x 1536          62.0     60.8     65.9     62.9     67.3
+//   4096 x 17920 x 1536          120      118      124      112      119      128
 //   4096 x 2048 x 1536           16.1     20.3     18.2     18.2     21.0
 //   4001 x 1536 x 8960           58.5     52.9     52.8     55.6     57.9
-//   16384 x 1536 x 8960          214      199      230      189      193
+//   16384 x 1536 x 8960          211      199      230      187      192      201
 //   1024 x 6144 x 4096           29.4     27.1     36.0     29.4     31.5
-//   6001 x 6144 x 4096           144      137      137      141      131
-//   3000 x 4096 x 14336          164      205      153      163      179
-//   4096 x 4096 x 4096           67.2     67.8     67.2     62.1     66.4
-//   8192 x 8192 x 8192           487      473      460      441      458
+//   6001 x 6144 x 4096           142      137      137      139      130      156
+//   1000 x 14336 x 4096          62.3     65.3     63.6     55.9     59.8     53.6
+//   4096 x 4096 x 4096           65.9     67.8     67.2     61.0     66.7     60.4
+//   4096 x 4096 x 14336          223      -        -        194      206      184
+//   8192 x 8192 x 8192           483      473      460      441      458      426
 // The gated product likewise, a block's three launches (tokens x hidden x inner size):
 //   4001 x 1536 x 8960           243      237      228      227      219
 //   1024 x 1536 x 8960           76.9     75.8     80.5     79.2     81.1
@@ -81,7 +84,9 @@ inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
   int64_t least = INT64_MAX;
   const auto consider = [&](Q8Kernel kernel, int tm, int np, int weight) {
     const Q8Plan t = plan(kernel, tm, np);
-    const int64_t rounds = (t.tiles + kCus - 1) / kCus, cost = rounds * weight * (rounds == 1 ? 6 : 5);
+    const int64_t rounds = (t.tiles + kCus - 1) / kCus;
+    const bool alone = rounds == 1 && kernel != kQ8Gemm256x256;
+    const int64_t cost = rounds * weight * (alone ? 6 : 5);
     if (cost < least) least = cost, best = t;
   };
   consider(kQ8Gemm128, 128, 8, 100);
@@ -89,6 +94,7 @@ inline Q8Plan q8_plan(int32_t rows, int32_t panels, int32_t kp) {
   consider(kQ8Gemm128x192, 128, 12, 135);
   consider(kQ8Gemm192x192, 192, 12, 189);
   consider(kQ8Gemm128x256, 128, 16, 168);
+  consider(kQ8Gemm256x256, 256, 16, 325);
   return best;
 }
 

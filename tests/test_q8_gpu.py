@@ -217,7 +217,7 @@ PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96),
             (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
             (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200),
             (3, 66000, 70), (2, 65553, 2100), (151, 16383, 72), (262, 16323, 600), (644, 16598, 70),
-            (517, 13074, 300), (193, 16455, 200)]
+            (517, 13074, 300), (193, 16455, 200), (644, 16405, 300), (771, 16440, 72)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -284,7 +284,7 @@ def mlp_bounds(rows, gate_up, gate_up_scale, down, down_scale):
 MLPS = [(1, 1536, 8960), (1, 64, 8), (2, 100, 36), (16, 1536, 8960), (5, 128, 17), (17, 896, 4864),
         (33, 300, 500), (64, 256, 1000), (65, 512, 1024), (150, 896, 4864), (260, 640, 1531),
         (515, 256, 768), (130, 512, 1100), (400, 2176, 750), (40, 64, 4201), (600, 128, 3500), (138, 70, 8192),
-        (757, 100, 5548), (166, 72, 8203), (2443, 40, 3093), (920, 200, 3081), (1014, 72, 2981)]
+        (757, 100, 5548), (166, 72, 8203), (2443, 40, 3093), (920, 200, 3081), (1014, 72, 2981), (1239, 40, 6249), (2321, 40, 4339)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -10,9 +10,10 @@ import pytest
 import test_q8_gpu
 from host_rules import rules
 
-FEW, T32X32, T32X64, T64X64, G64, G128, G128X192, G192X128, G128X256, G192X192 = range(10)
+FEW, T32X32, T32X64, T64X64, G64, G128, G128X192, G192X128, G128X256, G192X192, G256X256 = range(11)
 SHAPE = {T32X32: (32, 32), T32X64: (32, 64), T64X64: (64, 64), G64: (64, 64), G128: (128, 128),
-         G128X192: (128, 192), G192X128: (192, 128), G128X256: (128, 256), G192X192: (192, 192)}
+         G128X192: (128, 192), G192X128: (192, 128), G128X256: (128, 256), G192X192: (192, 192),
+         G256X256: (256, 256)}
 
 
 @functools.lru_cache(None)
@@ -42,7 +43,7 @@ def plan(rows, features, k):
     (512, 1536, 8960, T64X64), (400, 2048, 1536, G64), (512, 17920, 1536, G192X128),
     (4096, 2048, 1536, G128), (2048, 17920, 1536, G128X192), (4001, 1536, 8960, G192X128), (4096, 1536, 8960, G128X192),
     (16384, 1536, 8960, G128X256), (6001, 6144, 4096, G192X192), (3000, 4096, 14336, G192X128),
-    (8192, 8192, 8192, G128X256), (1, 1, 1, FEW), (65, 1, 1, T32X32)])
+    (8192, 8192, 8192, G256X256), (4096, 6144, 4096, G128X256), (1, 1, 1, FEW), (65, 1, 1, T32X32)])
 def test_kernels(rows, features, k, kernel):
     assert plan(rows, features, k)[0] == kernel
 
@@ -60,5 +61,5 @@ def test_work_groups_cover_every_result():
 
 
 def test_the_gpu_tests_reach_every_kernel():
-    assert {plan(*size)[0] for size in test_q8_gpu.PRODUCTS} == set(range(10))
-    assert {plan(m, 2 * inter, hidden)[0] for m, hidden, inter in test_q8_gpu.MLPS} == set(range(10))
+    assert {plan(*size)[0] for size in test_q8_gpu.PRODUCTS} == set(range(11))
+    assert {plan(m, 2 * inter, hidden)[0] for m, hidden, inter in test_q8_gpu.MLPS} == set(range(11))
