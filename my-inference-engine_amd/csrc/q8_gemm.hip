@@ -13,8 +13,8 @@
 // silu(g) u leaves in fp32: in bfloat16 the values between half the row's largest and the largest lie half a
 // step of the 8 bits apart, so one in eight of them would move by a whole step.
 //
-// Measured (rows in 8 bits, launches in a graph, several cards): 8192^3 426-435 us (2.53-2.58 POP/s; the library's
-// int8 product 2.06), 4096^3 60-61, 6001 x 6144 x 4096 130-137 us (the library's 180), 4096 x 17920 x 1536
+// Measured (rows in 8 bits, launches in a graph, several cards): 8192^3 426-459 us (2.40-2.58 POP/s; the library's
+// int8 product 2.06), 4096^3 60-61, 6001 x 6144 x 4096 130-137 (the library's 180), 4096 x 17920 x 1536
 // 112-122 (140), 4001 x 1536 x 8960 53-59 (70), 4096 x 2048 x 1536 16.1-20.1 (25.0).  What bounds the long ones is
 // power: the MFMAs alone run at 3.8 POP/s; with 128 x 128 tiles 8192^3 ran at 1.4 GHz (a stage of three work-groups
 // 900 cycles for 768 of MFMAs), and on zeros at 1.9 GHz and 3.1 POP/s.  Larger tiles move fewer bytes for a product
