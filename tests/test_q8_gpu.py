@@ -284,7 +284,8 @@ def mlp_bounds(rows, gate_up, gate_up_scale, down, down_scale):
 MLPS = [(1, 1536, 8960), (1, 64, 8), (2, 100, 36), (16, 1536, 8960), (5, 128, 17), (17, 896, 4864),
         (33, 300, 500), (64, 256, 1000), (65, 512, 1024), (150, 896, 4864), (260, 640, 1531),
         (515, 256, 768), (130, 512, 1100), (400, 2176, 750), (40, 64, 4201), (600, 128, 3500), (138, 70, 8192),
-        (757, 100, 5548), (166, 72, 8203), (2443, 40, 3093), (920, 200, 3081), (1014, 72, 2981), (1239, 40, 6249), (2321, 40, 4339)]
+        (757, 100, 5548), (166, 72, 8203), (2443, 40, 3093), (920, 200, 3081), (1014, 72, 2981), (1239, 40, 6249),
+        (2321, 40, 4339), (3, 64, 20000), (40, 48, 33001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -383,6 +384,36 @@ def test_quantized_weight_is_a_row_for_each_feature():
     check_rows(rows, w, 2 * U)
     assert torch.equal(got.data.cpu(), o8.packed(rows.values.cpu()).flatten())
     assert torch.equal(got.scale, rows.scale)
+
+
+@pytest.mark.parametrize("m,n", [(1, 40), (16, 300), (30, 200), (70, 130), (300, 1000), (600, 2100), (2048, 2100),
+                                 (1300, 6200)])
+def test_longest_sums(m, n):
+    """in_features 131,072 with every value at 127: 2,114,060,288, the largest sum in 32 bits."""
+    announce(f"longest sums {m} x {n}")
+    g = torch.Generator(device=DEV).manual_seed(m)
+    sign_x, sign_w = (torch.randint(0, 2, (c, 1), generator=g, device=DEV) * 2 - 1 for c in (m, n))
+    x = (sign_x * 0.375).bfloat16().expand(m, q8.MAX_IN).contiguous()
+    scale = torch.rand(n, generator=g, device=DEV) + 0.5
+    w = q8.Weight((sign_w * 127).to(torch.int8).expand(n, q8.MAX_IN).contiguous(), scale)
+    rows = q8.quantize(x)
+    total = (sign_x * sign_w.t() * (127 * 127 * q8.MAX_IN)).float()
+    want = (total * rows.scale[:, None] * scale).bfloat16()
+    assert torch.equal(q8.linear(rows, w), want) and torch.equal(q8.linear(x, w), want)
+
+
+def test_most_rows():
+    announce("most rows")
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn(q8.MAX_ROWS, 24, generator=g, device=DEV, dtype=torch.float16)
+    w = q8.quantize_weight(torch.randn(40, 24, generator=g, device=DEV, dtype=torch.float16))
+    norm = torch.randn(24, generator=g, device=DEV, dtype=torch.float16)
+    assert torch.equal(q8.linear(x, w)[-7:], q8.linear(x[-7:], w))
+    r, rows = q8.add_rmsnorm(x, norm, 1e-6, y=x)
+    want_r, want = q8.add_rmsnorm(x[-7:].clone(), norm, 1e-6, y=x[-7:])
+    assert torch.equal(r[-7:], want_r) and torch.equal(rows.dequantize()[-7:], want.dequantize())
+    with pytest.raises(AssertionError):
+        q8.quantize(x.new_empty(q8.MAX_ROWS + 1, 1))
 
 
 def test_past_two_gigabytes():
