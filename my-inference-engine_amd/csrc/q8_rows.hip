@@ -434,16 +434,17 @@ hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
     if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, 1>);
     else go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, kQ8FloatMax>);
   }
-  else if (p.Kp <= 1024)
-    go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, TILE>);
-  else if (p.Kp <= 1536)
-    go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, TILE>);
-  else if (p.Kp <= kQ8KeepK)
-    go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, TILE>);
-  else if constexpr (SRC == kQ8Rows && MT < 4)   // (q8_plan: no more than 32 rows of these)
-    go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
-  else
-    return hipErrorInvalidValue;
+  else if constexpr (TILE == kQrHalf) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
+  else if (p.Kp <= 1024) go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, TILE>);
+  else if (p.Kp <= 1536) go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, TILE>);
+  else if (p.Kp <= kQ8KeepK) {
+    if constexpr (NP < 4) go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, TILE>);
+    else return hipErrorInvalidValue;   // (q8_rows_shape: two panels at most)
+  } else {
+    // (q8_plan: no more than 32 rows of these)
+    if constexpr (SRC == kQ8Rows && MT < 4 && NP != 2) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
+    else return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 
@@ -451,15 +452,23 @@ template <typename E, bool GATED, int SRC>
 hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
   const int grid = std::min(p.panels, n_cus);
   if constexpr (SRC == kQ8Rows) {
+    // (two work-groups a CU: 64 x 6400 x 2048 5.7 -> 6.7 us, 64 x 8192 x 1536 4.8 -> 5.2)
     if (p.M > 32) return launch_rows_k<E, 4, 1, GATED, SRC>(p, grid, stream);
     if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
   }
-  // Few panels: half a panel a work-group (1536 x 8960 by one token 6.4 -> 5.8 us).
-  if constexpr (!GATED)
-    if (2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, 2 * p.panels, stream);
-  // Very many: four panels between two barriers.
+  const bool keep = SRC != kQ8Float && p.Kp <= kQ8KeepK;
+  // Few panels of many features: half a panel a work-group (1536 x 8960 by one token 6.4 -> 5.8 us).
+  if constexpr (!GATED && (SRC == kQ8Rows || SRC == kQ8Float))
+    if (!keep && 2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, 2 * p.panels, stream);
   if constexpr (SRC != kQ8Float)
-    if (p.panels >= 16 * n_cus) return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
+    if (keep && (SRC != kQ8Rows || p.Kp <= 1536)) {   // (else 16 rows in 8 bits x 6400 x 2048 3.5 -> 4.3 us)
+      const Q8RowsShape shape = q8_rows_shape(p.panels, p.Kp, n_cus);
+      const int most = std::min((p.panels + shape.panels - 1) / shape.panels, shape.per_cu * n_cus);
+      if (shape.panels == 4) return launch_rows_k<E, 1, 4, GATED, SRC>(p, most, stream);
+      if (shape.panels == 2) return launch_rows_k<E, 1, 2, GATED, SRC>(p, most, stream);
+    } else if (!keep && p.panels >= 16 * n_cus) {   // (16 x 100000 x 4096 94 -> 85 us; one token 78 and 79)
+      return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
+    }
   return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);
 }
 

@@ -16,6 +16,31 @@ enum Q8Kernel {
   kQ8Gemm128x256, kQ8Gemm192x192, kQ8Gemm256x256
 };
 
+// How the few-row kernel takes more panels than there are CUs, where x stays in registers (q8_pad(K) <= kQ8KeepK, 16
+// rows at most): panels between two barriers, and work-groups a CU.  More panels put more loads in flight and
+// share a barrier; a second work-group computes while the first waits, until registers (K past 1536) or an
+// uneven last round cost more.  Measured with the norm, weights from memory (us; panels x work-groups a CU):
+//   tokens x features x K        1 x 1    1 x 2    2 x 1    2 x 2    4 x 1
+//   16 x 6720 x 1536             6.63     7.35     6.37     6.24     6.86
+//   1 x 9728 x 896               5.53     5.01     4.87     5.35     4.60
+//   16 x 14400 x 1536            9.52     8.42     8.22     8.62     8.06
+//   1 x 17920 x 1536             9.02     7.85     7.90     7.42     8.36
+//   16 x 17920 x 1536            10.6     8.95     9.39     8.81     9.59
+//   16 x 28672 x 1536            13.1     11.4     11.3     10.0     10.9
+//   16 x 28672 x 896             11.5     9.53     9.55     8.41     8.28
+//   16 x 22016 x 2048            13.5     11.9     11.8     13.7     12.3
+//   1 x 96000 x 1536             34.5     25.9     25.2     24.6     23.9
+// (Over 45 sizes by 1, 4 and 16 tokens 0.5% behind the best of each, 1 x 1 always 18%.)
+struct Q8RowsShape {
+  int32_t panels, per_cu;
+};
+inline Q8RowsShape q8_rows_shape(int32_t panels, int32_t kp, int32_t cus) {
+  if (panels <= cus) return {1, 1};
+  if (panels <= 2 * cus || kp > 1536) return {2, 1};
+  if (kp > 1024 && panels > 4 * cus && panels <= 8 * cus) return {2, 2};
+  return {4, 1};
+}
+
 struct Q8Plan {
   int32_t kernel;   // Q8Kernel
   int32_t tiles;    // work-groups

@@ -217,7 +217,8 @@ PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96),
             (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
             (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200),
             (3, 66000, 70), (2, 65553, 2100), (151, 16383, 72), (262, 16323, 600), (644, 16598, 70),
-            (517, 13074, 300), (193, 16455, 200), (644, 16405, 300), (771, 16440, 72)]
+            (517, 13074, 300), (193, 16455, 200), (644, 16405, 300), (771, 16440, 72), (7, 5003, 70), (16, 7000, 1300), (5, 17900, 1500),
+            (16, 9001, 1400), (9, 20011, 1900), (12, 20000, 600), (10, 100, 2000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -285,7 +286,8 @@ MLPS = [(1, 1536, 8960), (1, 64, 8), (2, 100, 36), (16, 1536, 8960), (5, 128, 17
         (33, 300, 500), (64, 256, 1000), (65, 512, 1024), (150, 896, 4864), (260, 640, 1531),
         (515, 256, 768), (130, 512, 1100), (400, 2176, 750), (40, 64, 4201), (600, 128, 3500), (138, 70, 8192),
         (757, 100, 5548), (166, 72, 8203), (2443, 40, 3093), (920, 200, 3081), (1014, 72, 2981), (1239, 40, 6249),
-        (2321, 40, 4339), (3, 64, 20000), (40, 48, 33001)]
+        (2321, 40, 4339), (3, 64, 20000), (40, 48, 33001), (5, 200, 4700), (3, 2000, 3000),
+        (15, 1400, 5000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -24,14 +24,18 @@ int plan(int rows, int panels, int kp, int* tiles) {
   const mi_fa2::Q8Plan p = mi_fa2::q8_plan(rows, panels, kp);
   *tiles = p.tiles;
   return p.kernel;
-}""").plan
-    fn.argtypes = [ctypes.c_int] * 3 + [ctypes.POINTER(ctypes.c_int)]
+}
+int rows_shape(int panels, int kp) {
+  const mi_fa2::Q8RowsShape s = mi_fa2::q8_rows_shape(panels, kp, 256);
+  return 10 * s.panels + s.per_cu;
+}""")
+    fn.plan.argtypes = [ctypes.c_int] * 3 + [ctypes.POINTER(ctypes.c_int)]
     return fn
 
 
 def plan(rows, features, k):
     tiles = ctypes.c_int()
-    kernel = _library()(rows, -(-features // 16), -(-k // 128) * 128, ctypes.byref(tiles))
+    kernel = _library().plan(rows, -(-features // 16), -(-k // 128) * 128, ctypes.byref(tiles))
     return kernel, tiles.value
 
 
@@ -63,3 +67,21 @@ def test_work_groups_cover_every_result():
 def test_the_gpu_tests_reach_every_kernel():
     assert {plan(*size)[0] for size in test_q8_gpu.PRODUCTS} == set(range(11))
     assert {plan(m, 2 * inter, hidden)[0] for m, hidden, inter in test_q8_gpu.MLPS} == set(range(11))
+
+
+def rows_shape(features, k):
+    return divmod(_library().rows_shape(-(-features // 16), -(-k // 128) * 128), 10)
+
+
+@pytest.mark.parametrize("features,k,shape", [
+    (16, 16, (1, 1)), (4096, 2048, (1, 1)), (6720, 1536, (2, 1)), (9728, 896, (4, 1)), (17920, 1536, (2, 2)),
+    (28672, 896, (4, 1)), (28672, 1536, (2, 2)), (22016, 2048, (2, 1)), (151936, 1536, (4, 1)), (151936, 2048, (2, 1))])
+def test_few_rows(features, k, shape):
+    assert rows_shape(features, k) == shape
+
+
+def test_the_gpu_tests_reach_every_shape_of_few_rows():
+    every = {((1, 1), 2), ((1, 1), 3), ((1, 1), 4), ((2, 1), 2), ((2, 1), 3), ((2, 1), 4), ((2, 2), 3), ((4, 1), 2),
+             ((4, 1), 3)}
+    steps = lambda k: max(2, -(-(-(-k // 128) * 128) // 512))
+    assert {(rows_shape(n, k), steps(k)) for m, n, k in test_q8_gpu.PRODUCTS if m <= 16 and k <= 2048} == every
