@@ -17,12 +17,12 @@
 // the operands' order, while the first weights are on their way.
 //
 // Bound by the weight stream and a launch's fixed cost.  Measured (bf16, launches in a graph, weights in the
-// last-level cache; one token and 16): 2048 x 1536 with norm 3.5 and 5.0 us, rows in 8 bits already 2.6;
-// 17920 x 1536 8.3 and 10.1, 7.5 (3.6 TB/s); 151936 x 1536 41.1 and 45.7, 39.5 (5.9 TB/s; a large copy moves
-// 5.2).  Weights from memory: 17920 x 1536 9.9 and 11.4.  The norm of 16 rows costs 2.3 us here, where every
+// last-level cache; one token and 16): 2048 x 1536 with norm 3.5 and 4.8 us, rows in 8 bits already 2.5;
+// 17920 x 1536 7.0 and 8.8, 6.8 (4.1 TB/s); 151936 x 1536 41.6 and 45.6, 39.5 (5.9 TB/s; a large copy moves
+// 5.2).  Weights from memory: 17920 x 1536 8.3 and 9.5.  The norm of 16 rows costs 1.9 to 2.3 us here, where every
 // work-group does it over; a launch of its own costs 3.1.
-// Two tiles in flight a work-group instead of one: 17920 x 1536 by one token 7.3 -> 8.0 us, the feed-forward
-// block of 16 tokens with weights from memory 24.1 -> 23.6.
+// Two tiles in flight one behind the other in a work-group, a panel each, gained nothing (17920 x 1536 by one token 7.3
+// -> 8.0 us); two panels side by side and a second work-group on the CU do (q8_rule.h: 9.0 -> 7.4).
 // The tile kernel at the end of the file is for the sizes q8_rule.h says.
 #include "q8.h"
 
