@@ -14,15 +14,16 @@
  * zeros from n on, mi_q8_rows_bytes() bytes, 16-byte aligned; rows past the last keep what they hold.
  *
  * Weights in 8 bits.  int8 [out_features][in_features] and one fp32 scale for each out feature, the
- * values laid out by mi_q8_pack once, as rows are but with zeros past the last.  A gated weight (the gate and up rows of a feed-forward block,
- * gate rows first) is laid out for mi_q8_mlp and used by nothing else.
+ * values laid out by mi_q8_pack once, as rows are but with zeros past the last.  A gated weight (the gate
+ * and up rows of a feed-forward block, gate rows first) is laid out for mi_q8_mlp and used by nothing else.
  *
  * A product is sum_k x[m][k] w[n][k], a whole number in 32 bits (exact, in_features <= 131072), times
  * the two scales in fp32; bias and residual are added in fp32 and the sum is rounded once.
  *
  * Common rules.  dtype: 0 bf16, 1 fp16 (everything that is not int8 or fp32 here).  Row strides are in
  * elements, at least the row's length, any alignment of rows (rows whose addresses are multiples of 16
- * bytes are faster).  Rows of one stride may be columns of one tensor.  Sizes: in_features at most 131072, out_features at most 2^24, rows at most 2^21.
+ * bytes are faster).  Rows of one stride may be columns of one tensor.  Sizes: in_features at most 131072,
+ * out_features at most 2^24, rows at most 2^21.
  * All launches are asynchronous on `stream`, allocate nothing and may be captured in a graph.
  * Workspaces: 16-byte aligned, contents arbitrary, not shared by calls that may overlap in time.
  *

@@ -2,11 +2,11 @@
 //
 // A work-group of 4 waves (8) computes TM tokens by NP panels (64 x 64, a wave 32 x 32; 128 x 128, a wave 64 x 64;
 // up to 256 x 256, a wave 64 tokens by 128 features) with v_mfma_i32_32x32x32_i8.  W is the A operand, so a lane's
-// four sums in a row are four features of one token.  Both operands come in panels (q8.h): a stage of 64 of K is NP + TM / 16 loads of 1 KB
-// straight into LDS, and a 32 x 32 operand is read out of two panels' kilobytes, 16 lanes in a run, with no two
-// on a bank.  ST stages are in flight.  A stage's operands are read during the MFMAs of the stage before, behind
-// one barrier a stage; the loads ST stages ahead follow between the second half of the MFMAs (reads, then
-// MFMAs, then loads, without that: 6001 x 6144 x 4096 153-159 us where this took 148-152).
+// four sums in a row are four features of one token.  Both operands come in panels (q8.h): a stage of 64 of K is
+// NP + TM / 16 loads of 1 KB straight into LDS, and a 32 x 32 operand is read out of two panels' kilobytes, 16 lanes
+// in a run, with no two on a bank.  ST stages are in flight.  A stage's operands are read during the MFMAs of the
+// stage before, behind one barrier a stage; the loads ST stages ahead follow between the second half of the MFMAs
+// (reads, then MFMAs, then loads, without that: 6001 x 6144 x 4096 153-159 us where this took 148-152).
 // Results: the tile's scales wait in LDS, loaded with the first stage; the sums are scaled, meet bias and
 // residual in fp32, and leave through LDS as whole rows, past the caches (143 -> 121 us for 4001 x 17920 x 1536
 // against stores that stay in the L2).  GATED: quads of gate and up rows of the same features lie in one lane,

@@ -51,7 +51,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
   // A row is a wave's or a work-group's: its address is uniform.
   const int64_t urow = __builtin_amdgcn_readfirstlane(row);
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + urow * p.x_st;
-  const __amdgpu_buffer_rsrc_t xf = make_rsrc(static_cast<const float*>(p.x) + urow * p.x_st, SRC == kQ8Float ? p.n * 4 : 0);
+  const __amdgpu_buffer_rsrc_t xf =
+      make_rsrc(static_cast<const float*>(p.x) + urow * p.x_st, SRC == kQ8Float ? p.n * 4 : 0);
   const bool add = SRC == kQ8Norm && p.y;
   const uint16_t* y = add ? p.y + urow * p.y_st : nullptr;
   uint16_t* r = add ? p.r_out + urow * p.r_st : nullptr;
@@ -149,7 +150,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void q8_quant_kernel(const Q8Qua
   if (tid == 0)
     p.scale[row] = q8_scale(f, SRC == kQ8Norm ? rsqrtf(ss / (float)p.n + p.eps) : 1.f);
   const auto store = [&](int c, const float (&v)[8]) {
-    const u32x2 o = {q8_pack4<SRC != kQ8Float>(v[0], v[1], v[2], v[3], f), q8_pack4<SRC != kQ8Float>(v[4], v[5], v[6], v[7], f)};
+    const u32x2 o = {q8_pack4<SRC != kQ8Float>(v[0], v[1], v[2], v[3], f),
+                     q8_pack4<SRC != kQ8Float>(v[4], v[5], v[6], v[7], f)};
     *reinterpret_cast<u32x2*>(p.q + q8_at(row, c, p.np)) = o;
   };
   if constexpr (PER > 0) {

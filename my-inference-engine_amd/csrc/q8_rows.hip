@@ -362,7 +362,8 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_rows_kernel(const Q8Params p
 // A tile of NP panels by 16 MT tokens a work-group, its 8 waves' shares of K each from memory straight into
 // the MFMAs, D steps ahead: nothing is shared but the sums, so there is no barrier before the last.  A step is
 // (NP + MT) KB for NP MT MFMAs of 16 cycles: bound by the 64 bytes a CU's vector cache gives a cycle, and by
-// latency where there are few steps.  64 x 1536 x 8960 9.5-10.0 us (1.4 TB/s of weights), 150 x 896 x 4864 7.1-7.7.
+// latency where there are few steps.  64 x 1536 x 8960 9.5-10.0 us (1.4 TB/s of weights), 150 x 896 x 4864 7.1-7.7
+// (8 and 10 steps ahead 9.3 and 8.2, and 65 x 512 x 1024 4.2 -> 6.0).
 template <typename E, int MT, int NP, int D, bool GATED>
 __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p) {
   constexpr int U = NP * MT;

@@ -217,8 +217,8 @@ PRODUCTS = [(1, 16, 64), (1, 2048, 1536), (2, 1, 1), (3, 17, 129), (15, 48, 96),
             (257, 513, 520), (300, 1536, 1536), (513, 384, 896), (1025, 300, 1100), (70, 5000, 72),
             (400, 1503, 2100), (50, 8500, 130), (300, 2701, 300), (513, 8300, 72), (1300, 3333, 200),
             (3, 66000, 70), (2, 65553, 2100), (151, 16383, 72), (262, 16323, 600), (644, 16598, 70),
-            (517, 13074, 300), (193, 16455, 200), (644, 16405, 300), (771, 16440, 72), (7, 5003, 70), (16, 7000, 1300), (5, 17900, 1500),
-            (16, 9001, 1400), (9, 20011, 1900), (12, 20000, 600), (10, 100, 2000)]
+            (517, 13074, 300), (193, 16455, 200), (644, 16405, 300), (771, 16440, 72), (7, 5003, 70),
+            (16, 7000, 1300), (5, 17900, 1500), (16, 9001, 1400), (9, 20011, 1900), (12, 20000, 600), (10, 100, 2000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
