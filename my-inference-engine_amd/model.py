@@ -255,7 +255,7 @@ class Attention(nn.Module):
                         meta.slot_mapping32, cache.k_pool(layer), cache.v_pool(layer), cfg.num_heads,
                         cfg.num_kv_heads)
         a = self._attend(q, B, T, cache, layer, meta).view(n, self.q_size)
-        q8.linear(a, self.o_proj.weight, residual=res, out=res)
+        q8.linear(a, self.o_proj.weight, bias=self.o_proj.bias, residual=res, out=res)
 
     def _attend_packed(self, q, cache, layer, meta):
         """q [N, Hq, d] packed queries of a mixed step -> [N, Hq, d]: the leading one-token rows
@@ -380,6 +380,8 @@ class Qwen2ForCausalLM(nn.Module):
         old = [getattr(m, name) for m, name in held]
         assert all(type(linear) is nn.Linear and plain(linear) for linear in old), \
             "projections that are nn.Linear with nothing hooked on"
+        assert all(layer.mlp.gate_up_proj.bias is None and layer.mlp.down_proj.bias is None
+                   for layer in self.layers), "the feed-forward block in 8 bits has no bias"
         new = [Linear8(linear, name == "gate_up_proj") for (_, name), linear in zip(held, old)]
         self.head8 = q8.quantize_weight(self.embed_tokens.weight.detach()) if lm_head else None
         for (m, name), linear in zip(held, new):

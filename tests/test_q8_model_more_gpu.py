@@ -1,0 +1,38 @@
+"""The model with its projections in 8 bits: biases."""
+import pytest
+import torch
+import torch.nn as nn
+
+from conftest import announce
+from test_q8_model_gpu import CFG, cache_for, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(3, 1), (2, 20)])
+def test_the_output_projections_bias(shape, dtype):
+    """A layer's attention with a bias on its output projection and without: the two results are rounded once
+    each, so they differ by the bias within half a step of either (and four roundings in fp32 beside)."""
+    announce(f"[gpu] biased output projection, {shape} {dtype}")
+    model = make(dtype)
+    o = model.layers[0].self_attn.o_proj = nn.Linear(256, CFG.hidden_size, bias=True).cuda().to(dtype)
+    g = torch.Generator().manual_seed(5)
+    with torch.no_grad():
+        o.bias.copy_(torch.randn(CFG.hidden_size, generator=g) * 2)
+    model.requires_grad_(False).quantize_()
+    attn, norm = model.layers[0].self_attn, model.layers[0].input_layernorm
+    B, T = shape
+    x = torch.randn(B * T, CFG.hidden_size, generator=g).to(dtype).cuda()
+    cos, sin = model.rope_cos_sin(torch.arange(T, device="cuda").expand(B, T), dtype)
+
+    def result():
+        cache, res = cache_for(dtype), x.clone()
+        meta = cache.prepare([cache.alloc() for _ in range(B)], T, CFG.num_heads)
+        attn.q8_step(res, norm, (B, T, CFG.hidden_size), cos, sin, cache, 0, meta)
+        return res.cpu().double()
+    got, bias = result(), attn.o_proj.bias
+    attn.o_proj.bias = None
+    without, bias = result(), bias.cpu().double()
+    tol = torch.finfo(dtype).eps / 2 * (got.abs() + without.abs()) * 1.01 + 2.0 ** -22 * (got.abs() + bias.abs())
+    assert ((got - without - bias).abs() <= tol).all()
