@@ -420,11 +420,9 @@ class Qwen2ForCausalLM(nn.Module):
             cos, sin = self.rope_cos_sin(position_ids, x.dtype)
         x = self.run_layers(x, cos, sin, cache, meta)
         x, w = x[:, -1:], self.embed_tokens.weight
+        if self._head8_fits(x):
+            return self._head8_logits(x)
         rows = x.reshape(-1, x.shape[-1])
-        if (self.head8 is not None and plain(self.norm) and inference(x, w, self.norm.weight)
-                and self._own("lm_head")):
-            return q8.linear(rows, self.head8, norm_weight=self.norm.weight,
-                             eps=self.norm.eps).view(*x.shape[:-1], w.shape[0])
         if (x.is_cuda and rows.shape[0] <= few_rows.MAX_NORM_ROWS and plain(self.norm)
                 and inference(x, w, self.norm.weight)
                 and self._own("lm_head") and few_rows.linear_fits(rows, w, self.norm.weight)):
@@ -435,6 +433,17 @@ class Qwen2ForCausalLM(nn.Module):
     def _own(self, name):
         """Whether method `name` is this class's, replaced neither in a subclass nor on the instance."""
         return getattr(self, name) == getattr(Qwen2ForCausalLM, name).__get__(self)
+
+    def _head8_fits(self, x):
+        """Whether the logits of x, the last layer's output, are the 8-bit head's product with the norm in it."""
+        return (self.head8 is not None and plain(self.norm)
+                and inference(x, self.embed_tokens.weight, self.norm.weight) and self._own("lm_head"))
+
+    def _head8_logits(self, x):
+        """The same for every kind of step: with the norm's output rounded to 16 bits in between, values next to a
+        border would move by a step of the 8 bits."""
+        out = q8.linear(x.reshape(-1, x.shape[-1]), self.head8, norm_weight=self.norm.weight, eps=self.norm.eps)
+        return out.view(*x.shape[:-1], out.shape[1])
 
     def lm_head(self, x):
         """Tied-embedding logits (model.py:204-207)."""
@@ -522,5 +531,7 @@ class Qwen2ForCausalLM(nn.Module):
         x = self.embed_tokens(token_ids)[None]                      # [1, N, hidden]
         cos, sin = self.rope_cos_sin(meta.positions[None], x.dtype)
         x = self.run_layers(x, cos, sin, cache, meta)
-        x = self.norm(x[0, meta.last_idx.long()])
-        return self.lm_head(x)
+        x = x[0, meta.last_idx.long()]
+        if self._head8_fits(x):
+            return self._head8_logits(x)
+        return self.lm_head(self.norm(x))

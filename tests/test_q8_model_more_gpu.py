@@ -1,10 +1,13 @@
-"""The model with its projections in 8 bits: biases."""
+"""The model with its projections in 8 bits: biases, the head in every kind of step."""
 import pytest
 import torch
 import torch.nn as nn
 
+import test_q8_model_gpu as base
 from conftest import announce
-from test_q8_model_gpu import CFG, cache_for, make
+from kernels import q8
+from model import Qwen2ForCausalLM
+from test_q8_model_gpu import CFG, cache_for, make, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +39,27 @@ def test_the_output_projections_bias(shape, dtype):
     without, bias = result(), bias.cpu().double()
     tol = torch.finfo(dtype).eps / 2 * (got.abs() + without.abs()) * 1.01 + 2.0 ** -22 * (got.abs() + bias.abs())
     assert ((got - without - bias).abs() <= tol).all()
+
+
+def test_the_head_of_a_packed_step():
+    """A packed step's logits are the head's product with the norm in front, as an ordinary step's are."""
+    announce("[gpu] head in 8 bits of a packed step")
+    model = make().quantize_(lm_head=True)
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(1, 40, CFG.hidden_size, generator=g).bfloat16().cuda()
+    cache = cache_for()
+    counts = [1, 1, 30, 8]
+    meta = cache.prepare_packed([cache.alloc() for _ in counts], counts)
+    model.run_layers = lambda *a: x
+    got = model.forward_packed(tokens(g, 40), cache, meta)
+    last = x[0, [0, 1, 31, 39]]
+    want = q8.linear(last, model.head8, norm_weight=model.norm.weight, eps=CFG.rms_norm_eps)
+    assert torch.equal(got, want)
+
+
+def test_graphs_mixed_steps_and_an_engine_with_the_head(monkeypatch):
+    """The runs of a model whose layers alone are in 8 bits, with the head too."""
+    quantize_ = Qwen2ForCausalLM.quantize_
+    monkeypatch.setattr(Qwen2ForCausalLM, "quantize_", lambda model: quantize_(model, lm_head=True))
+    base.test_graphs_and_mixed_steps()
+    base.test_an_engine_serves_it()
