@@ -154,6 +154,8 @@ class DecodeGraphs:
         n = len(seqs)
         rows = self._bucket(n)
         cache = self.cache
+        if getattr(self.model, "head8", None) is not None:
+            self.model.refresh_head8()
         groups = cache.shared_groups(seqs) if self._may_share(rows) else None
         if groups is not None and not self._shared_ready(rows):
             groups = None

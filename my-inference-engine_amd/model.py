@@ -355,7 +355,7 @@ class Qwen2ForCausalLM(nn.Module):
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2).float() / cfg.head_dim))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        self.quantized, self.head8 = False, None   # quantize_
+        self.quantized, self.head8, self._head8_made = False, None, None   # quantize_
 
     @torch.no_grad()
     def init_random(self, std=0.02, seed=0):
@@ -371,8 +371,8 @@ class Qwen2ForCausalLM(nn.Module):
 
     @torch.no_grad()
     def quantize_(self, lm_head=False):
-        """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head) in 8
-        bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit weights are let go: capture decode
+        """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head, which
+        follows them when they change) in 8 bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit weights are let go: capture decode
         graphs after this, those captured before read memory that is no longer theirs."""
         held = [(m, name) for layer in self.layers
                 for m, name in ((layer.self_attn, "qkv_proj"), (layer.self_attn, "o_proj"),
@@ -383,11 +383,32 @@ class Qwen2ForCausalLM(nn.Module):
         assert all(layer.mlp.gate_up_proj.bias is None and layer.mlp.down_proj.bias is None
                    for layer in self.layers), "the feed-forward block in 8 bits has no bias"
         new = [Linear8(linear, name == "gate_up_proj") for (_, name), linear in zip(held, old)]
-        self.head8 = q8.quantize_weight(self.embed_tokens.weight.detach()) if lm_head else None
+        if lm_head:
+            self.head8, self._head8_made = q8.quantize_weight(self.embed_tokens.weight.detach()), self._embeddings()
         for (m, name), linear in zip(held, new):
             setattr(m, name, linear)
         self.quantized = True
         return self
+
+    def _embeddings(self):
+        """The embedding tensor and what changes with its contents."""
+        w = self.embed_tokens.weight
+        return w, w.data_ptr(), None if w.is_inference() else w._version
+
+    @torch.no_grad()
+    def refresh_head8(self):
+        """Bring the 8-bit head up to date with the embeddings, where they were changed since it was made: in
+        place, so that captured steps read it too.  Every step calls this, a captured one before its replay."""
+        if self.head8 is None:
+            return
+        made, now = self._head8_made, self._embeddings()
+        if made[0] is now[0] and made[1:] == now[1:]:
+            return
+        new, old = q8.quantize_weight(now[0].detach()), self.head8
+        assert new.sig == old.sig, f"embeddings [{old.out_features}, {old.in_features}] on {old.device}, as quantize_ saw"
+        old.data.copy_(new.data)
+        old.scale.copy_(new.scale)
+        self._head8_made = now
 
     def rope_cos_sin(self, position_ids, dtype):
         # position_ids [B, T] -> cos/sin [B, 1, T, head_dim] (model.py:151-155)
@@ -442,6 +463,7 @@ class Qwen2ForCausalLM(nn.Module):
     def _head8_logits(self, x):
         """The same for every kind of step: with the norm's output rounded to 16 bits in between, values next to a
         border would move by a step of the 8 bits."""
+        self.refresh_head8()
         out = q8.linear(x.reshape(-1, x.shape[-1]), self.head8, norm_weight=self.norm.weight, eps=self.norm.eps)
         return out.view(*x.shape[:-1], out.shape[1])
 
@@ -449,6 +471,7 @@ class Qwen2ForCausalLM(nn.Module):
         """Tied-embedding logits (model.py:204-207)."""
         w = self.embed_tokens.weight
         if self.head8 is not None:
+            self.refresh_head8()
             return q8.linear(x.reshape(-1, x.shape[-1]), self.head8).view(*x.shape[:-1], w.shape[0])
         if x.is_cuda:
             rows = x.reshape(-1, x.shape[-1])

@@ -1,10 +1,11 @@
-"""The model with its projections in 8 bits: biases, the head in every kind of step."""
+"""The model with its projections in 8 bits: biases, the head in every kind of step, weights that change."""
 import pytest
 import torch
 import torch.nn as nn
 
 import test_q8_model_gpu as base
 from conftest import announce
+from graphs import DecodeGraphs
 from kernels import q8
 from model import Qwen2ForCausalLM
 from test_q8_model_gpu import CFG, cache_for, make, tokens
@@ -63,3 +64,39 @@ def test_graphs_mixed_steps_and_an_engine_with_the_head(monkeypatch):
     monkeypatch.setattr(Qwen2ForCausalLM, "quantize_", lambda model: quantize_(model, lm_head=True))
     base.test_graphs_and_mixed_steps()
     base.test_an_engine_serves_it()
+
+
+def test_an_embedding_that_changes_changes_the_head():
+    announce("[gpu] head in 8 bits after the embedding changed")
+    model = make().quantize_(lm_head=True)
+    g = torch.Generator().manual_seed(7)
+    ids = tokens(g, 2, 5)
+
+    def logits(m):
+        cache = cache_for()
+        return m(ids, cache, [cache.alloc(), cache.alloc()])
+    def step(graphs, cache):
+        return graphs.run([cache.alloc()], [3]).clone()
+    cache = cache_for()
+    graphs = DecodeGraphs(model, cache, buckets=(1,))
+    logits(model)
+    step(graphs, cache)
+    other = make()
+    with torch.no_grad():
+        for m in (model, other):
+            m.embed_tokens.weight[5:9] *= 3.0
+    want = logits(other.quantize_(lm_head=True))
+    captured = step(graphs, cache)
+    assert torch.equal(logits(model), want)
+    c = cache_for()
+    assert torch.equal(captured, step(DecodeGraphs(other, c, buckets=(1,)), c))
+    # another tensor in its place, of the same values doubled
+    for m in (model, other):
+        m.embed_tokens.weight = nn.Parameter(m.embed_tokens.weight.detach() * 2, requires_grad=False)
+    fresh = make()
+    fresh.embed_tokens.weight = nn.Parameter(other.embed_tokens.weight.detach().clone(), requires_grad=False)
+    assert torch.equal(logits(model), logits(fresh.quantize_(lm_head=True)))
+    # of another size: nothing to bring up to date
+    model.embed_tokens.weight = nn.Parameter(torch.cat([model.embed_tokens.weight] * 2), requires_grad=False)
+    with pytest.raises(AssertionError, match="as quantize_ saw"):
+        logits(model)
