@@ -23,6 +23,9 @@ another graph of the bucket, whose attention reads them once; which rows share w
 slots and ids.  It is captured by capture_shared(), or when the first such step comes: two steps and a
 capture in the middle of serving, and device memory for its intermediates (51 MB of workspace and more).  A
 step for which that memory cannot be had replays the bucket's ordinary graph, which computes the same.
+
+A graph reads the weights where they lay when it was captured.  They may change in place; once a model's
+projections are replaced (quantize_) or its embeddings lie elsewhere, run() raises.
 """
 import numpy as np
 import torch
@@ -52,12 +55,23 @@ class DecodeGraphs:
         # is kept per stream, and a stream handle recycled by torch's pool while these graphs
         # exist would hand their workspace to unrelated calls.
         self._side = torch.cuda.Stream(device=cache.device)
+        self._held = self._weights()
         for rows in self.buckets:
             self._capture(rows)
 
     @property
     def max_rows(self):
         return self.buckets[-1]
+
+    def _weights(self):
+        held = getattr(self.model, "weights_held", None)     # (a model of another kind says nothing)
+        return held() if held is not None else None
+
+    def _check_weights(self):
+        """The graphs read the weights that the model had when they were captured."""
+        if self._weights() != self._held:
+            raise RuntimeError("the model's weights were replaced after its decode graphs were captured: "
+                               "capture new ones")
 
     def _bucket(self, n):
         for b in self.buckets:
@@ -68,6 +82,7 @@ class DecodeGraphs:
     def capture_shared(self, rows=None):
         """Capture the sharing graph of a bucket (default: of all that may replay one) now, so that no step
         has to.  Raises if there is no memory for it."""
+        self._check_weights()
         for bucket in self.buckets if rows is None else [self._bucket(rows)]:
             if self._may_share(bucket) and bucket not in self.shared_graphs:
                 self._capture(bucket, shared=True)
@@ -154,6 +169,7 @@ class DecodeGraphs:
         n = len(seqs)
         rows = self._bucket(n)
         cache = self.cache
+        self._check_weights()
         if getattr(self.model, "head8", None) is not None:
             self.model.refresh_head8()
         groups = cache.shared_groups(seqs) if self._may_share(rows) else None

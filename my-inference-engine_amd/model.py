@@ -356,6 +356,7 @@ class Qwen2ForCausalLM(nn.Module):
         inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2).float() / cfg.head_dim))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
         self.quantized, self.head8, self._head8_made = False, None, None   # quantize_
+        self._replaced = 0   # how often projections were replaced
 
     @torch.no_grad()
     def init_random(self, std=0.02, seed=0):
@@ -373,7 +374,7 @@ class Qwen2ForCausalLM(nn.Module):
     def quantize_(self, lm_head=False):
         """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head, which
         follows them when they change) in 8 bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit weights are let go: capture decode
-        graphs after this, those captured before read memory that is no longer theirs."""
+        graphs after this, those captured before refuse to run."""
         held = [(m, name) for layer in self.layers
                 for m, name in ((layer.self_attn, "qkv_proj"), (layer.self_attn, "o_proj"),
                                 (layer.mlp, "gate_up_proj"), (layer.mlp, "down_proj"))]
@@ -388,7 +389,13 @@ class Qwen2ForCausalLM(nn.Module):
         for (m, name), linear in zip(held, new):
             setattr(m, name, linear)
         self.quantized = True
+        self._replaced += 1
         return self
+
+    def weights_held(self):
+        """Another value when weights that a captured step reads have been replaced: projections by quantize_, the
+        embeddings by a tensor elsewhere."""
+        return self._replaced, self.embed_tokens.weight.data_ptr()
 
     def _embeddings(self):
         """The embedding tensor and what changes with its contents."""

@@ -1,8 +1,13 @@
-"""What Qwen2ForCausalLM.quantize_ refuses, on the CPU: no kernel runs here."""
+"""What Qwen2ForCausalLM.quantize_ refuses and what it means to graphs captured before, on the CPU: no kernel runs
+here."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 import torch.nn as nn
 
+from graphs import DecodeGraphs
+from kernels import q8
 from model import QwenConfig, Qwen2ForCausalLM
 
 CFG = QwenConfig(hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, intermediate_size=520,
@@ -20,3 +25,58 @@ def test_a_biased_feed_forward_block_is_refused(name):
         model.quantize_()
     assert not model.quantized
     assert all(type(layer.self_attn.qkv_proj) is nn.Linear for layer in model.layers)
+
+
+class Graph:
+    """A captured graph that counts its replays."""
+    replays = 0
+
+    def replay(self):
+        self.replays += 1
+
+
+def graphs_of(model):
+    """DecodeGraphs with a one-row graph as captured from model, over a cache that keeps nothing."""
+    graphs = object.__new__(DecodeGraphs)
+    event = SimpleNamespace(synchronize=lambda: None, record=lambda: None)
+    bufs = (torch.zeros(4), torch.zeros(1, 1), torch.zeros(4), torch.zeros(1, 1))
+    graph = Graph()
+    vars(graphs).update(
+        model=model, W=1, buckets=[1], graphs={1: (graph, torch.zeros(1, 1, 5), bufs, event)}, shared_graphs={},
+        cache=SimpleNamespace(device_tables=False, SHARED_MAX_ROWS=1, advance=lambda *a: None,
+                              pack_step=lambda *a, **k: None))
+    graphs._held = graphs._weights()
+    return graphs, graph
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """quantize_ on the CPU, for what it does around the kernels."""
+    monkeypatch.setattr(q8, "quantize_weight", lambda w, gated=False: SimpleNamespace(sig=tuple(w.shape)))
+
+
+@pytest.mark.parametrize("replace", ["projections", "projections and head", "embeddings"])
+def test_graphs_captured_before_weights_are_replaced_do_not_run(replace, stand_in):
+    """They read the replaced weights' memory, which is somebody else's by then."""
+    model = Qwen2ForCausalLM(CFG).bfloat16()
+    graphs, graph = graphs_of(model)
+    graphs.run([0], [3])
+    with torch.no_grad():
+        model.embed_tokens.weight[3] *= 2      # in place: the graph reads it
+    graphs.run([0], [3])
+    assert graph.replays == 2
+    if replace == "embeddings":
+        model.embed_tokens.weight = nn.Parameter(model.embed_tokens.weight.detach().clone())
+    else:
+        model.quantize_(lm_head=replace != "projections")
+    with pytest.raises(RuntimeError, match="replaced"):
+        graphs.run([0], [3])
+    with pytest.raises(RuntimeError, match="replaced"):
+        graphs.capture_shared()
+    assert graph.replays == 2
+
+
+def test_graphs_of_a_model_of_another_kind_run():
+    graphs, graph = graphs_of(SimpleNamespace(forward_meta=None))
+    graphs.run([0], [3])
+    assert graph.replays == 1
