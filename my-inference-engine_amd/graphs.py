@@ -24,8 +24,9 @@ slots and ids.  It is captured by capture_shared(), or when the first such step 
 capture in the middle of serving, and device memory for its intermediates (51 MB of workspace and more).  A
 step for which that memory cannot be had replays the bucket's ordinary graph, which computes the same.
 
-A graph reads the weights where they lay when it was captured.  They may change in place; once a model's
-projections are replaced (quantize_) or its embeddings lie elsewhere, run() raises.
+A graph reads the weights where they lay when it was captured.  They may change in place (but for buckets past the
+few-row kernels, which multiply by transposed copies of the gate/up and head weights: those stay as captured); once a
+model's projections are replaced (quantize_) or its embeddings lie elsewhere, run() raises.
 """
 import numpy as np
 import torch
@@ -56,6 +57,7 @@ class DecodeGraphs:
         # exist would hand their workspace to unrelated calls.
         self._side = torch.cuda.Stream(device=cache.device)
         self._held = self._weights()
+        self._copies = []           # of weights, that a graph may read
         for rows in self.buckets:
             self._capture(rows)
 
@@ -159,6 +161,9 @@ class DecodeGraphs:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph), torch.no_grad():
             logits = step()
+        # steps past the few-row kernels multiply by transposed copies, which a changed weight replaces
+        parameters = getattr(self.model, "parameters", list)
+        self._copies += [p._mi_transposed for p in parameters() if hasattr(p, "_mi_transposed")]
         kept = self.shared_graphs if shared else self.graphs
         kept[rows] = (graph, logits, bufs, torch.cuda.Event())
 
