@@ -388,6 +388,8 @@ class Qwen2ForCausalLM(nn.Module):
             self.head8, self._head8_made = q8.quantize_weight(self.embed_tokens.weight.detach()), self._embeddings()
         for (m, name), linear in zip(held, new):
             setattr(m, name, linear)
+        if lm_head:   # what larger steps multiplied by: the head's product takes its place
+            vars(self.embed_tokens.weight).pop("_mi_transposed", None)
         self.quantized = True
         self._replaced += 1
         return self

@@ -8,7 +8,7 @@ import torch.nn as nn
 
 from graphs import DecodeGraphs
 from kernels import q8
-from model import QwenConfig, Qwen2ForCausalLM
+from model import QwenConfig, Qwen2ForCausalLM, transposed
 
 CFG = QwenConfig(hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, intermediate_size=520,
                  vocab_size=512)
@@ -80,3 +80,11 @@ def test_graphs_of_a_model_of_another_kind_run():
     graphs, graph = graphs_of(SimpleNamespace(forward_meta=None))
     graphs.run([0], [3])
     assert graph.replays == 1
+
+
+@pytest.mark.parametrize("lm_head", [False, True])
+def test_the_transposed_embeddings_go_with_the_head_that_used_them(lm_head, stand_in):
+    model = Qwen2ForCausalLM(CFG).bfloat16()
+    transposed(model.embed_tokens.weight)
+    model.quantize_(lm_head=lm_head)
+    assert hasattr(model.embed_tokens.weight, "_mi_transposed") == (not lm_head)
