@@ -347,6 +347,10 @@ _PLAIN = (nn.Linear, Linear8, RMSNorm, Attention, MLP, Block)   # what plain() k
 
 
 class Qwen2ForCausalLM(nn.Module):
+    # what quantize_ sets (here, so that models saved whole before there was one have it too); _replaced: how often
+    # projections were replaced
+    quantized, head8, _head8_made, _replaced = False, None, None, 0
+
     def __init__(self, cfg=QWEN25_1P5B):
         super().__init__()
         self.cfg = cfg
@@ -355,8 +359,6 @@ class Qwen2ForCausalLM(nn.Module):
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2).float() / cfg.head_dim))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        self.quantized, self.head8, self._head8_made = False, None, None   # quantize_
-        self._replaced = 0   # how often projections were replaced
 
     @torch.no_grad()
     def init_random(self, std=0.02, seed=0):

@@ -1,5 +1,6 @@
 """What Qwen2ForCausalLM.quantize_ refuses and what it means to graphs captured before, on the CPU: no kernel runs
 here."""
+import pickle
 from types import SimpleNamespace
 
 import pytest
@@ -8,6 +9,7 @@ import torch.nn as nn
 
 from graphs import DecodeGraphs
 from kernels import q8
+from kv_cache import KVCache
 from model import QwenConfig, Qwen2ForCausalLM, transposed
 
 CFG = QwenConfig(hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, intermediate_size=520,
@@ -88,3 +90,15 @@ def test_the_transposed_embeddings_go_with_the_head_that_used_them(lm_head, stan
     transposed(model.embed_tokens.weight)
     model.quantize_(lm_head=lm_head)
     assert hasattr(model.embed_tokens.weight, "_mi_transposed") == (not lm_head)
+
+
+def test_a_model_saved_before_there_was_quantize_runs():
+    """Saved whole, a model comes back with the attributes that it had then."""
+    model = Qwen2ForCausalLM(CFG).init_random()
+    for name in ("quantized", "head8", "_head8_made", "_replaced"):
+        vars(model).pop(name, None)
+    old = pickle.loads(pickle.dumps(model))
+    caches = [KVCache(8, 16, "cpu", torch.float32, CFG.num_layers, CFG.num_kv_heads, CFG.head_dim) for _ in range(2)]
+    ids = torch.arange(5)[None]
+    got, want = (m(ids, c, [c.alloc()]) for m, c in zip((old, Qwen2ForCausalLM(CFG).init_random()), caches))
+    assert torch.equal(got, want) and old.weights_held()[0] == 0
