@@ -213,8 +213,12 @@ def _empty_rows(R, n, dtype, dev):
     return rows
 
 
+_ROWS_GO = "x: 16-bit rows (rows in 8 bits go to linear)"
+
+
 def quantize(x):
     """Rows x [rows, n] in 8 bits."""
+    assert type(x) is not Rows, _ROWS_GO
     dt, dev = _input(x)
     R, n = x.shape
     xp, xs = _rows(x, "x", dt, dev)
@@ -242,6 +246,7 @@ def _sig(t):
 def add_rmsnorm(x, weight, eps, y=None, residual_out=None):
     """x [rows, n] (+ y) -> (r, Rows): r = x + y rounded (x itself when y is None), and weight * rmsnorm(r)
     in 8 bits, with no rounding to 16 bits in between.  residual_out may be x or y (in place)."""
+    assert type(x) is not Rows, _ROWS_GO
     key = ("norm", x.shape, x.stride(), x.dtype, x.device, _sig(weight), _sig(y), _sig(residual_out))
     plan = _PLANS.get(key)
     if plan is None:
@@ -347,6 +352,7 @@ def mlp(x, gate_up, down, residual=None, norm_weight=None, eps=0.0, out=None):
     gate_up a gated Weight [2 * inter, hidden], down a Weight [hidden, inter].  The activation is held in 8 bits
     too, every row by its largest magnitude.  out may be residual and x."""
     assert type(gate_up) is Weight and type(down) is Weight, "gate_up, down: Weights"
+    assert type(x) is not Rows, _ROWS_GO
     key = ("mlp", x.shape, x.stride(), x.dtype, x.device, gate_up.sig, down.sig, _sig(residual),
            _sig(norm_weight), _sig(out))
     plan = _PLANS.get(key)
@@ -390,6 +396,7 @@ def qkv_rope(x, norm_weight, eps, w, bias, cos, sin, slot_mapping, k_pool, v_poo
     of a hidden size up to 2048 in one launch, more through `linear` and rope_kv_write (whose rows of cos and sin
     lie at multiples of 16 bytes), bitwise the same."""
     assert type(w) is Weight, "w: a Weight"
+    assert type(x) is not Rows, _ROWS_GO
     rows, hidden = x.shape
     if rows > FUSED_ROWS or hidden > FUSED_IN:
         qkv = linear(x, w, bias=bias, norm_weight=norm_weight, eps=eps)
