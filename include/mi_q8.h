@@ -7,9 +7,9 @@
  * in a model whose projections are held in 8 bits.
  *
  * Rows in 8 bits.  A row v of n numbers is held as n int8 and one fp32 scale:
- *   scale = max(max |v|, 2^-100) / 127,   value = round_half_even(v / scale), at most 127 in size.
- * A row that holds an infinity or a NaN has scale NaN (and zeros), so that whatever is computed from
- * it is NaN.  The values are laid out for the products: panels of 16 rows,
+ *   scale = max(max |v|, 2^-100) / 127,   value = round_half_even(v / scale), at most 127 in size
+ * (normalised rows: see mi_q8_add_rmsnorm).  A row that holds an infinity or a NaN has scale NaN (and zeros), so that
+ * whatever is computed from it is NaN.  The values are laid out for the products: panels of 16 rows,
  *   [ceil(rows / 16)][np / 64][4][16 rows][16 values], np = n rounded up to a multiple of 128,
  * zeros from n on, mi_q8_rows_bytes() bytes, 16-byte aligned; rows past the last keep what they hold.
  *
@@ -54,6 +54,9 @@ MI_Q8_API int mi_q8_quantize(int32_t dtype, const void* x, int64_t x_stride, voi
 /*
  * r = x + y, rounded (y NULL: r is x, and residual_out is not used); values and scale are the rows of
  * r * rsqrt(mean(r^2) + eps) * weight in 8 bits, taken in fp32 without a rounding in between.
+ * The largest |r * weight| counts as at least 2^-100.  The mean is fp32's, as mi_fa2_add_rmsnorm's is: of a finite row
+ * whose squares pass fp32 (bf16 numbers of 1.8e19 and more) the scale is 0, and the row zeros; where mean and eps are 0 the
+ * scale is infinite, and the row zeros times that.
  * residual_out may be x or y, and shares nothing with them otherwise.
  */
 typedef struct mi_q8_norm_args {
