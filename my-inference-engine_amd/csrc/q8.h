@@ -172,7 +172,6 @@ struct Q8QuantParams {
   int32_t M, n, np;
   int32_t spread;         // work-groups are dealt so that a panel's rows share an XCD
 };
-enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2, kQ8Rows = 3 };
 hipError_t launch_q8_quant(const Q8QuantParams& p, int dtype, int source, hipStream_t stream);
 
 struct Q8DequantParams {

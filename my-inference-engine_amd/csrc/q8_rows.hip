@@ -426,51 +426,51 @@ __global__ __launch_bounds__(kQrThreads, 2) void q8_tile_kernel(const Q8Params p
 namespace {
 
 template <typename E, int MT, int NP, bool GATED, int SRC, RowsTile TILE = kQrPanels>
-hipError_t launch_rows_k(const Q8Params& p, int grid, hipStream_t stream) {
-  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kQrThreads), 0, stream, p); };
-  // Steps a wave has in flight where x does not stay: one token's half tiles of 1536 x 8960 take all 18 at once
-  // (the feed-forward block 17.1 -> 15.4 us); with rows in 8 bits beside them 9 (6.0 us, 18: 7.1).
-  constexpr int kMany = SRC == kQ8Float && TILE == kQrHalf ? 18 : MT == 1 ? 9 : 6;
+hipError_t launch_rows_k(const Q8Params& p, const Q8RowsChoice& c, hipStream_t stream) {
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(c.grid), dim3(kQrThreads), 0, stream, p); };
   if constexpr (SRC == kQ8Float) {
-    if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, 1>);
-    else go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE, kQ8FloatMax>);
-  }
-  else if constexpr (TILE == kQrHalf) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
-  else if (p.Kp <= 1024) go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, TILE>);
-  else if (p.Kp <= 1536) go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, TILE>);
-  else if (p.Kp <= kQ8KeepK) {
-    if constexpr (NP < 4) go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, TILE>);
-    else return hipErrorInvalidValue;   // (q8_rows_shape: two panels at most)
-  } else {
+    constexpr int kSteps = TILE == kQrHalf ? 18 : 9;
+    if (c.steps != kSteps) return hipErrorInvalidValue;
+    if (p.M == 1) go(q8_rows_kernel<E, MT, NP, kSteps, GATED, SRC, false, TILE, 1>);
+    else go(q8_rows_kernel<E, MT, NP, kSteps, GATED, SRC, false, TILE, kQ8FloatMax>);
+  } else if (!c.keep) {
+    constexpr int kSteps = MT == 1 ? 9 : 6;
+    if (c.steps != kSteps) return hipErrorInvalidValue;
     // (q8_plan: no more than 32 rows of these)
-    if constexpr (SRC == kQ8Rows && MT < 4 && NP != 2) go(q8_rows_kernel<E, MT, NP, kMany, GATED, SRC, false, TILE>);
+    if constexpr (SRC == kQ8Rows && MT < 4 && NP != 2) go(q8_rows_kernel<E, MT, NP, kSteps, GATED, SRC, false, TILE>);
     else return hipErrorInvalidValue;
+  } else if constexpr (TILE == kQrHalf) {
+    return hipErrorInvalidValue;
+  } else {
+    switch (c.steps) {
+      case 2: go(q8_rows_kernel<E, MT, NP, 2, GATED, SRC, true, TILE>); break;
+      case 3: go(q8_rows_kernel<E, MT, NP, 3, GATED, SRC, true, TILE>); break;
+      case 4:   // (q8_rows_shape: two panels at most)
+        if constexpr (NP < 4) {
+          go(q8_rows_kernel<E, MT, NP, 4, GATED, SRC, true, TILE>);
+          break;
+        }
+        [[fallthrough]];
+      default: return hipErrorInvalidValue;
+    }
   }
   return hipGetLastError();
 }
 
 template <typename E, bool GATED, int SRC>
 hipError_t launch_rows_m(const Q8Params& p, int n_cus, hipStream_t stream) {
-  const int grid = std::min(p.panels, n_cus);
+  const Q8RowsChoice c = q8_rows_choice(p.M, p.panels, p.Kp, n_cus, static_cast<Q8Source>(SRC), GATED);
   if constexpr (SRC == kQ8Rows) {
-    // (two work-groups a CU: 64 x 6400 x 2048 5.7 -> 6.7 us, 64 x 8192 x 1536 4.8 -> 5.2)
-    if (p.M > 32) return launch_rows_k<E, 4, 1, GATED, SRC>(p, grid, stream);
-    if (p.M > 16) return launch_rows_k<E, 2, 1, GATED, SRC>(p, grid, stream);
+    if (c.mt == 4) return launch_rows_k<E, 4, 1, GATED, SRC>(p, c, stream);
+    if (c.mt == 2) return launch_rows_k<E, 2, 1, GATED, SRC>(p, c, stream);
   }
-  const bool keep = SRC != kQ8Float && p.Kp <= kQ8KeepK;
-  // Few panels of many features: half a panel a work-group (1536 x 8960 by one token 6.4 -> 5.8 us).
   if constexpr (!GATED && (SRC == kQ8Rows || SRC == kQ8Float))
-    if (!keep && 2 * p.panels <= n_cus) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, 2 * p.panels, stream);
-  if constexpr (SRC != kQ8Float)
-    if (keep && (SRC != kQ8Rows || p.Kp <= 1536)) {   // (else 16 rows in 8 bits x 6400 x 2048 3.5 -> 4.3 us)
-      const Q8RowsShape shape = q8_rows_shape(p.panels, p.Kp, n_cus);
-      const int most = std::min((p.panels + shape.panels - 1) / shape.panels, shape.per_cu * n_cus);
-      if (shape.panels == 4) return launch_rows_k<E, 1, 4, GATED, SRC>(p, most, stream);
-      if (shape.panels == 2) return launch_rows_k<E, 1, 2, GATED, SRC>(p, most, stream);
-    } else if (!keep && p.panels >= 16 * n_cus) {   // (16 x 100000 x 4096 94 -> 85 us; one token 78 and 79)
-      return launch_rows_k<E, 1, 4, GATED, SRC>(p, n_cus, stream);
-    }
-  return launch_rows_k<E, 1, 1, GATED, SRC>(p, grid, stream);
+    if (c.half) return launch_rows_k<E, 1, 1, GATED, SRC, kQrHalf>(p, c, stream);
+  if constexpr (SRC != kQ8Float) {
+    if (c.panels == 4) return launch_rows_k<E, 1, 4, GATED, SRC>(p, c, stream);
+    if (c.panels == 2) return launch_rows_k<E, 1, 2, GATED, SRC>(p, c, stream);
+  }
+  return launch_rows_k<E, 1, 1, GATED, SRC>(p, c, stream);
 }
 
 template <typename E, bool GATED>
@@ -485,9 +485,10 @@ hipError_t launch_rows_s(const Q8Params& p, int source, int n_cus, hipStream_t s
 }  // namespace
 
 hipError_t launch_q8_qkv_rope(const Q8Params& p, int dtype, int n_cus, hipStream_t stream) {
-  const int grid = std::min(p.panels, n_cus);
-  return dtype == 0 ? launch_rows_k<BF16, 1, 1, false, kQ8Norm, kQrPairs>(p, grid, stream)
-                    : launch_rows_k<FP16, 1, 1, false, kQ8Norm, kQrPairs>(p, grid, stream);
+  Q8RowsChoice c = q8_rows_choice(p.M, p.panels, p.Kp, n_cus, kQ8Norm, false);
+  c.grid = std::min(p.panels, n_cus);   // (a tile is a panel here)
+  return dtype == 0 ? launch_rows_k<BF16, 1, 1, false, kQ8Norm, kQrPairs>(p, c, stream)
+                    : launch_rows_k<FP16, 1, 1, false, kQ8Norm, kQrPairs>(p, c, stream);
 }
 
 hipError_t launch_q8_tile(const Q8Params& p, const Q8Plan& plan, int dtype, bool gated, hipStream_t stream) {

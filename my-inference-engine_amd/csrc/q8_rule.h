@@ -3,12 +3,17 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace mi_fa2 {
 
 constexpr int kQ8RowsMax = 64;    // rows that the few-row kernel takes
 constexpr int kQ8KeepK = 2048;    // (padded) in features whose rows it keeps in registers
 constexpr int kQ8FusedMax = 16;   // rows that it brings to 8 bits itself, of at most kQ8KeepK
 constexpr int kQ8FloatMax = 4, kQ8FloatK = 12288;   // fp32 rows that it does, and their most features
+
+// What a product's rows are (and what is brought to 8 bits): 16-bit rows, the same normalised, fp32 rows, rows in 8 bits.
+enum Q8Source { kQ8Plain = 0, kQ8Norm = 1, kQ8Float = 2, kQ8Rows = 3 };
 
 // (tokens by features)
 enum Q8Kernel {
@@ -39,6 +44,39 @@ inline Q8RowsShape q8_rows_shape(int32_t panels, int32_t kp, int32_t cus) {
   if (panels <= 2 * cus || kp > 1536) return {2, 1};
   if (kp > 1024 && panels > 4 * cus && panels <= 8 * cus) return {2, 2};
   return {4, 1};
+}
+
+// The variant of the few-row kernel.
+struct Q8RowsChoice {
+  int32_t mt;      // tokens by 16
+  int32_t panels;  // a tile's, or half: one panel's halves
+  int32_t half;
+  int32_t keep;    // x stays in registers
+  int32_t steps;   // of K that a wave takes at a time (keep: all of its share)
+  int32_t grid;
+};
+inline Q8RowsChoice q8_rows_choice(int32_t rows, int32_t panels, int32_t kp, int32_t cus, Q8Source source, bool gated) {
+  const bool keep = source != kQ8Float && kp <= kQ8KeepK;
+  Q8RowsChoice c{rows > 32 ? 4 : rows > 16 ? 2 : 1, 1, 0, keep, 0, std::min(panels, cus)};
+  // (from 17 rows on a panel at a time; two work-groups a CU: 64 x 6400 x 2048 5.7 -> 6.7 us, 64 x 8192 x 1536 4.8 ->
+  // 5.2)
+  if (c.mt == 1) {
+    if (!gated && !keep && 2 * panels <= cus) {
+      // few panels of many features: half a panel a work-group (1536 x 8960 by one token 6.4 -> 5.8 us)
+      c.half = 1;
+      c.grid = 2 * panels;
+    } else if (keep && (source != kQ8Rows || kp <= 1536)) {   // (else 16 rows in 8 bits x 6400 x 2048 3.5 -> 4.3 us)
+      const Q8RowsShape shape = q8_rows_shape(panels, kp, cus);
+      c.panels = shape.panels;
+      c.grid = std::min((panels + shape.panels - 1) / shape.panels, shape.per_cu * cus);
+    } else if (!keep && source != kQ8Float && panels >= 16 * cus) {   // (16 x 100000 x 4096 94 -> 85 us; one token 78
+      c.panels = 4;                                                   // and 79)
+    }
+  }
+  // Where x does not stay: one token's half tiles of 1536 x 8960 take all 18 steps of a wave at once (the feed-forward
+  // block 17.1 -> 15.4 us); with rows in 8 bits beside them 9 (6.0 us, 18: 7.1).
+  c.steps = keep ? std::max(2, (kp + 511) / 512) : source == kQ8Float && c.half ? 18 : c.mt == 1 ? 9 : 6;
+  return c;
 }
 
 struct Q8Plan {
