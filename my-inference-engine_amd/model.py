@@ -406,7 +406,6 @@ class Qwen2ForCausalLM(nn.Module):
         w = self.embed_tokens.weight
         return w, w.data_ptr(), None if w.is_inference() else w._version
 
-    @torch.no_grad()
     def refresh_head8(self):
         """Bring the 8-bit head up to date with the embeddings, where they were changed since it was made: in
         place, so that captured steps read it too.  Every step calls this, a captured one before its replay."""
@@ -415,10 +414,12 @@ class Qwen2ForCausalLM(nn.Module):
         made, now = self._head8_made, self._embeddings()
         if made[0] is now[0] and made[1:] == now[1:]:
             return
-        new, old = q8.quantize_weight(now[0].detach()), self.head8
-        assert new.sig == old.sig, f"embeddings [{old.out_features}, {old.in_features}] on {old.device}, as quantize_ saw"
-        old.data.copy_(new.data)
-        old.scale.copy_(new.scale)
+        with torch.inference_mode():   # (in which quantize_ may have made the head)
+            new, old = q8.quantize_weight(now[0].detach()), self.head8
+            assert new.sig == old.sig, \
+                f"embeddings [{old.out_features}, {old.in_features}] on {old.device}, as quantize_ saw"
+            old.data.copy_(new.data)
+            old.scale.copy_(new.scale)
         self._head8_made = now
 
     def rope_cos_sin(self, position_ids, dtype):

@@ -100,3 +100,15 @@ def test_an_embedding_that_changes_changes_the_head():
     model.embed_tokens.weight = nn.Parameter(torch.cat([model.embed_tokens.weight] * 2), requires_grad=False)
     with pytest.raises(AssertionError, match="as quantize_ saw"):
         logits(model)
+
+
+def test_a_head_made_in_inference_mode_follows_too():
+    model, other = make(), make()
+    with torch.inference_mode():
+        model.quantize_(lm_head=True)
+    ids = tokens(torch.Generator().manual_seed(8), 1, 4)
+    with torch.no_grad():
+        for m in (model, other):
+            m.embed_tokens.weight[5:9] *= 3.0
+        got, want = (m(ids, c, [c.alloc()]) for m, c in ((model, cache_for()), (other.quantize_(lm_head=True), cache_for())))
+    assert torch.equal(got, want)
