@@ -10,8 +10,9 @@
 // numbers would change by a whole step (a hundredth of the row's largest) for it.
 //
 // Bound by memory: 16,384 rows of 1,536 with their residual 35.6 us (176 MB, 4.9 TB/s; a large copy moves 5.2),
-// 4,096 rows without 5.5 us and 4,001 rows of 8,960 in fp32 28 us (6.4 TB/s: out of the last-level cache), one
-// row 2.9 us.  All of a thread's loads go out before the first is used.
+// 4,096 rows without 5.3 us where they lie in the caches, 7.3 out of memory (19 MB, 2.6 TB/s; before a product that
+// evicts them 6.1 to 8.3), 4,001 rows of 8,960 in fp32 28 us (6.4 TB/s: out of the last-level cache), one row 2.9 us.
+// All of a thread's loads go out before the first is used.
 #include "q8.h"
 
 #include <algorithm>

@@ -74,7 +74,9 @@ inline Q8RowsChoice q8_rows_choice(int32_t rows, int32_t panels, int32_t kp, int
     }
   }
   // Where x does not stay: one token's half tiles of 1536 x 8960 take all 18 steps of a wave at once (the feed-forward
-  // block 17.1 -> 15.4 us); with rows in 8 bits beside them 9 (6.0 us, 18: 7.1).
+  // block 17.1 -> 15.4 us); with rows in 8 bits beside them 9 (6.0 us, 18: 7.1).  Past 9,216 features, where a wave
+  // has more than 18, nothing shows of it: blocks of 1536 x 8192, 9216, 9472, 10240, 12288 13.8, 14.9, 15.6, 16.6,
+  // 17.9 us (weights from memory; 12416, in a launch more, 22.8).
   c.steps = keep ? std::max(2, (kp + 511) / 512) : source == kQ8Float && c.half ? 18 : c.mt == 1 ? 9 : 6;
   return c;
 }
