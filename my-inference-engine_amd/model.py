@@ -412,6 +412,8 @@ class Qwen2ForCausalLM(nn.Module):
         if self.head8 is None:
             return
         made, now = self._head8_made, self._embeddings()
+        if made is None:   # a head from elsewhere, or saved whole before this was kept: of the embeddings as they are
+            self._head8_made = made = now
         if made[0] is now[0] and made[1:] == now[1:]:
             return
         with torch.inference_mode():   # (in which quantize_ may have made the head)

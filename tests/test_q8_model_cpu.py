@@ -102,3 +102,12 @@ def test_a_model_saved_before_there_was_quantize_runs():
     ids = torch.arange(5)[None]
     got, want = (m(ids, c, [c.alloc()]) for m, c in zip((old, Qwen2ForCausalLM(CFG).init_random()), caches))
     assert torch.equal(got, want) and old.weights_held()[0] == 0
+
+
+def test_a_head_that_quantize_did_not_make_is_kept():
+    """Set by hand, or saved whole with the model before it was kept what the head was made of."""
+    model = Qwen2ForCausalLM(CFG)
+    model.head8 = head = SimpleNamespace()
+    model.refresh_head8()
+    model.refresh_head8()
+    assert model.head8 is head
