@@ -13,9 +13,10 @@ products is its model.py:49-55,81-84,107,112-138,204-207.
 
 A row of n numbers v is held as round(v / scale) with scale = max|v| / 127; a row with an infinity or a NaN has
 scale NaN, and so is everything computed from it.  A norm's mean is taken in fp32, as kernels.model_ops takes it: of a
-finite row whose squares pass that (bf16, 1.8e19 and more) it is infinite and the row comes out as zeros.  Inference only: no gradient is recorded.  Products are whole
-numbers, exact in 32 bits; scales, bias and residual are applied in fp32 and the result is rounded once.  No CPU
-path and no fallback: a missing library or a call that the kernels do not take raises.
+finite row whose squares pass that (bf16, 1.8e19 and more) it is infinite and the row comes out as zeros.  Inference
+only: no gradient is recorded.  Products are whole numbers, exact in 32 bits; scales, bias and residual are applied in
+fp32 and the result is rounded once.  No CPU path and no fallback: a missing library or a call that the kernels do not
+take raises.
 """
 import ctypes
 import os

@@ -375,8 +375,8 @@ class Qwen2ForCausalLM(nn.Module):
     @torch.no_grad()
     def quantize_(self, lm_head=False):
         """Hold the layers' projections (and, asked for, a copy of the tied embeddings as the output head, which
-        follows them when they change) in 8 bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit weights are let go: capture decode
-        graphs after this, those captured before refuse to run."""
+        follows them when they change) in 8 bits from now on.  The model is on the GPU, in bf16 or fp16.  The 16-bit
+        weights are let go: capture decode graphs after this, those captured before refuse to run."""
         held = [(m, name) for layer in self.layers
                 for m, name in ((layer.self_attn, "qkv_proj"), (layer.self_attn, "o_proj"),
                                 (layer.mlp, "gate_up_proj"), (layer.mlp, "down_proj"))]
